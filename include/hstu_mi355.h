@@ -264,6 +264,118 @@ typedef struct hstu_paged_fwd_params {
 HSTU_API int hstu_paged_fwd_workspace_size(const hstu_paged_fwd_params* params, uint64_t* workspace_bytes);
 HSTU_API int hstu_paged_fwd(const hstu_paged_fwd_params* params, void* workspace, uint64_t workspace_bytes, void* stream);
 
+/*
+ * 8-bit paged key / value cache: writing new rows, attention, eviction.  No counterpart in the reference, whose paged cache holds
+ * the type of q.  A cache of one layer is
+ *
+ *   k_cache  e4m3 [num_pages, num_heads_k, page_size / 32, 32, head_dim]   rows of a block of 32 tokens
+ *   v_cache  e4m3 [num_pages, num_heads_k, page_size / 32, head_dim, 32]   the same, tokens innermost
+ *   k_scale, v_scale  fp32 [num_pages, num_heads_k, page_size / 32]        a scale per block and head, a power of two
+ *   weights  fp32 [num_pages, num_heads_k, page_size]                      accumulated attention weights; may be NULL
+ *
+ * The rows of sequence b are those of its pages page_ids[page_offsets[b] : page_offsets[b + 1]] in order, the first cache_len[b] of
+ * them live.  Page ids outside [0, num_pages) stand for pages that are not there: nothing is read from them (their rows count as
+ * zeros) or written to them.  A page that a call writes to must stand in it once, and nowhere else in the call; a page that is
+ * only read may be shared by sequences.  head_dim is a multiple of 16 in [16, 256], page_size a multiple of 32; pointers to
+ * caches, q, k, v and out are 16-byte aligned.
+ */
+#define HSTU_PAGED_FP8_MAX_SEQ_LEN_K 16777216
+#define HSTU_PAGED_FP8_MAX_HEAD_DIM 256
+
+typedef struct hstu_paged_fp8_cache {
+    void* k_cache;
+    void* v_cache;
+    float* k_scale;
+    float* v_scale;
+    float* weights;
+    const void* cache_len;    /* [n_offsets - 1], index dtype */
+    const void* page_offsets; /* [n_offsets] */
+    const void* page_ids;     /* [n_page_ids] */
+    int64_t num_pages;
+    int64_t page_size;
+    int64_t n_page_ids;
+    int64_t num_heads_k;
+    int64_t head_dim;
+    int64_t n_offsets; /* batch + 1 */
+    int32_t index_dtype;
+    int32_t reserved0;
+} hstu_paged_fp8_cache;
+
+/*
+ * out = silu(alpha Q K^T) * silu_scale * M . V, the built-in mask of hstu_jagged_fwd with s_k = cache_len[b] (the rows of the call are
+ * in the cache already), no context rows; with window > 0 a row at position p sees of those keys only j > p - window and
+ * j < sinks, where a target row stands at the position of the first target.  Where cache.weights is given, the weights
+ * silu(...) * silu_scale * M are added up in magnitude over rows and query heads and added to it.  Rows of q that belong to no
+ * sequence, and rows past max_seq_len_q of one, come out as zeros; cache_len is cut at max_seq_len_k.
+ */
+typedef struct hstu_paged_fp8_fwd_params {
+    uint32_t struct_size; /* sizeof(hstu_paged_fp8_fwd_params) */
+    int32_t dtype;        /* of q and out: HSTU_DT_BF16 or HSTU_DT_FP16 */
+    hstu_paged_fp8_cache cache;
+    const void* q;          /* [total_q, num_heads_q, head_dim] */
+    void* out;              /* the same */
+    const void* seq_offset; /* [n_offsets] */
+    const void* num_target; /* [n_offsets - 1]; may be NULL */
+    int64_t total_q;
+    int64_t num_heads_q;
+    int64_t max_seq_len_q;
+    int64_t max_seq_len_k;
+    int64_t target_group_size;
+    int64_t window;
+    int64_t sinks;
+    double silu_scale; /* resolved: not 0 */
+    double alpha;
+} hstu_paged_fp8_fwd_params;
+
+HSTU_API int hstu_paged_fp8_fwd_workspace_size(const hstu_paged_fp8_fwd_params* params, uint64_t* workspace_bytes);
+HSTU_API int hstu_paged_fp8_fwd(const hstu_paged_fp8_fwd_params* params, void* workspace, uint64_t workspace_bytes, void* stream);
+HSTU_API const char* hstu_paged_fp8_fwd_kernel_name(const hstu_paged_fp8_fwd_params* params);
+
+/*
+ * Rows seq_offset[b] : seq_offset[b + 1] of k and v go to the positions cache_len[b], cache_len[b] + 1, ... of sequence b (cache_len is
+ * not changed; rows that its pages have no room for are dropped).  Every block touched gets a new scale, the smallest power of two
+ * that brings its largest finite magnitude, old rows included, to at most 448; codes round to nearest even, values that are not
+ * finite become NaN.  The rows of a touched block behind the new end are cleared; weights of new rows and of those become 0.
+ */
+typedef struct hstu_paged_fp8_append_params {
+    uint32_t struct_size; /* sizeof(hstu_paged_fp8_append_params) */
+    int32_t dtype;        /* of k and v: HSTU_DT_BF16 or HSTU_DT_FP16 */
+    hstu_paged_fp8_cache cache;
+    const void* k; /* [total, num_heads_k, head_dim] with these strides (elements, multiples of 8), head_dim contiguous */
+    const void* v;
+    const void* seq_offset; /* [n_offsets] */
+    int64_t total;
+    int64_t k_stride_row, k_stride_head;
+    int64_t v_stride_row, v_stride_head;
+    int64_t max_seq_len; /* of the rows of a sequence; rows past it are dropped */
+} hstu_paged_fp8_append_params;
+
+HSTU_API int hstu_paged_fp8_append(const hstu_paged_fp8_append_params* params, void* stream);
+
+/*
+ * Of each sequence at most `keep` rows stay (no more than the new pages hold): the first `sinks`, the last `recent`, and of the others
+ * those with the largest scores, ties to the lower index; a score is the fp32 sum of a row's weights over the key heads, in
+ * their order.  The rows that stay are moved in order to the new pages (new_page_ids[new_page_offsets[b] : ...]), with new
+ * scales and their weights; new_cache_len[b] is their number, kept[b] their old indices, -1 behind them.
+ */
+typedef struct hstu_paged_fp8_evict_params {
+    uint32_t struct_size; /* sizeof(hstu_paged_fp8_evict_params) */
+    uint32_t reserved0;
+    hstu_paged_fp8_cache cache; /* with weights */
+    const void* new_page_offsets; /* [n_offsets] */
+    const void* new_page_ids;     /* [n_new_page_ids] */
+    void* new_cache_len;          /* [n_offsets - 1], index dtype */
+    void* kept;                   /* [n_offsets - 1, keep], index dtype */
+    int64_t n_new_page_ids;
+    int64_t max_seq_len_k;
+    int64_t keep;
+    int64_t sinks;
+    int64_t recent;
+} hstu_paged_fp8_evict_params;
+
+HSTU_API int hstu_paged_fp8_evict_workspace_size(const hstu_paged_fp8_evict_params* params, uint64_t* workspace_bytes);
+HSTU_API int hstu_paged_fp8_evict(const hstu_paged_fp8_evict_params* params, void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* replaces aclGetRecentErrMsg (ascendc/common/torch_plugin/pytorch_npu_helper.hpp:649,662):
  * text of the calling thread's most recent failure; never NULL. */
 HSTU_API const char* hstu_last_error(void);

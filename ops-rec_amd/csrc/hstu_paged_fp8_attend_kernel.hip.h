@@ -1,0 +1,576 @@
+// HSTU attention over the 8-bit paged cache (gfx950).
+//
+//   S = Q K^T,  P = silu(alpha S) * silu_scale * M,  O = P V,  with K and V the codes of the cache times their blocks' scales
+//
+// A step is one block of 32 keys, which lies in one page and has one scale for K and one for V.  Both products run on
+// v_mfma_f32_32x32x16 in the type of q: e4m3 values times a power of two are exact there, and v_cvt_scalef32_pk multiplies by
+// the scale while it converts, so scales cost nothing.
+//   S^T[key][row] = K . Q^T     A = K: lane l % 32 takes key pi(l % 32) of the block, 16 dims of its half at a time; B = Q, in
+//                               registers from the start, the same dims
+//   O^T[dim][row] += V^T . P^T  A = V^T: lane l % 32 takes dim pi(l % 32) of a group of 32, the 16 keys of its half; B = P
+// The rows of the 32x32 result that a lane holds are 8 a + 4 half + b (a, b = 0 .. 3).  With pi(8 a + 4 h + b) = 16 h + 4 a + b a
+// lane's 16 values of S are the keys 16 half .. + 15 in order, which is what the second product wants of B when A's lanes load 16
+// consecutive keys: P goes from one product to the other in its registers, V (stored with the keys innermost) comes straight from
+// memory, and no value passes through LDS or another lane.  The same order of V's dims gives a lane 16 consecutive output dims.
+//
+// The columns of the result are rows of q: (row, query head of the key head's group) pairs, head fastest, so that grouped heads
+// share the keys that are read.
+#pragma once
+#include "hstu_paged_fp8_common.hip.h"
+
+namespace hstu {
+
+typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+
+// One 16-byte chunk of codes as eight + eight 16-bit values.
+struct Fp8Pair {
+    u32x4_t lo, hi;
+};
+template <typename Tag>
+__device__ __forceinline__ uint32_t fp8_two(uint32_t codes, float scale, bool hi);
+template <>
+__device__ __forceinline__ uint32_t fp8_two<bf16_tag>(uint32_t codes, float scale, bool hi)
+{
+    return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true))
+              : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false));
+}
+template <>
+__device__ __forceinline__ uint32_t fp8_two<f16_tag>(uint32_t codes, float scale, bool hi)
+{
+    return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, true))
+              : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, false));
+}
+template <typename Tag>
+__device__ __forceinline__ Fp8Pair fp8_widen(u32x4_t codes, float scale)
+{
+    Fp8Pair r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        r.lo[2 * i] = fp8_two<Tag>(codes[i], scale, false);
+        r.lo[2 * i + 1] = fp8_two<Tag>(codes[i], scale, true);
+        r.hi[2 * i] = fp8_two<Tag>(codes[2 + i], scale, false);
+        r.hi[2 * i + 1] = fp8_two<Tag>(codes[2 + i], scale, true);
+    }
+    return r;
+}
+
+// 0x80 in the place of each of four codes that is NaN (0x7f, 0xff), 0 elsewhere
+__device__ __forceinline__ uint32_t nan_codes(uint32_t codes) { return ((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+__device__ __forceinline__ u32x4_t load_codes(__amdgpu_buffer_rsrc_t rsrc, uint32_t offset)
+{
+    return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, static_cast<int>(offset), 0, 0));
+}
+
+// The blocks that some row of a range of rows sees, in at most three runs: the first tokens (sinks), what the window or the
+// whole history leaves up to the targets, and the targets' own groups.
+struct Fp8Runs {
+    int n_a, n_b, n_c;  // blocks of each
+    int b0, c0;         // first block of the second and of the third
+    __device__ __forceinline__ int count() const { return n_a + n_b + n_c; }
+    __device__ __forceinline__ int block(int n) const { return n < n_a ? n : (n < n_a + n_b ? b0 + n - n_a : c0 + n - n_a - n_b); }
+};
+
+// What a sequence's rows see: row i (position p = i + len - rows) sees the keys j <= p; a target row, of the last `targets`, not
+// the targets of the groups above its own; with a window only j > centre - window and j < sinks, the centre being p, or for a
+// target row the first target.
+struct Fp8Mask {
+    int len, delta, first_target, first_key, group, window, sinks;
+    bool targets;
+
+    __device__ __forceinline__ int lim(int i) const  // one past the last key
+    {
+        const int e = i + delta + 1;
+        return e < 0 ? 0 : (e > len ? len : e);
+    }
+    __device__ __forceinline__ int hole(int i) const  // keys [first_key, hole) are not seen
+    {
+        return targets && i >= first_target ? first_key + (i - first_target) / group * group : first_key;
+    }
+    __device__ __forceinline__ int low(int i) const  // keys [sinks, low) are not seen
+    {
+        const int centre = targets && i >= first_target ? first_key : i + delta;
+        return window > 0 ? centre - window + 1 : 0;
+    }
+};
+
+__device__ __forceinline__ Fp8Runs fp8_runs(const Fp8Mask& m, int i0, int i1)  // rows [i0, i1), i0 < i1
+{
+    Fp8Runs r;
+    const int end = (m.lim(i1 - 1) + kFp8Block - 1) / kFp8Block;
+    const int low = m.low(i0) > 0 ? m.low(i0) / kFp8Block : 0;
+    const int sinks = m.window > 0 && m.sinks > 0 ? (m.sinks + kFp8Block - 1) / kFp8Block : 0;
+    r.n_a = sinks < low ? (sinks < end ? sinks : end) : 0;
+    const int b = sinks < low ? low : 0;  // (0: the window reaches the first tokens, one run)
+    r.b0 = b;
+    // the blocks that lie whole in what even the first row does not see of the targets
+    int h0 = end, h1 = end;
+    const int hole = m.hole(i0);
+    if (hole > m.first_key && m.first_key >= 0) {
+        h0 = (m.first_key + kFp8Block - 1) / kFp8Block;
+        h1 = hole / kFp8Block;
+        if (h1 <= h0 || h0 < b) {
+            h0 = h1 = end;
+        }
+    }
+    h0 = h0 < end ? h0 : end;
+    h1 = h1 < end ? h1 : end;
+    r.n_b = h0 > b ? h0 - b : 0;
+    r.c0 = h1;
+    r.n_c = end > h1 ? end - h1 : 0;
+    return r;
+}
+
+// One sequence of a call: its rows of q, its pages and live keys, and what its rows see.
+struct Fp8Item {
+    Fp8Sequence seq;
+    int64_t q0, q1;  // rows of q
+    int n_rows;      // of them within the longest length allowed
+    Fp8Mask mask;
+};
+__device__ __forceinline__ Fp8Item fp8_item(const Fp8AttendArgs& a, int b)
+{
+    const Fp8Cache& c = a.c;
+    Fp8Item it;
+    it.seq = fp8_sequence(c, b);
+    it.seq.len = it.seq.len < a.max_k ? it.seq.len : a.max_k;
+    int64_t q0 = load_index_uniform(a.offs_q, b, c.idx64), q1 = load_index_uniform(a.offs_q, b + 1, c.idx64);
+    q0 = q0 < 0 ? 0 : (q0 > a.total_q ? a.total_q : q0);
+    q1 = q1 < q0 ? q0 : (q1 > a.total_q ? a.total_q : q1);
+    it.q0 = q0;
+    it.q1 = q1;
+    it.n_rows = static_cast<int>(q1 - q0 < a.max_q ? q1 - q0 : a.max_q);
+    int n_targets = 0;
+    if (a.num_target != nullptr && a.group > 0) {
+        const int64_t t = load_index_uniform(a.num_target, b, c.idx64);
+        n_targets = static_cast<int>(t < 0 ? 0 : (t > 0x3fffffff ? 0x3fffffff : t));
+    }
+    Fp8Mask& m = it.mask;
+    m.len = it.seq.len;
+    m.delta = it.seq.len - it.n_rows;
+    m.targets = n_targets > 0;
+    m.first_target = it.n_rows - n_targets;
+    m.first_key = it.seq.len - n_targets;
+    m.group = m.targets ? a.group : 1;
+    m.window = a.window;
+    m.sinks = a.sinks;
+    return it;
+}
+
+// Tag     : type of q and out
+// NC      : groups of 32 dims (dim is at most 32 NC, a multiple of 16)
+// NB      : columns of 32 rows of a wavefront
+// WK, WR  : wavefronts of a workgroup over the keys of a row tile, and over row tiles
+// WEIGHTS : the sums of |P| per key as well
+template <typename Tag, int NC, int NB, int WK, int WR, bool WEIGHTS>
+__global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(const Fp8AttendArgs a)
+{
+    constexpr int ROWS = 32 * NB;        // (row, head) pairs of a wavefront
+    constexpr int TILE = ROWS * WR;      // and of a workgroup
+    constexpr int CHUNK_WORDS = NB * 64 * 16;
+    __shared__ __attribute__((aligned(16))) float s_sum[WK > 1 ? 2 : 1][WK > 1 ? WK * CHUNK_WORDS : 4];
+
+    const Fp8Cache& c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    const int wk = WR > 1 ? 0 : wave, wr = WR > 1 ? wave : 0;
+    static_assert(WK == 1 || WR == 1, "keys or rows");
+
+    // slots: (pair of sequence and key head) x row tile x part; the tiles of a pair, which read the same keys, on one XCD
+    // (workgroup w runs on XCD w mod 8); parts of one tile have no keys in common and go to all of them
+    const int slot = static_cast<int>(blockIdx.x);
+    const int n_pairs = c.n_batch * c.n_heads;
+    int pair, part = 0, tile = 0;
+    if (a.row_tiles == 1) {
+        part = slot / n_pairs;
+        pair = slot - part * n_pairs;
+    } else {
+        const int per_pair = a.row_tiles * a.parts;
+        const int oct = slot / (8 * per_pair), rest = slot - oct * 8 * per_pair, in_pair = rest >> 3;
+        pair = oct * 8 + (rest & 7);
+        part = in_pair / a.row_tiles;
+        tile = a.row_tiles - 1 - (in_pair - part * a.row_tiles);  // (later rows see more keys: first)
+    }
+    pair = uniform(pair);
+    part = uniform(part);
+    tile = uniform(tile);
+    if (pair >= n_pairs) {
+        return;
+    }
+    const int b = uniform(pair / c.n_heads), g = pair - b * c.n_heads;
+
+    const Fp8Item item = fp8_item(a, b);
+    const Fp8Sequence& seq = item.seq;
+    const Fp8Mask& mask = item.mask;
+    const int64_t q0 = item.q0, q1 = item.q1;
+    const int n_rows = item.n_rows;
+    const int dim = c.dim;
+    uint16_t* const out = static_cast<uint16_t*>(a.out);
+
+    // rows of no sequence, and rows past the longest sequence allowed: zeros
+    if (tile == 0 && part == 0) {
+        const int64_t row_words = static_cast<int64_t>(a.n_heads_q) * dim, mine = static_cast<int64_t>(a.ratio) * dim;
+        const auto clear = [&](int64_t from, int64_t to) {
+            for (int64_t r = from; r < to; ++r) {
+                for (int64_t x = tid; x < mine; x += 64 * WK * WR) {
+                    out[r * row_words + g * mine + x] = 0;
+                }
+            }
+        };
+        clear(q0 + n_rows, q1);
+        if (b == 0) {
+            clear(0, q0);
+        }
+        if (b == c.n_batch - 1) {
+            clear(q1, a.total_q);
+        }
+    }
+
+    const int n_pairs_rows = n_rows * a.ratio;  // (row, head) pairs
+    if (tile * TILE >= n_pairs_rows) {
+        return;
+    }
+    const int m0 = tile * TILE + wr * ROWS;
+    const int m1 = m0 + ROWS < n_pairs_rows ? m0 + ROWS : n_pairs_rows;
+    // what this wavefront sweeps: its rows' blocks (all wavefronts of a tile's keys have the same rows)
+    Fp8Runs runs = {0, 0, 0, 0, 0};
+    int i_first = 0, i_last = 0;
+    if (m0 < m1) {
+        i_first = uniform(div_small(m0, a.ratio));
+        i_last = uniform(div_small(m1 - 1, a.ratio));
+        runs = fp8_runs(mask, i_first, i_last + 1);
+        runs = {uniform(runs.n_a), uniform(runs.n_b), uniform(runs.n_c), uniform(runs.b0), uniform(runs.c0)};
+    }
+    const int n_blocks = runs.count();
+    const int parts_used = a.parts == 1 ? 1 : uniform((n_blocks + a.chunk - 1) / a.chunk);
+    if (a.parts > 1 && part > 0 && part >= parts_used) {
+        return;
+    }
+    const int n_begin = a.parts == 1 ? 0 : part * a.chunk;
+    const int n_end = a.parts == 1 || part == a.parts - 1 ? n_blocks : (n_begin + a.chunk < n_blocks ? n_begin + a.chunk : n_blocks);
+
+    // q: the rows of this wavefront, 16 dims of this lane's half per group of 32
+    u32x4_t q[NB][NC][2];
+    int lim[NB], hole[NB], low[NB];
+    {
+        const uint32_t bytes = static_cast<uint32_t>(n_rows) * static_cast<uint32_t>(a.n_heads_q) * dim * 2u;
+        const __amdgpu_buffer_rsrc_t rsrc =
+            make_rsrc(static_cast<const uint16_t*>(a.q) + q0 * a.n_heads_q * static_cast<int64_t>(dim), bytes);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int m = m0 + nb * 32 + col, i = div_small(m < n_pairs_rows ? m : 0, a.ratio);
+            const bool there = m < n_pairs_rows;
+            const uint32_t at = (static_cast<uint32_t>(i) * a.n_heads_q + g * a.ratio + (m - i * a.ratio)) * dim * 2u;
+            lim[nb] = there ? mask.lim(i) : 0;
+            hole[nb] = mask.hole(i);
+            low[nb] = mask.low(i);
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int d = 32 * n + 16 * half + 8 * u;
+                    q[nb][n][u] = load_codes(rsrc, there && d < dim ? at + d * 2u : kOutOfRange);
+                }
+            }
+        }
+    }
+
+    // offsets of this lane's chunks within a block of codes; dims past the last read as zeros
+    const int pi = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);
+    const uint32_t block_bytes = static_cast<uint32_t>(kFp8Block) * dim;
+    uint32_t k_at[NC], v_at[NC];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        const int d = 32 * n + 16 * half;
+        k_at[n] = d < dim ? static_cast<uint32_t>(pi) * dim + d : kOutOfRange;
+        v_at[n] = 32 * n + pi < dim ? static_cast<uint32_t>(32 * n + pi) * kFp8Block + 16 * half : kOutOfRange;
+    }
+
+    f32x16_t acc[NB][NC];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            acc[nb][n] = f32x16_t{0.0f};
+        }
+    }
+
+    // bounds for the whole wavefront: a block inside them needs no mask
+    const int lim_min = mask.lim(i_first), low_max = mask.low(i_last), hole_max = uniform(mask.hole(i_last));
+
+    // Steps of this wavefront: blocks n_begin + wk, + WK, ...; the places and scales of 64 of them at a time, a step per lane.  They are
+    // looked up, and handed out by readlane, with every lane active: a lane that is not has no value that another may count on (the
+    // compiler may move a value between registers under the mask of a branch).
+    const int n_steps = n_end - n_begin - wk > 0 ? (n_end - n_begin - wk + WK - 1) / WK : 0;
+    int my_lin = -1;
+    float my_ks = 1.0f, my_vs = 1.0f;
+    const auto look_up = [&](int base) {  // (base < n_steps; lanes behind the last step take it too)
+        const int s = base + lane < n_steps ? base + lane : n_steps - 1;
+        my_lin = fp8_block(c, c.page_ids, seq.first, g, runs.block(n_begin + wk + s * WK));
+        const int at = my_lin >= 0 ? my_lin : 0;
+        my_ks = c.k_scale[at];
+        my_vs = c.v_scale[at];
+    };
+    const auto place_of = [&](int s) { return __builtin_amdgcn_readlane(my_lin, s & 63); };
+
+    struct Stage {
+        u32x4_t k[NC], v[NC];
+    };
+    const auto request = [&](Stage& st, int s) {
+        const int lin = place_of(s);
+        const int64_t at = static_cast<int64_t>(lin < 0 ? 0 : lin) * block_bytes;
+        const __amdgpu_buffer_rsrc_t kr = make_rsrc(c.k + at, lin < 0 ? 0u : block_bytes), vr = make_rsrc(c.v + at, lin < 0 ? 0u : block_bytes);
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            st.k[n] = load_codes(kr, k_at[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            st.v[n] = load_codes(vr, v_at[n]);
+        }
+    };
+    const auto sees_key = [&](int j, int nb) {  // whether this lane's row of column nb sees key j
+        return static_cast<bool>((j < lim[nb]) & ((j < mask.first_key) | (j >= hole[nb])) & ((j >= low[nb]) | (j < mask.sinks)));
+    };
+    const auto step = [&](Stage& st, int s, float ks, float vs) {
+        const int lin = place_of(s);
+        const int blk = runs.block(n_begin + wk + s * WK), c0 = blk * kFp8Block;
+        f32x16_t sc[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            sc[nb] = f32x16_t{0.0f};
+        }
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            const Fp8Pair kk = fp8_widen<Tag>(st.k[n], ks);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                sc[nb] = mfma32<Tag>(kk.lo, q[nb][n][0], sc[nb]);
+                sc[nb] = mfma32<Tag>(kk.hi, q[nb][n][1], sc[nb]);
+            }
+        }
+        const int end = c0 + kFp8Block;
+        const bool whole = end <= lim_min && (c0 >= low_max || end <= mask.sinks) && (end <= mask.first_key || c0 >= hole_max);
+        u32x4_t p[NB][2];
+        float sums[16];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            float w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float x = sc[nb][i];
+                w[i] = x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * a.c_exp));
+            }
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    w[i] = sees_key(c0 + 16 * half + i, nb) ? w[i] : 0.0f;
+                }
+            }
+            if constexpr (WEIGHTS) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    sums[i] = nb == 0 ? __builtin_fabsf(w[i]) : sums[i] + __builtin_fabsf(w[i]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    p[nb][u][i] = pack2<Tag>(w[8 * u + 2 * i], w[8 * u + 2 * i + 1]);
+                }
+            }
+        }
+        if (end > seq.len) {  // codes behind the last row may be anything, NaN among them: zero times that is not zero
+            const int left = seq.len - c0 - 16 * half;  // live keys of this lane's sixteen
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int n = left - 4 * i;
+                const uint32_t keep = n >= 4 ? 0xffffffffu : (n <= 0 ? 0u : (1u << (8 * n)) - 1u);
+#pragma unroll
+                for (int k = 0; k < NC; ++k) {
+                    st.v[k][i] &= keep;
+                }
+            }
+        }
+        // A key that some rows do not see must not reach them, and zero times NaN would.  The codes for NaN are found by their bits; where
+        // a block with a mask holds one, the products run on zeros in their place, and afterwards a product of ones there with the mask
+        // says which outputs are NaN.
+        bool poisoned = false;
+        if (!whole) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t bits = nan_codes(st.v[n][i]);
+                    any |= bits;
+                    st.v[n][i] &= ~((bits >> 7) * 0xffu);
+                }
+            }
+            poisoned = __any(any != 0);
+        }
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            const Fp8Pair vv = fp8_widen<Tag>(st.v[n], vs);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                acc[nb][n] = mfma32<Tag>(vv.lo, p[nb][0], acc[nb][n]);
+                acc[nb][n] = mfma32<Tag>(vv.hi, p[nb][1], acc[nb][n]);
+            }
+        }
+        if (poisoned) {  // (the codes are read again: nothing is kept for this case)
+            const __amdgpu_buffer_rsrc_t vr = make_rsrc(c.v + static_cast<int64_t>(lin < 0 ? 0 : lin) * block_bytes, lin < 0 ? 0u : block_bytes);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                u32x4_t sees[2];
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const int j = c0 + 16 * half + i;
+                    sees[i >> 3][(i >> 1) & 3] = pack2<Tag>(sees_key(j, nb) ? 1.0f : 0.0f, sees_key(j + 1, nb) ? 1.0f : 0.0f);
+                }
+#pragma unroll
+                for (int n = 0; n < NC; ++n) {
+                    u32x4_t ones = load_codes(vr, v_at[n]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        ones[i] = (nan_codes(ones[i]) >> 7) * 0x38u;  // the code of 1
+                    }
+                    const Fp8Pair oo = fp8_widen<Tag>(ones, 1.0f);
+                    f32x16_t hits = mfma32<Tag>(oo.lo, sees[0], f32x16_t{0.0f});
+                    hits = mfma32<Tag>(oo.hi, sees[1], hits);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        acc[nb][n][i] = hits[i] > 0.0f ? __builtin_nanf("") : acc[nb][n][i];
+                    }
+                }
+            }
+        }
+        if constexpr (WEIGHTS) {
+            // the sum over the 32 lanes of a half, halving the values a lane carries in each of four exchanges: lane x ends with the key
+            // whose bits are those of x, highest first
+#pragma unroll
+            for (int d = 16, width = 8; d >= 2; d >>= 1, width >>= 1) {
+#pragma unroll
+                for (int i = 0; i < width; ++i) {
+                    const bool upper = (lane & d) != 0;
+                    const float give = upper ? sums[i] : sums[i + width];
+                    const float keep = upper ? sums[i + width] : sums[i];
+                    sums[i] = keep + __shfl_xor(give, d, 64);
+                }
+            }
+            const float all = (sums[0] + __shfl_xor(sums[0], 1, 64)) * __builtin_fabsf(a.c_out);
+            if ((lane & 1) == 0) {
+                const int key = 16 * half + 8 * ((lane >> 4) & 1) + 4 * ((lane >> 3) & 1) + 2 * ((lane >> 2) & 1) + ((lane >> 1) & 1);
+                if (a.weight_partial != nullptr) {
+                    const int row_tile = tile * WR + wr;
+                    a.weight_partial[((static_cast<int64_t>(pair) * a.row_tiles * WR + row_tile) * a.max_blocks + blk) * kFp8Block + key] = all;
+                } else {
+                    if (lin >= 0) {
+                        unsafeAtomicAdd(c.weights + static_cast<int64_t>(lin) * kFp8Block + key, all);
+                    }
+                }
+            }
+        }
+    };
+    const auto scale_of = [&](float mine, int s) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), s & 63));
+    };
+
+    Stage st[2];
+    for (int base = 0; base < n_steps; base += 64) {
+        look_up(base);
+        const int stop = n_steps < base + 64 ? n_steps : base + 64;
+        request(st[0], base);
+        for (int s = base; s < stop; s += 2) {
+            if (s + 1 < stop) {
+                request(st[1], s + 1);
+            }
+            step(st[0], s, scale_of(my_ks, s), scale_of(my_vs, s));
+            if (s + 1 < stop) {
+                if (s + 2 < stop) {
+                    request(st[0], s + 2);
+                }
+                step(st[1], s + 1, scale_of(my_ks, s + 1), scale_of(my_vs, s + 1));
+            }
+        }
+    }
+
+    // ---- the sum over the wavefronts that shared the keys, and the store ----
+    const bool partial = a.parts > 1 && parts_used > 1;
+    float* const to_partial =
+        a.partial + (static_cast<int64_t>(pair * a.row_tiles + tile) * a.parts + part) * static_cast<int64_t>(TILE) * dim;
+    const auto row_at = [&](int m) {  // element index of a (row, head) pair in q and out
+        const int i = div_small(m, a.ratio);
+        return ((q0 + i) * a.n_heads_q + g * a.ratio + (m - i * a.ratio)) * static_cast<int64_t>(dim);
+    };
+    if constexpr (WK > 1) {
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            float* const s = s_sum[n & 1];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4_t x = {acc[nb][n][4 * i], acc[nb][n][4 * i + 1], acc[nb][n][4 * i + 2], acc[nb][n][4 * i + 3]};
+                    *reinterpret_cast<f32x4_t*>(s + wk * CHUNK_WORDS + (nb * 4 + i) * 256 + lane * 4) = x;
+                }
+            }
+            __syncthreads();
+            constexpr int T = 64 * WK;
+            static_assert(CHUNK_WORDS % (2 * T) == 0, "every lane has whole pairs to add");
+#pragma unroll
+            for (int r = 0; r < CHUNK_WORDS / (2 * T); ++r) {
+                const int word = 2 * (tid + r * T);
+                float x0 = 0.0f, x1 = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WK; ++w) {
+                    x0 += s[w * CHUNK_WORDS + word];
+                    x1 += s[w * CHUNK_WORDS + word + 1];
+                }
+                const int nb = word >> 10, i = ((word >> 8) & 3) * 4 + (word & 3), from = (word >> 2) & 63;
+                const int m = m0 + nb * 32 + (from & 31), d = 32 * n + 16 * (from >> 5) + i;
+                if (m < n_pairs_rows && d < dim) {
+                    if (partial) {
+                        float* const to = to_partial + static_cast<int64_t>(m - tile * TILE) * dim + d;
+                        to[0] = x0;
+                        to[1] = x1;
+                    } else {
+                        *reinterpret_cast<uint32_t*>(out + row_at(m) + d) = pack2<Tag>(x0 * a.c_out, x1 * a.c_out);
+                    }
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int m = m0 + nb * 32 + col;
+            if (m < n_pairs_rows) {
+                const int64_t at = row_at(m);
+#pragma unroll
+                for (int n = 0; n < NC; ++n) {
+                    const int d = 32 * n + 16 * half;
+                    if (d < dim) {
+                        if (partial) {
+                            f32x4_t* const to = reinterpret_cast<f32x4_t*>(to_partial + static_cast<int64_t>(m - tile * TILE) * dim + d);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                to[i] = f32x4_t{acc[nb][n][4 * i], acc[nb][n][4 * i + 1], acc[nb][n][4 * i + 2], acc[nb][n][4 * i + 3]};
+                            }
+                        } else {
+                            u32x4_t x[2];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                x[i >> 2][i & 3] = pack2<Tag>(acc[nb][n][2 * i] * a.c_out, acc[nb][n][2 * i + 1] * a.c_out);
+                            }
+                            *reinterpret_cast<u32x4_t*>(out + at + d) = x[0];
+                            *reinterpret_cast<u32x4_t*>(out + at + d + 8) = x[1];
+                        }
+                    }
+                }
+            }
+        }
+    }
+}
+
+}  // namespace hstu

@@ -1,0 +1,25 @@
+// The variants of the attention kernel over the 8-bit paged cache, by type of q (hstu_paged_fp8_kernels_*.hip).
+#pragma once
+#include "hstu_paged_fp8.h"
+
+namespace hstu {
+
+// how a workgroup's wavefronts are dealt: over the keys of one tile of rows, of one or two columns of 32, or over rows
+enum Fp8Shape { kFp8Keys = 0, kFp8KeysWide = 1, kFp8Rows = 2, kFp8Shapes = 3 };
+
+struct Fp8AttendVariant {
+    const char* name;
+    void (*kernel)(const Fp8AttendArgs);
+    int threads;
+    int wave_rows;  // (row, head) pairs of a wavefront
+    int tile_rows;  // and of a workgroup
+};
+
+// dims in groups of 32 that a variant is built for: the smallest of these that holds the head dim
+constexpr int kFp8Groups[] = {1, 2, 3, 4, 6, 8};
+constexpr int kFp8GroupCounts = 6;
+
+using Fp8AttendTable = Fp8AttendVariant[kFp8GroupCounts][kFp8Shapes][2];  // [2]: without and with weights
+extern const Fp8AttendTable kFp8AttendBf16, kFp8AttendF16;
+
+}  // namespace hstu

@@ -42,6 +42,9 @@ struct Fallbacks {
     PyObject* ln_mul = nullptr;           // _activation.ln_mul
     PyObject* in_linear_silu = nullptr;   // _activation.distance_in_linear_silu
     PyObject* in_linear_silu_backward = nullptr;
+    PyObject* paged_fp8 = nullptr;        // _paged_fp8.hstu_paged_fp8
+    PyObject* paged_fp8_append = nullptr;  // _paged_fp8.hstu_paged_fp8_append
+    PyObject* paged_fp8_evict = nullptr;   // _paged_fp8.hstu_paged_fp8_evict
 } fallbacks;
 
 template <typename R, typename... A>
@@ -374,6 +377,173 @@ Tensor paged(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& ca
                              deterministic);
 }
 
+// --------------------------------------------------------------------------------------------- 8-bit paged cache ----
+
+// The cache tensors and the index tensors as the library reads them; false when they are not in canonical form.
+bool describe_cache(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale, const Tensor* weights,
+                    const Tensor& cache_len, const Tensor& page_offsets, const Tensor& page_ids, hstu_paged_fp8_cache& c)
+{
+    if (!k_cache.defined() || !v_cache.defined() || !k_scale.defined() || !v_scale.defined() || !cache_len.defined() || !page_offsets.defined() ||
+        !page_ids.defined() || k_cache.dim() != 5 || v_cache.dim() != 5 || k_cache.numel() == 0) {
+        return false;
+    }
+    const at::Device device = k_cache.device();
+    const int64_t pages = k_cache.size(0), heads = k_cache.size(1), blocks = k_cache.size(2), dim = k_cache.size(4);
+    const at::ScalarType index = cache_len.scalar_type();
+    const auto scales = [&](const Tensor& t, int64_t last) {
+        return t.device() == device && t.scalar_type() == at::kFloat && t.dim() == 3 && t.size(0) == pages && t.size(1) == heads && t.size(2) == last &&
+               t.is_contiguous();
+    };
+    const auto codes = [&](const Tensor& t, int64_t rows, int64_t cols) {
+        return t.device() == device && t.scalar_type() == at::kFloat8_e4m3fn && t.size(0) == pages && t.size(1) == heads && t.size(2) == blocks &&
+               t.size(3) == rows && t.size(4) == cols && t.is_contiguous();
+    };
+    const auto vector = [&](const Tensor& t) { return t.dim() == 1 && t.scalar_type() == index && t.device() == device && t.is_contiguous(); };
+    if (!device.is_cuda() || (index != at::kInt && index != at::kLong) || !codes(k_cache, 32, dim) || !codes(v_cache, dim, 32) ||
+        !scales(k_scale, blocks) || !scales(v_scale, blocks) || (weights != nullptr && !scales(*weights, blocks * 32)) || !vector(cache_len) ||
+        !vector(page_offsets) || !vector(page_ids) || page_offsets.size(0) < 2 || cache_len.size(0) != page_offsets.size(0) - 1) {
+        return false;
+    }
+    std::memset(&c, 0, sizeof c);
+    c.k_cache = k_cache.data_ptr();
+    c.v_cache = v_cache.data_ptr();
+    c.k_scale = static_cast<float*>(k_scale.data_ptr());
+    c.v_scale = static_cast<float*>(v_scale.data_ptr());
+    c.weights = weights != nullptr ? static_cast<float*>(weights->data_ptr()) : nullptr;
+    c.cache_len = cache_len.data_ptr();
+    c.page_offsets = page_offsets.data_ptr();
+    c.page_ids = ptr(page_ids);
+    c.num_pages = pages;
+    c.page_size = blocks * 32;
+    c.n_page_ids = page_ids.numel();
+    c.num_heads_k = heads;
+    c.head_dim = dim;
+    c.n_offsets = page_offsets.size(0);
+    c.index_dtype = index == at::kLong ? HSTU_IDX_I64 : HSTU_IDX_I32;
+    return true;
+}
+
+bool is_index(const Tensor& t, const Tensor& like, int64_t n)
+{
+    return t.defined() && t.dim() == 1 && t.size(0) == n && t.scalar_type() == like.scalar_type() && t.device() == like.device() && t.is_contiguous();
+}
+
+bool is_half(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }
+
+const Tensor* given(const OptTensor& t) { return is_set(t) ? &*t : nullptr; }
+
+Tensor paged_fp8(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale, const Tensor& seq_offset,
+                 const Tensor& cache_len, const Tensor& page_offsets, const Tensor& page_ids, int64_t max_seq_len, int64_t max_seq_len_k,
+                 double silu_scale, const OptTensor& num_target, int64_t group, double alpha, int64_t window, int64_t sinks, const OptTensor& weights)
+{
+    hstu_paged_fp8_fwd_params p;
+    if (q.dim() == 3 && q.numel() != 0 && is_half(q) && q.is_contiguous() && q.device() == k_cache.device() &&
+        describe_cache(k_cache, v_cache, k_scale, v_scale, given(weights), cache_len, page_offsets, page_ids, p.cache) &&
+        is_index(seq_offset, cache_len, p.cache.n_offsets) && (!is_set(num_target) || is_index(*num_target, cache_len, p.cache.n_offsets - 1)) &&
+        q.size(2) == p.cache.head_dim) {
+        const c10::DeviceGuard guard(q.device());
+        p.struct_size = sizeof p;
+        p.dtype = dtype_code(q.scalar_type());
+        p.q = q.data_ptr();
+        p.seq_offset = seq_offset.data_ptr();
+        p.num_target = ptr(num_target);
+        p.total_q = q.size(0);
+        p.num_heads_q = q.size(1);
+        p.max_seq_len_q = max_seq_len;
+        p.max_seq_len_k = max_seq_len_k;
+        p.target_group_size = group;
+        p.window = window;
+        p.sinks = sinks;
+        p.silu_scale = silu_scale == 0.0 ? 1.0 / static_cast<double>(max_seq_len) : silu_scale;
+        p.alpha = alpha;
+        Tensor out = empty(q.sizes(), q.scalar_type(), q.device());
+        p.out = out.data_ptr();
+        uint64_t ws_bytes = 0;
+        if (hstu_paged_fp8_fwd_workspace_size(&p, &ws_bytes) == HSTU_OK) {  // (refused: the Python implementation says so in its words)
+            Tensor ws;
+            if (ws_bytes != 0) {
+                ws = empty({static_cast<int64_t>(ws_bytes)}, at::kByte, q.device());
+            }
+            const int rc = hstu_paged_fp8_fwd(&p, ptr(ws), ws_bytes, stream_of(q));
+            TORCH_CHECK(rc == HSTU_OK, "hstu_paged_fp8_fwd failed (", rc, "): ", hstu_last_error());
+            return out;
+        }
+    }
+    return in_python<Tensor>(fallbacks.paged_fp8, q, k_cache, v_cache, k_scale, v_scale, seq_offset, cache_len, page_offsets, page_ids, max_seq_len,
+                             max_seq_len_k, silu_scale, num_target, group, alpha, window, sinks, weights);
+}
+
+void paged_fp8_append(const Tensor& k, const Tensor& v, const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale,
+                      const Tensor& seq_offset, const Tensor& cache_len, const Tensor& page_offsets, const Tensor& page_ids, int64_t max_seq_len,
+                      const OptTensor& weights)
+{
+    hstu_paged_fp8_append_params p;
+    if (k.dim() == 3 && v.dim() == 3 && k.numel() != 0 && is_half(k) && v.scalar_type() == k.scalar_type() && k.device() == k_cache.device() &&
+        v.device() == k.device() && describe_cache(k_cache, v_cache, k_scale, v_scale, given(weights), cache_len, page_offsets, page_ids, p.cache) &&
+        is_index(seq_offset, cache_len, p.cache.n_offsets) && k.sizes() == v.sizes() && k.size(1) == p.cache.num_heads_k &&
+        k.size(2) == p.cache.head_dim && k.stride(2) == 1 && v.stride(2) == 1 && max_seq_len >= 1 && max_seq_len <= HSTU_PAGED_FP8_MAX_SEQ_LEN_K) {
+        const auto readable = [](const Tensor& t) {
+            return t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+        };
+        if (readable(k) && readable(v)) {
+            const c10::DeviceGuard guard(k.device());
+            p.struct_size = sizeof p;
+            p.dtype = dtype_code(k.scalar_type());
+            p.k = k.data_ptr();
+            p.v = v.data_ptr();
+            p.seq_offset = seq_offset.data_ptr();
+            p.total = k.size(0);
+            p.k_stride_row = k.stride(0);
+            p.k_stride_head = k.stride(1);
+            p.v_stride_row = v.stride(0);
+            p.v_stride_head = v.stride(1);
+            p.max_seq_len = max_seq_len;
+            if (hstu_paged_fp8_append(&p, stream_of(k)) == HSTU_OK) {
+                return;
+            }
+        }
+    }
+    py::gil_scoped_acquire gil;  // (held until the returned None is let go)
+    in_python<py::object>(fallbacks.paged_fp8_append, k, v, k_cache, v_cache, k_scale, v_scale, seq_offset, cache_len, page_offsets, page_ids,
+                          max_seq_len, weights);
+}
+
+std::tuple<Tensor, Tensor> paged_fp8_evict(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale,
+                                           const Tensor& weights, const Tensor& cache_len, const Tensor& page_offsets, const Tensor& page_ids,
+                                           const Tensor& new_page_offsets, const Tensor& new_page_ids, int64_t max_seq_len_k, int64_t keep,
+                                           int64_t sinks, int64_t recent)
+{
+    hstu_paged_fp8_evict_params p;
+    if (weights.defined() && keep >= 1 && keep <= HSTU_PAGED_FP8_MAX_SEQ_LEN_K && new_page_ids.defined() &&
+        describe_cache(k_cache, v_cache, k_scale, v_scale, &weights, cache_len, page_offsets, page_ids, p.cache) &&
+        is_index(new_page_offsets, cache_len, p.cache.n_offsets) && new_page_ids.dim() == 1 && is_index(new_page_ids, cache_len, new_page_ids.size(0))) {
+        const c10::DeviceGuard guard(k_cache.device());
+        Tensor new_len = empty({cache_len.size(0)}, cache_len.scalar_type(), cache_len.device());
+        Tensor kept = empty({cache_len.size(0), keep}, cache_len.scalar_type(), cache_len.device());
+        p.struct_size = sizeof p;
+        p.reserved0 = 0;
+        p.new_page_offsets = new_page_offsets.data_ptr();
+        p.new_page_ids = ptr(new_page_ids);
+        p.new_cache_len = new_len.data_ptr();
+        p.kept = kept.data_ptr();
+        p.n_new_page_ids = new_page_ids.size(0);
+        p.max_seq_len_k = max_seq_len_k;
+        p.keep = keep;
+        p.sinks = sinks;
+        p.recent = recent;
+        uint64_t ws_bytes = 0;
+        if (hstu_paged_fp8_evict_workspace_size(&p, &ws_bytes) == HSTU_OK) {
+            const Tensor ws = empty({static_cast<int64_t>(ws_bytes)}, at::kByte, k_cache.device());
+            const int rc = hstu_paged_fp8_evict(&p, ptr(ws), ws_bytes, stream_of(k_cache));
+            TORCH_CHECK(rc == HSTU_OK, "hstu_paged_fp8_evict failed (", rc, "): ", hstu_last_error());
+            return {new_len, kept};
+        }
+    }
+    py::gil_scoped_acquire gil;
+    return in_python<std::tuple<Tensor, Tensor>>(fallbacks.paged_fp8_evict, k_cache, v_cache, k_scale, v_scale, weights, cache_len, page_offsets,
+                                                 page_ids, new_page_offsets, new_page_ids, max_seq_len_k, keep, sinks, recent);
+}
+
 // ------------------------------------------------------------------------------------------------ layer operators ----
 
 Tensor ln_mul(const Tensor& x, const Tensor& u, const Tensor& gamma, const Tensor& beta)
@@ -683,6 +853,9 @@ TORCH_LIBRARY_IMPL(ops_rec, CUDA, m)
     m.impl("hstu_jagged_backward.equal", jagged_backward_equal);
     m.impl("hstu_jagged_backward.delta", jagged_backward_delta);
     m.impl("hstu_paged", paged);
+    m.impl("hstu_paged_fp8", paged_fp8);
+    m.impl("hstu_paged_fp8_append", paged_fp8_append);
+    m.impl("hstu_paged_fp8_evict", paged_fp8_evict);
     m.impl("ln_mul", ln_mul);
     m.impl("distance_in_linear_silu", in_linear_silu);
     m.impl("in_linear_silu_backward", in_linear_silu_backward);
@@ -698,13 +871,16 @@ TORCH_LIBRARY_IMPL(ops_rec, AutogradCUDA, m)
 PYBIND11_MODULE(_torch_binding, m)
 {
     m.def("set_fallbacks", [](py::object forward, py::object backward, py::object paged_fn, py::object ln_mul_fn, py::object projection,
-                              py::object projection_backward) {
+                              py::object projection_backward, py::object fp8, py::object fp8_append, py::object fp8_evict) {
         fallbacks.forward = forward.release().ptr();
         fallbacks.backward = backward.release().ptr();
         fallbacks.paged = paged_fn.release().ptr();
         fallbacks.ln_mul = ln_mul_fn.release().ptr();
         fallbacks.in_linear_silu = projection.release().ptr();
         fallbacks.in_linear_silu_backward = projection_backward.release().ptr();
+        fallbacks.paged_fp8 = fp8.release().ptr();
+        fallbacks.paged_fp8_append = fp8_append.release().ptr();
+        fallbacks.paged_fp8_evict = fp8_evict.release().ptr();
     });
     m.def("fp8_forward", &fp8_forward, py::call_guard<py::gil_scoped_release>());
 }

@@ -14,6 +14,7 @@ from __future__ import annotations
 import logging
 
 from . import _ops  # noqa: F401  (defines the attention operators)
+from . import _paged_fp8  # noqa: F401  (defines the operators of the 8-bit paged cache)
 from . import _activation  # noqa: F401  (defines ln_mul)
 from . import _dispatch  # noqa: F401  (the native kernels of both, where they are built)
 from . import ascendc  # noqa: F401

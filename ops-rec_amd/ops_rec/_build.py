@@ -30,6 +30,9 @@ SOURCES = [
     "hstu_kernels_bwd_f16.hip",
     "hstu_kernels_bwd_fused.hip",
     "hstu_kernels_fwd_pinned.hip",
+    "hstu_paged_fp8_mi355.hip",
+    "hstu_paged_fp8_kernels_bf16.hip",
+    "hstu_paged_fp8_kernels_f16.hip",
 ]
 # These kernels name the accumulator registers they keep their sums in (hstu_pinned_acc.hip.h); every other matrix result belongs in
 # vector registers, where the compiler would otherwise keep it in accumulators as well and copy each element out.
@@ -37,6 +40,9 @@ _VGPR_FORM = ("-mllvm", "-amdgpu-mfma-vgpr-form=1")
 SOURCE_FLAGS = {"hstu_kernels_bwd_fused.hip": _VGPR_FORM, "hstu_kernels_fwd_pinned.hip": _VGPR_FORM}
 # The same where it is operands that stay in accumulators (the compiler knows of those: none is named).
 OPERAND_SOURCE_FLAGS = {"in_linear_silu_kernels_rows.hip": _VGPR_FORM}
+# And where nothing is pinned, but two columns of scores and outputs of up to 128 dims leave no register over for a score's way out
+# of an accumulator: without the form these kernels keep up to 220 bytes a lane in scratch memory, with it none.
+SCORE_SOURCE_FLAGS = {"hstu_paged_fp8_kernels_bf16.hip": _VGPR_FORM, "hstu_paged_fp8_kernels_f16.hip": _VGPR_FORM}
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
     "-O3",
@@ -45,6 +51,12 @@ HIPCC_FLAGS = [
     "-fvisibility=hidden",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]  # fmt: skip
+
+
+def flags_of(source: str) -> list[str]:
+    """What a source is compiled with."""
+    tables = (SOURCE_FLAGS, OPERAND_SOURCE_FLAGS, SCORE_SOURCE_FLAGS)
+    return [*HIPCC_FLAGS, *(flag for table in tables for flag in table.get(source, ()))]
 
 
 def hipcc_path() -> str:
@@ -90,8 +102,7 @@ def build(verbose: bool = False, jobs: int | None = None, extra_flags: tuple = (
         objects = [os.path.join(obj_dir, os.path.splitext(s)[0] + ".o") for s in SOURCES]
         with ThreadPoolExecutor(max_workers=jobs) as pool:
             jobs_done = [
-                pool.submit(_run, [hipcc, *HIPCC_FLAGS, *SOURCE_FLAGS.get(s, OPERAND_SOURCE_FLAGS.get(s, ())), *extra_flags, "-c",
-                                   os.path.join(CSRC, s), "-o", o], verbose)
+                pool.submit(_run, [hipcc, *flags_of(s), *extra_flags, "-c", os.path.join(CSRC, s), "-o", o], verbose)
                 for s, o in zip(SOURCES, objects)
             ]
             for j in jobs_done:

@@ -15,7 +15,7 @@ import os
 
 import torch
 
-from . import _activation, _build, _ops
+from . import _activation, _build, _ops, _paged_fp8
 
 logger = logging.getLogger(__name__)
 
@@ -29,7 +29,8 @@ def _load():
     module = importlib.util.module_from_spec(importlib.util.spec_from_file_location(name, _build.BINDING_PATH, loader=loader))
     loader.exec_module(module)  # (its static registrations put the native kernels into the dispatcher)
     module.set_fallbacks(_ops._forward_impl, _ops._backward_impl, _ops.hstu_paged, _activation.ln_mul,
-                         _activation.distance_in_linear_silu, _activation.in_linear_silu_backward)  # fmt: skip
+                         _activation.distance_in_linear_silu, _activation.in_linear_silu_backward, _paged_fp8.hstu_paged_fp8,
+                         _paged_fp8.hstu_paged_fp8_append, _paged_fp8.hstu_paged_fp8_evict)  # fmt: skip
     return module
 
 

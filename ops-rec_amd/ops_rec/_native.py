@@ -31,6 +31,12 @@ EXPORTED_SYMBOLS = (
     "hstu_paged_fwd_workspace_size",
     "hstu_paged_fwd",
     "hstu_paged_fwd_kernel_name",
+    "hstu_paged_fp8_fwd_workspace_size",
+    "hstu_paged_fp8_fwd",
+    "hstu_paged_fp8_fwd_kernel_name",
+    "hstu_paged_fp8_append",
+    "hstu_paged_fp8_evict_workspace_size",
+    "hstu_paged_fp8_evict",
     "ln_mul_fwd",
     "ln_mul_fwd_kernel_name",
     "in_linear_silu_fwd",
@@ -112,6 +118,55 @@ class PagedParams(ctypes.Structure):
         ("num_pages", ctypes.c_int64),
         ("page_size", ctypes.c_int64),
         ("n_page_ids", ctypes.c_int64),
+    ]
+
+
+class PagedFp8Cache(ctypes.Structure):
+    """Mirror of ``hstu_paged_fp8_cache``."""
+
+    _fields_ = [
+        *((name, ctypes.c_void_p) for name in ("k_cache", "v_cache", "k_scale", "v_scale", "weights", "cache_len", "page_offsets", "page_ids")),
+        *((name, ctypes.c_int64) for name in ("num_pages", "page_size", "n_page_ids", "num_heads_k", "head_dim", "n_offsets")),
+        ("index_dtype", ctypes.c_int32),
+        ("reserved0", ctypes.c_int32),
+    ]
+
+
+class PagedFp8FwdParams(ctypes.Structure):
+    """Mirror of ``hstu_paged_fp8_fwd_params``."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32),
+        ("cache", PagedFp8Cache),
+        *((name, ctypes.c_void_p) for name in ("q", "out", "seq_offset", "num_target")),
+        *((name, ctypes.c_int64) for name in ("total_q", "num_heads_q", "max_seq_len_q", "max_seq_len_k", "target_group_size", "window", "sinks")),
+        ("silu_scale", ctypes.c_double),
+        ("alpha", ctypes.c_double),
+    ]
+
+
+class PagedFp8AppendParams(ctypes.Structure):
+    """Mirror of ``hstu_paged_fp8_append_params``."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32),
+        ("cache", PagedFp8Cache),
+        *((name, ctypes.c_void_p) for name in ("k", "v", "seq_offset")),
+        *((name, ctypes.c_int64) for name in ("total", "k_stride_row", "k_stride_head", "v_stride_row", "v_stride_head", "max_seq_len")),
+    ]
+
+
+class PagedFp8EvictParams(ctypes.Structure):
+    """Mirror of ``hstu_paged_fp8_evict_params``."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("reserved0", ctypes.c_uint32),
+        ("cache", PagedFp8Cache),
+        *((name, ctypes.c_void_p) for name in ("new_page_offsets", "new_page_ids", "new_cache_len", "kept")),
+        *((name, ctypes.c_int64) for name in ("n_new_page_ids", "max_seq_len_k", "keep", "sinks", "recent")),
     ]
 
 
@@ -247,6 +302,17 @@ def load() -> ctypes.CDLL:
     lib.hstu_paged_fwd.argtypes = [ctypes.POINTER(PagedParams), ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p]
     lib.hstu_paged_fwd_kernel_name.restype = ctypes.c_char_p
     lib.hstu_paged_fwd_kernel_name.argtypes = [ctypes.POINTER(PagedParams)]
+    for name, params, workspace in (("hstu_paged_fp8_fwd", PagedFp8FwdParams, True), ("hstu_paged_fp8_append", PagedFp8AppendParams, False),
+                                    ("hstu_paged_fp8_evict", PagedFp8EvictParams, True)):  # fmt: skip
+        call = getattr(lib, name)
+        call.restype = ctypes.c_int
+        call.argtypes = [ctypes.POINTER(params), *((ctypes.c_void_p, ctypes.c_uint64) if workspace else ()), ctypes.c_void_p]
+        if workspace:
+            size = getattr(lib, name + "_workspace_size")
+            size.restype = ctypes.c_int
+            size.argtypes = [ctypes.POINTER(params), ctypes.POINTER(ctypes.c_uint64)]
+    lib.hstu_paged_fp8_fwd_kernel_name.restype = ctypes.c_char_p
+    lib.hstu_paged_fp8_fwd_kernel_name.argtypes = [ctypes.POINTER(PagedFp8FwdParams)]
     lib.ln_mul_fwd.restype = ctypes.c_int
     lib.ln_mul_fwd.argtypes = [ctypes.POINTER(LnMulParams), ctypes.c_void_p]
     lib.ln_mul_fwd_kernel_name.restype = ctypes.c_char_p

@@ -2,13 +2,15 @@
 
 Same surface as the reference module (ops_rec/ascendc/attention/__init__.py:31-55): both
 ``ops_rec.ascendc.attention.hstu_jagged(...)`` and ``from ops_rec.ascendc.attention import
-hstu_jagged`` work, and an unknown name raises ``AttributeError`` listing what exists.
+hstu_jagged`` work, and an unknown name raises ``AttributeError`` listing what exists.  The ``hstu_paged_fp8*`` operators (an 8-bit paged cache)
+are an extension: the reference has none of the kind.
 """
 
 import torch
 
 _NS = torch.ops.ops_rec
-_OPS = ("hstu_jagged", "hstu_jagged_backward", "hstu_dense", "hstu_dense_backward", "hstu_paged")
+_OPS = ("hstu_jagged", "hstu_jagged_backward", "hstu_dense", "hstu_dense_backward", "hstu_paged",
+        "hstu_paged_fp8", "hstu_paged_fp8_append", "hstu_paged_fp8_evict")  # fmt: skip
 
 __all__ = [name for name in _OPS if hasattr(_NS, name)]
 for _name in __all__:
