@@ -121,6 +121,24 @@ __device__ __forceinline__ Fp8Runs fp8_runs(const Fp8Mask& m, int i0, int i1)  /
     return r;
 }
 
+// The blocks that every row of [i0, i1] sees whole: an interval, and the first few of the sinks.
+struct Fp8Whole {
+    int lo, hi, sinks;
+    __device__ __forceinline__ bool has(int blk) const { return static_cast<uint32_t>(blk - lo) < static_cast<uint32_t>(hi - lo) || blk < sinks; }
+};
+__device__ __forceinline__ Fp8Whole fp8_whole(const Fp8Mask& m, int i0, int i1)
+{
+    Fp8Whole w;
+    const int lim = m.lim(i0), low = m.low(i1);
+    const int end = m.hole(i1) > m.first_key ? (lim < m.first_key ? lim : m.first_key) : lim;  // (up to the targets where some are not seen)
+    w.lo = uniform(low > 0 ? (low + kFp8Block - 1) / kFp8Block : 0);
+    w.hi = uniform(end > 0 ? end / kFp8Block : 0);
+    w.hi = w.hi < w.lo ? w.lo : w.hi;
+    const int sinks = m.window > 0 ? (m.sinks < end ? m.sinks : end) : 0;
+    w.sinks = uniform(sinks > 0 ? sinks / kFp8Block : 0);
+    return w;
+}
+
 // One sequence of a call: its rows of q, its pages and live keys, and what its rows see.
 struct Fp8Item {
     Fp8Sequence seq;
@@ -157,6 +175,120 @@ __device__ __forceinline__ Fp8Item fp8_item(const Fp8AttendArgs& a, int b)
     return it;
 }
 
+// What a workgroup does: slots are (pair of sequence and key head) x row tile x part, the tiles of a pair, which read the same keys,
+// on one XCD (workgroup w runs on XCD w mod 8); parts of one tile have no keys in common and go to all of them.
+__device__ __forceinline__ void fp8_slot(const Fp8AttendArgs& a, int& pair, int& part, int& tile)
+{
+    const int slot = static_cast<int>(blockIdx.x), n_pairs = a.c.n_batch * a.c.n_heads;
+    if (a.row_tiles == 1) {
+        part = uniform(slot / n_pairs);
+        pair = slot - part * n_pairs;
+        tile = 0;
+    } else {
+        const int per_pair = a.row_tiles * a.parts, oct = uniform(slot / (8 * per_pair)), rest = slot - oct * 8 * per_pair, in_pair = rest >> 3;
+        pair = oct * 8 + (rest & 7);
+        part = uniform(in_pair / a.row_tiles);
+        tile = a.row_tiles - 1 - (in_pair - part * a.row_tiles);  // (later rows see more keys: first)
+    }
+}
+
+// Rows of no sequence, and rows past the longest sequence allowed: zeros.  For the workgroup of a pair's first tile and part.
+template <int THREADS>
+__device__ __forceinline__ void fp8_clear_rows(const Fp8AttendArgs& a, const Fp8Item& item, int b, int g, uint16_t* out)
+{
+    const int64_t pitch = static_cast<int64_t>(a.n_heads_q) * a.c.dim, mine = static_cast<int64_t>(a.ratio) * a.c.dim;
+    const auto clear = [&](int64_t from, int64_t to) {
+        for (int64_t r = from; r < to; ++r) {
+            for (int64_t x = threadIdx.x; x < mine; x += THREADS) {
+                out[r * pitch + g * mine + x] = 0;
+            }
+        }
+    };
+    clear(item.q0 + item.n_rows, item.q1);
+    if (b == 0) {
+        clear(0, item.q0);
+    }
+    if (b == a.c.n_batch - 1) {
+        clear(item.q1, a.total_q);
+    }
+}
+
+// x of another lane of its row of 16, as a DPP control says
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x)
+{
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+// halves the N values a lane carries: a lane with `upper` keeps the second half, and every lane adds what its partner gives away
+template <int CTRL, int N>
+__device__ __forceinline__ void halve(float (&v)[16], bool upper)
+{
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        const float give = upper ? v[i] : v[i + N / 2], keep = upper ? v[i + N / 2] : v[i];
+        v[i] = keep + dpp<CTRL>(give);
+    }
+}
+// The sums of 16 values over the 32 lanes of each half, in the vector unit alone (through LDS the exchanges took longer than the block's
+// products).  Returned to lanes 2 x and 2 x + 1 is that of the key whose bits are those of x, highest first.
+__device__ __forceinline__ float fp8_key_sum(float (&v)[16], int lane)
+{
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {  // rows of 16 lanes, in pairs: the odd row of one against the even row of the other
+        const u32x2_t r =
+            __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v[i]), __builtin_bit_cast(uint32_t, v[i + 8]), false, false);
+        const uint32_t one = r[0], other = r[1];  // (values: a bit cast of an element of a vector takes its first)
+        v[i] = __builtin_bit_cast(float, one) + __builtin_bit_cast(float, other);
+    }
+    halve<0x128, 8>(v, (lane & 8) != 0);  // row_ror:8
+    halve<0x141, 4>(v, (lane & 4) != 0);  // row_half_mirror: 7 - l of each eight
+    halve<0x4e, 2>(v, (lane & 2) != 0);   // quad_perm 2 3 0 1
+    return v[0] + dpp<0xb1>(v[0]);        // quad_perm 1 0 3 2
+}
+__device__ __forceinline__ void fp8_store_key_sum(const Fp8AttendArgs& a, float sum, int lane, int pair, int row_tile, int row_tiles, int blk, int lin)
+{
+    if ((lane & 1) == 0) {
+        const int key = 16 * (lane >> 5) + 8 * ((lane >> 4) & 1) + 4 * ((lane >> 3) & 1) + 2 * ((lane >> 2) & 1) + ((lane >> 1) & 1);
+        if (a.weight_partial != nullptr) {
+            a.weight_partial[((static_cast<int64_t>(pair) * row_tiles + row_tile) * a.max_blocks + blk) * kFp8Block + key] = sum;
+        } else if (lin >= 0) {  // (a page may be in two sequences)
+            unsafeAtomicAdd(a.c.weights + static_cast<int64_t>(lin) * kFp8Block + key, sum);
+        }
+    }
+}
+
+// Outputs that a value which is NaN reaches, of one block: a product of ones at the codes for NaN with the 0 / 1 mask counts, for every
+// (dim, row), the NaN that the row sees.  j0: the first key of this lane's half; v_at: where its codes are.  (The products proper
+// had zeros in the place of those codes.)
+template <typename Tag, int NC, typename Sees>
+__device__ __forceinline__ void fp8_poison(f32x16_t (&acc)[NC], const Fp8Cache& c, int lin, const uint32_t (&v_at)[NC], int j0, int len, Sees sees)
+{
+    const uint32_t bytes = static_cast<uint32_t>(kFp8Block) * c.dim;
+    const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(c.v + static_cast<int64_t>(lin < 0 ? 0 : lin) * bytes, lin < 0 ? 0u : bytes);
+    u32x4_t seen[2];
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+        const int j = j0 + i;
+        seen[i >> 3][(i >> 1) & 3] = pack2<Tag>(((j < len) & sees(j)) ? 1.0f : 0.0f, ((j + 1 < len) & sees(j + 1)) ? 1.0f : 0.0f);
+    }
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        u32x4_t ones = load_codes(rsrc, v_at[n]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            ones[i] = (nan_codes(ones[i]) >> 7) * 0x38u;  // the code of 1
+        }
+        const Fp8Pair oo = fp8_widen<Tag>(ones, 1.0f);
+        f32x16_t hits = mfma32<Tag>(oo.lo, seen[0], f32x16_t{0.0f});
+        hits = mfma32<Tag>(oo.hi, seen[1], hits);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            acc[n][i] = hits[i] > 0.0f ? __builtin_nanf("") : acc[n][i];
+        }
+        __builtin_amdgcn_sched_barrier(0);  // (a group of dims at a time: no registers are set aside for this)
+    }
+}
+
 // Tag     : type of q and out
 // NC      : groups of 32 dims (dim is at most 32 NC, a multiple of 16)
 // NB      : columns of 32 rows of a wavefront
@@ -176,24 +308,9 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
     const int wk = WR > 1 ? 0 : wave, wr = WR > 1 ? wave : 0;
     static_assert(WK == 1 || WR == 1, "keys or rows");
 
-    // slots: (pair of sequence and key head) x row tile x part; the tiles of a pair, which read the same keys, on one XCD
-    // (workgroup w runs on XCD w mod 8); parts of one tile have no keys in common and go to all of them
-    const int slot = static_cast<int>(blockIdx.x);
+    int pair, part, tile;
+    fp8_slot(a, pair, part, tile);
     const int n_pairs = c.n_batch * c.n_heads;
-    int pair, part = 0, tile = 0;
-    if (a.row_tiles == 1) {
-        part = slot / n_pairs;
-        pair = slot - part * n_pairs;
-    } else {
-        const int per_pair = a.row_tiles * a.parts;
-        const int oct = slot / (8 * per_pair), rest = slot - oct * 8 * per_pair, in_pair = rest >> 3;
-        pair = oct * 8 + (rest & 7);
-        part = in_pair / a.row_tiles;
-        tile = a.row_tiles - 1 - (in_pair - part * a.row_tiles);  // (later rows see more keys: first)
-    }
-    pair = uniform(pair);
-    part = uniform(part);
-    tile = uniform(tile);
     if (pair >= n_pairs) {
         return;
     }
@@ -207,25 +324,9 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
     const int dim = c.dim;
     uint16_t* const out = static_cast<uint16_t*>(a.out);
 
-    // rows of no sequence, and rows past the longest sequence allowed: zeros
     if (tile == 0 && part == 0) {
-        const int64_t row_words = static_cast<int64_t>(a.n_heads_q) * dim, mine = static_cast<int64_t>(a.ratio) * dim;
-        const auto clear = [&](int64_t from, int64_t to) {
-            for (int64_t r = from; r < to; ++r) {
-                for (int64_t x = tid; x < mine; x += 64 * WK * WR) {
-                    out[r * row_words + g * mine + x] = 0;
-                }
-            }
-        };
-        clear(q0 + n_rows, q1);
-        if (b == 0) {
-            clear(0, q0);
-        }
-        if (b == c.n_batch - 1) {
-            clear(q1, a.total_q);
-        }
+        fp8_clear_rows<64 * WK * WR>(a, item, b, g, out);
     }
-
     const int n_pairs_rows = n_rows * a.ratio;  // (row, head) pairs
     if (tile * TILE >= n_pairs_rows) {
         return;
@@ -295,8 +396,7 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
         }
     }
 
-    // bounds for the whole wavefront: a block inside them needs no mask
-    const int lim_min = mask.lim(i_first), low_max = mask.low(i_last), hole_max = uniform(mask.hole(i_last));
+    const Fp8Whole whole_blocks = fp8_whole(mask, i_first, i_last);  // these need no mask
 
     // Steps of this wavefront: blocks n_begin + wk, + WK, ...; the places and scales of 64 of them at a time, a step per lane.  They are
     // looked up, and handed out by readlane, with every lane active: a lane that is not has no value that another may count on (the
@@ -332,6 +432,7 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
     const auto sees_key = [&](int j, int nb) {  // whether this lane's row of column nb sees key j
         return static_cast<bool>((j < lim[nb]) & ((j < mask.first_key) | (j >= hole[nb])) & ((j >= low[nb]) | (j < mask.sinks)));
     };
+    bool poisoned = false;
     const auto step = [&](Stage& st, int s, float ks, float vs) {
         const int lin = place_of(s);
         const int blk = runs.block(n_begin + wk + s * WK), c0 = blk * kFp8Block;
@@ -350,7 +451,7 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
             }
         }
         const int end = c0 + kFp8Block;
-        const bool whole = end <= lim_min && (c0 >= low_max || end <= mask.sinks) && (end <= mask.first_key || c0 >= hole_max);
+        const bool whole = whole_blocks.has(blk);
         u32x4_t p[NB][2];
         float sums[16];
 #pragma unroll
@@ -394,9 +495,7 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
             }
         }
         // A key that some rows do not see must not reach them, and zero times NaN would.  The codes for NaN are found by their bits; where
-        // a block with a mask holds one, the products run on zeros in their place, and afterwards a product of ones there with the mask
-        // says which outputs are NaN.
-        bool poisoned = false;
+        // a block with a mask holds one, the products run on zeros in their place, and what they make NaN is seen to after the sweep.
         if (!whole) {
             uint32_t any = 0;
 #pragma unroll
@@ -408,7 +507,7 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
                     st.v[n][i] &= ~((bits >> 7) * 0xffu);
                 }
             }
-            poisoned = __any(any != 0);
+            poisoned = poisoned || __any(any != 0);
         }
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
@@ -419,58 +518,9 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
                 acc[nb][n] = mfma32<Tag>(vv.hi, p[nb][1], acc[nb][n]);
             }
         }
-        if (poisoned) {  // (the codes are read again: nothing is kept for this case)
-            const __amdgpu_buffer_rsrc_t vr = make_rsrc(c.v + static_cast<int64_t>(lin < 0 ? 0 : lin) * block_bytes, lin < 0 ? 0u : block_bytes);
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                u32x4_t sees[2];
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const int j = c0 + 16 * half + i;
-                    sees[i >> 3][(i >> 1) & 3] = pack2<Tag>(sees_key(j, nb) ? 1.0f : 0.0f, sees_key(j + 1, nb) ? 1.0f : 0.0f);
-                }
-#pragma unroll
-                for (int n = 0; n < NC; ++n) {
-                    u32x4_t ones = load_codes(vr, v_at[n]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        ones[i] = (nan_codes(ones[i]) >> 7) * 0x38u;  // the code of 1
-                    }
-                    const Fp8Pair oo = fp8_widen<Tag>(ones, 1.0f);
-                    f32x16_t hits = mfma32<Tag>(oo.lo, sees[0], f32x16_t{0.0f});
-                    hits = mfma32<Tag>(oo.hi, sees[1], hits);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        acc[nb][n][i] = hits[i] > 0.0f ? __builtin_nanf("") : acc[nb][n][i];
-                    }
-                }
-            }
-        }
         if constexpr (WEIGHTS) {
-            // the sum over the 32 lanes of a half, halving the values a lane carries in each of four exchanges: lane x ends with the key
-            // whose bits are those of x, highest first
-#pragma unroll
-            for (int d = 16, width = 8; d >= 2; d >>= 1, width >>= 1) {
-#pragma unroll
-                for (int i = 0; i < width; ++i) {
-                    const bool upper = (lane & d) != 0;
-                    const float give = upper ? sums[i] : sums[i + width];
-                    const float keep = upper ? sums[i + width] : sums[i];
-                    sums[i] = keep + __shfl_xor(give, d, 64);
-                }
-            }
-            const float all = (sums[0] + __shfl_xor(sums[0], 1, 64)) * __builtin_fabsf(a.c_out);
-            if ((lane & 1) == 0) {
-                const int key = 16 * half + 8 * ((lane >> 4) & 1) + 4 * ((lane >> 3) & 1) + 2 * ((lane >> 2) & 1) + ((lane >> 1) & 1);
-                if (a.weight_partial != nullptr) {
-                    const int row_tile = tile * WR + wr;
-                    a.weight_partial[((static_cast<int64_t>(pair) * a.row_tiles * WR + row_tile) * a.max_blocks + blk) * kFp8Block + key] = all;
-                } else {
-                    if (lin >= 0) {
-                        unsafeAtomicAdd(c.weights + static_cast<int64_t>(lin) * kFp8Block + key, all);
-                    }
-                }
-            }
+            const float all = fp8_key_sum(sums, lane) * __builtin_fabsf(a.c_out);
+            fp8_store_key_sum(a, all, lane, pair, tile * WR + wr, a.row_tiles * WR, blk, lin);
         }
     };
     const auto scale_of = [&](float mine, int s) {
@@ -492,6 +542,21 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
                     request(st[0], s + 2);
                 }
                 step(st[1], s + 1, scale_of(my_ks, s + 1), scale_of(my_vs, s + 1));
+            }
+        }
+    }
+
+    if (poisoned) {
+        for (int s = 0; s < n_steps; ++s) {
+            const int blk = runs.block(n_begin + wk + s * WK);
+            if (whole_blocks.has(blk)) {
+                continue;
+            }
+            const int lin = uniform(fp8_block(c, c.page_ids, seq.first, g, blk));
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                const auto sees = [&](int j) { return sees_key(j, nb); };
+                fp8_poison<Tag, NC>(acc[nb], c, lin, v_at, blk * kFp8Block + 16 * half, seq.len, sees);
             }
         }
     }

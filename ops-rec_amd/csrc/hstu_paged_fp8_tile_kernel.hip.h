@@ -1,0 +1,362 @@
+// HSTU attention over the 8-bit paged cache for tiles of many rows (gfx950): the arithmetic of hstu_paged_fp8_attend_kernel.hip.h with the
+// codes converted once per workgroup.
+//
+// A 32 x 32 block of scores costs 16 matrix instructions (248 ns on a SIMD alone) and, in the vector unit, 32 transcendental
+// instructions and some 60 others (230 ns; both together, from two wavefronts, 300 ns), and 64 conversions of codes (150 ns) in a
+// kernel whose wavefronts work alone.  Here the RG wavefronts of a share of the keys, 32 rows each, bring its blocks in together, each
+// a part of the chunks: codes two steps ahead in registers, converted (v_cvt_scalef32_pk) and left in LDS in the order of the
+// matrix operands, 16 bytes per lane, so that reads have no bank conflicts; two buffers for K and three for V, one barrier a step.  The
+// products of K(t) and of V(t - 1) go together, a chain of eight that wait for each other between four pairs that do not.  Four
+// wavefronts per workgroup and two workgroups per CU: what one leaves of a SIMD's units the other, which is nowhere in step with it, takes.
+// (Eight wavefronts half a step apart, one half multiplying while the other weighs, changing places at every barrier, took 10 %
+// longer: 288 against 266 us with wavefronts alone, on 16 x 4 key heads of 1024 rows and 2048 .. 8192 keys.)
+//   step t : S = K(t) Q and O += V(t - 1) P; convert K, V (t + 1) to LDS, request those of t + 3; P = silu(S) masked
+// The outputs of KG shares of the keys (every KG-th block) are added through LDS at the end, in a fixed order.
+#pragma once
+#include "hstu_paged_fp8_attend_kernel.hip.h"
+
+namespace hstu {
+
+template <typename Tag, int NC, int RG, int KG, bool WEIGHTS>
+__global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(NC <= 2 ? 4 : 2, NC <= 2 ? 4 : 2))) void hstu_paged_fp8_tile_kernel(const Fp8AttendArgs a)
+{
+    constexpr int WAVES = RG * KG, T = 64 * WAVES;
+    constexpr int TILE = 32 * RG;
+    constexpr int CHUNKS = (2 * NC + RG - 1) / RG;  // chunks of 1 KiB of codes that a wavefront brings in per block
+    constexpr int FRAG = 64 * 16;                   // bytes of an operand: 16 per lane
+    constexpr int BUFFER = 2 * NC * FRAG;           // K or V of a block, 16 bits a value
+    constexpr int SHARE = 5 * BUFFER;               // two of K, three of V
+    constexpr int SUMS = WAVES * 1024 * 4;          // a group of 32 dims of all wavefronts
+    constexpr int LDS = KG * SHARE > 2 * SUMS ? KG * SHARE : 2 * SUMS;
+    __shared__ __attribute__((aligned(16))) uint8_t s_mem[LDS];
+
+    const Fp8Cache& c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    const int rg = wave & (RG - 1), kg = wave / RG;
+
+    int pair, part, tile;
+    fp8_slot(a, pair, part, tile);
+    const int n_pairs = c.n_batch * c.n_heads;
+    if (pair >= n_pairs) {
+        return;
+    }
+    const int b = uniform(pair / c.n_heads), g = pair - b * c.n_heads;
+    const Fp8Item item = fp8_item(a, b);
+    const Fp8Sequence& seq = item.seq;
+    const Fp8Mask& mask = item.mask;
+    const int dim = c.dim;
+    uint16_t* const out = static_cast<uint16_t*>(a.out);
+    if (tile == 0 && part == 0) {
+        fp8_clear_rows<T>(a, item, b, g, out);
+    }
+    const int n_rows = item.n_rows * a.ratio;  // (row, head) pairs
+    const int t0 = tile * TILE, t1 = t0 + TILE < n_rows ? t0 + TILE : n_rows;
+    if (t0 >= t1) {
+        return;
+    }
+    // the tile's blocks, and the bounds inside which a block needs no mask for the tile, and for this wavefront's rows
+    const int ti0 = uniform(div_small(t0, a.ratio)), ti1 = uniform(div_small(t1 - 1, a.ratio));
+    Fp8Runs runs = fp8_runs(mask, ti0, ti1 + 1);
+    runs = {uniform(runs.n_a), uniform(runs.n_b), uniform(runs.n_c), uniform(runs.b0), uniform(runs.c0)};
+    const int n_blocks = runs.count();
+    const int parts_used = a.parts == 1 ? 1 : uniform((n_blocks + a.chunk - 1) / a.chunk);
+    if (part > 0 && part >= parts_used) {
+        return;
+    }
+    const int n_begin = a.parts == 1 ? 0 : part * a.chunk;
+    const int n_end = a.parts == 1 || part == a.parts - 1 ? n_blocks : (n_begin + a.chunk < n_blocks ? n_begin + a.chunk : n_blocks);
+    const int m0 = t0 + 32 * rg;
+    const bool rows_here = m0 < n_rows;
+    const int m1 = m0 + 32 < n_rows ? m0 + 32 : n_rows;
+    const int i_first = rows_here ? uniform(div_small(m0, a.ratio)) : ti0, i_last = rows_here ? uniform(div_small(m1 - 1, a.ratio)) : ti0;
+    const Fp8Whole whole = fp8_whole(mask, i_first, i_last), tile_whole = fp8_whole(mask, ti0, ti1);
+
+    // this lane's row of q
+    u32x4_t q[NC][2];
+    const int m = m0 + col, i_row = div_small(m < n_rows ? m : 0, a.ratio);
+    const int lim = m < n_rows ? mask.lim(i_row) : 0, hole = mask.hole(i_row), low = mask.low(i_row);
+    {
+        const uint32_t bytes = static_cast<uint32_t>(item.n_rows) * static_cast<uint32_t>(a.n_heads_q) * dim * 2u;
+        const __amdgpu_buffer_rsrc_t rsrc =
+            make_rsrc(static_cast<const uint16_t*>(a.q) + item.q0 * a.n_heads_q * static_cast<int64_t>(dim), bytes);
+        const uint32_t at = (static_cast<uint32_t>(i_row) * a.n_heads_q + g * a.ratio + (m - i_row * a.ratio)) * dim * 2u;
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int d = 32 * n + 16 * half + 8 * u;
+                q[n][u] = load_codes(rsrc, m < n_rows && d < dim ? at + d * 2u : kOutOfRange);
+            }
+        }
+    }
+    const auto sees_key = [&](int j) {
+        return static_cast<bool>((j < lim) & ((j < mask.first_key) | (j >= hole)) & ((j >= low) | (j < mask.sinks)));
+    };
+
+    // the chunks this wavefront brings in: number rg + RG i of the block's 2 NC, K first
+    const int pi = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);
+    const uint32_t block_bytes = static_cast<uint32_t>(kFp8Block) * dim;
+    uint32_t code_at[CHUNKS];
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+        const int n = rg + RG * i, d = 32 * n + 16 * half, dv = 32 * (n - NC) + pi;
+        const uint32_t k_at = d < dim ? static_cast<uint32_t>(pi) * dim + d : kOutOfRange;
+        const uint32_t v_at = dv < dim ? static_cast<uint32_t>(dv) * kFp8Block + 16 * half : kOutOfRange;
+        code_at[i] = n < NC ? k_at : (n < 2 * NC ? v_at : kOutOfRange);
+    }
+
+    // steps: blocks n_begin + kg, + KG, ...; the same number for every share, the last of some without a block, and an even one (requests
+    // then stand in one order at the loop's head, and a wait is for a block's own).  Places and scales of 64 steps, and of the 64
+    // behind them, a step per lane; looked up and handed out with every lane active.
+    const int n_steps = (n_end - n_begin + 2 * KG - 1) / (2 * KG) * 2;
+    const int mine = n_end - n_begin - kg > 0 ? (n_end - n_begin - kg + KG - 1) / KG : 0;
+    const auto block_of = [&](int s) { return runs.block(n_begin + kg + s * KG); };
+    int lin_a = -1, lin_b = -1;
+    float ks_a = 1.0f, ks_b = 1.0f, vs_a = 1.0f, vs_b = 1.0f;
+    int base = 0;
+    const auto look_up = [&](int first, int& lin, float& ks, float& vs) {
+        lin = -1;
+        if (first < mine) {
+            const int s = first + lane < mine ? first + lane : mine - 1;
+            const int at = fp8_block(c, c.page_ids, seq.first, g, block_of(s));
+            ks = c.k_scale[at >= 0 ? at : 0];
+            vs = c.v_scale[at >= 0 ? at : 0];
+            lin = first + lane < mine ? at : -1;
+        }
+    };
+    // lane s mod 64 of the first or the second of these: steps base .. base + 127
+    const auto pick = [&](int x_a, int x_b, int s) {
+        const int l_a = __builtin_amdgcn_readlane(x_a, s & 63), l_b = __builtin_amdgcn_readlane(x_b, s & 63);
+        return s < base + 64 ? l_a : l_b;
+    };
+    const auto lin_of = [&](int s) { return pick(lin_a, lin_b, s); };
+    const auto scale_of = [&](float x_a, float x_b, int s) {
+        return __builtin_bit_cast(float, pick(__builtin_bit_cast(int, x_a), __builtin_bit_cast(int, x_b), s));
+    };
+
+    u32x4_t raw[2][CHUNKS];
+    const auto request = [&](u32x4_t (&to)[CHUNKS], int t) {
+        const int lin = lin_of(t);
+        const int64_t at = static_cast<int64_t>(lin < 0 ? 0 : lin) * block_bytes;
+        const __amdgpu_buffer_rsrc_t kr = make_rsrc(c.k + at, lin < 0 ? 0u : block_bytes), vr = make_rsrc(c.v + at, lin < 0 ? 0u : block_bytes);
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) {
+            if (rg + RG * i < NC) {
+                to[i] = load_codes(kr, code_at[i]);
+            } else {
+                to[i] = load_codes(vr, code_at[i]);
+            }
+        }
+    };
+    bool poisoned = false;
+    const auto convert = [&](u32x4_t (&from)[CHUNKS], int t, uint8_t* to_k, uint8_t* to_v) {
+        const int blk = block_of(t);
+        const float ks = scale_of(ks_a, ks_b, t), vs = scale_of(vs_a, vs_b, t);
+        if (t < mine && !tile_whole.has(blk)) {
+            // codes behind the last row may be anything; NaN that some rows do not see: see the other kernel
+            const int left = seq.len - blk * kFp8Block - 16 * half;
+            uint32_t any = 0;
+#pragma unroll
+            for (int i = 0; i < CHUNKS; ++i) {
+                if (rg + RG * i >= NC) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int k = left - 4 * j;
+                        const uint32_t live = from[i][j] & (k >= 4 ? 0xffffffffu : (k <= 0 ? 0u : (1u << (8 * k)) - 1u));
+                        const uint32_t bits = nan_codes(live);
+                        any |= bits;
+                        from[i][j] = live & ~((bits >> 7) * 0xffu);
+                    }
+                }
+            }
+            poisoned = poisoned || __any(any != 0);
+        }
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) {
+            const int n = rg + RG * i;
+            if (n < 2 * NC) {
+                const Fp8Pair x = fp8_widen<Tag>(from[i], n < NC ? ks : vs);
+                uint8_t* const to = (n < NC ? to_k + 2 * n * FRAG : to_v + 2 * (n - NC) * FRAG) + lane * 16;
+                *reinterpret_cast<u32x4_t*>(to) = x.lo;
+                *reinterpret_cast<u32x4_t*>(to + FRAG) = x.hi;
+            }
+        }
+    };
+
+    f32x16_t acc[NC], sc;
+    u32x4_t p[2] = {u32x4_t{0u}, u32x4_t{0u}};
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        acc[n] = f32x16_t{0.0f};
+    }
+    const auto operand = [&](const uint8_t* from, int n) { return *reinterpret_cast<const u32x4_t*>(from + n * FRAG + lane * 16); };
+    // There is no branch around a product: ahead of the first step and behind the last they run on weights and values of zero.
+    const auto multiply = [&](const uint8_t* k, const uint8_t* v) {
+        sc = f32x16_t{0.0f};
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                sc = mfma32<Tag>(operand(k, 2 * n + u), q[n][u], sc);
+                acc[n] = mfma32<Tag>(operand(v, 2 * n + u), p[u], acc[n]);
+            }
+        }
+        // operands are read eight ahead of their products (left to itself the compiler reads each into the same registers and waits
+        // for it: 16 times the LDS's latency)
+        constexpr int N = 4 * NC, AHEAD = N < 8 ? N : 8;
+        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);  // LDS reads
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
+            if (i + AHEAD < N) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto weigh = [&](int t) {
+        const int blk = block_of(t), c0 = blk * kFp8Block;
+        float w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float x = sc[i];
+            w[i] = x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * a.c_exp));
+        }
+        if (t >= mine || !whole.has(blk)) {
+            const int end = t < mine ? lim : 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int j = c0 + 16 * half + i;
+                w[i] = ((j < end) & ((j < mask.first_key) | (j >= hole)) & ((j >= low) | (j < mask.sinks))) ? w[i] : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[u][i] = pack2<Tag>(w[8 * u + 2 * i], w[8 * u + 2 * i + 1]);
+            }
+        }
+        if constexpr (WEIGHTS) {
+            if (t < mine && rows_here) {
+                const int lin = lin_of(t);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    w[i] = __builtin_fabsf(w[i]);
+                }
+                const float all = fp8_key_sum(w, lane) * __builtin_fabsf(a.c_out);
+                fp8_store_key_sum(a, all, lane, pair, tile * RG + rg, a.row_tiles * RG, blk, lin);
+            }
+        }
+    };
+
+    uint8_t* const share = s_mem + kg * SHARE;
+    uint8_t *v_last = share + 4 * BUFFER, *v_now = share + 2 * BUFFER, *v_next = share + 3 * BUFFER;  // V of t - 1, t, t + 1
+    const auto step = [&](u32x4_t (&next)[CHUNKS], int t, int turn) {
+        multiply(share + turn * BUFFER, v_last);
+        convert(next, t + 1, share + (turn ^ 1) * BUFFER, v_next);
+        request(next, t + 3);
+        weigh(t);
+        __syncthreads();
+        uint8_t* const free = v_last;
+        v_last = v_now;
+        v_now = v_next;
+        v_next = free;
+    };
+    for (int x = rg; x < 2 * NC; x += RG) {
+        *reinterpret_cast<u32x4_t*>(v_last + x * FRAG + lane * 16) = u32x4_t{0u};
+    }
+    look_up(0, lin_a, ks_a, vs_a);
+    look_up(64, lin_b, ks_b, vs_b);
+    request(raw[0], 0);
+    request(raw[1], 1);
+    convert(raw[0], 0, share, v_now);
+    request(raw[0], 2);
+    __syncthreads();
+    for (int t = 0; t < n_steps; t += 2) {
+        if (t >= base + 64) {
+            base += 64;
+            lin_a = lin_b;
+            ks_a = ks_b;
+            vs_a = vs_b;
+            look_up(base + 64, lin_b, ks_b, vs_b);
+            // (waited for here, every 64 steps: where paths meet, the compiler would wait for these loads, and so for the codes asked
+            // for before them, in every step)
+            __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+        }
+        step(raw[1], t, 0);
+        step(raw[0], t + 1, 1);
+    }
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        acc[n] = mfma32<Tag>(operand(v_last, 2 * n), p[0], acc[n]);
+        acc[n] = mfma32<Tag>(operand(v_last, 2 * n + 1), p[1], acc[n]);
+    }
+    // (flags where K and V were: with room of their own two workgroups of four shares' worth of buffers do not fit a CU)
+    int* const s_poison = reinterpret_cast<int*>(s_mem);
+    __syncthreads();
+    if (tid < KG) {
+        s_poison[tid] = 0;
+    }
+    __syncthreads();
+    if (poisoned) {
+        s_poison[kg] = 1;
+    }
+    __syncthreads();
+    const bool any_poison = s_poison[kg] != 0;
+    __syncthreads();  // (the sums go there next)
+    if (any_poison) {
+        uint32_t v_at[NC];
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            v_at[n] = 32 * n + pi < dim ? static_cast<uint32_t>(32 * n + pi) * kFp8Block + 16 * half : kOutOfRange;
+        }
+        for (int s = 0; s < mine; ++s) {
+            const int blk = block_of(s);
+            if (!tile_whole.has(blk)) {
+                fp8_poison<Tag, NC>(acc, c, uniform(fp8_block(c, c.page_ids, seq.first, g, blk)), v_at, blk * kFp8Block + 16 * half, seq.len, sees_key);
+            }
+        }
+    }
+
+    // ---- the sum over the shares, and the store ----
+    const bool partial = a.parts > 1 && parts_used > 1;
+    float* const to_partial =
+        a.partial + (static_cast<int64_t>(pair * a.row_tiles + tile) * a.parts + part) * static_cast<int64_t>(TILE) * dim;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        float* const s = reinterpret_cast<float*>(s_mem) + (n & 1) * (SUMS / 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4_t x = {acc[n][4 * i], acc[n][4 * i + 1], acc[n][4 * i + 2], acc[n][4 * i + 3]};
+            *reinterpret_cast<f32x4_t*>(s + wave * 1024 + i * 256 + lane * 4) = x;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < RG * 512 / T; ++r) {  // (two values per thread and turn)
+            const int word = 2 * (tid + r * T);
+            float x0 = 0.0f, x1 = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KG; ++k) {
+                x0 += s[k * RG * 1024 + word];
+                x1 += s[k * RG * 1024 + word + 1];
+            }
+            const int i = ((word >> 8) & 3) * 4 + (word & 3), from = (word >> 2) & 63;
+            const int row = t0 + 32 * (word >> 10) + (from & 31), d = 32 * n + 16 * (from >> 5) + i;
+            if (row < n_rows && d < dim) {
+                if (partial) {
+                    float* const to = to_partial + static_cast<int64_t>(row - t0) * dim + d;
+                    to[0] = x0;
+                    to[1] = x1;
+                } else {
+                    const int ir = div_small(row, a.ratio);
+                    const int64_t at = ((item.q0 + ir) * a.n_heads_q + g * a.ratio + (row - ir * a.ratio)) * static_cast<int64_t>(dim) + d;
+                    *reinterpret_cast<uint32_t*>(out + at) = pack2<Tag>(x0 * a.c_out, x1 * a.c_out);
+                }
+            }
+        }
+    }
+}
+
+}  // namespace hstu
