@@ -33,7 +33,7 @@ struct Fp8AttendArgs {
     const void* offs_q;
     const void* num_target;  // or null
     void* out;
-    float* partial;         // [slots][parts][rows of a tile][dim], for launches of more than one part
+    float* partial;         // [total_parts * n_heads][row_tiles][rows of a tile][dim], where there are parts
     float* weight_partial;  // [n_batch * n_heads][row_tiles][max_blocks * 32], for weights over more than one row tile
     int64_t total_q;
     int n_heads_q;
@@ -43,9 +43,11 @@ struct Fp8AttendArgs {
     int group;
     int window;  // 0: none
     int sinks;
-    int row_tiles;   // of a (sequence, key head) pair, at most
-    int parts;       // a tile's keys are dealt to so many workgroups
-    int chunk;       // blocks of one part
+    int row_tiles;    // of a (sequence, key head) pair, at most
+    int total_parts;  // the keys of the sequences are dealt to so many parts in all; 0: a sequence is one part
+    int parts;        // of each sequence, where they are not dealt by length (more than 64 sequences)
+    int chunk;        // blocks of a part: at least (dealt by length), or exactly
+    int most_blocks;  // that a row tile sweeps, at most
     int max_blocks;  // pitch of weight_partial, in blocks
     float c_exp;     // -alpha * log2(e): silu(alpha s) = alpha * s / (1 + 2^(c_exp s))
     float c_out;     // alpha * silu_scale

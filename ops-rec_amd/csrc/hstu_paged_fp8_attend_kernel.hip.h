@@ -175,21 +175,82 @@ __device__ __forceinline__ Fp8Item fp8_item(const Fp8AttendArgs& a, int b)
     return it;
 }
 
-// What a workgroup does: slots are (pair of sequence and key head) x row tile x part, the tiles of a pair, which read the same keys,
-// on one XCD (workgroup w runs on XCD w mod 8); parts of one tile have no keys in common and go to all of them.
-__device__ __forceinline__ void fp8_slot(const Fp8AttendArgs& a, int& pair, int& part, int& tile)
+// Which share of a sequence's keys a workgroup takes.  Tiles whose keys take long are dealt to several workgroups, in parts of as
+// many blocks each, `chunk`, whatever the sequence: with up to 64 sequences, a lane of a wavefront for each, the lengths are
+// looked at, and the chunk is what makes total_parts of them all -- sum ceil(blocks / chunk) is at most sum blocks / chunk + the
+// number of sequences.  (Cut alike by the longest length allowed, parts of short sequences have nothing to do: 3 x 2 key heads
+// of 30011 .. 120011 keys, d 256, 70 us in such parts, 47 in these.)  First come the first parts of all sequences, the longest first,
+// then their second parts, and so on: what starts late is short.
+struct Fp8Deal {
+    int b;      // the sequence; -1: none
+    int part;   // of its
+    int parts;
+    int chunk;
+    int slot;   // number of the part among all
+};
+struct Fp8DealLanes {
+    int chunk, parts, rank;  // of the sequence of this lane: its parts (0: no sequence), and how many come before it
+    // number of the first of the p-th parts of all
+    __device__ __forceinline__ int count(int p) const { return static_cast<int>(__popcll(__ballot(parts > p))); }
+};
+__device__ __forceinline__ Fp8DealLanes fp8_deal_lanes(const Fp8AttendArgs& a)
 {
-    const int slot = static_cast<int>(blockIdx.x), n_pairs = a.c.n_batch * a.c.n_heads;
-    if (a.row_tiles == 1) {
-        part = uniform(slot / n_pairs);
-        pair = slot - part * n_pairs;
-        tile = 0;
-    } else {
-        const int per_pair = a.row_tiles * a.parts, oct = uniform(slot / (8 * per_pair)), rest = slot - oct * 8 * per_pair, in_pair = rest >> 3;
-        pair = oct * 8 + (rest & 7);
-        part = uniform(in_pair / a.row_tiles);
-        tile = a.row_tiles - 1 - (in_pair - part * a.row_tiles);  // (later rows see more keys: first)
+    const int lane = threadIdx.x & 63, n = a.c.n_batch;
+    const int64_t len = load_index(a.c.cache_len, lane < n ? lane : 0, a.c.idx64);
+    const int keys = static_cast<int>(len < 0 ? 0 : (len < a.max_k ? len : a.max_k));
+    const int all = (keys + kFp8Block - 1) / kFp8Block, blocks = lane < n ? (all < a.most_blocks ? all : a.most_blocks) : -1;
+    int sum = blocks > 0 ? blocks : 0;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        sum += __shfl_xor(sum, d, 64);
     }
+    Fp8DealLanes r;
+    const int even = uniform((sum + a.total_parts - n - 1) / (a.total_parts - n));
+    r.chunk = even > a.chunk ? even : a.chunk;
+    const int parts = div_small((blocks > 0 ? blocks : 0) + r.chunk - 1, r.chunk);
+    r.parts = lane < n ? (parts > 1 ? parts : 1) : 0;
+    r.rank = 0;
+    for (int l = 0; l < n; ++l) {
+        const int other = __builtin_amdgcn_readlane(blocks, l);
+        r.rank += (other > blocks) | ((other == blocks) & (l < lane)) ? 1 : 0;
+    }
+    return r;
+}
+__device__ __forceinline__ Fp8Deal fp8_deal(const Fp8AttendArgs& a, int n)  // the n-th part of all
+{
+    if (a.total_parts == 0) {
+        return {n < a.c.n_batch ? n : -1, 0, 1, 0x3fffffff, n};
+    }
+    if (a.c.n_batch > 64) {
+        const int b = uniform(n / a.parts);
+        return {b < a.c.n_batch ? b : -1, n - b * a.parts, a.parts, a.chunk, n};
+    }
+    const Fp8DealLanes l = fp8_deal_lanes(a);
+    int part = 0, rank = n, count = l.count(0);
+    while (rank >= count && count > 0) {
+        rank -= count;
+        count = l.count(++part);
+    }
+    const uint64_t mine = __ballot((l.rank == rank) & (l.parts > part));
+    const int b = mine != 0 ? __builtin_ctzll(mine) : -1;
+    return {b, part, mine != 0 ? __builtin_amdgcn_readlane(l.parts, b >= 0 ? b : 0) : 1, l.chunk, n};
+}
+
+// What a workgroup does: slots are (part, key head) x row tile, the tiles of a part and head, which read the same keys, on one XCD
+// (workgroup w runs on XCD w mod 8).
+__device__ __forceinline__ Fp8Deal fp8_slot(const Fp8AttendArgs& a, int& g, int& tile)
+{
+    const int slot = static_cast<int>(blockIdx.x);
+    int unit = slot;
+    tile = 0;
+    if (a.row_tiles > 1) {
+        const int oct = uniform(slot / (8 * a.row_tiles)), rest = slot - oct * 8 * a.row_tiles;
+        unit = oct * 8 + (rest & 7);
+        tile = a.row_tiles - 1 - (rest >> 3);  // (later rows see more keys: first)
+    }
+    const int n = uniform(unit / a.c.n_heads);
+    g = unit - n * a.c.n_heads;
+    return fp8_deal(a, n);
 }
 
 // Rows of no sequence, and rows past the longest sequence allowed: zeros.  For the workgroup of a pair's first tile and part.
@@ -308,13 +369,12 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
     const int wk = WR > 1 ? 0 : wave, wr = WR > 1 ? wave : 0;
     static_assert(WK == 1 || WR == 1, "keys or rows");
 
-    int pair, part, tile;
-    fp8_slot(a, pair, part, tile);
-    const int n_pairs = c.n_batch * c.n_heads;
-    if (pair >= n_pairs) {
+    int g, tile;
+    const Fp8Deal deal = fp8_slot(a, g, tile);
+    if (deal.b < 0) {
         return;
     }
-    const int b = uniform(pair / c.n_heads), g = pair - b * c.n_heads;
+    const int b = deal.b, part = deal.part, pair = b * c.n_heads + g;
 
     const Fp8Item item = fp8_item(a, b);
     const Fp8Sequence& seq = item.seq;
@@ -333,22 +393,18 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
     }
     const int m0 = tile * TILE + wr * ROWS;
     const int m1 = m0 + ROWS < n_pairs_rows ? m0 + ROWS : n_pairs_rows;
-    // what this wavefront sweeps: its rows' blocks (all wavefronts of a tile's keys have the same rows)
-    Fp8Runs runs = {0, 0, 0, 0, 0};
-    int i_first = 0, i_last = 0;
-    if (m0 < m1) {
-        i_first = uniform(div_small(m0, a.ratio));
-        i_last = uniform(div_small(m1 - 1, a.ratio));
-        runs = fp8_runs(mask, i_first, i_last + 1);
-        runs = {uniform(runs.n_a), uniform(runs.n_b), uniform(runs.n_c), uniform(runs.b0), uniform(runs.c0)};
-    }
+    // what the workgroup sweeps: the blocks of its tile's rows
+    const int t0 = tile * TILE, t1 = t0 + TILE < n_pairs_rows ? t0 + TILE : n_pairs_rows;
+    Fp8Runs runs = fp8_runs(mask, uniform(div_small(t0, a.ratio)), uniform(div_small(t1 - 1, a.ratio)) + 1);
+    runs = {uniform(runs.n_a), uniform(runs.n_b), uniform(runs.n_c), uniform(runs.b0), uniform(runs.c0)};
+    const int i_first = uniform(div_small(m0 < m1 ? m0 : t0, a.ratio)), i_last = uniform(div_small(m0 < m1 ? m1 - 1 : t0, a.ratio));
     const int n_blocks = runs.count();
-    const int parts_used = a.parts == 1 ? 1 : uniform((n_blocks + a.chunk - 1) / a.chunk);
-    if (a.parts > 1 && part > 0 && part >= parts_used) {
+    const int parts_used = deal.parts == 1 ? 1 : uniform((n_blocks + deal.chunk - 1) / deal.chunk);
+    if (part > 0 && part >= parts_used) {
         return;
     }
-    const int n_begin = a.parts == 1 ? 0 : part * a.chunk;
-    const int n_end = a.parts == 1 || part == a.parts - 1 ? n_blocks : (n_begin + a.chunk < n_blocks ? n_begin + a.chunk : n_blocks);
+    const int n_begin = deal.parts == 1 ? 0 : part * deal.chunk;
+    const int n_end = part == deal.parts - 1 || n_blocks - n_begin < deal.chunk ? n_blocks : n_begin + deal.chunk;
 
     // q: the rows of this wavefront, 16 dims of this lane's half per group of 32
     u32x4_t q[NB][NC][2];
@@ -518,7 +574,7 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
                 acc[nb][n] = mfma32<Tag>(vv.hi, p[nb][1], acc[nb][n]);
             }
         }
-        if constexpr (WEIGHTS) {
+        if (WEIGHTS && m0 < m1) {
             const float all = fp8_key_sum(sums, lane) * __builtin_fabsf(a.c_out);
             fp8_store_key_sum(a, all, lane, pair, tile * WR + wr, a.row_tiles * WR, blk, lin);
         }
@@ -562,9 +618,8 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
     }
 
     // ---- the sum over the wavefronts that shared the keys, and the store ----
-    const bool partial = a.parts > 1 && parts_used > 1;
-    float* const to_partial =
-        a.partial + (static_cast<int64_t>(pair * a.row_tiles + tile) * a.parts + part) * static_cast<int64_t>(TILE) * dim;
+    const bool partial = parts_used > 1 && deal.parts > 1;
+    float* const to_partial = a.partial + (static_cast<int64_t>(deal.slot * c.n_heads + g) * a.row_tiles + tile) * TILE * dim;
     const auto row_at = [&](int m) {  // element index of a (row, head) pair in q and out
         const int i = div_small(m, a.ratio);
         return ((q0 + i) * a.n_heads_q + g * a.ratio + (m - i * a.ratio)) * static_cast<int64_t>(dim);

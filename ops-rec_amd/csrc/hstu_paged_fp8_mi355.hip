@@ -136,6 +136,7 @@ struct Plan {
     Fp8AttendArgs a;
     int64_t slots;
     uint64_t partial_bytes, weight_bytes;
+    bool split;  // some sequence may have more than one part
 };
 
 // Which variant, and how the keys of a tile are dealt to workgroups.
@@ -149,7 +150,10 @@ Plan plan(const hstu_paged_fp8_fwd_params* p)
         ++groups;
     }
     const Fp8AttendTable& table = p->dtype == HSTU_DT_BF16 ? kFp8AttendBf16 : kFp8AttendF16;
-    const int shape = rows <= 32 ? kFp8Keys : (rows <= 128 ? kFp8KeysWide : kFp8Rows);
+    // Up to 32 rows a wavefront of its own takes whatever keys it can get; up to 64 two share the conversion of codes; more rows go in
+    // tiles of 128 where those fill the machine's places for them, else of 64, whose keys go to two shares of a workgroup (24 x 4
+    // pairs, 100 .. 260 rows in a window of 1024: 42 us, 57 in tiles of 128; 16 x 4 pairs of 1024 rows on 2048 .. 8192 keys 301 and 265).
+    const int shape = rows <= 32 ? kFp8Keys : (rows <= 64 || pairs * ceil_div(rows, 128) < 512 ? kFp8KeysWide : kFp8Rows);
     const bool weights = p->cache.weights != nullptr;
     r.v = &table[groups][shape][weights ? 1 : 0];
     Fp8AttendArgs& a = r.a;
@@ -172,25 +176,41 @@ Plan plan(const hstu_paged_fp8_fwd_params* p)
     a.c_out = static_cast<float>(p->alpha * p->silu_scale);
     a.row_tiles = static_cast<int>(ceil_div(rows, r.v->tile_rows));
     a.max_blocks = static_cast<int>(ceil_div(p->max_seq_len_k, kBlock));
-    // the most blocks that a tile sweeps
-    int64_t blocks = a.max_blocks;
+    a.most_blocks = a.max_blocks;
     if (a.window > 0) {
-        blocks = std::min<int64_t>(blocks, ceil_div(a.window + r.v->tile_rows / ratio, kBlock) + 2 + ceil_div(a.sinks, kBlock));
+        const int64_t seen = ceil_div(a.window + r.v->tile_rows / ratio, kBlock) + 2 + ceil_div(a.sinks, kBlock);
+        a.most_blocks = static_cast<int>(std::min<int64_t>(a.most_blocks, seen));
     }
+    // Parts (fp8_deal), where there are fewer workgroups than the machine has places: as many as it has, by the registers of the variants.
+    // More cost more than they spare: 64 x 4 pairs of one row on 2048 .. 8192 keys 74 us without, 81 in 512 and 87 in 1024; 3 x 2 pairs,
+    // d 256, on 30011 .. 120011 51 in 256, 56 in 512 to 1024; 32 x 4 of 49 .. 64 rows, d 64, on 501 .. 4001 31 in 1024, 45 without;
+    // 32 x 4 of 40 .. 64, d 128, with weights 58 in 512, 68 in 1024, 87 without.  Parts of a few blocks are not worth their sums.
+    const int64_t batch = p->cache.n_offsets - 1, per_part = p->cache.num_heads_k * a.row_tiles;
+    const bool narrow = groups < 2, wide = groups >= 4;  // up to 64 dims, more than 128
+    const int64_t places = shape == kFp8Keys ? (narrow ? 512 : 256) : (wide ? 256 : (narrow || shape == kFp8Rows ? 1024 : 512));
+    const int64_t total = places / per_part, waves = r.v->threads / 64;
+    const int least = static_cast<int>(shape == kFp8Rows ? 32 : (shape == kFp8Keys ? 4 * waves : 8));
+    a.total_parts = 0;
     a.parts = 1;
-    a.chunk = static_cast<int>(blocks);
-    if (shape != kFp8Rows) {
-        const int64_t tiles = pairs * a.row_tiles, waves = r.v->threads / 64;
-        const int64_t wanted = std::min(ceil_div(768, tiles), blocks / (4 * waves));
-        if (wanted > 1) {
-            a.chunk = static_cast<int>(ceil_div(blocks, wanted));
-            a.parts = static_cast<int>(ceil_div(blocks, a.chunk));
+    a.chunk = a.most_blocks;
+    if (2 * total >= 3 * batch && a.most_blocks > least) {
+        if (batch <= 64) {
+            a.chunk = least;
+            a.total_parts = static_cast<int>(total);
+        } else {
+            a.parts = static_cast<int>(std::min(ceil_div(total, batch), ceil_div(a.most_blocks, least)));
+            a.chunk = static_cast<int>(ceil_div(a.most_blocks, a.parts));
+            a.total_parts = static_cast<int>(batch * a.parts);
         }
+    } else if (shape == kFp8Rows && batch <= 64) {  // one part each, the longest sequences first
+        a.total_parts = static_cast<int>(batch + 1);
     }
-    r.partial_bytes = a.parts > 1 ? static_cast<uint64_t>(pairs) * a.row_tiles * a.parts * r.v->tile_rows * p->cache.head_dim * 4 : 0;
+    r.split = a.chunk < a.most_blocks;
+    r.partial_bytes = r.split ? static_cast<uint64_t>(a.total_parts) * per_part * r.v->tile_rows * p->cache.head_dim * 4 : 0;
     const int64_t wave_tiles = static_cast<int64_t>(a.row_tiles) * (r.v->tile_rows / r.v->wave_rows);
     r.weight_bytes = weights && wave_tiles > 1 ? static_cast<uint64_t>(pairs) * wave_tiles * a.max_blocks * kBlock * 4 : 0;
-    r.slots = a.row_tiles == 1 ? pairs * a.parts : ceil_div(pairs, 8) * 8 * a.row_tiles * a.parts;
+    const int64_t units = (a.total_parts > 0 ? a.total_parts : batch) * p->cache.num_heads_k;
+    r.slots = a.row_tiles == 1 ? units : ceil_div(units, 8) * 8 * a.row_tiles;
     return r;
 }
 
@@ -294,9 +314,10 @@ HSTU_API int hstu_paged_fp8_fwd(const hstu_paged_fp8_fwd_params* p, void* worksp
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const unsigned pairs = static_cast<unsigned>(a.c.n_batch) * a.c.n_heads;
     hipLaunchKernelGGL(r.v->kernel, dim3(static_cast<unsigned>(r.slots)), dim3(r.v->threads), 0, s, a);
-    if (a.parts > 1) {
+    if (r.split) {
         const auto join = p->dtype == HSTU_DT_BF16 ? hstu_paged_fp8_join_kernel<bf16_tag> : hstu_paged_fp8_join_kernel<f16_tag>;
-        hipLaunchKernelGGL(join, dim3(pairs, a.row_tiles), dim3(256), 0, s, a, r.v->tile_rows);
+        hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(ceil_div(static_cast<int64_t>(r.v->tile_rows) * a.c.dim, 1024)), a.row_tiles, pairs), dim3(256), 0, s, a,
+                           r.v->tile_rows);
     }
     if (a.weight_partial != nullptr) {
         const int tiles = a.row_tiles * (r.v->tile_rows / r.v->wave_rows);

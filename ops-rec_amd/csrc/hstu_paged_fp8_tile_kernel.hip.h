@@ -18,7 +18,7 @@
 namespace hstu {
 
 template <typename Tag, int NC, int RG, int KG, bool WEIGHTS>
-__global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(NC <= 2 ? 4 : 2, NC <= 2 ? 4 : 2))) void hstu_paged_fp8_tile_kernel(const Fp8AttendArgs a)
+__global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(NC <= 2 ? 4 : (WEIGHTS ? 2 : 3), NC <= 2 ? 4 : (WEIGHTS ? 2 : 3)))) void hstu_paged_fp8_tile_kernel(const Fp8AttendArgs a)
 {
     constexpr int WAVES = RG * KG, T = 64 * WAVES;
     constexpr int TILE = 32 * RG;
@@ -35,13 +35,12 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(NC
     const int col = lane & 31, half = lane >> 5;
     const int rg = wave & (RG - 1), kg = wave / RG;
 
-    int pair, part, tile;
-    fp8_slot(a, pair, part, tile);
-    const int n_pairs = c.n_batch * c.n_heads;
-    if (pair >= n_pairs) {
+    int g, tile;
+    const Fp8Deal deal = fp8_slot(a, g, tile);
+    if (deal.b < 0) {
         return;
     }
-    const int b = uniform(pair / c.n_heads), g = pair - b * c.n_heads;
+    const int b = deal.b, part = deal.part, pair = b * c.n_heads + g;
     const Fp8Item item = fp8_item(a, b);
     const Fp8Sequence& seq = item.seq;
     const Fp8Mask& mask = item.mask;
@@ -60,12 +59,12 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(NC
     Fp8Runs runs = fp8_runs(mask, ti0, ti1 + 1);
     runs = {uniform(runs.n_a), uniform(runs.n_b), uniform(runs.n_c), uniform(runs.b0), uniform(runs.c0)};
     const int n_blocks = runs.count();
-    const int parts_used = a.parts == 1 ? 1 : uniform((n_blocks + a.chunk - 1) / a.chunk);
+    const int parts_used = deal.parts == 1 ? 1 : uniform((n_blocks + deal.chunk - 1) / deal.chunk);
     if (part > 0 && part >= parts_used) {
         return;
     }
-    const int n_begin = a.parts == 1 ? 0 : part * a.chunk;
-    const int n_end = a.parts == 1 || part == a.parts - 1 ? n_blocks : (n_begin + a.chunk < n_blocks ? n_begin + a.chunk : n_blocks);
+    const int n_begin = deal.parts == 1 ? 0 : part * deal.chunk;
+    const int n_end = part == deal.parts - 1 || n_blocks - n_begin < deal.chunk ? n_blocks : n_begin + deal.chunk;
     const int m0 = t0 + 32 * rg;
     const bool rows_here = m0 < n_rows;
     const int m1 = m0 + 32 < n_rows ? m0 + 32 : n_rows;
@@ -202,9 +201,9 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(NC
                 acc[n] = mfma32<Tag>(operand(v, 2 * n + u), p[u], acc[n]);
             }
         }
-        // operands are read eight ahead of their products (left to itself the compiler reads each into the same registers and waits
+        // operands are read six ahead of their products (left to itself the compiler reads each into the same registers and waits
         // for it: 16 times the LDS's latency)
-        constexpr int N = 4 * NC, AHEAD = N < 8 ? N : 8;
+        constexpr int N = 4 * NC, AHEAD = N < 6 ? N : 6;
         __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);  // LDS reads
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -321,9 +320,8 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(NC
     }
 
     // ---- the sum over the shares, and the store ----
-    const bool partial = a.parts > 1 && parts_used > 1;
-    float* const to_partial =
-        a.partial + (static_cast<int64_t>(pair * a.row_tiles + tile) * a.parts + part) * static_cast<int64_t>(TILE) * dim;
+    const bool partial = parts_used > 1 && deal.parts > 1;
+    float* const to_partial = a.partial + (static_cast<int64_t>(deal.slot * c.n_heads + g) * a.row_tiles + tile) * TILE * dim;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
         float* const s = reinterpret_cast<float*>(s_mem) + (n & 1) * (SUMS / 4);
