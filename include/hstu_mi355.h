@@ -277,7 +277,7 @@ HSTU_API int hstu_paged_fwd(const hstu_paged_fwd_params* params, void* workspace
  * them live.  Page ids outside [0, num_pages) stand for pages that are not there: nothing is read from them (their rows count as
  * zeros) or written to them.  A page that a call writes to must stand in it once, and nowhere else in the call; a page that is
  * only read may be shared by sequences.  head_dim is a multiple of 16 in [16, 256], page_size a multiple of 32; pointers to
- * caches, q, k, v and out are 16-byte aligned.
+ * caches, weights, q, k, v and out are 16-byte aligned.
  */
 #define HSTU_PAGED_FP8_MAX_SEQ_LEN_K 16777216
 #define HSTU_PAGED_FP8_MAX_HEAD_DIM 256

@@ -5,8 +5,11 @@
 namespace hstu {
 
 constexpr int kFp8Block = 32;         // tokens that share a scale, and keys of one step of the attention kernel
+constexpr int kFp8JoinEnough = 1024;  // workgroups of the joins that fill the machine
 constexpr int kFp8AppendThreads = 128;
-constexpr int kFp8SelectThreads = 1024;
+constexpr int kFp8AppendEnough = 8192;  // workgroups of the append from which on one takes several blocks
+constexpr int kFp8SelectKeys = 32768;   // scores that the selecting kernel holds in LDS
+constexpr int kFp8SelectFew = 2048;     // longest sequence of its variant with few threads
 
 // The cache of one layer, and whose pages are whose.
 struct Fp8Cache {
@@ -34,6 +37,7 @@ struct Fp8AttendArgs {
     const void* num_target;  // or null
     void* out;
     float* partial;         // [total_parts * n_heads][row_tiles][rows of a tile][dim], where there are parts
+    int2* joins;            // [n_batch * n_heads][row_tiles] how many parts a tile was done in, and the first of them; where there are parts
     float* weight_partial;  // [n_batch * n_heads][row_tiles][max_blocks * 32], for weights over more than one row tile
     int64_t total_q;
     int n_heads_q;
@@ -61,6 +65,7 @@ struct Fp8AppendArgs {
     int64_t total;
     int64_t k_row, k_head, v_row, v_head;  // strides, in elements
     int max_rows;
+    int in_turn;  // blocks that a workgroup takes one after the other
 };
 
 struct Fp8EvictArgs {
@@ -69,7 +74,8 @@ struct Fp8EvictArgs {
     const void* new_page_ids;
     void* new_len;    // [n_batch], of the index type
     void* kept;       // [n_batch][keep], of the index type
-    uint32_t* keys;   // workspace [n_batch][max_k]: the scores in an order that compares as integers
+    uint32_t* keys;   // workspace [n_batch][key_pitch], for more scores than fit LDS: in an order that compares as integers
+    int64_t key_pitch;
     int n_new_page_ids;
     int max_k;
     int keep;

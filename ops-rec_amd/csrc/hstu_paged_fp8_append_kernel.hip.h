@@ -1,10 +1,10 @@
 // New key and value rows written into the 8-bit paged cache (gfx950).
 //
-// One workgroup per (block of 32 tokens that the call touches, key head, K or V, sequence).  It reads the
-// new rows of its block and, in the first block of a sequence, the rows that are there already (decoded with the block's old
-// scale); the largest finite magnitude of all of them gives the block's scale, a power of two, so that dividing by it rounds
-// nothing, live rows move to a larger scale by a change of exponent alone (only what falls below the smallest normal code
-// rounds), and writing the same rows again changes nothing.  The whole block is written: rows behind the new end are cleared.
+// One workgroup per (some blocks of 32 tokens that the call touches, one after the other, key head, K or V, sequence).  It reads the
+// new rows of a block, those of the next one on their way meanwhile, and, in the first block of a sequence, the rows that are there already
+// (decoded with the block's old scale); the largest finite magnitude of all of them gives the block's scale, a power of two, so that
+// dividing by it rounds nothing, live rows move to a larger scale by a change of exponent alone (only what falls below the smallest
+// normal code rounds), and writing the same rows again changes nothing.  The whole block is written: rows behind the new end are cleared.
 //   K: 16 bytes of a row per lane, 8 codes out, at the row's place.
 //   V: the block is stored with the tokens innermost (what the attention kernel's matrix instruction reads); a lane takes two
 //      dims of 16 tokens, 4 bytes a load -- a wavefront's lanes read 256 bytes of a row together -- and has 16 bytes of each dim
@@ -15,13 +15,16 @@
 
 namespace hstu {
 
-template <typename Tag, int DS>
+// a row of a block that the call brings rows [live, fill) of
+__device__ __forceinline__ int64_t clamp_row(int row, int live, int fill) { return row < live ? live : (row < fill ? row : fill - 1); }
+
+template <typename Tag, int DS, bool TURNS>
 __global__ __launch_bounds__(kFp8AppendThreads) void hstu_paged_fp8_append_kernel(const Fp8AppendArgs a)
 {
     constexpr int T = kFp8AppendThreads;
     constexpr int KP = kFp8Block * DS / 8 / T;     // 8-dim pieces per lane
     constexpr int VP = DS / T > 0 ? DS / T : 1;  // (dim pair, 16 tokens) units per lane
-    __shared__ uint32_t s_top[kFp8AppendThreads / 64];
+    __shared__ uint32_t s_top[2][T / 64];
 
     const Fp8Cache& c = a.c;
     const int b = static_cast<int>(blockIdx.z), g = static_cast<int>(blockIdx.y >> 1);
@@ -33,144 +36,222 @@ __global__ __launch_bounds__(kFp8AppendThreads) void hstu_paged_fp8_append_kerne
     const int room = fp8_room(c, seq.n_pages) - seq.len;
     int n_new = static_cast<int>(r1 > r0 ? r1 - r0 : 0);
     n_new = n_new < room ? n_new : room;
-    const int blk = seq.len / kFp8Block + static_cast<int>(blockIdx.x);
-    const int start = blk * kFp8Block, end = seq.len + n_new;
-    if (n_new <= 0 || start >= end) {
+    const int first = seq.len / kFp8Block + static_cast<int>(blockIdx.x) * a.in_turn, end = seq.len + n_new;
+    int n_blocks = (end + kFp8Block - 1) / kFp8Block - first;
+    n_blocks = n_blocks < a.in_turn ? n_blocks : a.in_turn;
+    if (n_new <= 0 || n_blocks <= 0) {
         return;
     }
-    const int lin = uniform(fp8_block(c, c.page_ids, seq.first, g, blk));
-    if (lin < 0) {
-        return;  // no such page: the rows have no place
-    }
-    const int live = seq.len > start ? seq.len - start : 0;            // rows of the block that are there already
-    const int fill = end - start < kFp8Block ? end - start : kFp8Block;  // ... and that are there after the call
-    const int64_t row0 = r0 + start - seq.len;                          // input row of the block's row 0 (only rows from `live` on exist)
-    const int t = threadIdx.x;
-    const int dim = c.dim;
-    const int64_t codes_at = static_cast<int64_t>(lin) * kFp8Block * dim;
+    const int t = threadIdx.x, dim = c.dim;
+    // input row of row 0 of block n of these, and the block's rows that are there before and after the call
+    const auto row_of = [&](int n) { return r0 + static_cast<int64_t>(first + n) * kFp8Block - seq.len; };
+    const auto live_of = [&](int n) { const int start = (first + n) * kFp8Block; return seq.len > start ? seq.len - start : 0; };
+    const auto fill_of = [&](int n) { const int rest = end - (first + n) * kFp8Block; return rest < kFp8Block ? rest : kFp8Block; };
 
     if ((blockIdx.y & 1) == 0) {
         const uint16_t* const src = static_cast<const uint16_t*>(a.k) + static_cast<int64_t>(g) * a.k_head;
-        uint8_t* const dst = c.k + codes_at;
-        const float old_scale = live > 0 ? c.k_scale[lin] : 0.0f;
         const int cpr = dim >> 3, pieces = kFp8Block * cpr;
-        float x[KP][8];
-        uint32_t top = 0;
+        int rows[KP], cols[KP];
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
-            const int p = t + i * T, row = div_small(p, cpr), col = (p - row * cpr) * 8;
+            const int p = t + i * T, row = div_small(p, cpr);
+            rows[i] = p < pieces ? row : kFp8Block;  // (of no block)
+            cols[i] = (p - row * cpr) * 8;
+        }
+        u32x4_t raw[KP];
+        const auto request = [&](int n) {
+            const uint16_t* const from = src + row_of(n) * a.k_row;
+            const int live = live_of(n), fill = fill_of(n);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[i][j] = 0.0f;
+            for (int i = 0; i < KP; ++i) {  // (a row that the call does not bring: one that it does, for nothing)
+                raw[i] = u32x4_t{0u};
+                if (TURNS || (rows[i] >= live && rows[i] < fill)) {
+                    raw[i] = *reinterpret_cast<const u32x4_t*>(from + clamp_row(rows[i], live, fill) * a.k_row + cols[i]);
+                }
             }
-            if (p < pieces && row >= live && row < fill) {
-                const u32x4_t w = *reinterpret_cast<const u32x4_t*>(src + (row0 + row) * a.k_row + col);
+        };
+        int next = uniform(fp8_block(c, c.page_ids, seq.first, g, first));
+        request(0);
+        for (int n = 0; n < (TURNS ? n_blocks : 1); ++n) {
+            const int lin = next, live = live_of(n), fill = fill_of(n);
+            uint8_t* const dst = c.k + static_cast<int64_t>(lin < 0 ? 0 : lin) * kFp8Block * dim;
+            const bool old = live > 0 && lin >= 0;  // (in the first block of a sequence only)
+            u32x2_t was[KP];
+            float old_scale = 0.0f;
+            if (old) {
+                old_scale = c.k_scale[lin];
+#pragma unroll
+                for (int i = 0; i < KP; ++i) {
+                    was[i] = *reinterpret_cast<const u32x2_t*>(dst + (rows[i] < live ? rows[i] * dim + cols[i] : 0));
+                }
+            }
+            float x[KP][8];
+#pragma unroll
+            for (int i = 0; i < KP; ++i) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    x[i][2 * j] = lo_to_float<Tag>(w[j]);
-                    x[i][2 * j + 1] = hi_to_float<Tag>(w[j]);
-                }
-            } else if (p < pieces && row < live) {
-                const u32x2_t w = *reinterpret_cast<const u32x2_t*>(dst + row * dim + col);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const f32x2_t lo = fp8_values2<false>(w[j]), hi = fp8_values2<true>(w[j]);
-                    x[i][4 * j] = lo[0] * old_scale;
-                    x[i][4 * j + 1] = lo[1] * old_scale;
-                    x[i][4 * j + 2] = hi[0] * old_scale;
-                    x[i][4 * j + 3] = hi[1] * old_scale;
+                    x[i][2 * j] = rows[i] < fill ? lo_to_float<Tag>(raw[i][j]) : 0.0f;
+                    x[i][2 * j + 1] = rows[i] < fill ? hi_to_float<Tag>(raw[i][j]) : 0.0f;
                 }
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t m = finite_bits(x[i][j]);
-                top = m > top ? m : top;
+            if (TURNS && n + 1 < n_blocks) {
+                next = uniform(fp8_block(c, c.page_ids, seq.first, g, first + n + 1));
+                request(n + 1);
             }
-        }
-        const uint32_t field = fp8_scale_field(block_top<T / 64>(top, s_top));
-        const float inverse = fp8_inverse_of(field);
+            if (old) {
 #pragma unroll
-        for (int i = 0; i < KP; ++i) {
-            const int p = t + i * T, row = div_small(p, cpr), col = (p - row * cpr) * 8;
-            u32x2_t w;
+                for (int i = 0; i < KP; ++i) {
+                    if (rows[i] < live) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                uint32_t codes = fp8_codes2<false>(x[i][4 * j], x[i][4 * j + 1], inverse, 0u);
-                w[j] = fp8_codes2<true>(x[i][4 * j + 2], x[i][4 * j + 3], inverse, codes);
-            }
-            if (p < pieces) {
-                *reinterpret_cast<u32x2_t*>(dst + row * dim + col) = w;
-            }
-        }
-        if (t == 0) {
-            c.k_scale[lin] = fp8_scale_of(field);
-        }
-        if (c.weights != nullptr && t >= live && t < kFp8Block) {
-            c.weights[static_cast<int64_t>(lin) * kFp8Block + t] = 0.0f;
-        }
-    } else {
-        const uint16_t* const src = static_cast<const uint16_t*>(a.v) + static_cast<int64_t>(g) * a.v_head;
-        uint8_t* const dst = c.v + codes_at;
-        const float old_scale = live > 0 ? c.v_scale[lin] : 0.0f;
-        const int pairs = dim >> 1;
-        float x[VP][2][16];  // [unit][dim of the pair][token]
-        uint32_t top = 0;
-#pragma unroll
-        for (int u = 0; u < VP; ++u) {
-            const int n = t + u * T, half = n >= pairs ? 1 : 0, d = 2 * (n - half * pairs);
-            const bool mine = n < 2 * pairs;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int row = 16 * half + i;
-                x[u][0][i] = x[u][1][i] = 0.0f;
-                if (mine && row >= live && row < fill) {
-                    const uint32_t w = *reinterpret_cast<const uint32_t*>(src + (row0 + row) * a.v_row + d);
-                    x[u][0][i] = lo_to_float<Tag>(w);
-                    x[u][1][i] = hi_to_float<Tag>(w);
-                }
-            }
-            if (live > 16 * half && mine) {  // (the first block of a sequence only)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const u32x4_t w = *reinterpret_cast<const u32x4_t*>(dst + (d + e) * kFp8Block + 16 * half);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const f32x2_t lo = fp8_values2<false>(w[j]), hi = fp8_values2<true>(w[j]);
-                        const float old[4] = {lo[0], lo[1], hi[0], hi[1]};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            x[u][e][4 * j + i] = 16 * half + 4 * j + i < live ? old[i] * old_scale : x[u][e][4 * j + i];
+                        for (int j = 0; j < 2; ++j) {
+                            const f32x2_t lo = fp8_values2<false>(was[i][j]), hi = fp8_values2<true>(was[i][j]);
+                            x[i][4 * j] = lo[0] * old_scale;
+                            x[i][4 * j + 1] = lo[1] * old_scale;
+                            x[i][4 * j + 2] = hi[0] * old_scale;
+                            x[i][4 * j + 3] = hi[1] * old_scale;
                         }
                     }
                 }
             }
+            uint32_t top = 0;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const uint32_t m0 = finite_bits(x[u][0][i]), m1 = finite_bits(x[u][1][i]);
-                top = m0 > top ? m0 : top;
-                top = m1 > top ? m1 : top;
+            for (int i = 0; i < KP; ++i) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t m = finite_bits(x[i][j]);
+                    top = m > top ? m : top;
+                }
+            }
+            const uint32_t field = fp8_scale_field(block_top<T / 64>(top, s_top[n & 1]));
+            const float inverse = fp8_inverse_of(field);
+            if (lin >= 0) {  // (otherwise there is no such page: the rows have no place)
+#pragma unroll
+                for (int i = 0; i < KP; ++i) {
+                    u32x2_t w;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t codes = fp8_codes2<false>(x[i][4 * j], x[i][4 * j + 1], inverse, 0u);
+                        w[j] = fp8_codes2<true>(x[i][4 * j + 2], x[i][4 * j + 3], inverse, codes);
+                    }
+                    if (rows[i] < kFp8Block) {
+                        *reinterpret_cast<u32x2_t*>(dst + rows[i] * dim + cols[i]) = w;
+                    }
+                }
+                if (t == 0) {
+                    c.k_scale[lin] = fp8_scale_of(field);
+                }
+                if (c.weights != nullptr && t >= live && t < kFp8Block) {
+                    c.weights[static_cast<int64_t>(lin) * kFp8Block + t] = 0.0f;
+                }
             }
         }
-        const uint32_t field = fp8_scale_field(block_top<T / 64>(top, s_top));
-        const float inverse = fp8_inverse_of(field);
+    } else {
+        const uint16_t* const src = static_cast<const uint16_t*>(a.v) + static_cast<int64_t>(g) * a.v_head;
+        const int pairs = dim >> 1;
+        int halves[VP], dims[VP];
 #pragma unroll
         for (int u = 0; u < VP; ++u) {
-            const int n = t + u * T, half = n >= pairs ? 1 : 0, d = 2 * (n - half * pairs);
+            const int m = t + u * T;
+            halves[u] = m >= pairs ? (m < 2 * pairs ? 16 : 2 * kFp8Block) : 0;  // first of the 16 tokens
+            dims[u] = m >= 2 * pairs ? 0 : 2 * (m >= pairs ? m - pairs : m);
+        }
+        uint32_t raw[VP][16];
+        const auto request = [&](int n) {
+            const uint16_t* const from = src + row_of(n) * a.v_row;
+            const int live = live_of(n), fill = fill_of(n);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                u32x4_t w;
+            for (int u = 0; u < VP; ++u) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t codes = fp8_codes2<false>(x[u][e][4 * j], x[u][e][4 * j + 1], inverse, 0u);
-                    w[j] = fp8_codes2<true>(x[u][e][4 * j + 2], x[u][e][4 * j + 3], inverse, codes);
-                }
-                if (n < 2 * pairs) {
-                    *reinterpret_cast<u32x4_t*>(dst + (d + e) * kFp8Block + 16 * half) = w;
+                for (int i = 0; i < 16; ++i) {
+                    raw[u][i] = 0u;
+                    if (TURNS || (halves[u] + i >= live && halves[u] + i < fill)) {
+                        raw[u][i] = *reinterpret_cast<const uint32_t*>(from + clamp_row(halves[u] + i, live, fill) * a.v_row + dims[u]);
+                    }
                 }
             }
-        }
-        if (t == 0) {
-            c.v_scale[lin] = fp8_scale_of(field);
+        };
+        int next = uniform(fp8_block(c, c.page_ids, seq.first, g, first));
+        request(0);
+        for (int n = 0; n < (TURNS ? n_blocks : 1); ++n) {
+            const int lin = next, live = live_of(n), fill = fill_of(n);
+            uint8_t* const dst = c.v + static_cast<int64_t>(lin < 0 ? 0 : lin) * kFp8Block * dim;
+            const bool old = live > 0 && lin >= 0;
+            u32x4_t was[VP][2];
+            float old_scale = 0.0f;
+            if (old) {
+                old_scale = c.v_scale[lin];
+#pragma unroll
+                for (int u = 0; u < VP; ++u) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        was[u][e] = *reinterpret_cast<const u32x4_t*>(dst + (dims[u] + e) * kFp8Block + (halves[u] & 16));
+                    }
+                }
+            }
+            float x[VP][2][16];  // [unit][dim of the pair][token]
+#pragma unroll
+            for (int u = 0; u < VP; ++u) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    x[u][0][i] = halves[u] + i < fill ? lo_to_float<Tag>(raw[u][i]) : 0.0f;
+                    x[u][1][i] = halves[u] + i < fill ? hi_to_float<Tag>(raw[u][i]) : 0.0f;
+                }
+            }
+            if (TURNS && n + 1 < n_blocks) {
+                next = uniform(fp8_block(c, c.page_ids, seq.first, g, first + n + 1));
+                request(n + 1);
+            }
+            if (old) {
+#pragma unroll
+                for (int u = 0; u < VP; ++u) {
+                    if (halves[u] < live) {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const f32x2_t lo = fp8_values2<false>(was[u][e][j]), hi = fp8_values2<true>(was[u][e][j]);
+                                const float had[4] = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    x[u][e][4 * j + i] = halves[u] + 4 * j + i < live ? had[i] * old_scale : x[u][e][4 * j + i];
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+            uint32_t top = 0;
+#pragma unroll
+            for (int u = 0; u < VP; ++u) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t m0 = finite_bits(x[u][0][i]), m1 = finite_bits(x[u][1][i]);
+                    top = m0 > top ? m0 : top;
+                    top = m1 > top ? m1 : top;
+                }
+            }
+            const uint32_t field = fp8_scale_field(block_top<T / 64>(top, s_top[n & 1]));
+            const float inverse = fp8_inverse_of(field);
+            if (lin >= 0) {
+#pragma unroll
+                for (int u = 0; u < VP; ++u) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        u32x4_t w;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t codes = fp8_codes2<false>(x[u][e][4 * j], x[u][e][4 * j + 1], inverse, 0u);
+                            w[j] = fp8_codes2<true>(x[u][e][4 * j + 2], x[u][e][4 * j + 3], inverse, codes);
+                        }
+                        if (halves[u] < kFp8Block) {
+                            *reinterpret_cast<u32x4_t*>(dst + (dims[u] + e) * kFp8Block + halves[u]) = w;
+                        }
+                    }
+                }
+                if (t == 0) {
+                    c.v_scale[lin] = fp8_scale_of(field);
+                }
+            }
         }
     }
 }

@@ -186,7 +186,7 @@ struct Fp8Deal {
     int part;   // of its
     int parts;
     int chunk;
-    int slot;   // number of the part among all
+    int slot;   // number of the part among all, in the order of the sequences (of a sequence that has one: unused)
 };
 struct Fp8DealLanes {
     int chunk, parts, rank;  // of the sequence of this lane: its parts (0: no sequence), and how many come before it
@@ -233,7 +233,16 @@ __device__ __forceinline__ Fp8Deal fp8_deal(const Fp8AttendArgs& a, int n)  // t
     }
     const uint64_t mine = __ballot((l.rank == rank) & (l.parts > part));
     const int b = mine != 0 ? __builtin_ctzll(mine) : -1;
-    return {b, part, mine != 0 ? __builtin_amdgcn_readlane(l.parts, b >= 0 ? b : 0) : 1, l.chunk, n};
+    const int parts = mine != 0 ? __builtin_amdgcn_readlane(l.parts, b >= 0 ? b : 0) : 1;
+    int ahead = 0;  // parts of the sequences before
+    if (parts > 1) {
+        ahead = static_cast<int>(threadIdx.x & 63) < b ? l.parts : 0;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            ahead += __shfl_xor(ahead, d, 64);
+        }
+    }
+    return {b, part, parts, l.chunk, uniform(ahead) + part};
 }
 
 // What a workgroup does: slots are (part, key head) x row tile, the tiles of a part and head, which read the same keys, on one XCD
@@ -402,6 +411,9 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
     const int parts_used = deal.parts == 1 ? 1 : uniform((n_blocks + deal.chunk - 1) / deal.chunk);
     if (part > 0 && part >= parts_used) {
         return;
+    }
+    if (part == 0 && a.joins != nullptr && threadIdx.x == 0) {
+        a.joins[pair * a.row_tiles + tile] = int2{parts_used < deal.parts ? parts_used : deal.parts, deal.slot};
     }
     const int n_begin = deal.parts == 1 ? 0 : part * deal.chunk;
     const int n_end = part == deal.parts - 1 || n_blocks - n_begin < deal.chunk ? n_blocks : n_begin + deal.chunk;

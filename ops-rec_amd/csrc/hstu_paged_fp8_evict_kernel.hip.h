@@ -24,6 +24,8 @@ __device__ __forceinline__ void store_index(void* p, int64_t i, int64_t value, i
     }
 }
 
+typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+
 // How many rows of a sequence stay, and how many of them stay whatever their score.
 struct Fp8Budget {
     int len, keep, sinks, recent;
@@ -41,19 +43,50 @@ __device__ __forceinline__ Fp8Budget fp8_budget(const Fp8EvictArgs& a, const Fp8
     return r;
 }
 
-// One workgroup per sequence.  A row's score is the sum of its weights over the key heads, in their order, in fp32.  The keep-th
-// largest among the rows that are not kept anyway is found by its bits, eight at a time from the top (four histograms in LDS
-// over the scores, which stay where the first pass left them); rows above it stay, and of those equal to it the first few.  The
-// kept rows' indices are written in order.
-__global__ __launch_bounds__(kFp8SelectThreads) void hstu_paged_fp8_select_kernel(const Fp8EvictArgs a)
+// Adds `x` over the lanes and wavefronts ahead of this one: the sum before it, and that of all in `all`.  `s` has a word per wavefront.
+template <int WAVES>
+__device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t (&s)[WAVES], uint32_t& all)
 {
-    constexpr int T = kFp8SelectThreads, WAVES = T / 64;
-    __shared__ uint32_t s_hist[256];
-    __shared__ uint32_t s_above[2][WAVES], s_equal[2][WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t until = x;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t below = static_cast<uint32_t>(__shfl_up(static_cast<int>(until), d, 64));
+        until += lane >= d ? below : 0u;
+    }
+    __syncthreads();  // (s of an earlier sum has been read)
+    if (lane == 63) {
+        s[wave] = until;
+    }
+    __syncthreads();
+    uint32_t before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        before += w < wave ? s[w] : 0u;
+        all += s[w];
+    }
+    return before + until - x;
+}
+
+// One workgroup per sequence.  A row's score is the sum of its weights over the key heads, in their order, in fp32.  The last of the
+// places that are left beside the rows kept anyway goes to the k-th largest score, which is found by its bits, eleven, eleven and
+// ten at a time from the top: histograms in LDS (2048 bins: with the eight bits of sign and exponent alone most scores of a sequence
+// fall into a few, whose additions then wait for each other) over the scores, in LDS too up to kFp8SelectKeys of them, else
+// where the first pass left them.  Rows above it stay, and of those equal to it the first few: every thread counts those of a
+// stretch of rows, one sum over the workgroup says where its indices go.
+// T threads and KEYS scores in LDS: 1024 and kFp8SelectKeys, or for short sequences few (500 rows: 9.5 us with 1024 threads, 6.5 with 256).
+template <int T, int KEYS>
+__global__ __launch_bounds__(T) void hstu_paged_fp8_select_kernel(const Fp8EvictArgs a)
+{
+    constexpr int WAVES = T / 64, BINS = 2048, OWN = BINS / T;
+    __shared__ __attribute__((aligned(16))) uint32_t s_keys[KEYS];
+    __shared__ uint32_t s_hist[BINS];
+    __shared__ uint32_t s_sum[WAVES];
     __shared__ uint32_t s_pick[2];
 
     const Fp8Cache& c = a.c;
-    const int b = static_cast<int>(blockIdx.x), tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63;
+    const int b = static_cast<int>(blockIdx.x), tid = threadIdx.x;
     const Fp8Sequence seq = fp8_sequence(c, b);
     const Fp8Sequence to = fp8_pages(a.new_page_offsets, a.n_new_page_ids, c.idx64, b);
     const Fp8Budget n = fp8_budget(a, seq, to.n_pages);
@@ -64,110 +97,120 @@ __global__ __launch_bounds__(kFp8SelectThreads) void hstu_paged_fp8_select_kerne
     for (int i = n.keep + tid; i < a.keep; i += T) {
         store_index(a.kept, kept + i, -1, c.idx64);
     }
-    if (n.keep == n.len) {
-        for (int i = tid; i < n.keep; i += T) {
-            store_index(a.kept, kept + i, i, c.idx64);
-        }
-        return;
-    }
-    // rows [sinks, len - recent) compete for the places left; there are fewer places than rows
+    // rows [lo, hi) compete for the places that are left; the others stay
     const int lo = n.sinks, hi = n.len - n.recent;
     const int places = n.keep - n.sinks - n.recent;
-    uint32_t* const keys = a.keys + static_cast<int64_t>(b) * a.max_k;
-    const int64_t head_pitch = static_cast<int64_t>(c.blocks_per_page) * kFp8Block;
-    for (int j = lo + tid; j < hi; j += T) {
-        const int lin = fp8_block(c, c.page_ids, seq.first, 0, j / kFp8Block);
-        float score = 0.0f;
-        if (lin >= 0) {
-            const float* const w = c.weights + static_cast<int64_t>(lin) * kFp8Block + (j & (kFp8Block - 1));
-            score = w[0];
-            for (int h = 1; h < c.n_heads; ++h) {
-                score += w[h * head_pitch];
-            }
-        }
-        keys[j] = score_key(score);
-    }
-    uint32_t prefix = 0, left = static_cast<uint32_t>(places);  // of the rows whose top bits are `prefix`, `left` stay
-    if (places > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += T) {
-                s_hist[i] = 0;
-            }
-            __syncthreads();
-            for (int j = lo + tid; j < hi; j += T) {
-                const uint32_t k = keys[j];
-                if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) {
-                    atomicAdd(&s_hist[(k >> shift) & 255u], 1u);
-                }
-            }
-            __syncthreads();
-            if (wave == 0) {
-                // lane l has the digits 255 - 4 l .. 252 - 4 l: counts from the top
-                uint32_t mine[4], sum = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    mine[i] = s_hist[255 - 4 * lane - i];
-                    sum += mine[i];
-                }
-                uint32_t before = sum;
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) {
-                    const uint32_t up = static_cast<uint32_t>(__shfl_up(static_cast<int>(before), d, 64));
-                    before += lane >= d ? up : 0u;
-                }
-                before -= sum;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (before < left && before + mine[i] >= left) {  // (true for one digit of one lane)
-                        s_pick[0] = static_cast<uint32_t>(255 - 4 * lane - i);
-                        s_pick[1] = left - before;
-                    }
-                    before += mine[i];
-                }
-            }
-            __syncthreads();
-            prefix |= s_pick[0] << shift;
-            left = s_pick[1];
-        }
-    }
-    // rows above `prefix` stay, and the first `left` of those equal to it; none where there are no places
-    const uint32_t none = places > 0 ? 0u : 1u;
-    uint32_t n_kept = static_cast<uint32_t>(n.sinks), n_equal = 0;
-    for (int i = tid; i < n.sinks; i += T) {
+    const bool all_stay = n.keep == n.len;
+    for (int i = tid; i < (all_stay ? n.keep : n.sinks); i += T) {
         store_index(a.kept, kept + i, i, c.idx64);
     }
-    int turn = 0;
-    for (int base = lo; base < hi && none == 0; base += T, turn ^= 1) {
-        const int j = base + tid;
-        const uint32_t k = j < hi ? keys[j] : 0u;
-        const bool above = j < hi && k > prefix, equal = j < hi && k == prefix;
-        const uint64_t m_above = __ballot(above), m_equal = __ballot(equal);
-        if (lane == 0) {
-            s_above[turn][wave] = static_cast<uint32_t>(__popcll(m_above));
-            s_equal[turn][wave] = static_cast<uint32_t>(__popcll(m_equal));
-        }
-        __syncthreads();
-        uint32_t a_before = 0, e_before = 0, a_all = 0, e_all = 0;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            a_before += w < wave ? s_above[turn][w] : 0u;
-            e_before += w < wave ? s_equal[turn][w] : 0u;
-            a_all += s_above[turn][w];
-            e_all += s_equal[turn][w];
-        }
-        const uint64_t below = (uint64_t{1} << lane) - 1;
-        const uint32_t a_rank = a_before + static_cast<uint32_t>(__popcll(m_above & below));
-        const uint32_t e_rank = n_equal + e_before + static_cast<uint32_t>(__popcll(m_equal & below));
-        const uint32_t e_kept = (e_rank < left ? e_rank : left) - (n_equal < left ? n_equal : left);  // equal rows of this turn that stay, before mine
-        if (above || (equal && e_rank < left)) {
-            store_index(a.kept, kept + n_kept + a_rank + e_kept, j, c.idx64);
-        }
-        const uint32_t e_after = n_equal + e_all;
-        n_kept += a_all + (e_after < left ? e_after : left) - (n_equal < left ? n_equal : left);
-        n_equal = e_after;
+    if (all_stay) {
+        return;
     }
     for (int i = tid; i < n.recent; i += T) {
         store_index(a.kept, kept + n.keep - n.recent + i, hi + i, c.idx64);
+    }
+    if (places == 0) {
+        return;
+    }
+    // scores of four rows at a time (of one block: lo is rounded down to a multiple of four, what lies ahead of it scores nothing)
+    const int first = lo & ~3, rows = (hi - first + 3) & ~3;
+    const bool in_lds = rows <= KEYS;
+    uint32_t* const far = a.keys + static_cast<int64_t>(b) * a.key_pitch;
+    const int64_t head_pitch = static_cast<int64_t>(c.blocks_per_page) * kFp8Block;
+    for (int r = 4 * tid; r < rows; r += 4 * T) {
+        const int j = first + r, lin = fp8_block(c, c.page_ids, seq.first, 0, j / kFp8Block);
+        f32x4_t score = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (lin >= 0) {
+            const float* const w = c.weights + static_cast<int64_t>(lin) * kFp8Block + (j & (kFp8Block - 1));
+            for (int h0 = 0; h0 < c.n_heads; h0 += 4) {  // (four heads on their way together)
+                f32x4_t v[4];
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    v[h] = *reinterpret_cast<const f32x4_t*>(w + (h0 + h < c.n_heads ? h0 + h : h0) * head_pitch);
+                }
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    if (h0 + h < c.n_heads) {
+                        score = h0 + h == 0 ? v[0] : score + v[h];
+                    }
+                }
+            }
+        }
+        u32x4_t k;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float s = score[i];
+            k[i] = score_key(s);
+        }
+        *reinterpret_cast<u32x4_t*>((in_lds ? s_keys : far) + r) = k;
+    }
+    const auto keys_of = [&](int r) { return *reinterpret_cast<const u32x4_t*>((in_lds ? s_keys : far) + r); };  // four, r a multiple of four
+    const auto competes = [&](int r) { return first + r >= lo && first + r < hi; };
+    __syncthreads();
+    uint32_t prefix = 0, left = static_cast<uint32_t>(places);  // of the rows whose top bits are `prefix`, `left` stay
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
+        for (int i = tid; i < BINS; i += T) {
+            s_hist[i] = 0;
+        }
+        __syncthreads();
+        for (int r = 4 * tid; r < rows; r += 4 * T) {
+            const u32x4_t four = keys_of(r);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t k = four[i];
+                if (competes(r + i) && (pass == 0 || (k >> (shift + bits)) == (prefix >> (shift + bits)))) {
+                    atomicAdd(&s_hist[(k >> shift) & ((1u << bits) - 1u)], 1u);
+                }
+            }
+        }
+        __syncthreads();
+        // thread t has OWN digits from BINS - 1 - OWN t down: counts from the top
+        uint32_t count[OWN], sum = 0, all;
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) {
+            count[i] = s_hist[BINS - 1 - OWN * tid - i];
+            sum += count[i];
+        }
+        uint32_t before = sum_before<WAVES>(sum, s_sum, all);
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) {
+            if (before < left && before + count[i] >= left) {  // (true for one digit of one thread)
+                s_pick[0] = static_cast<uint32_t>(BINS - 1 - OWN * tid - i);
+                s_pick[1] = left - before;
+            }
+            before += count[i];
+        }
+        __syncthreads();
+        prefix |= s_pick[0] << shift;
+        left = s_pick[1];
+    }
+    // rows above `prefix` stay, and the first `left` of those equal to it
+    const int stretch = ((rows + T - 1) / T + 3) & ~3, r0 = tid * stretch < rows ? tid * stretch : rows, r1 = r0 + stretch < rows ? r0 + stretch : rows;
+    uint32_t above = 0, equal = 0;
+    for (int r = r0; r < r1; r += 4) {
+        const u32x4_t four = keys_of(r);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            above += competes(r + i) && four[i] > prefix ? 1u : 0u;
+            equal += competes(r + i) && four[i] == prefix ? 1u : 0u;
+        }
+    }
+    uint32_t all;
+    uint32_t ties = sum_before<WAVES>(equal, s_sum, all);
+    uint32_t at = sum_before<WAVES>(above, s_sum, all) + (ties < left ? ties : left) + static_cast<uint32_t>(n.sinks);
+    for (int r = r0; r < r1; r += 4) {
+        const u32x4_t four = keys_of(r);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool tied = competes(r + i) && four[i] == prefix;
+            if (competes(r + i) && (four[i] > prefix || (tied && ties < left))) {
+                store_index(a.kept, kept + at++, first + r + i, c.idx64);
+            }
+            ties += tied ? 1u : 0u;
+        }
     }
 }
 
@@ -178,7 +221,6 @@ __global__ __launch_bounds__(kFp8AppendThreads) void hstu_paged_fp8_move_kernel(
 {
     constexpr int T = kFp8AppendThreads;
     constexpr int KP = kFp8Block * DS / 8 / T;
-    constexpr int VP = DS / T > 0 ? DS / T : 1;
     __shared__ uint32_t s_top[T / 64];
     __shared__ int s_block[kFp8Block];  // where a row of the new block comes from: the block's number, and its place in it
     __shared__ int s_slot[kFp8Block];
@@ -263,44 +305,45 @@ __global__ __launch_bounds__(kFp8AppendThreads) void hstu_paged_fp8_move_kernel(
             c.k_scale[lin] = fp8_scale_of(field);
         }
     } else {
+        // a lane has a row of the new block, and of its dims a quarter: a load takes a byte of 32 rows, which came from few blocks, for two
+        // dims, so that its lanes meet in few lines (two dims of 64 lanes' own, a row at a time: 64 lines a load, 106 us where this takes 55)
         uint8_t* const dst = c.v + lin * pitch;
-        const int pairs = dim >> 1;
-        float x[VP][2][16];
-        uint32_t top = 0;
+        const int quarter = dim >> 2, row = t & 31, d0 = (t >> 5) * quarter;
+        const int from = s_block[row];
+        const float scale = s_scale[row];
+        const uint8_t* const src = c.v + (from >= 0 ? from : 0) * pitch + d0 * kFp8Block + s_slot[row];
+        uint32_t byte[DS / 4];
 #pragma unroll
-        for (int u = 0; u < VP; ++u) {
-            const int m = t + u * T, half = m >= pairs ? 1 : 0, d = 2 * (m - half * pairs);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int row = 16 * half + i, from = m < 2 * pairs ? s_block[row] : -1;
-                x[u][0][i] = x[u][1][i] = 0.0f;
-                if (from >= 0) {
-                    const uint8_t* const src = c.v + from * pitch + d * kFp8Block + s_slot[row];
-                    const f32x2_t two = fp8_values2<false>(static_cast<uint32_t>(src[0]) | static_cast<uint32_t>(src[kFp8Block]) << 8);
-                    x[u][0][i] = two[0] * s_scale[row];
-                    x[u][1][i] = two[1] * s_scale[row];
-                }
-                const uint32_t m0 = finite_bits(x[u][0][i]), m1 = finite_bits(x[u][1][i]);
-                top = m0 > top ? m0 : top;
-                top = m1 > top ? m1 : top;
+        for (int i = 0; i < DS / 4; ++i) {
+            byte[i] = 0u;
+            if (from >= 0 && i < quarter) {
+                byte[i] = src[i * kFp8Block];
             }
+        }
+        uint32_t top = 0;
+        float x[DS / 4];
+#pragma unroll
+        for (int i = 0; i < DS / 4; ++i) {
+            const f32x2_t two = fp8_values2<false>(byte[i]);
+            x[i] = two[0] * scale;
+            const uint32_t m = finite_bits(x[i]);
+            top = m > top ? m : top;
         }
         const uint32_t field = fp8_scale_field(block_top<T / 64>(top, s_top));
         const float inverse = fp8_inverse_of(field);
 #pragma unroll
-        for (int u = 0; u < VP; ++u) {
-            const int m = t + u * T, half = m >= pairs ? 1 : 0, d = 2 * (m - half * pairs);
+        for (int i = 0; i < DS / 4; i += 4) {
+            // four dims of this row, and of the rows of four lanes one dim each
+            uint32_t mine = fp8_codes2<false>(x[i], x[i + 1], inverse, 0u);
+            mine = fp8_codes2<true>(x[i + 2], x[i + 3], inverse, mine);
+            uint32_t w = 0;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                u32x4_t w;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t codes = fp8_codes2<false>(x[u][e][4 * j], x[u][e][4 * j + 1], inverse, 0u);
-                    w[j] = fp8_codes2<true>(x[u][e][4 * j + 2], x[u][e][4 * j + 3], inverse, codes);
-                }
-                if (m < 2 * pairs) {
-                    *reinterpret_cast<u32x4_t*>(dst + (d + e) * kFp8Block + 16 * half) = w;
-                }
+            for (int l = 0; l < 4; ++l) {
+                const uint32_t theirs = static_cast<uint32_t>(__shfl(static_cast<int>(mine), (t & 60) + l, 64));
+                w |= (theirs >> (8 * (t & 3)) & 0xffu) << (8 * l);
+            }
+            if (i < quarter) {
+                *reinterpret_cast<uint32_t*>(dst + (d0 + i + (t & 3)) * kFp8Block + (row & ~3)) = w;
             }
         }
         if (t == 0) {

@@ -5,66 +5,72 @@
 
 namespace hstu {
 
-// Adds the parts of tiles whose keys were dealt to several workgroups, in their order.  Four values of a row per thread; a workgroup
-// per (256 of them, row tile, pair).
+// Adds the parts of tiles whose keys were dealt to several workgroups, in a fixed order.  Four values of a row per lane, a workgroup
+// for every gridDim.x-th so many of a (row tile, pair).  Where a value has many parts, which is where there are few values, the four
+// wavefronts take a quarter of the parts each.  Bound by the latency of two loads, the record that the attention kernel has left of a
+// tile's parts and the parts, so there are hardly more workgroups than run at once: 64 pairs of 8 tiles of 128 x 128, the half of them in
+// two parts, 11 us, and 22 in 8192 workgroups that found the parts for themselves; 128 pairs of one tile 6, and 9 in twice as many.
 template <typename Tag>
 __global__ __launch_bounds__(256) void hstu_paged_fp8_join_kernel(const Fp8AttendArgs a, int tile_rows)
 {
+    __shared__ f32x4_t s_sum[3][64];
     const Fp8Cache& c = a.c;
     const int pair = static_cast<int>(blockIdx.z), tile = static_cast<int>(blockIdx.y);
     const int b = uniform(pair / c.n_heads), g = pair - b * c.n_heads;
-    const bool by_length = c.n_batch <= 64;
-    Fp8DealLanes lanes = {a.chunk, 0, 0};
-    int all_parts = a.parts, rank = 0;
-    if (by_length) {
-        lanes = fp8_deal_lanes(a);
-        all_parts = __builtin_amdgcn_readlane(lanes.parts, b);
-        rank = __builtin_amdgcn_readlane(lanes.rank, b);
-    }
+    const int2 join = a.joins[pair * a.row_tiles + tile];
     const Fp8Item item = fp8_item(a, b);
     const int n_rows = item.n_rows * a.ratio;  // (row, head) pairs
-    const int m0 = tile * tile_rows, m1 = m0 + tile_rows < n_rows ? m0 + tile_rows : n_rows;
-    if (m0 >= m1 || all_parts == 1) {
-        return;
+    const int m0 = tile * tile_rows, m1 = m0 + tile_rows < n_rows ? m0 + tile_rows : n_rows, parts = uniform(join.x);
+    if (m0 >= m1 || parts <= 1) {
+        return;  // (no rows, of which nothing stands in joins, or the one part has written them)
     }
-    const int n_blocks = fp8_runs(item.mask, div_small(m0, a.ratio), div_small(m1 - 1, a.ratio) + 1).count();
-    int parts = uniform((n_blocks + lanes.chunk - 1) / lanes.chunk);
-    parts = parts < all_parts ? parts : all_parts;
-    if (parts <= 1) {
-        return;  // (the one part has written the rows)
-    }
-    const int dim = c.dim, pieces = dim >> 2, x = static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x);
-    const bool here = x < (m1 - m0) * pieces;  // (every lane takes part in finding the parts)
+    const int dim = c.dim, pieces = dim >> 2, n_pieces = (m1 - m0) * pieces;
+    const bool quarters = parts > 4;
+    const int wave = uniform(static_cast<int>(threadIdx.x) >> 6), lane = threadIdx.x & 63;
+    const int share = quarters ? (parts + 3) >> 2 : parts, first = quarters ? wave * share : 0;
+    const int last = first + share < parts ? first + share : parts;
+    const int step = quarters ? 64 : 256, mine = quarters ? lane : static_cast<int>(threadIdx.x);
     const int64_t tile_words = static_cast<int64_t>(tile_rows) * dim, pitch = static_cast<int64_t>(c.n_heads) * a.row_tiles * tile_words;
-    const float* const from = a.partial + (static_cast<int64_t>(g) * a.row_tiles + tile) * tile_words + (here ? 4 * x : 0);
-    f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    int before = 0;  // parts of all sequences ahead of the p-th ones
-    for (int p0 = 0; p0 < parts; p0 += 8) {
-        f32x4_t v[8];
+    const float* const tile_at = a.partial + uniform(join.y) * pitch + (static_cast<int64_t>(g) * a.row_tiles + tile) * tile_words;
+    for (int x0 = static_cast<int>(blockIdx.x) * step; x0 < n_pieces; x0 += static_cast<int>(gridDim.x) * step) {
+        const int x = x0 + mine;
+        const bool here = x < n_pieces;
+        const float* const from = tile_at + (here ? 4 * x : 0);
+        f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int p0 = first; p0 < last; p0 += 8) {
+            f32x4_t v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int p = p0 + i;
-            const int slot = by_length ? before + rank : b * a.parts + p;
-            before += by_length ? lanes.count(p) : 0;
-            v[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            if (p < parts) {
-                v[i] = *reinterpret_cast<const f32x4_t*>(from + slot * pitch);
+            for (int i = 0; i < 8; ++i) {
+                const int p = p0 + i;
+                v[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+                if (p < last) {
+                    v[i] = *reinterpret_cast<const f32x4_t*>(from + p * pitch);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                sum += v[i];
             }
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            sum += v[i];
+        if (quarters) {
+            __syncthreads();  // (read by the first wavefront in the turn before)
+            if (wave > 0) {
+                s_sum[wave - 1][lane] = sum;
+            }
+            __syncthreads();
+            if (wave == 0) {
+                sum = ((sum + s_sum[0][lane]) + s_sum[1][lane]) + s_sum[2][lane];
+            }
+        }
+        if (here && (wave == 0 || !quarters)) {
+            const int r = div_small(x, pieces), d = 4 * (x - r * pieces), m = m0 + r, i = div_small(m, a.ratio);
+            const int64_t at = ((item.q0 + i) * a.n_heads_q + g * a.ratio + (m - i * a.ratio)) * static_cast<int64_t>(dim) + d;
+            u32x2_t w;
+            w[0] = pack2<Tag>(sum[0] * a.c_out, sum[1] * a.c_out);
+            w[1] = pack2<Tag>(sum[2] * a.c_out, sum[3] * a.c_out);
+            *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(a.out) + at) = w;
         }
     }
-    if (!here) {
-        return;
-    }
-    const int r = div_small(x, pieces), d = 4 * (x - r * pieces), m = m0 + r, i = div_small(m, a.ratio);
-    const int64_t at = ((item.q0 + i) * a.n_heads_q + g * a.ratio + (m - i * a.ratio)) * static_cast<int64_t>(dim) + d;
-    u32x2_t w;
-    w[0] = pack2<Tag>(sum[0] * a.c_out, sum[1] * a.c_out);
-    w[1] = pack2<Tag>(sum[2] * a.c_out, sum[3] * a.c_out);
-    *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(a.out) + at) = w;
 }
 
 // Adds the sums of |P| of several row tiles to the weights, in the order of the tiles.  A workgroup per (eight blocks, pair); a tile

@@ -52,8 +52,8 @@ int check_cache(const hstu_paged_fp8_cache& c)
     if (c.num_pages * c.num_heads_k * (c.page_size / kBlock) > INT32_MAX) {
         return set_error(HSTU_ERR_INVALID, "the cache has more than 2^31 - 1 blocks of %d tokens and head", kBlock);
     }
-    if (!aligned16(c.k_cache) || !aligned16(c.v_cache)) {
-        return set_error(HSTU_ERR_INVALID, "k_cache and v_cache must be 16-byte aligned");
+    if (!aligned16(c.k_cache) || !aligned16(c.v_cache) || !aligned16(c.weights)) {
+        return set_error(HSTU_ERR_INVALID, "k_cache, v_cache and weights must be 16-byte aligned");
     }
     return HSTU_OK;
 }
@@ -135,8 +135,9 @@ struct Plan {
     const Fp8AttendVariant* v;
     Fp8AttendArgs a;
     int64_t slots;
-    uint64_t partial_bytes, weight_bytes;
+    uint64_t partial_bytes, join_bytes, weight_bytes;
     bool split;  // some sequence may have more than one part
+    uint64_t bytes() const { return partial_bytes + join_bytes + weight_bytes; }
 };
 
 // Which variant, and how the keys of a tile are dealt to workgroups.
@@ -163,6 +164,7 @@ Plan plan(const hstu_paged_fp8_fwd_params* p)
     a.num_target = p->num_target;
     a.out = p->out;
     a.partial = nullptr;
+    a.joins = nullptr;
     a.weight_partial = nullptr;
     a.total_q = p->total_q;
     a.n_heads_q = static_cast<int>(p->num_heads_q);
@@ -207,6 +209,7 @@ Plan plan(const hstu_paged_fp8_fwd_params* p)
     }
     r.split = a.chunk < a.most_blocks;
     r.partial_bytes = r.split ? static_cast<uint64_t>(a.total_parts) * per_part * r.v->tile_rows * p->cache.head_dim * 4 : 0;
+    r.join_bytes = r.split ? static_cast<uint64_t>(ceil_div(pairs * a.row_tiles, 2)) * 16 : 0;
     const int64_t wave_tiles = static_cast<int64_t>(a.row_tiles) * (r.v->tile_rows / r.v->wave_rows);
     r.weight_bytes = weights && wave_tiles > 1 ? static_cast<uint64_t>(pairs) * wave_tiles * a.max_blocks * kBlock * 4 : 0;
     const int64_t units = (a.total_parts > 0 ? a.total_parts : batch) * p->cache.num_heads_k;
@@ -217,11 +220,18 @@ Plan plan(const hstu_paged_fp8_fwd_params* p)
 // ---------------------------------------------------------------------------------------------------------- append ----
 
 using AppendKernel = void (*)(const Fp8AppendArgs);
-// by type and head dims up to 64, 128, 256: what a lane holds
-const AppendKernel kAppend[2][3] = {
-    {hstu_paged_fp8_append_kernel<bf16_tag, 64>, hstu_paged_fp8_append_kernel<bf16_tag, 128>, hstu_paged_fp8_append_kernel<bf16_tag, 256>},
-    {hstu_paged_fp8_append_kernel<f16_tag, 64>, hstu_paged_fp8_append_kernel<f16_tag, 128>, hstu_paged_fp8_append_kernel<f16_tag, 256>},
-};
+template <typename Tag, bool TURNS>
+constexpr AppendKernel append_by_dim(int slot)
+{
+    return slot == 0 ? hstu_paged_fp8_append_kernel<Tag, 64, TURNS>
+                     : (slot == 1 ? hstu_paged_fp8_append_kernel<Tag, 128, TURNS> : hstu_paged_fp8_append_kernel<Tag, 256, TURNS>);
+}
+// head dims up to 64, 128, 256: what a lane holds
+AppendKernel append_kernel(bool bf16, bool turns, int slot)
+{
+    return bf16 ? (turns ? append_by_dim<bf16_tag, true>(slot) : append_by_dim<bf16_tag, false>(slot))
+                : (turns ? append_by_dim<f16_tag, true>(slot) : append_by_dim<f16_tag, false>(slot));
+}
 int dim_slot(int64_t dim) { return dim <= 64 ? 0 : (dim <= 128 ? 1 : 2); }
 
 bool bad_stride(int64_t s) { return s < 0 || s % 8 != 0; }
@@ -229,6 +239,7 @@ bool bad_stride(int64_t s) { return s < 0 || s % 8 != 0; }
 // ---------------------------------------------------------------------------------------------------------- evict ----
 
 using EvictKernel = void (*)(const Fp8EvictArgs);
+const EvictKernel kSelect = hstu_paged_fp8_select_kernel<1024, kFp8SelectKeys>, kSelectFew = hstu_paged_fp8_select_kernel<256, kFp8SelectFew + 8>;
 const EvictKernel kMove[3] = {hstu_paged_fp8_move_kernel<64>, hstu_paged_fp8_move_kernel<128>, hstu_paged_fp8_move_kernel<256>};
 
 int check_evict(const hstu_paged_fp8_evict_params* p)
@@ -264,7 +275,9 @@ int check_evict(const hstu_paged_fp8_evict_params* p)
     return HSTU_OK;
 }
 
-uint64_t evict_workspace(const hstu_paged_fp8_evict_params* p) { return static_cast<uint64_t>(p->cache.n_offsets - 1) * p->max_seq_len_k * 4; }
+// scores of the longest sequence allowed, in whole fours and where its first may be rounded down; none where LDS holds them
+int64_t evict_pitch(const hstu_paged_fp8_evict_params* p) { return p->max_seq_len_k + 8 <= kFp8SelectKeys ? 0 : ceil_div(p->max_seq_len_k, 4) * 4 + 8; }
+uint64_t evict_workspace(const hstu_paged_fp8_evict_params* p) { return static_cast<uint64_t>(p->cache.n_offsets - 1) * evict_pitch(p) * 4; }
 
 }  // namespace
 
@@ -280,7 +293,7 @@ HSTU_API int hstu_paged_fp8_fwd_workspace_size(const hstu_paged_fp8_fwd_params* 
         return set_error(HSTU_ERR_NULLPTR, "workspace_bytes is NULL");
     }
     const Plan r = plan(p);
-    *bytes = r.partial_bytes + r.weight_bytes;
+    *bytes = r.bytes();
     return HSTU_OK;
 }
 
@@ -300,24 +313,27 @@ HSTU_API int hstu_paged_fp8_fwd(const hstu_paged_fp8_fwd_params* p, void* worksp
     if (r.slots > INT32_MAX) {
         return set_error(HSTU_ERR_INVALID, "the call has more tiles than a launch can hold");
     }
-    if (r.partial_bytes + r.weight_bytes > 0) {
-        if (workspace == nullptr || workspace_bytes < r.partial_bytes + r.weight_bytes) {
+    if (r.bytes() > 0) {
+        if (workspace == nullptr || workspace_bytes < r.bytes()) {
             return set_error(HSTU_ERR_WORKSPACE, "workspace of %llu bytes, %llu are needed", (unsigned long long)(workspace ? workspace_bytes : 0),
-                             (unsigned long long)(r.partial_bytes + r.weight_bytes));
+                             (unsigned long long)r.bytes());
         }
         if (!aligned16(workspace)) {
             return set_error(HSTU_ERR_INVALID, "workspace must be 16-byte aligned");
         }
         a.partial = r.partial_bytes > 0 ? static_cast<float*>(workspace) : nullptr;
-        a.weight_partial = r.weight_bytes > 0 ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + r.partial_bytes) : nullptr;
+        uint8_t* const joins = static_cast<uint8_t*>(workspace) + r.partial_bytes;
+        a.joins = r.join_bytes > 0 ? reinterpret_cast<int2*>(joins) : nullptr;
+        a.weight_partial = r.weight_bytes > 0 ? reinterpret_cast<float*>(joins + r.join_bytes) : nullptr;
     }
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const unsigned pairs = static_cast<unsigned>(a.c.n_batch) * a.c.n_heads;
     hipLaunchKernelGGL(r.v->kernel, dim3(static_cast<unsigned>(r.slots)), dim3(r.v->threads), 0, s, a);
     if (r.split) {
         const auto join = p->dtype == HSTU_DT_BF16 ? hstu_paged_fp8_join_kernel<bf16_tag> : hstu_paged_fp8_join_kernel<f16_tag>;
-        hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(ceil_div(static_cast<int64_t>(r.v->tile_rows) * a.c.dim, 1024)), a.row_tiles, pairs), dim3(256), 0, s, a,
-                           r.v->tile_rows);
+        const int64_t most = ceil_div(static_cast<int64_t>(r.v->tile_rows) * a.c.dim, 256),
+                      enough = ceil_div(kFp8JoinEnough, static_cast<int64_t>(a.row_tiles) * pairs);
+        hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(std::min(most, enough)), a.row_tiles, pairs), dim3(256), 0, s, a, r.v->tile_rows);
     }
     if (a.weight_partial != nullptr) {
         const int tiles = a.row_tiles * (r.v->tile_rows / r.v->wave_rows);
@@ -367,10 +383,14 @@ HSTU_API int hstu_paged_fp8_append(const hstu_paged_fp8_append_params* p, void* 
     a.v_head = p->v_stride_head;
     const int64_t most = std::min(p->max_seq_len, p->total);
     a.max_rows = static_cast<int>(most);
-    // n rows that begin anywhere in a block touch at most so many
-    const int64_t blocks = (most + 2 * kBlock - 2) / kBlock;
-    hipLaunchKernelGGL(kAppend[p->dtype == HSTU_DT_BF16 ? 0 : 1][dim_slot(a.c.dim)],
-                       dim3(static_cast<unsigned>(blocks), 2u * static_cast<unsigned>(a.c.n_heads), static_cast<unsigned>(a.c.n_batch)),
+    // n rows that begin anywhere in a block touch at most so many.  Where that leaves enough workgroups, one takes several blocks in turn
+    // (64512 of f16 rows, 8 key heads, 128 dims, of 32 ragged sequences: 116 us in workgroups of one, 109, 105 and 110 of two to four, 121 of twelve),
+    // and their number along a sequence is odd: workgroups go to the eight dies in turn, and by an even number the last ones of all the
+    // sequences, which the short ones do not need, would fall to the same dies (of four: 158 us)
+    const int64_t blocks = (most + 2 * kBlock - 2) / kBlock, all = blocks * 2 * a.c.n_heads * a.c.n_batch;
+    a.in_turn = static_cast<int>(std::min<int64_t>(std::max<int64_t>(all / kFp8AppendEnough, 1), 3));
+    hipLaunchKernelGGL(append_kernel(p->dtype == HSTU_DT_BF16, a.in_turn > 1, dim_slot(a.c.dim)),
+                       dim3(static_cast<unsigned>(ceil_div(blocks, a.in_turn) | 1), 2u * static_cast<unsigned>(a.c.n_heads), static_cast<unsigned>(a.c.n_batch)),
                        dim3(kFp8AppendThreads), 0, static_cast<hipStream_t>(stream), a);
     return launched("hstu_paged_fp8_append_kernel");
 }
@@ -394,7 +414,7 @@ HSTU_API int hstu_paged_fp8_evict(const hstu_paged_fp8_evict_params* p, void* wo
     if (rc != HSTU_OK) {
         return rc;
     }
-    if (workspace == nullptr || workspace_bytes < evict_workspace(p)) {
+    if (evict_workspace(p) > 0 && (workspace == nullptr || workspace_bytes < evict_workspace(p))) {
         return set_error(HSTU_ERR_WORKSPACE, "workspace of %llu bytes, %llu are needed", (unsigned long long)(workspace ? workspace_bytes : 0),
                          (unsigned long long)evict_workspace(p));
     }
@@ -404,14 +424,20 @@ HSTU_API int hstu_paged_fp8_evict(const hstu_paged_fp8_evict_params* p, void* wo
     a.new_page_ids = p->new_page_ids;
     a.new_len = p->new_cache_len;
     a.kept = p->kept;
+    if (evict_workspace(p) > 0 && !aligned16(workspace)) {
+        return set_error(HSTU_ERR_INVALID, "workspace must be 16-byte aligned");
+    }
     a.keys = static_cast<uint32_t*>(workspace);
+    a.key_pitch = evict_pitch(p);
     a.n_new_page_ids = static_cast<int>(p->n_new_page_ids);
     a.max_k = static_cast<int>(p->max_seq_len_k);
     a.keep = static_cast<int>(p->keep);
     a.sinks = static_cast<int>(std::min<int64_t>(p->sinks, p->keep));
     a.recent = static_cast<int>(std::min<int64_t>(p->recent, p->keep));
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(hstu_paged_fp8_select_kernel, dim3(static_cast<unsigned>(a.c.n_batch)), dim3(kFp8SelectThreads), 0, s, a);
+    const bool few = a.max_k <= kFp8SelectFew;
+    const EvictKernel select = few ? kSelectFew : kSelect;
+    hipLaunchKernelGGL(select, dim3(static_cast<unsigned>(a.c.n_batch)), dim3(few ? 256 : 1024), 0, s, a);
     const int64_t most = std::min(p->keep, p->max_seq_len_k);
     hipLaunchKernelGGL(kMove[dim_slot(a.c.dim)],
                        dim3(static_cast<unsigned>(ceil_div(most, kBlock)), 2u * static_cast<unsigned>(a.c.n_heads), static_cast<unsigned>(a.c.n_batch)),

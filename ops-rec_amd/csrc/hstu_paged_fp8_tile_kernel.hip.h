@@ -63,6 +63,9 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(NC
     if (part > 0 && part >= parts_used) {
         return;
     }
+    if (part == 0 && a.joins != nullptr && threadIdx.x == 0) {
+        a.joins[pair * a.row_tiles + tile] = int2{parts_used < deal.parts ? parts_used : deal.parts, deal.slot};
+    }
     const int n_begin = deal.parts == 1 ? 0 : part * deal.chunk;
     const int n_end = part == deal.parts - 1 || n_blocks - n_begin < deal.chunk ? n_blocks : n_begin + deal.chunk;
     const int m0 = t0 + 32 * rg;

@@ -533,7 +533,7 @@ std::tuple<Tensor, Tensor> paged_fp8_evict(const Tensor& k_cache, const Tensor& 
         p.recent = recent;
         uint64_t ws_bytes = 0;
         if (hstu_paged_fp8_evict_workspace_size(&p, &ws_bytes) == HSTU_OK) {
-            const Tensor ws = empty({static_cast<int64_t>(ws_bytes)}, at::kByte, k_cache.device());
+            const Tensor ws = ws_bytes != 0 ? empty({static_cast<int64_t>(ws_bytes)}, at::kByte, k_cache.device()) : Tensor();
             const int rc = hstu_paged_fp8_evict(&p, ptr(ws), ws_bytes, stream_of(k_cache));
             TORCH_CHECK(rc == HSTU_OK, "hstu_paged_fp8_evict failed (", rc, "): ", hstu_last_error());
             return {new_len, kept};
