@@ -329,31 +329,28 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(NC
     for (int n = 0; n < NC; ++n) {
         float* const s = reinterpret_cast<float*>(s_mem) + (n & 1) * (SUMS / 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4; ++i) {  // (16 bytes at a time, their places exchanged so that neither side has bank conflicts)
             const f32x4_t x = {acc[n][4 * i], acc[n][4 * i + 1], acc[n][4 * i + 2], acc[n][4 * i + 3]};
-            *reinterpret_cast<f32x4_t*>(s + wave * 1024 + i * 256 + lane * 4) = x;
+            *reinterpret_cast<f32x4_t*>(s + wave * 1024 + 4 * (i * 64 + (lane ^ (2 * i + 8 * half)))) = x;
         }
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < RG * 512 / T; ++r) {  // (two values per thread and turn)
-            const int word = 2 * (tid + r * T);
-            float x0 = 0.0f, x1 = 0.0f;
+        for (int r = 0; r < 4 / KG; ++r) {  // four dims per lane, eight lanes together the 32 of a row
+            const int word = tid + r * T, i = word & 3, h = (word >> 2) & 1, row_in = word >> 3;
+            const float* const from = s + (row_in >> 5) * 1024 + 4 * (i * 64 + ((32 * h + (row_in & 31)) ^ (2 * i + 8 * h)));
+            f32x4_t x = *reinterpret_cast<const f32x4_t*>(from);
 #pragma unroll
-            for (int k = 0; k < KG; ++k) {
-                x0 += s[k * RG * 1024 + word];
-                x1 += s[k * RG * 1024 + word + 1];
+            for (int k = 1; k < KG; ++k) {
+                x += *reinterpret_cast<const f32x4_t*>(from + k * RG * 1024);
             }
-            const int i = ((word >> 8) & 3) * 4 + (word & 3), from = (word >> 2) & 63;
-            const int row = t0 + 32 * (word >> 10) + (from & 31), d = 32 * n + 16 * (from >> 5) + i;
+            const int row = t0 + row_in, d = 32 * n + 16 * h + 4 * i;
             if (row < n_rows && d < dim) {
                 if (partial) {
-                    float* const to = to_partial + static_cast<int64_t>(row - t0) * dim + d;
-                    to[0] = x0;
-                    to[1] = x1;
+                    *reinterpret_cast<f32x4_t*>(to_partial + static_cast<int64_t>(row_in) * dim + d) = x;
                 } else {
                     const int ir = div_small(row, a.ratio);
                     const int64_t at = ((item.q0 + ir) * a.n_heads_q + g * a.ratio + (row - ir * a.ratio)) * static_cast<int64_t>(dim) + d;
-                    *reinterpret_cast<uint32_t*>(out + at) = pack2<Tag>(x0 * a.c_out, x1 * a.c_out);
+                    *reinterpret_cast<u32x2_t*>(out + at) = u32x2_t{pack2<Tag>(x[0] * a.c_out, x[1] * a.c_out), pack2<Tag>(x[2] * a.c_out, x[3] * a.c_out)};
                 }
             }
         }
