@@ -179,7 +179,7 @@ __device__ __forceinline__ Fp8Item fp8_item(const Fp8AttendArgs& a, int b)
 // many blocks each, `chunk`, whatever the sequence: with up to 64 sequences, a lane of a wavefront for each, the lengths are
 // looked at, and the chunk is what makes total_parts of them all -- sum ceil(blocks / chunk) is at most sum blocks / chunk + the
 // number of sequences.  (Cut alike by the longest length allowed, parts of short sequences have nothing to do: 3 x 2 key heads
-// of 30011 .. 120011 keys, d 256, 70 us in such parts, 47 in these.)  First come the first parts of all sequences, the longest first,
+// of 30011 .. 120011 keys, d 256, 70 us in such parts, 48 in these.)  First come the first parts of all sequences, the longest first,
 // then their second parts, and so on: what starts late is short.
 struct Fp8Deal {
     int b;      // the sequence; -1: none
@@ -361,15 +361,14 @@ __device__ __forceinline__ void fp8_poison(f32x16_t (&acc)[NC], const Fp8Cache& 
 
 // Tag     : type of q and out
 // NC      : groups of 32 dims (dim is at most 32 NC, a multiple of 16)
-// NB      : columns of 32 rows of a wavefront
 // WK, WR  : wavefronts of a workgroup over the keys of a row tile, and over row tiles
 // WEIGHTS : the sums of |P| per key as well
-template <typename Tag, int NC, int NB, int WK, int WR, bool WEIGHTS>
+template <typename Tag, int NC, int WK, int WR, bool WEIGHTS>
 __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(const Fp8AttendArgs a)
 {
-    constexpr int ROWS = 32 * NB;        // (row, head) pairs of a wavefront
-    constexpr int TILE = ROWS * WR;      // and of a workgroup
-    constexpr int CHUNK_WORDS = NB * 64 * 16;
+    constexpr int ROWS = 32;         // (row, head) pairs of a wavefront
+    constexpr int TILE = ROWS * WR;  // and of a workgroup
+    constexpr int CHUNK_WORDS = 64 * 16;
     __shared__ __attribute__((aligned(16))) float s_sum[WK > 1 ? 2 : 1][WK > 1 ? WK * CHUNK_WORDS : 4];
 
     const Fp8Cache& c = a.c;
@@ -419,27 +418,20 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
     const int n_end = part == deal.parts - 1 || n_blocks - n_begin < deal.chunk ? n_blocks : n_begin + deal.chunk;
 
     // q: the rows of this wavefront, 16 dims of this lane's half per group of 32
-    u32x4_t q[NB][NC][2];
-    int lim[NB], hole[NB], low[NB];
+    u32x4_t q[NC][2];
+    const int m = m0 + col, i_row = div_small(m < n_pairs_rows ? m : 0, a.ratio);
+    const int lim = m < n_pairs_rows ? mask.lim(i_row) : 0, hole = mask.hole(i_row), low = mask.low(i_row);
     {
         const uint32_t bytes = static_cast<uint32_t>(n_rows) * static_cast<uint32_t>(a.n_heads_q) * dim * 2u;
         const __amdgpu_buffer_rsrc_t rsrc =
             make_rsrc(static_cast<const uint16_t*>(a.q) + q0 * a.n_heads_q * static_cast<int64_t>(dim), bytes);
+        const uint32_t at = (static_cast<uint32_t>(i_row) * a.n_heads_q + g * a.ratio + (m - i_row * a.ratio)) * dim * 2u;
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            const int m = m0 + nb * 32 + col, i = div_small(m < n_pairs_rows ? m : 0, a.ratio);
-            const bool there = m < n_pairs_rows;
-            const uint32_t at = (static_cast<uint32_t>(i) * a.n_heads_q + g * a.ratio + (m - i * a.ratio)) * dim * 2u;
-            lim[nb] = there ? mask.lim(i) : 0;
-            hole[nb] = mask.hole(i);
-            low[nb] = mask.low(i);
+        for (int n = 0; n < NC; ++n) {
 #pragma unroll
-            for (int n = 0; n < NC; ++n) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int d = 32 * n + 16 * half + 8 * u;
-                    q[nb][n][u] = load_codes(rsrc, there && d < dim ? at + d * 2u : kOutOfRange);
-                }
+            for (int u = 0; u < 2; ++u) {
+                const int d = 32 * n + 16 * half + 8 * u;
+                q[n][u] = load_codes(rsrc, m < n_pairs_rows && d < dim ? at + d * 2u : kOutOfRange);
             }
         }
     }
@@ -455,13 +447,10 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
         v_at[n] = 32 * n + pi < dim ? static_cast<uint32_t>(32 * n + pi) * kFp8Block + 16 * half : kOutOfRange;
     }
 
-    f32x16_t acc[NB][NC];
+    f32x16_t acc[NC];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            acc[nb][n] = f32x16_t{0.0f};
-        }
+    for (int n = 0; n < NC; ++n) {
+        acc[n] = f32x16_t{0.0f};
     }
 
     const Fp8Whole whole_blocks = fp8_whole(mask, i_first, i_last);  // these need no mask
@@ -497,57 +486,40 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
             st.v[n] = load_codes(vr, v_at[n]);
         }
     };
-    const auto sees_key = [&](int j, int nb) {  // whether this lane's row of column nb sees key j
-        return static_cast<bool>((j < lim[nb]) & ((j < mask.first_key) | (j >= hole[nb])) & ((j >= low[nb]) | (j < mask.sinks)));
+    const auto sees_key = [&](int j) {  // whether this lane's row sees key j
+        return static_cast<bool>((j < lim) & ((j < mask.first_key) | (j >= hole)) & ((j >= low) | (j < mask.sinks)));
     };
     bool poisoned = false;
     const auto step = [&](Stage& st, int s, float ks, float vs) {
         const int lin = place_of(s);
         const int blk = runs.block(n_begin + wk + s * WK), c0 = blk * kFp8Block;
-        f32x16_t sc[NB];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            sc[nb] = f32x16_t{0.0f};
-        }
+        f32x16_t sc = f32x16_t{0.0f};
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
             const Fp8Pair kk = fp8_widen<Tag>(st.k[n], ks);
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                sc[nb] = mfma32<Tag>(kk.lo, q[nb][n][0], sc[nb]);
-                sc[nb] = mfma32<Tag>(kk.hi, q[nb][n][1], sc[nb]);
-            }
+            sc = mfma32<Tag>(kk.lo, q[n][0], sc);
+            sc = mfma32<Tag>(kk.hi, q[n][1], sc);
         }
         const int end = c0 + kFp8Block;
         const bool whole = whole_blocks.has(blk);
-        u32x4_t p[NB][2];
-        float sums[16];
+        u32x4_t p[2];
+        float w[16];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            float w[16];
+        for (int i = 0; i < 16; ++i) {
+            const float x = sc[i];
+            w[i] = x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * a.c_exp));
+        }
+        if (!whole) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float x = sc[nb][i];
-                w[i] = x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * a.c_exp));
+                w[i] = sees_key(c0 + 16 * half + i) ? w[i] : 0.0f;
             }
-            if (!whole) {
+        }
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    w[i] = sees_key(c0 + 16 * half + i, nb) ? w[i] : 0.0f;
-                }
-            }
-            if constexpr (WEIGHTS) {
+        for (int u = 0; u < 2; ++u) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    sums[i] = nb == 0 ? __builtin_fabsf(w[i]) : sums[i] + __builtin_fabsf(w[i]);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    p[nb][u][i] = pack2<Tag>(w[8 * u + 2 * i], w[8 * u + 2 * i + 1]);
-                }
+            for (int i = 0; i < 4; ++i) {
+                p[u][i] = pack2<Tag>(w[8 * u + 2 * i], w[8 * u + 2 * i + 1]);
             }
         }
         if (end > seq.len) {  // codes behind the last row may be anything, NaN among them: zero times that is not zero
@@ -580,14 +552,15 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
             const Fp8Pair vv = fp8_widen<Tag>(st.v[n], vs);
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                acc[nb][n] = mfma32<Tag>(vv.lo, p[nb][0], acc[nb][n]);
-                acc[nb][n] = mfma32<Tag>(vv.hi, p[nb][1], acc[nb][n]);
-            }
+            acc[n] = mfma32<Tag>(vv.lo, p[0], acc[n]);
+            acc[n] = mfma32<Tag>(vv.hi, p[1], acc[n]);
         }
         if (WEIGHTS && m0 < m1) {
-            const float all = fp8_key_sum(sums, lane) * __builtin_fabsf(a.c_out);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                w[i] = __builtin_fabsf(w[i]);
+            }
+            const float all = fp8_key_sum(w, lane) * __builtin_fabsf(a.c_out);
             fp8_store_key_sum(a, all, lane, pair, tile * WR + wr, a.row_tiles * WR, blk, lin);
         }
     };
@@ -621,11 +594,7 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
                 continue;
             }
             const int lin = uniform(fp8_block(c, c.page_ids, seq.first, g, blk));
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                const auto sees = [&](int j) { return sees_key(j, nb); };
-                fp8_poison<Tag, NC>(acc[nb], c, lin, v_at, blk * kFp8Block + 16 * half, seq.len, sees);
-            }
+            fp8_poison<Tag, NC>(acc, c, lin, v_at, blk * kFp8Block + 16 * half, seq.len, sees_key);
         }
     }
 
@@ -641,64 +610,47 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
         for (int n = 0; n < NC; ++n) {
             float* const s = s_sum[n & 1];
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const f32x4_t x = {acc[nb][n][4 * i], acc[nb][n][4 * i + 1], acc[nb][n][4 * i + 2], acc[nb][n][4 * i + 3]};
-                    *reinterpret_cast<f32x4_t*>(s + wk * CHUNK_WORDS + (nb * 4 + i) * 256 + lane * 4) = x;
-                }
+            for (int i = 0; i < 4; ++i) {  // (16 bytes at a time, their places exchanged so that neither side has bank conflicts)
+                const f32x4_t x = {acc[n][4 * i], acc[n][4 * i + 1], acc[n][4 * i + 2], acc[n][4 * i + 3]};
+                *reinterpret_cast<f32x4_t*>(s + wk * CHUNK_WORDS + 4 * (i * 64 + (lane ^ (2 * i + 8 * half)))) = x;
             }
             __syncthreads();
-            constexpr int T = 64 * WK;
-            static_assert(CHUNK_WORDS % (2 * T) == 0, "every lane has whole pairs to add");
-#pragma unroll
-            for (int r = 0; r < CHUNK_WORDS / (2 * T); ++r) {
-                const int word = 2 * (tid + r * T);
-                float x0 = 0.0f, x1 = 0.0f;
+            // four dims per lane, eight lanes together the 32 of a row
+            const int i = tid & 3, h = (tid >> 2) & 1, row = tid >> 3, mr = m0 + row, d = 32 * n + 16 * h + 4 * i;
+            if (tid < CHUNK_WORDS / 4 && mr < n_pairs_rows && d < dim) {
+                f32x4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int w = 0; w < WK; ++w) {
-                    x0 += s[w * CHUNK_WORDS + word];
-                    x1 += s[w * CHUNK_WORDS + word + 1];
+                    x += *reinterpret_cast<const f32x4_t*>(s + w * CHUNK_WORDS + 4 * (i * 64 + ((32 * h + row) ^ (2 * i + 8 * h))));
                 }
-                const int nb = word >> 10, i = ((word >> 8) & 3) * 4 + (word & 3), from = (word >> 2) & 63;
-                const int m = m0 + nb * 32 + (from & 31), d = 32 * n + 16 * (from >> 5) + i;
-                if (m < n_pairs_rows && d < dim) {
-                    if (partial) {
-                        float* const to = to_partial + static_cast<int64_t>(m - tile * TILE) * dim + d;
-                        to[0] = x0;
-                        to[1] = x1;
-                    } else {
-                        *reinterpret_cast<uint32_t*>(out + row_at(m) + d) = pack2<Tag>(x0 * a.c_out, x1 * a.c_out);
-                    }
+                if (partial) {
+                    *reinterpret_cast<f32x4_t*>(to_partial + static_cast<int64_t>(mr - tile * TILE) * dim + d) = x;
+                } else {
+                    *reinterpret_cast<u32x2_t*>(out + row_at(mr) + d) = u32x2_t{pack2<Tag>(x[0] * a.c_out, x[1] * a.c_out), pack2<Tag>(x[2] * a.c_out, x[3] * a.c_out)};
                 }
             }
         }
-    } else {
+        static_assert(64 * WK * 4 >= CHUNK_WORDS, "a lane for every four values");
+    } else if (m < n_pairs_rows) {
+        const int64_t at = row_at(m);
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            const int m = m0 + nb * 32 + col;
-            if (m < n_pairs_rows) {
-                const int64_t at = row_at(m);
+        for (int n = 0; n < NC; ++n) {
+            const int d = 32 * n + 16 * half;
+            if (d < dim) {
+                if (partial) {
+                    f32x4_t* const to = reinterpret_cast<f32x4_t*>(to_partial + static_cast<int64_t>(m - tile * TILE) * dim + d);
 #pragma unroll
-                for (int n = 0; n < NC; ++n) {
-                    const int d = 32 * n + 16 * half;
-                    if (d < dim) {
-                        if (partial) {
-                            f32x4_t* const to = reinterpret_cast<f32x4_t*>(to_partial + static_cast<int64_t>(m - tile * TILE) * dim + d);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                to[i] = f32x4_t{acc[nb][n][4 * i], acc[nb][n][4 * i + 1], acc[nb][n][4 * i + 2], acc[nb][n][4 * i + 3]};
-                            }
-                        } else {
-                            u32x4_t x[2];
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                x[i >> 2][i & 3] = pack2<Tag>(acc[nb][n][2 * i] * a.c_out, acc[nb][n][2 * i + 1] * a.c_out);
-                            }
-                            *reinterpret_cast<u32x4_t*>(out + at + d) = x[0];
-                            *reinterpret_cast<u32x4_t*>(out + at + d + 8) = x[1];
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        to[i] = f32x4_t{acc[n][4 * i], acc[n][4 * i + 1], acc[n][4 * i + 2], acc[n][4 * i + 3]};
                     }
+                } else {
+                    u32x4_t x[2];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        x[i >> 2][i & 3] = pack2<Tag>(acc[n][2 * i] * a.c_out, acc[n][2 * i + 1] * a.c_out);
+                    }
+                    *reinterpret_cast<u32x4_t*>(out + at + d) = x[0];
+                    *reinterpret_cast<u32x4_t*>(out + at + d + 8) = x[1];
                 }
             }
         }

@@ -151,10 +151,12 @@ Plan plan(const hstu_paged_fp8_fwd_params* p)
         ++groups;
     }
     const Fp8AttendTable& table = p->dtype == HSTU_DT_BF16 ? kFp8AttendBf16 : kFp8AttendF16;
-    // Up to 32 rows a wavefront of its own takes whatever keys it can get; up to 64 two share the conversion of codes; more rows go in
-    // tiles of 128 where those fill the machine's places for them, else of 64, whose keys go to two shares of a workgroup (24 x 4
-    // pairs, 100 .. 260 rows in a window of 1024: 42 us, 57 in tiles of 128; 16 x 4 pairs of 1024 rows on 2048 .. 8192 keys 301 and 265).
-    const int shape = rows <= 32 ? kFp8Keys : (rows <= 64 || pairs * ceil_div(rows, 128) < 512 ? kFp8KeysWide : kFp8Rows);
+    // A workgroup's wavefronts share the keys of a tile of 32 rows, each converting what it reads, unless there are enough rows that tiles
+    // of 128, whose wavefronts share the conversion, fill the machine: 8 x 4 key heads of 512 rows on 2048 .. 8192 keys 85 us and 99 in
+    // tiles of 64 of two shares of the keys, 16 x 4 of 1024 278 and 257; 64 x 4 of 64 rows 100 and 142.  Up to 64 dims, where a conversion
+    // costs half as much, later: 24 x 4 of 512 rows, d 64, 113 and 142, 64 x 4 on 500 .. 1500 keys 77 and 72.
+    const bool narrow = groups < 2, wide = groups >= 4;  // up to 64 dims, more than 128
+    const int shape = pairs * (rows / 128) >= (narrow ? 1024 : 512) ? kFp8Rows : kFp8Keys;
     const bool weights = p->cache.weights != nullptr;
     r.v = &table[groups][shape][weights ? 1 : 0];
     Fp8AttendArgs& a = r.a;
@@ -183,19 +185,18 @@ Plan plan(const hstu_paged_fp8_fwd_params* p)
         const int64_t seen = ceil_div(a.window + r.v->tile_rows / ratio, kBlock) + 2 + ceil_div(a.sinks, kBlock);
         a.most_blocks = static_cast<int>(std::min<int64_t>(a.most_blocks, seen));
     }
-    // Parts (fp8_deal), where there are fewer workgroups than the machine has places: as many as it has, by the registers of the variants.
-    // More cost more than they spare: 64 x 4 pairs of one row on 2048 .. 8192 keys 74 us without, 81 in 512 and 87 in 1024; 3 x 2 pairs,
-    // d 256, on 30011 .. 120011 51 in 256, 56 in 512 to 1024; 32 x 4 of 49 .. 64 rows, d 64, on 501 .. 4001 31 in 1024, 45 without;
-    // 32 x 4 of 40 .. 64, d 128, with weights 58 in 512, 68 in 1024, 87 without.  Parts of a few blocks are not worth their sums.
+    // Parts (fp8_deal), where there are fewer workgroups than the machine has places, by the registers of the variants.  More cost more
+    // than they spare: 24 x 4 pairs of up to 8 rows on 2000 .. 8000 keys 45 us without, 32 in 256, 39 in 512; 2 x 4 pairs, d 256, of up to
+    // 256 rows 71, 37 and 46.  Nor are parts of a few blocks worth their sums: 2 x 4 pairs, d 64, on 500 .. 1500 keys 10 us without and 14 in
+    // parts, on 2000 .. 8000 26 and 18.
     const int64_t batch = p->cache.n_offsets - 1, per_part = p->cache.num_heads_k * a.row_tiles;
-    const bool narrow = groups < 2, wide = groups >= 4;  // up to 64 dims, more than 128
-    const int64_t places = shape == kFp8Keys ? (narrow ? 512 : 256) : (wide ? 256 : (narrow || shape == kFp8Rows ? 1024 : 512));
+    const int64_t places = shape == kFp8Keys || wide ? 256 : 1024;
     const int64_t total = places / per_part, waves = r.v->threads / 64;
-    const int least = static_cast<int>(shape == kFp8Rows ? 32 : (shape == kFp8Keys ? 4 * waves : 8));
+    const int least = static_cast<int>(shape == kFp8Rows ? 32 : 4 * waves);
     a.total_parts = 0;
     a.parts = 1;
     a.chunk = a.most_blocks;
-    if (2 * total >= 3 * batch && a.most_blocks > least) {
+    if (2 * total >= 3 * batch && a.most_blocks > 2 * least) {
         if (batch <= 64) {
             a.chunk = least;
             a.total_parts = static_cast<int>(total);
@@ -210,7 +211,7 @@ Plan plan(const hstu_paged_fp8_fwd_params* p)
     r.split = a.chunk < a.most_blocks;
     r.partial_bytes = r.split ? static_cast<uint64_t>(a.total_parts) * per_part * r.v->tile_rows * p->cache.head_dim * 4 : 0;
     r.join_bytes = r.split ? static_cast<uint64_t>(ceil_div(pairs * a.row_tiles, 2)) * 16 : 0;
-    const int64_t wave_tiles = static_cast<int64_t>(a.row_tiles) * (r.v->tile_rows / r.v->wave_rows);
+    const int64_t wave_tiles = static_cast<int64_t>(a.row_tiles) * (r.v->tile_rows / 32);
     r.weight_bytes = weights && wave_tiles > 1 ? static_cast<uint64_t>(pairs) * wave_tiles * a.max_blocks * kBlock * 4 : 0;
     const int64_t units = (a.total_parts > 0 ? a.total_parts : batch) * p->cache.num_heads_k;
     r.slots = a.row_tiles == 1 ? units : ceil_div(units, 8) * 8 * a.row_tiles;
@@ -336,9 +337,9 @@ HSTU_API int hstu_paged_fp8_fwd(const hstu_paged_fp8_fwd_params* p, void* worksp
         hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(std::min(most, enough)), a.row_tiles, pairs), dim3(256), 0, s, a, r.v->tile_rows);
     }
     if (a.weight_partial != nullptr) {
-        const int tiles = a.row_tiles * (r.v->tile_rows / r.v->wave_rows);
+        const int tiles = a.row_tiles * (r.v->tile_rows / 32);
         hipLaunchKernelGGL(hstu_paged_fp8_weights_kernel, dim3(static_cast<unsigned>(ceil_div(a.max_blocks, 8)), pairs), dim3(256), 0, s, a,
-                           r.v->wave_rows, tiles);
+                           32, tiles);
     }
     return launched(r.v->name);
 }

@@ -3,37 +3,37 @@
 //
 // A 32 x 32 block of scores costs 16 matrix instructions (248 ns on a SIMD alone) and, in the vector unit, 32 transcendental
 // instructions and some 60 others (230 ns; both together, from two wavefronts, 300 ns), and 64 conversions of codes (150 ns) in a
-// kernel whose wavefronts work alone.  Here the RG wavefronts of a share of the keys, 32 rows each, bring its blocks in together, each
-// a part of the chunks: codes two steps ahead in registers, converted (v_cvt_scalef32_pk) and left in LDS in the order of the
-// matrix operands, 16 bytes per lane, so that reads have no bank conflicts; two buffers for K and three for V, one barrier a step.  The
-// products of K(t) and of V(t - 1) go together, a chain of eight that wait for each other between four pairs that do not.  Four
-// wavefronts per workgroup and two workgroups per CU: what one leaves of a SIMD's units the other, which is nowhere in step with it, takes.
-// (Eight wavefronts half a step apart, one half multiplying while the other weighs, changing places at every barrier, took 10 %
-// longer: 288 against 266 us with wavefronts alone, on 16 x 4 key heads of 1024 rows and 2048 .. 8192 keys.)
+// kernel whose wavefronts work alone.  Here four wavefronts, 32 rows each, bring the same blocks in together, each a part of the
+// chunks: codes two steps ahead in registers, converted (v_cvt_scalef32_pk) and left in LDS in the order of the matrix operands, 16
+// bytes per lane, so that reads have no bank conflicts; two buffers for K and three for V, one barrier a step.  The products of K(t)
+// and of V(t - 1) go together, a chain of eight that wait for each other between four pairs that do not.  Up to 128 dims three
+// workgroups fit a CU, and what one leaves of a SIMD's units another, which is nowhere in step with it, takes.  Bound by the vector
+// unit: 16 x 4 key heads of 1024 rows on 2048 .. 8192 keys, d 128, 258 us (698 TFLOP/s), 32 such batches of 5120 keys 850 TFLOP/s;
+// wavefronts that convert for themselves take 278 us.  (Eight wavefronts half a step apart, one half multiplying while the other
+// weighs, changing places at every barrier, took 288; two shares of the keys for tiles of 64 rows lost to wavefronts alone.)
 //   step t : S = K(t) Q and O += V(t - 1) P; convert K, V (t + 1) to LDS, request those of t + 3; P = silu(S) masked
-// The outputs of KG shares of the keys (every KG-th block) are added through LDS at the end, in a fixed order.
 #pragma once
 #include "hstu_paged_fp8_attend_kernel.hip.h"
 
 namespace hstu {
 
-template <typename Tag, int NC, int RG, int KG, bool WEIGHTS>
-__global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(NC <= 2 ? 4 : (WEIGHTS ? 2 : 3), NC <= 2 ? 4 : (WEIGHTS ? 2 : 3)))) void hstu_paged_fp8_tile_kernel(const Fp8AttendArgs a)
+constexpr int kFp8TileThreads = 256, kFp8TileRows = 128;
+
+template <typename Tag, int NC, bool WEIGHTS>
+__global__ __launch_bounds__(kFp8TileThreads) __attribute__((amdgpu_waves_per_eu(NC <= 2 ? 4 : (WEIGHTS ? 2 : 3), NC <= 2 ? 4 : (WEIGHTS ? 2 : 3)))) void hstu_paged_fp8_tile_kernel(const Fp8AttendArgs a)
 {
-    constexpr int WAVES = RG * KG, T = 64 * WAVES;
-    constexpr int TILE = 32 * RG;
+    constexpr int T = kFp8TileThreads, RG = T / 64, TILE = kFp8TileRows;
     constexpr int CHUNKS = (2 * NC + RG - 1) / RG;  // chunks of 1 KiB of codes that a wavefront brings in per block
     constexpr int FRAG = 64 * 16;                   // bytes of an operand: 16 per lane
     constexpr int BUFFER = 2 * NC * FRAG;           // K or V of a block, 16 bits a value
-    constexpr int SHARE = 5 * BUFFER;               // two of K, three of V
-    constexpr int SUMS = WAVES * 1024 * 4;          // a group of 32 dims of all wavefronts
-    constexpr int LDS = KG * SHARE > 2 * SUMS ? KG * SHARE : 2 * SUMS;
+    constexpr int BUFFERS = 5 * BUFFER;             // two of K, three of V
+    constexpr int SUMS = RG * 1024 * 4;             // a group of 32 dims of all wavefronts
+    constexpr int LDS = BUFFERS > 2 * SUMS ? BUFFERS : 2 * SUMS;
     __shared__ __attribute__((aligned(16))) uint8_t s_mem[LDS];
 
     const Fp8Cache& c = a.c;
-    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int tid = threadIdx.x, lane = tid & 63, rg = uniform(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
-    const int rg = wave & (RG - 1), kg = wave / RG;
 
     int g, tile;
     const Fp8Deal deal = fp8_slot(a, g, tile);
@@ -108,12 +108,11 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(NC
         code_at[i] = n < NC ? k_at : (n < 2 * NC ? v_at : kOutOfRange);
     }
 
-    // steps: blocks n_begin + kg, + KG, ...; the same number for every share, the last of some without a block, and an even one (requests
-    // then stand in one order at the loop's head, and a wait is for a block's own).  Places and scales of 64 steps, and of the 64
-    // behind them, a step per lane; looked up and handed out with every lane active.
-    const int n_steps = (n_end - n_begin + 2 * KG - 1) / (2 * KG) * 2;
-    const int mine = n_end - n_begin - kg > 0 ? (n_end - n_begin - kg + KG - 1) / KG : 0;
-    const auto block_of = [&](int s) { return runs.block(n_begin + kg + s * KG); };
+    // a step is a block; an even number of steps, the last perhaps without one (requests then stand in one order at the loop's head, and
+    // a wait is for a block's own).  Places and scales of 64 steps, and of the 64 behind them, a step per lane; looked up and handed
+    // out with every lane active.
+    const int mine = n_end - n_begin > 0 ? n_end - n_begin : 0, n_steps = (mine + 1) / 2 * 2;
+    const auto block_of = [&](int s) { return runs.block(n_begin + s); };
     int lin_a = -1, lin_b = -1;
     float ks_a = 1.0f, ks_b = 1.0f, vs_a = 1.0f, vs_b = 1.0f;
     int base = 0;
@@ -253,11 +252,10 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(NC
         }
     };
 
-    uint8_t* const share = s_mem + kg * SHARE;
-    uint8_t *v_last = share + 4 * BUFFER, *v_now = share + 2 * BUFFER, *v_next = share + 3 * BUFFER;  // V of t - 1, t, t + 1
+    uint8_t *v_last = s_mem + 4 * BUFFER, *v_now = s_mem + 2 * BUFFER, *v_next = s_mem + 3 * BUFFER;  // V of t - 1, t, t + 1
     const auto step = [&](u32x4_t (&next)[CHUNKS], int t, int turn) {
-        multiply(share + turn * BUFFER, v_last);
-        convert(next, t + 1, share + (turn ^ 1) * BUFFER, v_next);
+        multiply(s_mem + turn * BUFFER, v_last);
+        convert(next, t + 1, s_mem + (turn ^ 1) * BUFFER, v_next);
         request(next, t + 3);
         weigh(t);
         __syncthreads();
@@ -273,7 +271,7 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(NC
     look_up(64, lin_b, ks_b, vs_b);
     request(raw[0], 0);
     request(raw[1], 1);
-    convert(raw[0], 0, share, v_now);
+    convert(raw[0], 0, s_mem, v_now);
     request(raw[0], 2);
     __syncthreads();
     for (int t = 0; t < n_steps; t += 2) {
@@ -295,18 +293,18 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(NC
         acc[n] = mfma32<Tag>(operand(v_last, 2 * n), p[0], acc[n]);
         acc[n] = mfma32<Tag>(operand(v_last, 2 * n + 1), p[1], acc[n]);
     }
-    // (flags where K and V were: with room of their own two workgroups of four shares' worth of buffers do not fit a CU)
+    // (a flag where K and V were)
     int* const s_poison = reinterpret_cast<int*>(s_mem);
     __syncthreads();
-    if (tid < KG) {
-        s_poison[tid] = 0;
+    if (tid == 0) {
+        *s_poison = 0;
     }
     __syncthreads();
     if (poisoned) {
-        s_poison[kg] = 1;
+        *s_poison = 1;
     }
     __syncthreads();
-    const bool any_poison = s_poison[kg] != 0;
+    const bool any_poison = *s_poison != 0;
     __syncthreads();  // (the sums go there next)
     if (any_poison) {
         uint32_t v_at[NC];
@@ -322,7 +320,7 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(NC
         }
     }
 
-    // ---- the sum over the shares, and the store ----
+    // ---- the store ----
     const bool partial = parts_used > 1 && deal.parts > 1;
     float* const to_partial = a.partial + (static_cast<int64_t>(deal.slot * c.n_heads + g) * a.row_tiles + tile) * TILE * dim;
 #pragma unroll
@@ -331,18 +329,14 @@ __global__ __launch_bounds__(64 * RG * KG) __attribute__((amdgpu_waves_per_eu(NC
 #pragma unroll
         for (int i = 0; i < 4; ++i) {  // (16 bytes at a time, their places exchanged so that neither side has bank conflicts)
             const f32x4_t x = {acc[n][4 * i], acc[n][4 * i + 1], acc[n][4 * i + 2], acc[n][4 * i + 3]};
-            *reinterpret_cast<f32x4_t*>(s + wave * 1024 + 4 * (i * 64 + (lane ^ (2 * i + 8 * half)))) = x;
+            *reinterpret_cast<f32x4_t*>(s + rg * 1024 + 4 * (i * 64 + (lane ^ (2 * i + 8 * half)))) = x;
         }
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < 4 / KG; ++r) {  // four dims per lane, eight lanes together the 32 of a row
+        for (int r = 0; r < 4; ++r) {  // four dims per lane, eight lanes together the 32 of a row
             const int word = tid + r * T, i = word & 3, h = (word >> 2) & 1, row_in = word >> 3;
             const float* const from = s + (row_in >> 5) * 1024 + 4 * (i * 64 + ((32 * h + (row_in & 31)) ^ (2 * i + 8 * h)));
-            f32x4_t x = *reinterpret_cast<const f32x4_t*>(from);
-#pragma unroll
-            for (int k = 1; k < KG; ++k) {
-                x += *reinterpret_cast<const f32x4_t*>(from + k * RG * 1024);
-            }
+            const f32x4_t x = *reinterpret_cast<const f32x4_t*>(from);
             const int row = t0 + row_in, d = 32 * n + 16 * h + 4 * i;
             if (row < n_rows && d < dim) {
                 if (partial) {

@@ -4,15 +4,14 @@
 
 namespace hstu {
 
-// how a workgroup's wavefronts are dealt: over the keys of one tile of rows, of one or two columns of 32, or over rows
-enum Fp8Shape { kFp8Keys = 0, kFp8KeysWide = 1, kFp8Rows = 2, kFp8Shapes = 3 };
+// how a workgroup's wavefronts are dealt: over the keys of one tile of 32 rows, or over four tiles
+enum Fp8Shape { kFp8Keys = 0, kFp8Rows = 1, kFp8Shapes = 2 };
 
 struct Fp8AttendVariant {
     const char* name;
     void (*kernel)(const Fp8AttendArgs);
     int threads;
-    int wave_rows;  // (row, head) pairs of a wavefront
-    int tile_rows;  // and of a workgroup
+    int tile_rows;  // (row, head) pairs of a workgroup; a wavefront has 32
 };
 
 // dims in groups of 32 that a variant is built for: the smallest of these that holds the head dim
