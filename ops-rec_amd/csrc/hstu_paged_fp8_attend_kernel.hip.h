@@ -17,6 +17,7 @@
 // share the keys that are read.
 #pragma once
 #include "hstu_paged_fp8_common.hip.h"
+#include "hstu_paged_fp8_variants.h"
 
 namespace hstu {
 
@@ -359,23 +360,23 @@ __device__ __forceinline__ void fp8_poison(f32x16_t (&acc)[NC], const Fp8Cache& 
     }
 }
 
+// that a variant's registers allow without scratch
+constexpr int fp8_wavefronts_per_simd(int nc, bool weights) { return nc <= 2 ? (nc == 2 && weights ? 3 : 4) : (nc <= 4 ? 2 : 1); }
+
 // Tag     : type of q and out
 // NC      : groups of 32 dims (dim is at most 32 NC, a multiple of 16)
-// WK, WR  : wavefronts of a workgroup over the keys of a row tile, and over row tiles
+// WK      : wavefronts of a workgroup, over the keys of a tile of rows
 // WEIGHTS : the sums of |P| per key as well
-template <typename Tag, int NC, int WK, int WR, bool WEIGHTS>
-__global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(const Fp8AttendArgs a)
+template <typename Tag, int NC, int WK, bool WEIGHTS>
+__global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wavefronts_per_simd(NC, WEIGHTS)))) void hstu_paged_fp8_attend_kernel(const Fp8AttendArgs a)
 {
-    constexpr int ROWS = 32;         // (row, head) pairs of a wavefront
-    constexpr int TILE = ROWS * WR;  // and of a workgroup
+    constexpr int T = 64 * WK, TILE = kFp8KeysRows;
     constexpr int CHUNK_WORDS = 64 * 16;
-    __shared__ __attribute__((aligned(16))) float s_sum[WK > 1 ? 2 : 1][WK > 1 ? WK * CHUNK_WORDS : 4];
+    __shared__ __attribute__((aligned(16))) float s_sum[2][WK * CHUNK_WORDS];
 
     const Fp8Cache& c = a.c;
-    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int tid = threadIdx.x, lane = tid & 63, wk = uniform(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
-    const int wk = WR > 1 ? 0 : wave, wr = WR > 1 ? wave : 0;
-    static_assert(WK == 1 || WR == 1, "keys or rows");
 
     int g, tile;
     const Fp8Deal deal = fp8_slot(a, g, tile);
@@ -393,19 +394,17 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
     uint16_t* const out = static_cast<uint16_t*>(a.out);
 
     if (tile == 0 && part == 0) {
-        fp8_clear_rows<64 * WK * WR>(a, item, b, g, out);
+        fp8_clear_rows<T>(a, item, b, g, out);
     }
     const int n_pairs_rows = n_rows * a.ratio;  // (row, head) pairs
-    if (tile * TILE >= n_pairs_rows) {
+    const int m0 = tile * TILE, m1 = m0 + TILE < n_pairs_rows ? m0 + TILE : n_pairs_rows;
+    if (m0 >= m1) {
         return;
     }
-    const int m0 = tile * TILE + wr * ROWS;
-    const int m1 = m0 + ROWS < n_pairs_rows ? m0 + ROWS : n_pairs_rows;
     // what the workgroup sweeps: the blocks of its tile's rows
-    const int t0 = tile * TILE, t1 = t0 + TILE < n_pairs_rows ? t0 + TILE : n_pairs_rows;
-    Fp8Runs runs = fp8_runs(mask, uniform(div_small(t0, a.ratio)), uniform(div_small(t1 - 1, a.ratio)) + 1);
+    const int i_first = uniform(div_small(m0, a.ratio)), i_last = uniform(div_small(m1 - 1, a.ratio));
+    Fp8Runs runs = fp8_runs(mask, i_first, i_last + 1);
     runs = {uniform(runs.n_a), uniform(runs.n_b), uniform(runs.n_c), uniform(runs.b0), uniform(runs.c0)};
-    const int i_first = uniform(div_small(m0 < m1 ? m0 : t0, a.ratio)), i_last = uniform(div_small(m0 < m1 ? m1 - 1 : t0, a.ratio));
     const int n_blocks = runs.count();
     const int parts_used = deal.parts == 1 ? 1 : uniform((n_blocks + deal.chunk - 1) / deal.chunk);
     if (part > 0 && part >= parts_used) {
@@ -555,13 +554,13 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
             acc[n] = mfma32<Tag>(vv.lo, p[0], acc[n]);
             acc[n] = mfma32<Tag>(vv.hi, p[1], acc[n]);
         }
-        if (WEIGHTS && m0 < m1) {
+        if constexpr (WEIGHTS) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 w[i] = __builtin_fabsf(w[i]);
             }
             const float all = fp8_key_sum(w, lane) * __builtin_fabsf(a.c_out);
-            fp8_store_key_sum(a, all, lane, pair, tile * WR + wr, a.row_tiles * WR, blk, lin);
+            fp8_store_key_sum(a, all, lane, pair, tile, a.row_tiles, blk, lin);
         }
     };
     const auto scale_of = [&](float mine, int s) {
@@ -601,56 +600,31 @@ __global__ __launch_bounds__(64 * WK * WR) void hstu_paged_fp8_attend_kernel(con
     // ---- the sum over the wavefronts that shared the keys, and the store ----
     const bool partial = parts_used > 1 && deal.parts > 1;
     float* const to_partial = a.partial + (static_cast<int64_t>(deal.slot * c.n_heads + g) * a.row_tiles + tile) * TILE * dim;
-    const auto row_at = [&](int m) {  // element index of a (row, head) pair in q and out
-        const int i = div_small(m, a.ratio);
-        return ((q0 + i) * a.n_heads_q + g * a.ratio + (m - i * a.ratio)) * static_cast<int64_t>(dim);
-    };
-    if constexpr (WK > 1) {
 #pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            float* const s = s_sum[n & 1];
+    for (int n = 0; n < NC; ++n) {
+        float* const s = s_sum[n & 1];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {  // (16 bytes at a time, their places exchanged so that neither side has bank conflicts)
-                const f32x4_t x = {acc[n][4 * i], acc[n][4 * i + 1], acc[n][4 * i + 2], acc[n][4 * i + 3]};
-                *reinterpret_cast<f32x4_t*>(s + wk * CHUNK_WORDS + 4 * (i * 64 + (lane ^ (2 * i + 8 * half)))) = x;
-            }
-            __syncthreads();
-            // four dims per lane, eight lanes together the 32 of a row
-            const int i = tid & 3, h = (tid >> 2) & 1, row = tid >> 3, mr = m0 + row, d = 32 * n + 16 * h + 4 * i;
-            if (tid < CHUNK_WORDS / 4 && mr < n_pairs_rows && d < dim) {
+        for (int i = 0; i < 4; ++i) {  // (16 bytes at a time, their places exchanged so that neither side has bank conflicts)
+            const f32x4_t x = {acc[n][4 * i], acc[n][4 * i + 1], acc[n][4 * i + 2], acc[n][4 * i + 3]};
+            *reinterpret_cast<f32x4_t*>(s + wk * CHUNK_WORDS + 4 * (i * 64 + (lane ^ (2 * i + 8 * half)))) = x;
+        }
+        __syncthreads();
+        constexpr int FOURS = CHUNK_WORDS / 4;
+#pragma unroll
+        for (int r = 0; r < (FOURS + T - 1) / T; ++r) {  // four dims per lane, eight lanes together the 32 of a row
+            const int four = tid + r * T, i = four & 3, h = (four >> 2) & 1, row = four >> 3, mr = m0 + row, d = 32 * n + 16 * h + 4 * i;
+            if (four < FOURS && mr < n_pairs_rows && d < dim) {
                 f32x4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int w = 0; w < WK; ++w) {
                     x += *reinterpret_cast<const f32x4_t*>(s + w * CHUNK_WORDS + 4 * (i * 64 + ((32 * h + row) ^ (2 * i + 8 * h))));
                 }
                 if (partial) {
-                    *reinterpret_cast<f32x4_t*>(to_partial + static_cast<int64_t>(mr - tile * TILE) * dim + d) = x;
+                    *reinterpret_cast<f32x4_t*>(to_partial + static_cast<int64_t>(row) * dim + d) = x;
                 } else {
-                    *reinterpret_cast<u32x2_t*>(out + row_at(mr) + d) = u32x2_t{pack2<Tag>(x[0] * a.c_out, x[1] * a.c_out), pack2<Tag>(x[2] * a.c_out, x[3] * a.c_out)};
-                }
-            }
-        }
-        static_assert(64 * WK * 4 >= CHUNK_WORDS, "a lane for every four values");
-    } else if (m < n_pairs_rows) {
-        const int64_t at = row_at(m);
-#pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            const int d = 32 * n + 16 * half;
-            if (d < dim) {
-                if (partial) {
-                    f32x4_t* const to = reinterpret_cast<f32x4_t*>(to_partial + static_cast<int64_t>(m - tile * TILE) * dim + d);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        to[i] = f32x4_t{acc[n][4 * i], acc[n][4 * i + 1], acc[n][4 * i + 2], acc[n][4 * i + 3]};
-                    }
-                } else {
-                    u32x4_t x[2];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        x[i >> 2][i & 3] = pack2<Tag>(acc[n][2 * i] * a.c_out, acc[n][2 * i + 1] * a.c_out);
-                    }
-                    *reinterpret_cast<u32x4_t*>(out + at + d) = x[0];
-                    *reinterpret_cast<u32x4_t*>(out + at + d + 8) = x[1];
+                    const int ir = div_small(mr, a.ratio);
+                    const int64_t at = ((q0 + ir) * a.n_heads_q + g * a.ratio + (mr - ir * a.ratio)) * static_cast<int64_t>(dim) + d;
+                    *reinterpret_cast<u32x2_t*>(out + at) = u32x2_t{pack2<Tag>(x[0] * a.c_out, x[1] * a.c_out), pack2<Tag>(x[2] * a.c_out, x[3] * a.c_out)};
                 }
             }
         }

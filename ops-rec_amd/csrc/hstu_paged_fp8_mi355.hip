@@ -151,14 +151,16 @@ Plan plan(const hstu_paged_fp8_fwd_params* p)
         ++groups;
     }
     const Fp8AttendTable& table = p->dtype == HSTU_DT_BF16 ? kFp8AttendBf16 : kFp8AttendF16;
-    // A workgroup's wavefronts share the keys of a tile of 32 rows, each converting what it reads, unless there are enough rows that tiles
-    // of 128, whose wavefronts share the conversion, fill the machine: 8 x 4 key heads of 512 rows on 2048 .. 8192 keys 85 us and 99 in
-    // tiles of 64 of two shares of the keys, 16 x 4 of 1024 278 and 257; 64 x 4 of 64 rows 100 and 142.  Up to 64 dims, where a conversion
-    // costs half as much, later: 24 x 4 of 512 rows, d 64, 113 and 142, 64 x 4 on 500 .. 1500 keys 77 and 72.
-    const bool narrow = groups < 2, wide = groups >= 4;  // up to 64 dims, more than 128
-    const int shape = pairs * (rows / 128) >= (narrow ? 1024 : 512) ? kFp8Rows : kFp8Keys;
-    const bool weights = p->cache.weights != nullptr;
-    r.v = &table[groups][shape][weights ? 1 : 0];
+    // A workgroup's wavefronts share the keys of a tile of 32 rows, each converting what it reads: as many of them as a CU's registers take,
+    // or half as many where there are more tiles than places for whole ones, so that one starts while another works (64 x 4 pairs of
+    // 33 .. 40 rows on 200 .. 400 keys 14 us and 20 in whole ones, on 1500 .. 3000 38 and 45; of 8 .. 16 on 1500 .. 3000, as many tiles as
+    // places, 31 and 32; 32 x 4 of them on 500 .. 1500 21 and 17).  Where tiles of 128 rows fill the machine their wavefronts share the
+    // conversion (16 x 4 of 1024 rows on 2000 .. 8000 keys 221 us, 241 in tiles of 32; 24 x 4 of 512 190 and 184): at 97 .. 128 dims and
+    // without weights only, elsewhere it is the other way round (d 96 191 and 189, d 64 165 and 139, with weights 329 and 307).
+    const bool narrow = groups < 2;  // up to 64 dims a CU's registers take two workgroups
+    const bool weights = p->cache.weights != nullptr, by_tile = groups == 3 && !weights && pairs * (rows / kFp8TileRows) >= 512;
+    const bool half = pairs * ceil_div(rows, kFp8KeysRows) > (narrow ? 512 : 256);
+    r.v = by_tile ? &table.tile : &table.keys[groups][half ? 1 : 0][weights ? 1 : 0];
     Fp8AttendArgs& a = r.a;
     a.c = describe(p->cache);
     a.q = p->q;
@@ -190,9 +192,8 @@ Plan plan(const hstu_paged_fp8_fwd_params* p)
     // 256 rows 71, 37 and 46.  Nor are parts of a few blocks worth their sums: 2 x 4 pairs, d 64, on 500 .. 1500 keys 10 us without and 14 in
     // parts, on 2000 .. 8000 26 and 18.
     const int64_t batch = p->cache.n_offsets - 1, per_part = p->cache.num_heads_k * a.row_tiles;
-    const int64_t places = shape == kFp8Keys || wide ? 256 : 1024;
-    const int64_t total = places / per_part, waves = r.v->threads / 64;
-    const int least = static_cast<int>(shape == kFp8Rows ? 32 : 4 * waves);
+    const int64_t total = (by_tile ? 1024 : 256) / per_part;
+    const int least = by_tile ? 32 : 4 * (r.v->threads / 64);
     a.total_parts = 0;
     a.parts = 1;
     a.chunk = a.most_blocks;
@@ -205,7 +206,9 @@ Plan plan(const hstu_paged_fp8_fwd_params* p)
             a.chunk = static_cast<int>(ceil_div(a.most_blocks, a.parts));
             a.total_parts = static_cast<int>(batch * a.parts);
         }
-    } else if (shape == kFp8Rows && batch <= 64) {  // one part each, the longest sequences first
+    } else if ((by_tile || (half && a.most_blocks >= 128)) && batch <= 64) {
+        // one part each, the longest sequences first: where workgroups follow one another and a late long one is waited for (24 x 4 pairs of
+        // 50 .. 250 rows on 2000 .. 8000 keys, d 128, 86 us and 92 in the order they come in; on 500 .. 1500, where looking costs more, 32 and 29)
         a.total_parts = static_cast<int>(batch + 1);
     }
     r.split = a.chunk < a.most_blocks;

@@ -6,10 +6,9 @@
 // kernel whose wavefronts work alone.  Here four wavefronts, 32 rows each, bring the same blocks in together, each a part of the
 // chunks: codes two steps ahead in registers, converted (v_cvt_scalef32_pk) and left in LDS in the order of the matrix operands, 16
 // bytes per lane, so that reads have no bank conflicts; two buffers for K and three for V, one barrier a step.  The products of K(t)
-// and of V(t - 1) go together, a chain of eight that wait for each other between four pairs that do not.  Up to 128 dims three
-// workgroups fit a CU, and what one leaves of a SIMD's units another, which is nowhere in step with it, takes.  Bound by the vector
-// unit: 16 x 4 key heads of 1024 rows on 2048 .. 8192 keys, d 128, 258 us (698 TFLOP/s), 32 such batches of 5120 keys 850 TFLOP/s;
-// wavefronts that convert for themselves take 278 us.  (Eight wavefronts half a step apart, one half multiplying while the other
+// and of V(t - 1) go together, a chain of eight that wait for each other between four pairs that do not.  Three workgroups fit a CU,
+// and what one leaves of a SIMD's units another, which is nowhere in step with it, takes.  Bound by the vector unit: 16 x 4 key heads of
+// 1024 rows on 2048 .. 8192 keys, d 128, 256 us (705 TFLOP/s), 64 such sequences of 5120 keys 850 TFLOP/s.  (Eight wavefronts half a step apart, one half multiplying while the other
 // weighs, changing places at every barrier, took 288; two shares of the keys for tiles of 64 rows lost to wavefronts alone.)
 //   step t : S = K(t) Q and O += V(t - 1) P; convert K, V (t + 1) to LDS, request those of t + 3; P = silu(S) masked
 #pragma once
@@ -17,10 +16,8 @@
 
 namespace hstu {
 
-constexpr int kFp8TileThreads = 256, kFp8TileRows = 128;
-
-template <typename Tag, int NC, bool WEIGHTS>
-__global__ __launch_bounds__(kFp8TileThreads) __attribute__((amdgpu_waves_per_eu(NC <= 2 ? 4 : (WEIGHTS ? 2 : 3), NC <= 2 ? 4 : (WEIGHTS ? 2 : 3)))) void hstu_paged_fp8_tile_kernel(const Fp8AttendArgs a)
+template <typename Tag, int NC>
+__global__ __launch_bounds__(kFp8TileThreads) __attribute__((amdgpu_waves_per_eu(3, 3))) void hstu_paged_fp8_tile_kernel(const Fp8AttendArgs a)
 {
     constexpr int T = kFp8TileThreads, RG = T / 64, TILE = kFp8TileRows;
     constexpr int CHUNKS = (2 * NC + RG - 1) / RG;  // chunks of 1 KiB of codes that a wavefront brings in per block
@@ -237,17 +234,6 @@ __global__ __launch_bounds__(kFp8TileThreads) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 p[u][i] = pack2<Tag>(w[8 * u + 2 * i], w[8 * u + 2 * i + 1]);
-            }
-        }
-        if constexpr (WEIGHTS) {
-            if (t < mine && rows_here) {
-                const int lin = lin_of(t);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    w[i] = __builtin_fabsf(w[i]);
-                }
-                const float all = fp8_key_sum(w, lane) * __builtin_fabsf(a.c_out);
-                fp8_store_key_sum(a, all, lane, pair, tile * RG + rg, a.row_tiles * RG, blk, lin);
             }
         }
     };

@@ -1,5 +1,5 @@
-"""Attention over the 8-bit paged cache where rows are many: the kernel for tiles of 128 rows, which a call reaches that allows for enough
-of them, and keys dealt to several workgroups, by the lengths of up to 64 sequences and alike for more."""
+"""Attention over the 8-bit paged cache where rows are many: workgroups of half the wavefronts and the kernel for tiles of 128 rows, which
+a call reaches that allows for enough rows, and keys dealt to several workgroups, by the lengths of up to 64 sequences and alike for more."""
 
 import pytest
 import torch
@@ -8,7 +8,7 @@ import paged_fp8_reference as R
 from test_gpu_paged_fp8 import DEV, TYPES, call, check, queries
 
 pytestmark = pytest.mark.gpu
-MOST = 20480  # rows that a call may allow for: 160 tiles of 128, and 8 key heads of sequences then fill the machine with them
+MOST = 20480  # rows that a call may allow for: 160 tiles of 128, and 4 sequences of 2 key heads then fill the machine with them
 WEIGHTS = pytest.mark.parametrize("weights", [False, True], ids=["plain", "weights"])
 
 
@@ -23,11 +23,13 @@ def kernels_of(run):
     return " ".join(e.name for e in prof.events())
 
 
-@pytest.mark.parametrize("dim,max_q,tiles", [(64, 300, False), (64, MOST, True), (128, MOST, True), (128, 300, False), (256, MOST, False)], ids=str)
-def test_the_kernel_that_these_tests_are_for_is_the_one_that_runs(dim, max_q, tiles):
+@pytest.mark.parametrize("dim,max_q,kernel", [(64, 300, "attend_kernel<hstu::bf16_tag, 2, 8,"), (64, MOST, "attend_kernel<hstu::bf16_tag, 2, 4,"),
+                                              (128, MOST, "tile_kernel<hstu::bf16_tag, 4>"), (128, 300, "attend_kernel<hstu::bf16_tag, 4, 8,"),
+                                              (160, MOST, "attend_kernel<hstu::bf16_tag, 6, 2,"), (256, 300, "attend_kernel<hstu::bf16_tag, 8, 4,")], ids=str)  # fmt: skip
+def test_the_kernel_that_these_tests_are_for_is_the_one_that_runs(dim, max_q, kernel):
     c = R.make([700] * 4, dim=dim, seed=1, device=DEV)
     q, offs = queries([300] * 4, 2, dim, torch.bfloat16), R.offsets([300] * 4, device=DEV)
-    assert ("hstu_paged_fp8_tile_kernel" in kernels_of(lambda: call(c, q, offs, [300], max_q=max_q))) == tiles
+    assert kernel in kernels_of(lambda: call(c, q, offs, [300], max_q=max_q))
 
 
 @TYPES
@@ -39,13 +41,13 @@ def test_head_dims(dim, dtype, weights):
 
 @pytest.mark.parametrize("heads,heads_k", [(8, 2), (6, 2), (16, 16), (3, 3)], ids=str)
 def test_grouped_heads(heads, heads_k):
-    check([200, 70, 331, 40], [200, 3, 90, 33], heads=heads, heads_k=heads_k, dim=64, seed=heads, max_q=MOST)
+    check([200, 70, 331, 40], [200, 3, 90, 33], heads=heads, heads_k=heads_k, dim=112, seed=heads, max_q=MOST)
 
 
 @pytest.mark.parametrize("rows", [33, 130, 300], ids=lambda n: f"rows{n}")
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (32, 32), (33, 31), (64, 0), (100, 4), (500, 100), (2000, 10), (64, 1000)], ids=str)
 def test_windows(rows, window, sinks):
-    check([rows + 600, rows, rows + 31, rows + 97], [rows] * 4, window=window, sinks=sinks, dim=32, page=32, seed=window + rows, max_q=MOST)
+    check([rows + 600, rows, rows + 31, rows + 97], [rows] * 4, window=window, sinks=sinks, dim=128, page=32, seed=window + rows, max_q=MOST)
 
 
 @WEIGHTS
@@ -83,7 +85,8 @@ def test_what_a_row_does_not_see_reaches_nothing(window, targets):
 
 
 def test_keys_past_64_and_past_128_steps():
-    check([32 * 150 + 9, 32 * 64, 32 * 65, 32 * 63 + 1], [130, 1, 33, 2], dim=64, page=256, seed=1, max_q=MOST)
+    check([32 * 150 + 9, 32 * 64, 32 * 65, 32 * 63 + 1], [130, 1, 33, 2], dim=128, page=256, seed=1, max_q=MOST)
+    check([32 * 4 * 130 + 9, 32 * 64 * 4, 32], [40, 1, 32], dim=16, page=256, seed=1, max_q=MOST)
 
 
 def test_pages_that_are_none_and_pages_of_two_sequences():
@@ -91,6 +94,7 @@ def test_pages_that_are_none_and_pages_of_two_sequences():
     ids = c["page_ids"]
     ids[2], ids[9] = -1, 1 << 30
     ids[7], ids[8] = ids[0], ids[1]  # the second sequence begins as the first
+    check([200, 290, 300, 290], [150, 200, 1, 290], dim=128, cache=c, max_q=MOST)
     check([200, 290, 300, 290], [150, 200, 1, 290], dim=128, cache=c, weights=True, max_q=MOST)
 
 
