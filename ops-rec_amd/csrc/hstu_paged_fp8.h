@@ -5,6 +5,9 @@
 namespace hstu {
 
 constexpr int kFp8Block = 32;         // tokens that share a scale, and keys of one step of the attention kernel
+constexpr int kFp8MostKeys = 1 << 24; // rows of a sequence in the cache, at most (what places are found by is exact up to there)
+constexpr int kFp8MostSlots = 1 << 22;  // workgroups of an attention launch, of up to 512 threads: a grid has less than 2^32 threads
+constexpr int64_t kFp8WeightBytes = int64_t{512} << 20;  // of partial sums of weights in the workspace of a call, at most (but for one row tile)
 constexpr int kFp8JoinEnough = 1024;  // workgroups of the joins that fill the machine
 constexpr int kFp8AppendThreads = 128;
 constexpr int kFp8AppendEnough = 8192;  // workgroups of the append from which on one takes several blocks
@@ -47,7 +50,8 @@ struct Fp8AttendArgs {
     int group;
     int window;  // 0: none
     int sinks;
-    int row_tiles;    // of a (sequence, key head) pair, at most
+    int row_tiles;    // of a (sequence, key head) pair that the launch takes, at most
+    int tile_first;   // the first of them
     int total_parts;  // the keys of the sequences are dealt to so many parts in all; 0: a sequence is one part
     int parts;        // of each sequence, where they are not dealt by length (more than 64 sequences)
     int chunk;        // blocks of a part: at least (dealt by length), or exactly

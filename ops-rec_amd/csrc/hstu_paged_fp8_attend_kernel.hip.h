@@ -246,7 +246,7 @@ __device__ __forceinline__ Fp8Deal fp8_deal(const Fp8AttendArgs& a, int n)  // t
     return {b, part, parts, l.chunk, uniform(ahead) + part};
 }
 
-// What a workgroup does: slots are (part, key head) x row tile, the tiles of a part and head, which read the same keys, on one XCD
+// What a workgroup does: slots are (part, key head) x row tile of the launch, the tiles of a part and head, which read the same keys, on one XCD
 // (workgroup w runs on XCD w mod 8).
 __device__ __forceinline__ Fp8Deal fp8_slot(const Fp8AttendArgs& a, int& g, int& tile)
 {
@@ -393,11 +393,11 @@ __global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wav
     const int dim = c.dim;
     uint16_t* const out = static_cast<uint16_t*>(a.out);
 
-    if (tile == 0 && part == 0) {
+    if (a.tile_first + tile == 0 && part == 0) {
         fp8_clear_rows<T>(a, item, b, g, out);
     }
     const int n_pairs_rows = n_rows * a.ratio;  // (row, head) pairs
-    const int m0 = tile * TILE, m1 = m0 + TILE < n_pairs_rows ? m0 + TILE : n_pairs_rows;
+    const int m0 = (a.tile_first + tile) * TILE, m1 = m0 + TILE < n_pairs_rows ? m0 + TILE : n_pairs_rows;
     if (m0 >= m1) {
         return;
     }

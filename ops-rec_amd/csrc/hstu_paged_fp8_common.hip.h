@@ -28,7 +28,7 @@ __device__ __forceinline__ Fp8Sequence fp8_pages(const void* offsets, int n_ids,
 __device__ __forceinline__ int fp8_room(const Fp8Cache& c, int n_pages)
 {
     const int64_t room = static_cast<int64_t>(n_pages) * c.blocks_per_page * kFp8Block;
-    return static_cast<int>(room < 0x3fffffff ? room : 0x3fffffff);
+    return static_cast<int>(room < kFp8MostKeys ? room : kFp8MostKeys);
 }
 
 __device__ __forceinline__ Fp8Sequence fp8_sequence(const Fp8Cache& c, int b)

@@ -20,7 +20,7 @@ __global__ __launch_bounds__(256) void hstu_paged_fp8_join_kernel(const Fp8Atten
     const int2 join = a.joins[pair * a.row_tiles + tile];
     const Fp8Item item = fp8_item(a, b);
     const int n_rows = item.n_rows * a.ratio;  // (row, head) pairs
-    const int m0 = tile * tile_rows, m1 = m0 + tile_rows < n_rows ? m0 + tile_rows : n_rows, parts = uniform(join.x);
+    const int m0 = (a.tile_first + tile) * tile_rows, m1 = m0 + tile_rows < n_rows ? m0 + tile_rows : n_rows, parts = uniform(join.x);
     if (m0 >= m1 || parts <= 1) {
         return;  // (no rows, of which nothing stands in joins, or the one part has written them)
     }
@@ -73,9 +73,9 @@ __global__ __launch_bounds__(256) void hstu_paged_fp8_join_kernel(const Fp8Atten
     }
 }
 
-// Adds the sums of |P| of several row tiles to the weights, in the order of the tiles.  A workgroup per (eight blocks, pair); a tile
-// has left sums for the blocks that its rows see.
-__global__ __launch_bounds__(256) void hstu_paged_fp8_weights_kernel(const Fp8AttendArgs a, int tile_rows, int tiles)
+// Adds the sums of |P| of the launch's row tiles, of 32 rows each, to the weights, in the order of the tiles.  A workgroup per (eight
+// blocks, pair); a tile has left sums for the blocks that its rows see.
+__global__ __launch_bounds__(256) void hstu_paged_fp8_weights_kernel(const Fp8AttendArgs a)
 {
     const Fp8Cache& c = a.c;
     const int pair = static_cast<int>(blockIdx.y), blk = static_cast<int>(blockIdx.x) * 8 + static_cast<int>(threadIdx.x >> 5);
@@ -86,11 +86,11 @@ __global__ __launch_bounds__(256) void hstu_paged_fp8_weights_kernel(const Fp8At
         return;
     }
     float sum = 0.0f;
-    for (int t = 0; t < tiles && t * tile_rows < n_pairs_rows; ++t) {
-        const int m0 = t * tile_rows, m1 = m0 + tile_rows < n_pairs_rows ? m0 + tile_rows : n_pairs_rows;
+    for (int t = 0; t < a.row_tiles && (a.tile_first + t) * kFp8KeysRows < n_pairs_rows; ++t) {
+        const int m0 = (a.tile_first + t) * kFp8KeysRows, m1 = m0 + kFp8KeysRows < n_pairs_rows ? m0 + kFp8KeysRows : n_pairs_rows;
         const Fp8Runs r = fp8_runs(item.mask, div_small(m0, a.ratio), div_small(m1 - 1, a.ratio) + 1);
         if (blk < r.n_a || (blk >= r.b0 && blk < r.b0 + r.n_b) || (blk >= r.c0 && blk < r.c0 + r.n_c)) {
-            sum += a.weight_partial[((static_cast<int64_t>(pair) * tiles + t) * a.max_blocks + blk) * kFp8Block + key];
+            sum += a.weight_partial[((static_cast<int64_t>(pair) * a.row_tiles + t) * a.max_blocks + blk) * kFp8Block + key];
         }
     }
     const int lin = fp8_block(c, c.page_ids, item.seq.first, g, blk);

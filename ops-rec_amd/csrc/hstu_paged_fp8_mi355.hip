@@ -134,7 +134,7 @@ int check_fwd(const hstu_paged_fp8_fwd_params* p)
 struct Plan {
     const Fp8AttendVariant* v;
     Fp8AttendArgs a;
-    int64_t slots;
+    int64_t units, all_tiles;  // (part, key head) pairs, row tiles
     uint64_t partial_bytes, join_bytes, weight_bytes;
     bool split;  // some sequence may have more than one part
     uint64_t bytes() const { return partial_bytes + join_bytes + weight_bytes; }
@@ -181,6 +181,7 @@ Plan plan(const hstu_paged_fp8_fwd_params* p)
     a.c_exp = static_cast<float>(-p->alpha * 1.4426950408889634);
     a.c_out = static_cast<float>(p->alpha * p->silu_scale);
     a.row_tiles = static_cast<int>(ceil_div(rows, r.v->tile_rows));
+    a.tile_first = 0;
     a.max_blocks = static_cast<int>(ceil_div(p->max_seq_len_k, kBlock));
     a.most_blocks = a.max_blocks;
     if (a.window > 0) {
@@ -213,11 +214,18 @@ Plan plan(const hstu_paged_fp8_fwd_params* p)
     }
     r.split = a.chunk < a.most_blocks;
     r.partial_bytes = r.split ? static_cast<uint64_t>(a.total_parts) * per_part * r.v->tile_rows * p->cache.head_dim * 4 : 0;
-    r.join_bytes = r.split ? static_cast<uint64_t>(ceil_div(pairs * a.row_tiles, 2)) * 16 : 0;
-    const int64_t wave_tiles = static_cast<int64_t>(a.row_tiles) * (r.v->tile_rows / 32);
-    r.weight_bytes = weights && wave_tiles > 1 ? static_cast<uint64_t>(pairs) * wave_tiles * a.max_blocks * kBlock * 4 : 0;
+    // A launch takes as many row tiles as its sums of weights have room for in 512 MiB, and as a grid holds; the others follow in launches
+    // of their own.
+    const uint64_t tile_bytes = static_cast<uint64_t>(pairs) * a.max_blocks * kBlock * 4;
     const int64_t units = (a.total_parts > 0 ? a.total_parts : batch) * p->cache.num_heads_k;
-    r.slots = a.row_tiles == 1 ? units : ceil_div(units, 8) * 8 * a.row_tiles;
+    r.all_tiles = a.row_tiles;
+    a.row_tiles = static_cast<int>(std::min<int64_t>(a.row_tiles, std::max<int64_t>(kFp8MostSlots / (units + 7), 1)));
+    if (weights) {
+        a.row_tiles = static_cast<int>(std::min<int64_t>(a.row_tiles, std::max<int64_t>(static_cast<int64_t>(kFp8WeightBytes / tile_bytes), 1)));
+    }
+    r.units = units;
+    r.join_bytes = r.split ? static_cast<uint64_t>(ceil_div(pairs * a.row_tiles, 2)) * 16 : 0;
+    r.weight_bytes = weights && a.row_tiles > 1 ? a.row_tiles * tile_bytes : 0;
     return r;
 }
 
@@ -314,9 +322,6 @@ HSTU_API int hstu_paged_fp8_fwd(const hstu_paged_fp8_fwd_params* p, void* worksp
     }
     Plan r = plan(p);
     Fp8AttendArgs& a = r.a;
-    if (r.slots > INT32_MAX) {
-        return set_error(HSTU_ERR_INVALID, "the call has more tiles than a launch can hold");
-    }
     if (r.bytes() > 0) {
         if (workspace == nullptr || workspace_bytes < r.bytes()) {
             return set_error(HSTU_ERR_WORKSPACE, "workspace of %llu bytes, %llu are needed", (unsigned long long)(workspace ? workspace_bytes : 0),
@@ -332,17 +337,19 @@ HSTU_API int hstu_paged_fp8_fwd(const hstu_paged_fp8_fwd_params* p, void* worksp
     }
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const unsigned pairs = static_cast<unsigned>(a.c.n_batch) * a.c.n_heads;
-    hipLaunchKernelGGL(r.v->kernel, dim3(static_cast<unsigned>(r.slots)), dim3(r.v->threads), 0, s, a);
-    if (r.split) {
-        const auto join = p->dtype == HSTU_DT_BF16 ? hstu_paged_fp8_join_kernel<bf16_tag> : hstu_paged_fp8_join_kernel<f16_tag>;
-        const int64_t most = ceil_div(static_cast<int64_t>(r.v->tile_rows) * a.c.dim, 256),
-                      enough = ceil_div(kFp8JoinEnough, static_cast<int64_t>(a.row_tiles) * pairs);
-        hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(std::min(most, enough)), a.row_tiles, pairs), dim3(256), 0, s, a, r.v->tile_rows);
-    }
-    if (a.weight_partial != nullptr) {
-        const int tiles = a.row_tiles * (r.v->tile_rows / 32);
-        hipLaunchKernelGGL(hstu_paged_fp8_weights_kernel, dim3(static_cast<unsigned>(ceil_div(a.max_blocks, 8)), pairs), dim3(256), 0, s, a,
-                           32, tiles);
+    for (const int tiles = a.row_tiles; a.tile_first < r.all_tiles; a.tile_first += tiles) {
+        a.row_tiles = static_cast<int>(std::min<int64_t>(tiles, r.all_tiles - a.tile_first));
+        const int64_t slots = a.row_tiles == 1 ? r.units : ceil_div(r.units, 8) * 8 * a.row_tiles;
+        hipLaunchKernelGGL(r.v->kernel, dim3(static_cast<unsigned>(slots)), dim3(r.v->threads), 0, s, a);
+        if (r.split) {
+            const auto join = p->dtype == HSTU_DT_BF16 ? hstu_paged_fp8_join_kernel<bf16_tag> : hstu_paged_fp8_join_kernel<f16_tag>;
+            const int64_t most = ceil_div(static_cast<int64_t>(r.v->tile_rows) * a.c.dim, 256),
+                          enough = ceil_div(kFp8JoinEnough, static_cast<int64_t>(a.row_tiles) * pairs);
+            hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(std::min(most, enough)), a.row_tiles, pairs), dim3(256), 0, s, a, r.v->tile_rows);
+        }
+        if (a.weight_partial != nullptr) {
+            hipLaunchKernelGGL(hstu_paged_fp8_weights_kernel, dim3(static_cast<unsigned>(ceil_div(a.max_blocks, 8)), pairs), dim3(256), 0, s, a);
+        }
     }
     return launched(r.v->name);
 }

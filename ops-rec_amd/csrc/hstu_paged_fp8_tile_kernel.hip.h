@@ -43,11 +43,11 @@ __global__ __launch_bounds__(kFp8TileThreads) __attribute__((amdgpu_waves_per_eu
     const Fp8Mask& mask = item.mask;
     const int dim = c.dim;
     uint16_t* const out = static_cast<uint16_t*>(a.out);
-    if (tile == 0 && part == 0) {
+    if (a.tile_first + tile == 0 && part == 0) {
         fp8_clear_rows<T>(a, item, b, g, out);
     }
     const int n_rows = item.n_rows * a.ratio;  // (row, head) pairs
-    const int t0 = tile * TILE, t1 = t0 + TILE < n_rows ? t0 + TILE : n_rows;
+    const int t0 = (a.tile_first + tile) * TILE, t1 = t0 + TILE < n_rows ? t0 + TILE : n_rows;
     if (t0 >= t1) {
         return;
     }

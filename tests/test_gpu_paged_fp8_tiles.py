@@ -135,6 +135,20 @@ def test_a_window_with_targets_past_the_blocks_it_allows_for(weights):
     check([9000, 9000], [800, 30], targets=[790, 20], group=2000, window=2100, sinks=40, heads=1, heads_k=1, dim=64, page=128, seed=9, weights=weights)
 
 
+@pytest.mark.parametrize("dim", [32, 256])
+def test_sums_of_weights_that_the_workspace_does_not_hold_at_once(dim):
+    """A call that allows for 2^24 keys: 128 MiB for the sums of a tile of 32 rows, of which the launch takes four; ten in three launches."""
+    check([700], [300], dim=dim, weights=True, seed=1, max_k=1 << 24)
+    check([700, 300], [300, 300], dim=dim, weights=True, seed=1, max_k=1 << 24)
+    check([700] + [40] * 4, [300] + [1] * 4, dim=dim, weights=True, seed=1, max_k=1 << 24)  # a tile in a launch
+
+
+def test_more_tiles_than_a_grid_holds():
+    """2048 sequences of 16 heads that may have 20480 rows each: 21 million tiles of 32."""
+    lens = [1 + i % 50 for i in range(2048)]
+    check(lens, [1 if i % 7 else min(40, n) for i, n in enumerate(lens)], heads=16, heads_k=16, dim=16, page=64, seed=3, max_q=MOST, silu_scale=0.1)
+
+
 @pytest.mark.parametrize("dim,max_q", [(128, MOST), (128, 10880), (64, 200)], ids=["tiles", "tiles-in-parts", "parts"])
 def test_the_same_bits_every_time(dim, max_q):
     lens = [6000, 300, 300, 200]
