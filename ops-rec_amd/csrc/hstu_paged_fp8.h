@@ -12,7 +12,7 @@ constexpr int kFp8JoinEnough = 1024;  // workgroups of the joins that fill the m
 constexpr int kFp8AppendThreads = 128;
 constexpr int kFp8AppendEnough = 8192;  // workgroups of the append from which on one takes several blocks
 constexpr int kFp8SelectKeys = 32768;   // scores that the selecting kernel holds in LDS
-constexpr int kFp8SelectFew = 2048;     // longest sequence of its variant with few threads
+constexpr int kFp8SelectFew = 1024;     // longest sequence of its variant with few threads
 
 // The cache of one layer, and whose pages are whose.
 struct Fp8Cache {

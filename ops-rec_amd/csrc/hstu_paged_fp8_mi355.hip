@@ -395,7 +395,7 @@ HSTU_API int hstu_paged_fp8_append(const hstu_paged_fp8_append_params* p, void* 
     const int64_t most = std::min(p->max_seq_len, p->total);
     a.max_rows = static_cast<int>(most);
     // n rows that begin anywhere in a block touch at most so many.  Where that leaves enough workgroups, one takes several blocks in turn
-    // (64512 of f16 rows, 8 key heads, 128 dims, of 32 ragged sequences: 116 us in workgroups of one, 109, 105 and 110 of two to four, 121 of twelve),
+    // (72000 f16 rows, 8 key heads, 128 dims, of 32 ragged sequences: 116 us in workgroups of one, 109, 105 and 110 of two to four, 121 of twelve),
     // and their number along a sequence is odd: workgroups go to the eight dies in turn, and by an even number the last ones of all the
     // sequences, which the short ones do not need, would fall to the same dies (of four: 158 us)
     const int64_t blocks = (most + 2 * kBlock - 2) / kBlock, all = blocks * 2 * a.c.n_heads * a.c.n_batch;
