@@ -131,7 +131,7 @@ def hstu_paged_fp8(q, k_cache, v_cache, k_scale, v_scale, seq_offset, cache_len,
     group) and the first ``sinks``.  ``silu_scale`` 0 means ``1 / max_seq_len``.
 
     ``weights``, where given, gets for every live key and key head the sum over rows and query heads of the magnitudes of the
-    attention weights added to it.  Returns the type and shape of ``q``; rows of no sequence come out as zeros."""
+    attention weights added to it.  Returns the type and shape of ``q``; rows of no sequence come out as zeros.  There is no backward."""
     _check(q.dim() == 3, "The q should be 3D in jagged layout")
     _check(q.dtype in (torch.bfloat16, torch.float16), f"q must be bfloat16 or float16, but it is {q.dtype}")
     _check_cache(k_cache, v_cache, k_scale, v_scale, weights)
