@@ -178,8 +178,9 @@ __device__ __forceinline__ Fp8Item fp8_item(const Fp8AttendArgs& a, int b)
 
 // Which share of a sequence's keys a workgroup takes.  Tiles whose keys take long are dealt to several workgroups, in parts of as
 // many blocks each, `chunk`, whatever the sequence: with up to 64 sequences, a lane of a wavefront for each, the lengths are
-// looked at, and the chunk is what makes total_parts of them all -- sum ceil(blocks / chunk) is at most sum blocks / chunk + the
-// number of sequences.  (Cut alike by the longest length allowed, parts of short sequences have nothing to do: 3 x 2 key heads
+// looked at, and the chunk is what makes hardly fewer than total_parts of them all -- sum ceil(blocks / chunk) is at most sum blocks / chunk +
+// the number of sequences, and about half that number less on average (16 x 4 pairs of 1024 rows on 2048 .. 8192 keys 259 us by the bound,
+// 248 by the half).  (Cut alike by the longest length allowed, parts of short sequences have nothing to do: 3 x 2 key heads
 // of 30011 .. 120011 keys, d 256, 70 us in such parts, 48 in these.)  First come the first parts of all sequences, the longest first,
 // then their second parts, and so on: what starts late is short.
 struct Fp8Deal {
@@ -200,16 +201,26 @@ __device__ __forceinline__ Fp8DealLanes fp8_deal_lanes(const Fp8AttendArgs& a)
     const int64_t len = load_index(a.c.cache_len, lane < n ? lane : 0, a.c.idx64);
     const int keys = static_cast<int>(len < 0 ? 0 : (len < a.max_k ? len : a.max_k));
     const int all = (keys + kFp8Block - 1) / kFp8Block, blocks = lane < n ? (all < a.most_blocks ? all : a.most_blocks) : -1;
-    int sum = blocks > 0 ? blocks : 0;
+    const auto over_lanes = [](int x) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        sum += __shfl_xor(sum, d, 64);
-    }
+        for (int d = 1; d < 64; d <<= 1) {
+            x += __shfl_xor(x, d, 64);
+        }
+        return uniform(x);
+    };
+    const int mine = blocks > 0 ? blocks : 0, sum = over_lanes(mine);
     Fp8DealLanes r;
-    const int even = uniform((sum + a.total_parts - n - 1) / (a.total_parts - n));
-    r.chunk = even > a.chunk ? even : a.chunk;
-    const int parts = div_small((blocks > 0 ? blocks : 0) + r.chunk - 1, r.chunk);
-    r.parts = lane < n ? (parts > 1 ? parts : 1) : 0;
+    // the first that makes no more than total_parts: sequences' last parts taken to be a half, or a quarter of a part on average, or nothing
+#pragma unroll
+    for (int lost = 2; lost <= 4; ++lost) {
+        const int whole = a.total_parts - div_small(lost * n, 4), even = uniform((sum + whole - 1) / whole);
+        r.chunk = even > a.chunk ? even : a.chunk;
+        const int parts = div_small(mine + r.chunk - 1, r.chunk);
+        r.parts = lane < n ? (parts > 1 ? parts : 1) : 0;
+        if (lost == 4 || over_lanes(r.parts) <= a.total_parts) {
+            break;
+        }
+    }
     r.rank = 0;
     for (int l = 0; l < n; ++l) {
         const int other = __builtin_amdgcn_readlane(blocks, l);
