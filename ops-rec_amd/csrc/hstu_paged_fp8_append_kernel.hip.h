@@ -85,22 +85,30 @@ __global__ __launch_bounds__(kFp8AppendThreads) void hstu_paged_fp8_append_kerne
                     was[i] = *reinterpret_cast<const u32x2_t*>(dst + (rows[i] < live ? rows[i] * dim + cols[i] : 0));
                 }
             }
-            float x[KP][8];
+            u32x4_t now[KP];
 #pragma unroll
             for (int i = 0; i < KP; ++i) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    x[i][2 * j] = rows[i] < fill ? lo_to_float<Tag>(raw[i][j]) : 0.0f;
-                    x[i][2 * j + 1] = rows[i] < fill ? hi_to_float<Tag>(raw[i][j]) : 0.0f;
+                now[i] = raw[i];
+                if (fill < kFp8Block && rows[i] >= fill) {
+                    now[i] = u32x4_t{0u};
                 }
             }
             if (TURNS && n + 1 < n_blocks) {
                 next = uniform(fp8_block(c, c.page_ids, seq.first, g, first + n + 1));
                 request(n + 1);
             }
-            if (old) {
+            u32x2_t w[KP];
+            uint32_t field;
+            if (old) {  // with the rows that are there, in fp32
+                float x[KP][8];
+                uint32_t top = 0;
 #pragma unroll
                 for (int i = 0; i < KP; ++i) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        x[i][2 * j] = lo_to_float<Tag>(now[i][j]);
+                        x[i][2 * j + 1] = hi_to_float<Tag>(now[i][j]);
+                    }
                     if (rows[i] < live) {
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
@@ -111,30 +119,48 @@ __global__ __launch_bounds__(kFp8AppendThreads) void hstu_paged_fp8_append_kerne
                             x[i][4 * j + 3] = hi[1] * old_scale;
                         }
                     }
-                }
-            }
-            uint32_t top = 0;
 #pragma unroll
-            for (int i = 0; i < KP; ++i) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t m = finite_bits(x[i][j]);
-                    top = m > top ? m : top;
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t m = finite_bits(x[i][j]);
+                        top = m > top ? m : top;
+                    }
                 }
-            }
-            const uint32_t field = fp8_scale_field(block_top<T / 64>(top, s_top[n & 1]));
-            const float inverse = fp8_inverse_of(field);
-            if (lin >= 0) {  // (otherwise there is no such page: the rows have no place)
+                field = fp8_scale_field(block_top<T / 64>(top, s_top[n & 1]));
+                const float inverse = fp8_inverse_of(field);
 #pragma unroll
                 for (int i = 0; i < KP; ++i) {
-                    u32x2_t w;
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const uint32_t codes = fp8_codes2<false>(x[i][4 * j], x[i][4 * j + 1], inverse, 0u);
-                        w[j] = fp8_codes2<true>(x[i][4 * j + 2], x[i][4 * j + 3], inverse, codes);
+                        w[i][j] = fp8_codes2<true>(x[i][4 * j + 2], x[i][4 * j + 3], inverse, codes);
                     }
+                }
+            } else {
+                FiniteTop<Tag> top;
+#pragma unroll
+                for (int i = 0; i < KP; ++i) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t word = now[i][j];
+                        top.take(word);
+                    }
+                }
+                field = fp8_scale_field(block_top<T / 64>(top.bits(), s_top[n & 1]));
+                const float scale = fp8_scale_of(field);
+#pragma unroll
+                for (int i = 0; i < KP; ++i) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t a0 = now[i][2 * j], a1 = now[i][2 * j + 1];
+                        w[i][j] = fp8_codes2<Tag, true>(a1, scale, fp8_codes2<Tag, false>(a0, scale, 0u));
+                    }
+                }
+            }
+            if (lin >= 0) {  // (otherwise there is no such page: the rows have no place)
+#pragma unroll
+                for (int i = 0; i < KP; ++i) {
                     if (rows[i] < kFp8Block) {
-                        *reinterpret_cast<u32x2_t*>(dst + rows[i] * dim + cols[i]) = w;
+                        *reinterpret_cast<u32x2_t*>(dst + rows[i] * dim + cols[i]) = w[i];
                     }
                 }
                 if (t == 0) {
@@ -188,22 +214,33 @@ __global__ __launch_bounds__(kFp8AppendThreads) void hstu_paged_fp8_append_kerne
                     }
                 }
             }
-            float x[VP][2][16];  // [unit][dim of the pair][token]
+            uint32_t now[VP][16];
 #pragma unroll
             for (int u = 0; u < VP; ++u) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    x[u][0][i] = halves[u] + i < fill ? lo_to_float<Tag>(raw[u][i]) : 0.0f;
-                    x[u][1][i] = halves[u] + i < fill ? hi_to_float<Tag>(raw[u][i]) : 0.0f;
+                    now[u][i] = raw[u][i];
+                    if (fill < kFp8Block && halves[u] + i >= fill) {
+                        now[u][i] = 0u;
+                    }
                 }
             }
             if (TURNS && n + 1 < n_blocks) {
                 next = uniform(fp8_block(c, c.page_ids, seq.first, g, first + n + 1));
                 request(n + 1);
             }
+            u32x4_t w[VP][2];
+            uint32_t field;
             if (old) {
+                float x[VP][2][16];  // [unit][dim of the pair][token]
+                uint32_t top = 0;
 #pragma unroll
                 for (int u = 0; u < VP; ++u) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        x[u][0][i] = lo_to_float<Tag>(now[u][i]);
+                        x[u][1][i] = hi_to_float<Tag>(now[u][i]);
+                    }
                     if (halves[u] < live) {
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
@@ -218,33 +255,55 @@ __global__ __launch_bounds__(kFp8AppendThreads) void hstu_paged_fp8_append_kerne
                             }
                         }
                     }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const uint32_t m0 = finite_bits(x[u][0][i]), m1 = finite_bits(x[u][1][i]);
+                        top = m0 > top ? m0 : top;
+                        top = m1 > top ? m1 : top;
+                    }
+                }
+                field = fp8_scale_field(block_top<T / 64>(top, s_top[n & 1]));
+                const float inverse = fp8_inverse_of(field);
+#pragma unroll
+                for (int u = 0; u < VP; ++u) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t codes = fp8_codes2<false>(x[u][e][4 * j], x[u][e][4 * j + 1], inverse, 0u);
+                            w[u][e][j] = fp8_codes2<true>(x[u][e][4 * j + 2], x[u][e][4 * j + 3], inverse, codes);
+                        }
+                    }
+                }
+            } else {
+                FiniteTop<Tag> top;
+#pragma unroll
+                for (int u = 0; u < VP; ++u) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        top.take(now[u][i]);
+                    }
+                }
+                field = fp8_scale_field(block_top<T / 64>(top.bits(), s_top[n & 1]));
+                const float scale = fp8_scale_of(field);
+#pragma unroll
+                for (int u = 0; u < VP; ++u) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {  // four tokens: codes of both dims of two and two, then of one dim of all four
+                        const uint32_t ab = fp8_codes2<Tag, true>(now[u][4 * j + 1], scale, fp8_codes2<Tag, false>(now[u][4 * j], scale, 0u));
+                        const uint32_t cd = fp8_codes2<Tag, true>(now[u][4 * j + 3], scale, fp8_codes2<Tag, false>(now[u][4 * j + 2], scale, 0u));
+                        w[u][0][j] = __builtin_amdgcn_perm(cd, ab, 0x06040200u);
+                        w[u][1][j] = __builtin_amdgcn_perm(cd, ab, 0x07050301u);
+                    }
                 }
             }
-            uint32_t top = 0;
-#pragma unroll
-            for (int u = 0; u < VP; ++u) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint32_t m0 = finite_bits(x[u][0][i]), m1 = finite_bits(x[u][1][i]);
-                    top = m0 > top ? m0 : top;
-                    top = m1 > top ? m1 : top;
-                }
-            }
-            const uint32_t field = fp8_scale_field(block_top<T / 64>(top, s_top[n & 1]));
-            const float inverse = fp8_inverse_of(field);
             if (lin >= 0) {
 #pragma unroll
                 for (int u = 0; u < VP; ++u) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        u32x4_t w;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t codes = fp8_codes2<false>(x[u][e][4 * j], x[u][e][4 * j + 1], inverse, 0u);
-                            w[j] = fp8_codes2<true>(x[u][e][4 * j + 2], x[u][e][4 * j + 3], inverse, codes);
-                        }
                         if (halves[u] < kFp8Block) {
-                            *reinterpret_cast<u32x4_t*>(dst + (dims[u] + e) * kFp8Block + halves[u]) = w;
+                            *reinterpret_cast<u32x4_t*>(dst + (dims[u] + e) * kFp8Block + halves[u]) = w[u][e];
                         }
                     }
                 }

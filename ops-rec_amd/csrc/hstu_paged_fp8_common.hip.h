@@ -71,16 +71,45 @@ __device__ __forceinline__ uint32_t finite_bits(float x)
     return m < 0x7f800000u ? m : 0u;
 }
 
-// the code of a value over its scale, in the low or high half of `old`: at most 448 in magnitude or not finite; what is not
-// finite becomes NaN (e4m3 has no infinity)
+// the codes of two values over their scale, in the low or high half of `old`: at most 448 in magnitude or not finite; what is not
+// finite becomes NaN (e4m3 has no infinity, and the instruction makes NaN of one)
 template <bool HI>
 __device__ __forceinline__ uint32_t fp8_codes2(float a, float b, float inverse, uint32_t old)
 {
-    const float nan = __builtin_nanf("");
-    a = finite_bits(a) == (__builtin_bit_cast(uint32_t, a) & 0x7fffffffu) ? a * inverse : nan;
-    b = finite_bits(b) == (__builtin_bit_cast(uint32_t, b) & 0x7fffffffu) ? b * inverse : nan;
-    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(a, b, static_cast<int>(old), HI));
+    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(a * inverse, b * inverse, static_cast<int>(old), HI));
 }
+
+typedef __attribute__((ext_vector_type(2))) short s16x2_t;
+
+// the same of a word of two 16-bit values, in one instruction
+template <typename Tag, bool HI>
+__device__ __forceinline__ uint32_t fp8_codes2(uint32_t word, float scale, uint32_t old)
+{
+    const s16x2_t was = __builtin_bit_cast(s16x2_t, old);
+    if constexpr (__is_same(Tag, bf16_tag)) {
+        typedef __attribute__((ext_vector_type(2))) __bf16 two_t;
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(was, __builtin_bit_cast(two_t, word), scale, HI));
+    } else {
+        typedef __attribute__((ext_vector_type(2))) _Float16 two_t;
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(was, __builtin_bit_cast(two_t, word), scale, HI));
+    }
+}
+
+// The largest finite magnitude among 16-bit values, two at a time: magnitudes moved up by as much as makes those that are not finite negative.
+template <typename Tag>
+struct FiniteTop {
+    static constexpr short kUp = __is_same(Tag, bf16_tag) ? 0x80 : 0x400;
+    s16x2_t top = {0, 0};
+    __device__ __forceinline__ void take(uint32_t word)
+    {
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(s16x2_t, word & 0x7fff7fffu) + s16x2_t{kUp, kUp});
+    }
+    __device__ __forceinline__ uint32_t bits() const  // as a float's
+    {
+        const int a = top[0], b = top[1], most = a > b ? a : b;
+        return __builtin_bit_cast(uint32_t, lo_to_float<Tag>(static_cast<uint32_t>(most > kUp ? most - kUp : 0)));
+    }
+};
 
 typedef __attribute__((ext_vector_type(2))) float f32x2_t;
 // two codes of a word (the low or the high ones) as floats
