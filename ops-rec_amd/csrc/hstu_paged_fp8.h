@@ -10,7 +10,6 @@ constexpr int kFp8MostSlots = 1 << 22;  // workgroups of an attention launch, of
 constexpr int64_t kFp8WeightBytes = int64_t{512} << 20;  // of partial sums of weights in the workspace of a call, at most (but for one row tile)
 constexpr int kFp8JoinEnough = 1024;  // workgroups of the joins that fill the machine
 constexpr int kFp8AppendThreads = 128;
-constexpr int kFp8AppendEnough = 8192;  // workgroups of the append from which on one takes several blocks
 constexpr int kFp8SelectKeys = 32768;   // scores that the selecting kernel holds in LDS
 constexpr int kFp8SelectFew = 1024;     // longest sequence of its variant with few threads
 
@@ -69,7 +68,6 @@ struct Fp8AppendArgs {
     int64_t total;
     int64_t k_row, k_head, v_row, v_head;  // strides, in elements
     int max_rows;
-    int in_turn;  // blocks that a workgroup takes one after the other
 };
 
 struct Fp8EvictArgs {

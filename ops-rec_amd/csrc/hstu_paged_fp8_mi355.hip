@@ -232,18 +232,11 @@ Plan plan(const hstu_paged_fp8_fwd_params* p)
 // ---------------------------------------------------------------------------------------------------------- append ----
 
 using AppendKernel = void (*)(const Fp8AppendArgs);
-template <typename Tag, bool TURNS>
-constexpr AppendKernel append_by_dim(int slot)
-{
-    return slot == 0 ? hstu_paged_fp8_append_kernel<Tag, 64, TURNS>
-                     : (slot == 1 ? hstu_paged_fp8_append_kernel<Tag, 128, TURNS> : hstu_paged_fp8_append_kernel<Tag, 256, TURNS>);
-}
-// head dims up to 64, 128, 256: what a lane holds
-AppendKernel append_kernel(bool bf16, bool turns, int slot)
-{
-    return bf16 ? (turns ? append_by_dim<bf16_tag, true>(slot) : append_by_dim<bf16_tag, false>(slot))
-                : (turns ? append_by_dim<f16_tag, true>(slot) : append_by_dim<f16_tag, false>(slot));
-}
+// by type and head dims up to 64, 128, 256: what a lane holds
+const AppendKernel kAppend[2][3] = {
+    {hstu_paged_fp8_append_kernel<bf16_tag, 64>, hstu_paged_fp8_append_kernel<bf16_tag, 128>, hstu_paged_fp8_append_kernel<bf16_tag, 256>},
+    {hstu_paged_fp8_append_kernel<f16_tag, 64>, hstu_paged_fp8_append_kernel<f16_tag, 128>, hstu_paged_fp8_append_kernel<f16_tag, 256>},
+};
 int dim_slot(int64_t dim) { return dim <= 64 ? 0 : (dim <= 128 ? 1 : 2); }
 
 bool bad_stride(int64_t s) { return s < 0 || s % 8 != 0; }
@@ -394,14 +387,12 @@ HSTU_API int hstu_paged_fp8_append(const hstu_paged_fp8_append_params* p, void* 
     a.v_head = p->v_stride_head;
     const int64_t most = std::min(p->max_seq_len, p->total);
     a.max_rows = static_cast<int>(most);
-    // n rows that begin anywhere in a block touch at most so many.  Where that leaves enough workgroups, one takes several blocks in turn
-    // (72000 f16 rows, 8 key heads, 128 dims, of 32 ragged sequences: 116 us in workgroups of one, 109, 105 and 110 of two to four, 121 of twelve),
-    // and their number along a sequence is odd: workgroups go to the eight dies in turn, and by an even number the last ones of all the
-    // sequences, which the short ones do not need, would fall to the same dies (of four: 158 us)
-    const int64_t blocks = (most + 2 * kBlock - 2) / kBlock, all = blocks * 2 * a.c.n_heads * a.c.n_batch;
-    a.in_turn = static_cast<int>(std::min<int64_t>(std::max<int64_t>(all / kFp8AppendEnough, 1), 3));
-    hipLaunchKernelGGL(append_kernel(p->dtype == HSTU_DT_BF16, a.in_turn > 1, dim_slot(a.c.dim)),
-                       dim3(static_cast<unsigned>(ceil_div(blocks, a.in_turn) | 1), 2u * static_cast<unsigned>(a.c.n_heads), static_cast<unsigned>(a.c.n_batch)),
+    // n rows that begin anywhere in a block touch at most so many.  The number of workgroups along a sequence is odd: they go to the eight
+    // dies in turn, and by a multiple of eight the last ones of all the sequences, which the short ones do not need, would fall to the
+    // same dies (32 of 16128 blocks in all: 158 us where 106 is usual)
+    const int64_t blocks = ((most + 2 * kBlock - 2) / kBlock) | 1;
+    hipLaunchKernelGGL(kAppend[p->dtype == HSTU_DT_BF16 ? 0 : 1][dim_slot(a.c.dim)],
+                       dim3(static_cast<unsigned>(blocks), 2u * static_cast<unsigned>(a.c.n_heads), static_cast<unsigned>(a.c.n_batch)),
                        dim3(kFp8AppendThreads), 0, static_cast<hipStream_t>(stream), a);
     return launched("hstu_paged_fp8_append_kernel");
 }
