@@ -11,7 +11,7 @@
 //      to store, without an exchange between lanes.
 // Blocks without older rows stay 16-bit words: an instruction converts two values and divides by the scale, two more find the largest
 // of two; blocks with them are added up in fp32.  Bound by the bytes of the rows and codes (72000 f16 rows, 8 key heads, 128 dims: 446 MB in
-// 86 us; 136 when all values went through fp32; two to four blocks in turn, the next one's rows on their way, 90 to 95).
+// 86 us; 136 when all values went through fp32; two to four blocks a workgroup, the next one's rows on their way, 90 to 95).
 #pragma once
 #include "hstu_paged_fp8_common.hip.h"
 

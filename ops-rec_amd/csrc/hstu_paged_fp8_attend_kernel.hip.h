@@ -512,7 +512,11 @@ __global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wav
         }
         const int end = c0 + kFp8Block;
         const bool whole = whole_blocks.has(blk);
-        u32x4_t p[2];
+        // P goes into the second product rounded to the type of q.  What that leaves of half the keys (0 .. 7 and 16 .. 23 of a block) goes into a
+        // product of its own, so that P adds less to the error than the output's rounding: bf16 outputs of few rows would else be 1.4 to
+        // 1.5 times as far off as rounding them alone, and are 1.2 times.  (64 rows of one query 74 us without, 77; 32 x 4 pairs of 49 .. 64 rows
+        // 22 and 24; both halves 78 and 26.5.)
+        u32x4_t p[2], rest;
         float w[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -529,8 +533,21 @@ __global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wav
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                p[u][i] = pack2<Tag>(w[8 * u + 2 * i], w[8 * u + 2 * i + 1]);
+                const float w0 = w[8 * u + 2 * i], w1 = w[8 * u + 2 * i + 1];
+                const uint32_t two = pack2<Tag>(w0, w1);
+                p[u][i] = two;
+                if (u == 0) {
+                    rest[i] = pack2<Tag>(w0 - lo_to_float<Tag>(two), w1 - hi_to_float<Tag>(two));
+                }
             }
+        }
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            top = __builtin_fmaxf(top, __builtin_fabsf(w[i]));
+        }
+        if (__any(top > (__is_same(Tag, bf16_tag) ? 3.3895314e38f : 65504.0f))) {  // (infinite in the type of q: nothing is left of it, not NaN)
+            rest = u32x4_t{0u};
         }
         if (end > seq.len) {  // codes behind the last row may be anything, NaN among them: zero times that is not zero
             const int left = seq.len - c0 - 16 * half;  // live keys of this lane's sixteen
@@ -564,6 +581,7 @@ __global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wav
             const Fp8Pair vv = fp8_widen<Tag>(st.v[n], vs);
             acc[n] = mfma32<Tag>(vv.lo, p[0], acc[n]);
             acc[n] = mfma32<Tag>(vv.hi, p[1], acc[n]);
+            acc[n] = mfma32<Tag>(vv.lo, rest, acc[n]);
         }
         if constexpr (WEIGHTS) {
 #pragma unroll

@@ -160,3 +160,18 @@ def test_the_same_bits_every_time(dim, max_q):
         got = (call(c, q, offs, [200], weights=w, max_q=max_q), w)
         first = first or got
         assert all(torch.equal(a, b) for a, b in zip(first, got))
+
+
+@TYPES
+def test_weights_past_the_type_of_q_are_infinite(dtype):
+    """P rounds to infinity there: an output is infinite with the sign of the value, and a row that sees no such key is what it was."""
+    c = R.make([1, 40], heads_k=1, dim=32, page=32, seed=1, device=DEV)
+    where, offs = [int(c["page_ids"][i]) for i in (0, 1)], R.offsets([1, 1], device=DEV)
+    q = queries([1, 1], 1, 32, dtype)
+    want = call(c, q, offs, [1], silu_scale=1.0)
+    k = c["k_cache"][where[0], 0, 0, 0].float() * c["k_scale"][where[0], 0, 0]
+    v = c["v_cache"][where[0], 0, 0, :, 0].float() * c["v_scale"][where[0], 0, 0]
+    q[0, 0] = torch.sign(k) * (60000.0 if dtype == torch.float16 else 3e38)
+    got = call(c, q, offs, [1], silu_scale=1.0)
+    assert torch.equal(got[1], want[1])
+    assert (got[0, 0][v > 0] == float("inf")).all() and (got[0, 0][v < 0] == -float("inf")).all()
