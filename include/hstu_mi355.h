@@ -276,8 +276,8 @@ HSTU_API int hstu_paged_fwd(const hstu_paged_fwd_params* params, void* workspace
  * The rows of sequence b are those of its pages page_ids[page_offsets[b] : page_offsets[b + 1]] in order, the first cache_len[b] of
  * them live.  Page ids outside [0, num_pages) stand for pages that are not there: nothing is read from them (their rows count as
  * zeros) or written to them.  A page that a call writes to must stand in it once, and nowhere else in the call; a page that is
- * only read may be shared by sequences.  head_dim is a multiple of 16 in [16, 256], page_size a multiple of 32; pointers to
- * caches, weights, q, k, v and out are 16-byte aligned.
+ * only read may be shared by sequences.  head_dim is a multiple of 16 in [16, 256], page_size a multiple of 32; a sequence ends at
+ * 2^24 rows, whatever its pages hold; pointers to caches, weights, q, k, v and out are 16-byte aligned.
  */
 #define HSTU_PAGED_FP8_MAX_SEQ_LEN_K 16777216
 #define HSTU_PAGED_FP8_MAX_HEAD_DIM 256
@@ -355,7 +355,7 @@ HSTU_API int hstu_paged_fp8_append(const hstu_paged_fp8_append_params* params, v
 /*
  * Of each sequence at most `keep` rows stay (no more than the new pages hold): the first `sinks`, the last `recent`, and of the others
  * those with the largest scores, ties to the lower index; a score is the fp32 sum of a row's weights over the key heads, in
- * their order.  The rows that stay are moved in order to the new pages (new_page_ids[new_page_offsets[b] : ...]), with new
+ * their order.  cache_len is cut at max_seq_len_k.  The rows that stay are moved in order to the new pages (new_page_ids[new_page_offsets[b] : ...]), with new
  * scales and their weights; new_cache_len[b] is their number, kept[b] their old indices, -1 behind them.
  */
 typedef struct hstu_paged_fp8_evict_params {
