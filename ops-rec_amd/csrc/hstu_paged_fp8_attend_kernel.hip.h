@@ -3,8 +3,8 @@
 //   S = Q K^T,  P = silu(alpha S) * silu_scale * M,  O = P V,  with K and V the codes of the cache times their blocks' scales
 //
 // A step is one block of 32 keys, which lies in one page and has one scale for K and one for V.  Both products run on
-// v_mfma_f32_32x32x16 in the type of q: e4m3 values times a power of two are exact there, and v_cvt_scalef32_pk multiplies by
-// the scale while it converts, so scales cost nothing.
+// v_mfma_f32_32x32x16 in the type of q, which holds an e4m3 value exactly; bf16 also holds it times the scale, a power of two, which
+// v_cvt_scalef32_pk multiplies by while it converts, so that scales cost nothing.  fp16 does not: see Fp8Unit.
 //   S^T[key][row] = K . Q^T     A = K: lane l % 32 takes key pi(l % 32) of the block, 16 dims of its half at a time; B = Q, in
 //                               registers from the start, the same dims
 //   O^T[dim][row] += V^T . P^T  A = V^T: lane l % 32 takes dim pi(l % 32) of a group of 32, the 16 keys of its half; B = P
@@ -59,6 +59,108 @@ __device__ __forceinline__ Fp8Pair fp8_widen(u32x4_t codes, float scale)
     }
     return r;
 }
+
+// A cache has no type, and fp16 does not hold what a code times its scale may be (from 65520 on it would be infinite, and zero times that NaN
+// in rows that do not see the key; below 2^-14 it would be rounded), nor what a weight may be before alpha and silu_scale.  So for rows of fp16
+// the products run on the codes themselves, which fp16 holds exactly.  A block's scale of K goes into the exponent of silu, and the weights go
+// into the second product times both scales, in units of their row's own.  Of a row of dim values up to m a score in units of K's scale is at most
+// 448 dim m; the unit is the power of two that puts this bound, times the largest product of both scales of the blocks that the row has seen a key
+// of, below 2^15, and grows, the row's sums with it, when a block has a larger one.  Weights are then rounded to multiples of 2^-24 of a unit at
+// worst, 2^-37 of what the bound says, where a score's own sum in fp32 is good to 2^-24 of it.  (A row is a column of the result: a lane holds of its
+// own row only, and so does the lane of the same row in the other half.)  It costs no instruction an element: x / (1 + e) * 2^n is
+// x / (e 2^-n + 2^-n).  bf16 reaches as far as fp32 and needs none of this.
+struct Fp8Unit {
+    int most;     // exponents of a block's two scales may add up to `most` - `up`
+    int up;       // the unit is 2^-up; ahead of the first block smaller than any needs
+    bool finite;  // the row
+    static __device__ __forceinline__ int exponent(float power_of_two) { return static_cast<int>(__builtin_bit_cast(uint32_t, power_of_two) >> 23 & 0xffu) - 127; }
+    // what `x` is in the two lanes of this lane's row, the larger of them
+    static __device__ __forceinline__ uint32_t of_row(uint32_t x)
+    {
+        const u32x2_t two = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        const uint32_t lower = two[0], upper = two[1];
+        return lower > upper ? lower : upper;
+    }
+    template <int NC>
+    __device__ __forceinline__ Fp8Unit(const u32x4_t (&q)[NC][2], int dim)
+    {
+        typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
+        u16x2_t top = {0, 0};
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t word = q[n][i >> 2][i & 3];
+                top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, word & 0x7fff7fffu));
+            }
+        }
+        const uint32_t a = top[0], b = top[1], m = of_row(a > b ? a : b);
+        finite = m < 0x7c00u;
+        const int bits = 32 - __builtin_clz(static_cast<uint32_t>(dim) - 1);  // dim <= 2^bits, codes <= 2^9
+        most = 15 - (__builtin_amdgcn_frexp_expf(lo_to_float<f16_tag>(m)) + 9 + bits);
+        up = most + 1024;
+    }
+    // Makes the unit large enough for a block whose scales' exponents add up to `by`, of which this row sees keys (`sees`, the same in both lanes of
+    // a row).
+    template <int NC>
+    __device__ __forceinline__ void fit(f32x16_t (&acc)[NC], int by, bool sees)
+    {
+        const bool small = sees & (up + by > most);
+        if (__any(small)) {
+            const int change = small ? most - by - up : 0;
+            up += change;
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    acc[n][i] = __builtin_ldexpf(acc[n][i], change);
+                }
+            }
+        }
+    }
+    // What the denominators of a block's weights are multiplied by.  (`most` is at most 30; of a score, below 2^33, 2^-64 leaves nothing in fp16; a
+    // row that sees no key of the block has scores of zero.)
+    __device__ __forceinline__ float denominator(int by) const
+    {
+        const int n = up + by;
+        return __builtin_ldexpf(1.0f, -(n > 64 ? 64 : (n < -64 ? -64 : n)));
+    }
+    // what a weight in units is multiplied by, without the scale of V of exponent `v`
+    __device__ __forceinline__ float weight(int v) const { return __builtin_ldexpf(1.0f, -up - v); }
+    template <int NC>
+    __device__ __forceinline__ void undo(f32x16_t (&acc)[NC]) const
+    {
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                acc[n][i] = __builtin_ldexpf(acc[n][i], -up);
+            }
+        }
+    }
+};
+// whether some of a lane's 16 scores, or of the other's of its row, is not zero
+__device__ __forceinline__ bool fp8_some_score(const float (&x)[16])
+{
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float one = x[i];
+        bits |= __builtin_bit_cast(uint32_t, one);
+    }
+    return Fp8Unit::of_row(bits & 0x7fffffffu) != 0;
+}
+// silu of 16 scores x (in units of a scale 2^k) without alpha, in units of a row: x / (1 + 2^(c_exp 2^k x)) times 1 / g.  `most`: of k, that leaves
+// the product finite (a score of 0 has a weight of 0).
+__device__ __forceinline__ void fp8_weights_in_units(float (&x)[16], float c_exp, int k, int most, float g)
+{
+    const float c = __builtin_ldexpf(c_exp, k < most ? k : most);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        x[i] = x[i] * __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_amdgcn_exp2f(x[i] * c), g, g));
+    }
+}
+__device__ __forceinline__ int fp8_most_scale(float c_exp) { return uniform(127 - __builtin_amdgcn_frexp_expf(c_exp)); }
 
 // 0x80 in the place of each of four codes that is NaN (0x7f, 0xff), 0 elsewhere
 __device__ __forceinline__ uint32_t nan_codes(uint32_t codes) { return ((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
@@ -344,11 +446,13 @@ __device__ __forceinline__ void fp8_store_key_sum(const Fp8AttendArgs& a, float 
     }
 }
 
+constexpr uint32_t kV32 = 32 * kFp8Block;  // bytes of 32 dims of V of a block
+
 // Outputs that a value which is NaN reaches, of one block: a product of ones at the codes for NaN with the 0 / 1 mask counts, for every
-// (dim, row), the NaN that the row sees.  j0: the first key of this lane's half; v_at: where its codes are.  (The products proper
+// (dim, row), the NaN that the row sees.  j0: the first key of this lane's half; v_at: where its codes of the first 32 dims are.  (The products proper
 // had zeros in the place of those codes.)
 template <typename Tag, int NC, typename Sees>
-__device__ __forceinline__ void fp8_poison(f32x16_t (&acc)[NC], const Fp8Cache& c, int lin, const uint32_t (&v_at)[NC], int j0, int len, Sees sees)
+__device__ __forceinline__ void fp8_poison(f32x16_t (&acc)[NC], const Fp8Cache& c, int lin, uint32_t v_at, int j0, int len, Sees sees)
 {
     const uint32_t bytes = static_cast<uint32_t>(kFp8Block) * c.dim;
     const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(c.v + static_cast<int64_t>(lin < 0 ? 0 : lin) * bytes, lin < 0 ? 0u : bytes);
@@ -360,7 +464,7 @@ __device__ __forceinline__ void fp8_poison(f32x16_t (&acc)[NC], const Fp8Cache& 
     }
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-        u32x4_t ones = load_codes(rsrc, v_at[n]);
+        u32x4_t ones = load_codes(rsrc, v_at + n * kV32);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             ones[i] = (nan_codes(ones[i]) >> 7) * 0x38u;  // the code of 1
@@ -387,6 +491,7 @@ template <typename Tag, int NC, int WK, bool WEIGHTS>
 __global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wavefronts_per_simd(NC, WEIGHTS)))) void hstu_paged_fp8_attend_kernel(const Fp8AttendArgs a)
 {
     constexpr int T = 64 * WK, TILE = kFp8KeysRows;
+    constexpr bool F16 = __is_same(Tag, f16_tag);
     constexpr int CHUNK_WORDS = 64 * 16;
     __shared__ __attribute__((aligned(16))) float s_sum[2][WK * CHUNK_WORDS];
 
@@ -454,13 +559,13 @@ __global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wav
     // offsets of this lane's chunks within a block of codes; dims past the last read as zeros
     const int pi = 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);
     const uint32_t block_bytes = static_cast<uint32_t>(kFp8Block) * dim;
-    uint32_t k_at[NC], v_at[NC];
+    uint32_t k_at[NC];
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
         const int d = 32 * n + 16 * half;
         k_at[n] = d < dim ? static_cast<uint32_t>(pi) * dim + d : kOutOfRange;
-        v_at[n] = 32 * n + pi < dim ? static_cast<uint32_t>(32 * n + pi) * kFp8Block + 16 * half : kOutOfRange;
     }
+    const uint32_t v_at = static_cast<uint32_t>(pi) * kFp8Block + 16 * half;  // (32 dims on: kV32 on; V of a dim past the last lies past the block)
 
     f32x16_t acc[NC];
 #pragma unroll
@@ -498,25 +603,31 @@ __global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wav
         }
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-            st.v[n] = load_codes(vr, v_at[n]);
+            st.v[n] = load_codes(vr, v_at + n * kV32);
         }
     };
     const auto sees_key = [&](int j) {  // whether this lane's row sees key j
         return static_cast<bool>((j < lim) & ((j < mask.first_key) | (j >= hole)) & ((j >= low) | (j < mask.sinks)));
     };
     bool poisoned = false;
+    Fp8Unit unit(q, dim);  // (fp16)
+    const int most_scale = fp8_most_scale(a.c_exp);
     const auto step = [&](Stage& st, int s, float ks, float vs) {
         const int lin = place_of(s);
         const int blk = runs.block(n_begin + wk + s * WK), c0 = blk * kFp8Block;
+        const bool whole = whole_blocks.has(blk);
+        const int by = Fp8Unit::exponent(ks) + Fp8Unit::exponent(vs);
+        if (F16 && whole) {
+            unit.fit<NC>(acc, by, true);
+        }
         f32x16_t sc = f32x16_t{0.0f};
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-            const Fp8Pair kk = fp8_widen<Tag>(st.k[n], ks);
+            const Fp8Pair kk = fp8_widen<Tag>(st.k[n], F16 ? 1.0f : ks);
             sc = mfma32<Tag>(kk.lo, q[n][0], sc);
             sc = mfma32<Tag>(kk.hi, q[n][1], sc);
         }
         const int end = c0 + kFp8Block;
-        const bool whole = whole_blocks.has(blk);
         // P goes into the second product rounded to the type of q.  What that leaves of half the keys (0 .. 7 and 16 .. 23 of a block) goes into a
         // product of its own, so that P adds less to the error than the output's rounding: bf16 outputs of few rows would else be 1.4 to
         // 1.5 times as far off as rounding them alone, and are 1.2 times.  (64 rows of one query 74 us without, 77; 32 x 4 pairs of 49 .. 64 rows
@@ -526,13 +637,19 @@ __global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wav
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float x = sc[i];
-            w[i] = x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * a.c_exp));
+            w[i] = F16 ? x : x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * a.c_exp));
         }
         if (!whole) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 w[i] = sees_key(c0 + 16 * half + i) ? w[i] : 0.0f;
             }
+            if constexpr (F16) {
+                unit.fit<NC>(acc, by, fp8_some_score(w));
+            }
+        }
+        if constexpr (F16) {
+            fp8_weights_in_units(w, a.c_exp, Fp8Unit::exponent(ks), most_scale, unit.denominator(by));
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -546,12 +663,15 @@ __global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wav
                 }
             }
         }
-        float top = 0.0f;
+        bool beyond = !unit.finite;  // what is infinite in the type of q leaves nothing, not NaN
+        if constexpr (!F16) {
+            float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            top = __builtin_fmaxf(top, __builtin_fabsf(w[i]));
+            for (int i = 0; i < 8; ++i) {
+                top = __builtin_fmaxf(top, __builtin_fabsf(w[i]));
+            }
+            beyond = top > 3.3895314e38f;
         }
-        const bool beyond = top > (__is_same(Tag, bf16_tag) ? 3.3895314e38f : 65504.0f);  // (infinite in the type of q: nothing is left, not NaN)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             rest[i] = beyond ? 0u : rest[i];
@@ -585,7 +705,7 @@ __global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wav
         }
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-            const Fp8Pair vv = fp8_widen<Tag>(st.v[n], vs);
+            const Fp8Pair vv = fp8_widen<Tag>(st.v[n], F16 ? 1.0f : vs);
             acc[n] = mfma32<Tag>(vv.lo, p[0], acc[n]);
             acc[n] = mfma32<Tag>(vv.hi, p[1], acc[n]);
             acc[n] = mfma32<Tag>(vv.lo, rest, acc[n]);
@@ -593,7 +713,7 @@ __global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wav
         if constexpr (WEIGHTS) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                w[i] = __builtin_fabsf(w[i]);
+                w[i] = F16 ? __builtin_fabsf(w[i]) * unit.weight(Fp8Unit::exponent(vs)) : __builtin_fabsf(w[i]);
             }
             const float all = fp8_key_sum(w, lane) * __builtin_fabsf(a.c_out);
             fp8_store_key_sum(a, all, lane, pair, tile, a.row_tiles, blk, lin);
@@ -633,7 +753,11 @@ __global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wav
         }
     }
 
+    if constexpr (F16) {
+        unit.undo<NC>(acc);
+    }
     // ---- the sum over the wavefronts that shared the keys, and the store ----
+    const int lane_e = lane_here(), tid_e = 64 * wk + lane_e, half_e = lane_e >> 5;
     const bool partial = parts_used > 1 && deal.parts > 1;
     float* const to_partial = a.partial + (static_cast<int64_t>(deal.slot * c.n_heads + g) * a.row_tiles + tile) * TILE * dim;
 #pragma unroll
@@ -642,13 +766,13 @@ __global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wav
 #pragma unroll
         for (int i = 0; i < 4; ++i) {  // (16 bytes at a time, their places exchanged so that neither side has bank conflicts)
             const f32x4_t x = {acc[n][4 * i], acc[n][4 * i + 1], acc[n][4 * i + 2], acc[n][4 * i + 3]};
-            *reinterpret_cast<f32x4_t*>(s + wk * CHUNK_WORDS + 4 * (i * 64 + (lane ^ (2 * i + 8 * half)))) = x;
+            *reinterpret_cast<f32x4_t*>(s + wk * CHUNK_WORDS + 4 * (i * 64 + (lane_e ^ (2 * i + 8 * half_e)))) = x;
         }
         __syncthreads();
         constexpr int FOURS = CHUNK_WORDS / 4;
 #pragma unroll
         for (int r = 0; r < (FOURS + T - 1) / T; ++r) {  // four dims per lane, eight lanes together the 32 of a row
-            const int four = tid + r * T, i = four & 3, h = (four >> 2) & 1, row = four >> 3, mr = m0 + row, d = 32 * n + 16 * h + 4 * i;
+            const int four = tid_e + r * T, i = four & 3, h = (four >> 2) & 1, row = four >> 3, mr = m0 + row, d = 32 * n + 16 * h + 4 * i;
             if (four < FOURS && mr < n_pairs_rows && d < dim) {
                 f32x4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll

@@ -50,6 +50,21 @@ __device__ __forceinline__ int fp8_block(const Fp8Cache& c, const void* ids, int
     return static_cast<uint64_t>(id) < static_cast<uint64_t>(c.num_pages) ? static_cast<int>(at) : -1;
 }
 
+// This lane's number, worked out where it stands: for what follows a loop, which would else keep a register through it.
+__device__ __forceinline__ int lane_here()
+{
+    uint32_t none = 0;
+    asm volatile("" : "+s"(none));
+    return static_cast<int>(__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none)));
+}
+
+// A value that is the same in all lanes, and what is worked out from it, likewise.
+__device__ __forceinline__ int here(int x)
+{
+    asm volatile("" : "+s"(x));
+    return x;
+}
+
 // A block's scale from the bits of the largest finite magnitude in it: the smallest power of two, from 2^-126 up, that brings it
 // to at most 448 = 1.75 * 2^8; 1 for a block of zeros.  Returned as the exponent field of the scale.
 __device__ __forceinline__ uint32_t fp8_scale_field(uint32_t top)

@@ -22,6 +22,7 @@ template <typename Tag, int NC>
 __global__ __launch_bounds__(kFp8TileThreads) __attribute__((amdgpu_waves_per_eu(3, 3))) void hstu_paged_fp8_tile_kernel(const Fp8AttendArgs a)
 {
     constexpr int T = kFp8TileThreads, RG = T / 64, TILE = kFp8TileRows;
+    constexpr bool F16 = __is_same(Tag, f16_tag);
     constexpr int CHUNKS = (2 * NC + RG - 1) / RG;  // chunks of 1 KiB of codes that a wavefront brings in per block
     constexpr int FRAG = 64 * 16;                   // bytes of an operand: 16 per lane
     constexpr int BUFFER = 2 * NC * FRAG;           // K or V of a block, 16 bits a value
@@ -176,7 +177,7 @@ __global__ __launch_bounds__(kFp8TileThreads) __attribute__((amdgpu_waves_per_eu
         for (int i = 0; i < CHUNKS; ++i) {
             const int n = rg + RG * i;
             if (n < 2 * NC) {
-                const Fp8Pair x = fp8_widen<Tag>(from[i], n < NC ? ks : vs);
+                const Fp8Pair x = fp8_widen<Tag>(from[i], F16 ? 1.0f : (n < NC ? ks : vs));
                 uint8_t* const to = (n < NC ? to_k + 2 * n * FRAG : to_v + 2 * (n - NC) * FRAG) + lane * 16;
                 *reinterpret_cast<u32x4_t*>(to) = x.lo;
                 *reinterpret_cast<u32x4_t*>(to + FRAG) = x.hi;
@@ -215,14 +216,17 @@ __global__ __launch_bounds__(kFp8TileThreads) __attribute__((amdgpu_waves_per_eu
         }
         __builtin_amdgcn_sched_barrier(0);
     };
+    Fp8Unit unit(q, dim);  // (fp16)
+    const int most_scale = fp8_most_scale(a.c_exp);
     const auto weigh = [&](int t) {
         const int blk = block_of(t), c0 = blk * kFp8Block;
         float w[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float x = sc[i];
-            w[i] = x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * a.c_exp));
+            w[i] = F16 ? x : x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * a.c_exp));
         }
+        bool sees = true;  // (this lane's row, a key of the block)
         if (t >= mine || !whole.has(blk)) {
             const int end = t < mine ? lim : 0;
 #pragma unroll
@@ -230,6 +234,12 @@ __global__ __launch_bounds__(kFp8TileThreads) __attribute__((amdgpu_waves_per_eu
                 const int j = c0 + 16 * half + i;
                 w[i] = ((j < end) & ((j < mask.first_key) | (j >= hole)) & ((j >= low) | (j < mask.sinks))) ? w[i] : 0.0f;
             }
+            sees = F16 && fp8_some_score(w);
+        }
+        if constexpr (F16) {
+            const int k = Fp8Unit::exponent(scale_of(ks_a, ks_b, t)), v = Fp8Unit::exponent(scale_of(vs_a, vs_b, t));
+            unit.fit<NC>(acc, k + v, sees);  // (the sums are of the blocks before this one)
+            fp8_weights_in_units(w, a.c_exp, k, most_scale, unit.denominator(k + v));
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -284,7 +294,7 @@ __global__ __launch_bounds__(kFp8TileThreads) __attribute__((amdgpu_waves_per_eu
     // (a flag where K and V were)
     int* const s_poison = reinterpret_cast<int*>(s_mem);
     __syncthreads();
-    if (tid == 0) {
+    if (rg == 0 && lane_here() == 0) {
         *s_poison = 0;
     }
     __syncthreads();
@@ -295,20 +305,21 @@ __global__ __launch_bounds__(kFp8TileThreads) __attribute__((amdgpu_waves_per_eu
     const bool any_poison = *s_poison != 0;
     __syncthreads();  // (the sums go there next)
     if (any_poison) {
-        uint32_t v_at[NC];
-#pragma unroll
-        for (int n = 0; n < NC; ++n) {
-            v_at[n] = 32 * n + pi < dim ? static_cast<uint32_t>(32 * n + pi) * kFp8Block + 16 * half : kOutOfRange;
-        }
+        const int lane_p = lane_here(), col_p = lane_p & 31, half_p = lane_p >> 5, pi_p = 16 * ((col_p >> 2) & 1) + 4 * (col_p >> 3) + (col_p & 3);
+        const uint32_t v_at = static_cast<uint32_t>(pi_p) * kFp8Block + 16 * half_p;
         for (int s = 0; s < mine; ++s) {
             const int blk = block_of(s);
             if (!tile_whole.has(blk)) {
-                fp8_poison<Tag, NC>(acc, c, uniform(fp8_block(c, c.page_ids, seq.first, g, blk)), v_at, blk * kFp8Block + 16 * half, seq.len, sees_key);
+                fp8_poison<Tag, NC>(acc, c, uniform(fp8_block(c, c.page_ids, seq.first, g, blk)), v_at, blk * kFp8Block + 16 * half_p, seq.len, sees_key);
             }
         }
     }
 
+    if constexpr (F16) {
+        unit.undo<NC>(acc);
+    }
     // ---- the store ----
+    const int lane_e = lane_here(), tid_e = 64 * rg + lane_e, half_e = lane_e >> 5, ratio = here(a.ratio);
     const bool partial = parts_used > 1 && deal.parts > 1;
     float* const to_partial = a.partial + (static_cast<int64_t>(deal.slot * c.n_heads + g) * a.row_tiles + tile) * TILE * dim;
 #pragma unroll
@@ -317,12 +328,12 @@ __global__ __launch_bounds__(kFp8TileThreads) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
         for (int i = 0; i < 4; ++i) {  // (16 bytes at a time, their places exchanged so that neither side has bank conflicts)
             const f32x4_t x = {acc[n][4 * i], acc[n][4 * i + 1], acc[n][4 * i + 2], acc[n][4 * i + 3]};
-            *reinterpret_cast<f32x4_t*>(s + rg * 1024 + 4 * (i * 64 + (lane ^ (2 * i + 8 * half)))) = x;
+            *reinterpret_cast<f32x4_t*>(s + rg * 1024 + 4 * (i * 64 + (lane_e ^ (2 * i + 8 * half_e)))) = x;
         }
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < 4; ++r) {  // four dims per lane, eight lanes together the 32 of a row
-            const int word = tid + r * T, i = word & 3, h = (word >> 2) & 1, row_in = word >> 3;
+            const int word = tid_e + r * T, i = word & 3, h = (word >> 2) & 1, row_in = word >> 3;
             const float* const from = s + (row_in >> 5) * 1024 + 4 * (i * 64 + ((32 * h + (row_in & 31)) ^ (2 * i + 8 * h)));
             const f32x4_t x = *reinterpret_cast<const f32x4_t*>(from);
             const int row = t0 + row_in, d = 32 * n + 16 * h + 4 * i;
@@ -330,8 +341,8 @@ __global__ __launch_bounds__(kFp8TileThreads) __attribute__((amdgpu_waves_per_eu
                 if (partial) {
                     *reinterpret_cast<f32x4_t*>(to_partial + static_cast<int64_t>(row_in) * dim + d) = x;
                 } else {
-                    const int ir = div_small(row, a.ratio);
-                    const int64_t at = ((item.q0 + ir) * a.n_heads_q + g * a.ratio + (row - ir * a.ratio)) * static_cast<int64_t>(dim) + d;
+                    const int ir = div_small(row, ratio);
+                    const int64_t at = ((item.q0 + ir) * a.n_heads_q + g * ratio + (row - ir * ratio)) * static_cast<int64_t>(dim) + d;
                     *reinterpret_cast<u32x2_t*>(out + at) = u32x2_t{pack2<Tag>(x[0] * a.c_out, x[1] * a.c_out), pack2<Tag>(x[2] * a.c_out, x[3] * a.c_out)};
                 }
             }

@@ -1,0 +1,106 @@
+"""The 8-bit paged cache away from magnitudes of one: what a cache holds has no type, so a call must do with it what the definition says
+whatever the type of q holds.  Against the definition in 64 bits (paged_fp8_reference), or bit for bit where powers of two move from one factor to
+another."""
+
+import numpy as np
+import pytest
+import torch
+
+import ops_rec
+import paged_fp8_reference as R
+from test_gpu_paged_fp8 import DEV, TYPES, call, check, compare, queries
+from test_gpu_paged_fp8_tiles import MOST
+
+pytestmark = pytest.mark.gpu
+OPS = ops_rec.ascendc.attention
+# the kernel that shares keys, the same in parts and with weights, the one of half the wavefronts, the one of tiles of 128 rows (lens, counts, dim, more)
+KERNELS = pytest.mark.parametrize("lens,counts,dim,kw", [
+    ([300, 140], [40, 7], 64, {}), ([9000, 40], [1, 3], 64, {}), ([300, 140], [70, 7], 128, dict(weights=True)), ([300, 140], [70, 7], 64, dict(max_q=MOST)),
+    ([300, 140, 77, 40], [70, 7, 77, 1], 128, dict(max_q=MOST)), ([300, 140], [5, 7], 256, {})], ids=["keys", "parts", "weights", "half", "tile", "d256"])  # fmt: skip
+
+
+def cache(lens, dim, seed=1, **kw):
+    return R.make(lens, dim=dim, heads_k=2, page=64, seed=seed, device=DEV, **kw)
+
+
+@TYPES
+@KERNELS
+@pytest.mark.parametrize("shift", [-40, -9, 17, 60])
+def test_a_power_of_two_in_the_scales_is_one_in_the_result(lens, counts, dim, kw, dtype, shift):
+    """V 2^shift as large and silu_scale as much smaller, K and alpha likewise: no product changes but by that power, so no bit of the result does."""
+    kw, scale, alpha = dict(kw), 1 / 64, 1 / 16
+    weights = kw.pop("weights", False)
+    q, offs = queries(counts, 2, dim, dtype), R.offsets(counts, device=DEV)
+
+    def run(k_shift, v_shift):
+        c = cache(lens, dim)
+        c["k_scale"] *= 2.0**k_shift
+        c["v_scale"] *= 2.0**v_shift
+        w = torch.zeros_like(c["weights"]) if weights else None
+        return call(c, q, offs, counts, alpha=alpha * 2.0**-k_shift, silu_scale=scale * 2.0**-v_shift, weights=w, **kw), w
+
+    want, want_w = run(0, 0)
+    assert want.isfinite().all() and want.any()
+    for k_shift, v_shift in ((shift, 0), (0, shift), (shift, -shift)):
+        got, w = run(k_shift, v_shift)
+        assert torch.equal(got, want)
+        assert not weights or torch.equal(w * 2.0**v_shift, want_w)
+
+
+@KERNELS
+@pytest.mark.parametrize("targets", [False, True], ids=["causal", "targets"])
+def test_values_past_the_type_of_q(lens, counts, dim, kw, targets):
+    """Values of up to some 1e6 read by fp16 rows, half the blocks of them so: finite outputs are finite, and no row has anything of what it does not see."""
+    c = cache(lens, dim)
+    c["v_scale"].view(-1)[::2] *= 2.0**14
+    kw = dict(kw, targets=[min(n, 30) for n in counts], group=1) if targets else kw
+    check(lens, counts, dim=dim, dtype=torch.float16, cache=c, seed=1, silu_scale=1e-7, **kw)
+
+
+@KERNELS
+def test_keys_and_scores_past_the_type_of_q(lens, counts, dim, kw):
+    """Keys of up to some 1e6, and scores of a few 1e6, whose weights are scaled down to a type that ends at 65504."""
+    c = cache(lens, dim)
+    c["k_scale"] *= 2.0**16
+    check(lens, counts, dim=dim, dtype=torch.float16, cache=c, seed=1, alpha=1.0, silu_scale=1e-10, **kw)
+
+
+@KERNELS
+def test_rows_of_very_different_weights(lens, counts, dim, kw):
+    """Rows of q from 2^-16 to 2^-1 beside each other, blocks of V over 2^16: a row's error is in proportion to its own weights."""
+    kw = dict(kw)
+    weights = kw.pop("weights", False)
+    c = cache(lens, dim)
+    n = c["v_scale"].view(-1)
+    n *= torch.exp2(torch.arange(n.numel(), device=DEV) * 5 % 17 - 8)
+    q, offs = queries(counts, 2, dim, torch.float16), R.offsets(counts, device=DEV)
+    q *= torch.exp2(torch.arange(len(q), device=DEV) * 7 % 16 - 16.0).view(-1, 1, 1).half()
+    want, off, *_ = R.book(c).attend(q, offs, c["cache_len"], kw.get("max_q", max(counts)), alpha=1.0, silu_scale=2.0**-4)
+    # A weight times its block's scale goes into the product as a multiple of 2^-24 of a unit, which rounds by half of that.  The unit puts a bound of
+    # the row's scores, 448 dim times its largest value, with the scale of V at 2^12.8 or above (powers of two that may each be almost twice
+    # what they bound); codes of V are at most 448.
+    book, o = R.book(c), offs.tolist()
+    for b, s_k in enumerate(lens):
+        for h in range(2):
+            top = [np.nanmax(scale) for scale in book.scales]
+            bound = 448 * dim * abs(q[o[b] : o[b + 1], h].cpu().double().numpy()).max(1, keepdims=True) * top[0] * top[1]
+            off[o[b] : o[b + 1], h] += 2.0**-4 * bound * 2.0 ** (-25 - 12.8) * 448 * s_k
+    w = torch.zeros_like(c["weights"]) if weights else None
+    compare(call(c, q, offs, counts, alpha=1.0, silu_scale=2.0**-4, weights=w, **kw), want, off)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16-in-the-cache"])
+@pytest.mark.parametrize("dim,max_q", [(64, None), (128, MOST)], ids=["keys", "tile"])
+def test_candidates_at_the_top_of_fp16(dim, max_q, dtype):
+    """Rows of +-65504, whose codes stand for 65536, and what a cache written in bf16 holds beyond, in one candidate: the others do not see it."""
+    lens, counts, targets = [200, 200, 200, 200], [40] * 4, [30] * 4
+    c = R.make([n - m for n, m in zip(lens, counts)], room=lens, dim=dim, heads_k=2, page=64, seed=2, device=DEV)
+    g = torch.Generator().manual_seed(3)
+    k, v = (torch.randn(160, 2, dim, generator=g).to(dtype).to(DEV) for _ in range(2))
+    top = 65504.0 if dtype == torch.float16 else 3e5
+    v[20, :, ::3], v[20, :, 1::3], v[60, :, 5], k[100, 0, 7] = top, -top, 63488.0, top
+    offs = R.offsets(counts, device=DEV)
+    OPS.hstu_paged_fp8_append(k, v, c["k_cache"], c["v_cache"], c["k_scale"], c["v_scale"], offs, c["cache_len"], c["page_offsets"], c["page_ids"], 40)
+    c["cache_len"] = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    got = check(lens, counts, dim=dim, dtype=torch.float16, cache=c, seed=4, targets=targets, group=1, alpha=2.0**-20, silu_scale=2.0**2, max_q=max_q)
+    assert got.isfinite().all()
