@@ -64,14 +64,15 @@ __device__ __forceinline__ Fp8Pair fp8_widen(u32x4_t codes, float scale)
 // in rows that do not see the key; below 2^-14 it would be rounded), nor what a weight may be before alpha and silu_scale.  So for rows of fp16
 // the products run on the codes themselves, which fp16 holds exactly.  A block's scale of K goes into the exponent of silu, and the weights go
 // into the second product times both scales, in units of their row's own.  Of a row of dim values up to m a score in units of K's scale is at most
-// 448 dim m; the unit is the power of two that puts this bound, times the largest product of both scales of the blocks that the row has seen a key
-// of, below 2^15, and grows, the row's sums with it, when a block has a larger one.  Weights are then rounded to multiples of 2^-24 of a unit at
-// worst, 2^-37 of what the bound says, where a score's own sum in fp32 is good to 2^-24 of it.  (A row is a column of the result: a lane holds of its
-// own row only, and so does the lane of the same row in the other half.)  It costs no instruction an element: x / (1 + e) * 2^n is
-// x / (e 2^-n + 2^-n).  bf16 reaches as far as fp32 and needs none of this.
+// 448 dim m; the unit is a power of two that puts this bound, times the scales of a block that the row has seen a key of, below 2^11, and is
+// changed, the row's sums with it, by a block whose scales' product is 2^5 times that block's or more, or less than 2^-8 of it.  Weights are then rounded to
+// multiples of 2^-24 of a unit at worst, 2^-25 of what the bound says for their block; a score's own sum in fp32 is good to 2^-24 of it.  (A row is a column
+// of the result: a lane holds of its own row only, and so does the lane of the same row in the other half.  Nothing that a row does not see changes
+// its unit, and a block that holds one value of 1e30 leaves the sums of other blocks as they are.)  It costs no instruction an
+// element: x / (1 + e) * 2^n is x / (e 2^-n + 2^-n).  bf16 reaches as far as fp32 and needs none of this.
 struct Fp8Unit {
-    int most;     // exponents of a block's two scales may add up to `most` - `up`
-    int up;       // the unit is 2^-up; ahead of the first block smaller than any needs
+    int own;      // exponent of the unit's reciprocal for a block with scales of 1
+    int up;       // and as it is: the unit is 2^-up; ahead of the first block one that none fits
     bool finite;  // the row
     static __device__ __forceinline__ int exponent(float power_of_two) { return static_cast<int>(__builtin_bit_cast(uint32_t, power_of_two) >> 23 & 0xffu) - 127; }
     // what `x` is in the two lanes of this lane's row, the larger of them
@@ -97,17 +98,17 @@ struct Fp8Unit {
         const uint32_t a = top[0], b = top[1], m = of_row(a > b ? a : b);
         finite = m < 0x7c00u;
         const int bits = 32 - __builtin_clz(static_cast<uint32_t>(dim) - 1);  // dim <= 2^bits, codes <= 2^9
-        most = 15 - (__builtin_amdgcn_frexp_expf(lo_to_float<f16_tag>(m)) + 9 + bits);
-        up = most + 1024;
+        own = 11 - (__builtin_amdgcn_frexp_expf(lo_to_float<f16_tag>(m)) + 9 + bits);
+        up = own + 1024;
     }
-    // Makes the unit large enough for a block whose scales' exponents add up to `by`, of which this row sees keys (`sees`, the same in both lanes of
+    // Makes the unit fit a block whose scales' exponents add up to `by`, of which this row sees keys (`sees`, the same in both lanes of
     // a row).
     template <int NC>
     __device__ __forceinline__ void fit(f32x16_t (&acc)[NC], int by, bool sees)
     {
-        const bool small = sees & (up + by > most);
-        if (__any(small)) {
-            const int change = small ? most - by - up : 0;
+        const bool other = sees & (static_cast<uint32_t>(up + by - own + 8) > 12u);
+        if (__any(other)) {
+            const int change = other ? own - by - up : 0;
             up += change;
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
@@ -118,8 +119,8 @@ struct Fp8Unit {
             }
         }
     }
-    // What the denominators of a block's weights are multiplied by.  (`most` is at most 30; of a score, below 2^33, 2^-64 leaves nothing in fp16; a
-    // row that sees no key of the block has scores of zero.)
+    // What the denominators of a block's weights are multiplied by.  (For a row that sees a key of the block it is between 2^-30 and 2^25; one that
+    // does not has scores of zero.)
     __device__ __forceinline__ float denominator(int by) const
     {
         const int n = up + by;

@@ -76,31 +76,36 @@ def test_rows_of_very_different_weights(lens, counts, dim, kw):
     q, offs = queries(counts, 2, dim, torch.float16), R.offsets(counts, device=DEV)
     q *= torch.exp2(torch.arange(len(q), device=DEV) * 7 % 16 - 16.0).view(-1, 1, 1).half()
     want, off, *_ = R.book(c).attend(q, offs, c["cache_len"], kw.get("max_q", max(counts)), alpha=1.0, silu_scale=2.0**-4)
-    # A weight times its block's scale goes into the product as a multiple of 2^-24 of a unit, which rounds by half of that.  The unit puts a bound of
-    # the row's scores, 448 dim times its largest value, with the scale of V at 2^12.8 or above (powers of two that may each be almost twice
-    # what they bound); codes of V are at most 448.
+    # A weight times its block's scales goes into the product as a multiple of 2^-24 of a unit, which rounds by half of that.  The unit puts a bound of
+    # the row's scores, 448 dim times its largest value, with the scales of the block at 2^0.8 or above (2^11 / 2^8, and powers of two that
+    # may be almost twice what they bound); codes of V are at most 448.
     book, o = R.book(c), offs.tolist()
     for b, s_k in enumerate(lens):
         for h in range(2):
-            top = [np.nanmax(scale) for scale in book.scales]
-            bound = 448 * dim * abs(q[o[b] : o[b + 1], h].cpu().double().numpy()).max(1, keepdims=True) * top[0] * top[1]
-            off[o[b] : o[b + 1], h] += 2.0**-4 * bound * 2.0 ** (-25 - 12.8) * 448 * s_k
+            products = np.concatenate([(book.scales[0] * book.scales[1])[pid, h] for pid in book._pages(b)])[: -(-s_k // 32)]
+            bound = 448 * dim * abs(q[o[b] : o[b + 1], h].cpu().double().numpy()).max(1, keepdims=True) * products.sum() * 32
+            off[o[b] : o[b + 1], h] += 2.0**-4 * bound * 2.0 ** (-25 - 0.8) * 448
     w = torch.zeros_like(c["weights"]) if weights else None
     compare(call(c, q, offs, counts, alpha=1.0, silu_scale=2.0**-4, weights=w, **kw), want, off)
 
 
-@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16-in-the-cache"])
+@pytest.mark.parametrize("dtype,top", [(torch.float16, 65504.0), (torch.bfloat16, 3e5), (torch.bfloat16, 1e30)], ids=["fp16", "bf16-in-the-cache", "1e30"])
 @pytest.mark.parametrize("dim,max_q", [(64, None), (128, MOST)], ids=["keys", "tile"])
-def test_candidates_at_the_top_of_fp16(dim, max_q, dtype):
+def test_candidates_past_fp16(dim, max_q, dtype, top):
     """Rows of +-65504, whose codes stand for 65536, and what a cache written in bf16 holds beyond, in one candidate: the others do not see it."""
     lens, counts, targets = [200, 200, 200, 200], [40] * 4, [30] * 4
     c = R.make([n - m for n, m in zip(lens, counts)], room=lens, dim=dim, heads_k=2, page=64, seed=2, device=DEV)
     g = torch.Generator().manual_seed(3)
     k, v = (torch.randn(160, 2, dim, generator=g).to(dtype).to(DEV) for _ in range(2))
-    top = 65504.0 if dtype == torch.float16 else 3e5
     v[20, :, ::3], v[20, :, 1::3], v[60, :, 5], k[100, 0, 7] = top, -top, 63488.0, top
     offs = R.offsets(counts, device=DEV)
     OPS.hstu_paged_fp8_append(k, v, c["k_cache"], c["v_cache"], c["k_scale"], c["v_scale"], offs, c["cache_len"], c["page_offsets"], c["page_ids"], 40)
     c["cache_len"] = torch.tensor(lens, dtype=torch.int32, device=DEV)
-    got = check(lens, counts, dim=dim, dtype=torch.float16, cache=c, seed=4, targets=targets, group=1, alpha=2.0**-20, silu_scale=2.0**2, max_q=max_q)
-    assert got.isfinite().all()
+    q, tgt = queries(counts, 2, dim, torch.float16, 4), torch.tensor(targets, dtype=torch.int32, device=DEV)
+    kw = dict(group=1, alpha=2.0**-20, silu_scale=2.0**2)
+    want, off, *_ = R.book(c).attend(q, offs, c["cache_len"], 40, num_target=tgt, **kw)
+    got = call(c, q, offs, counts, num_target=tgt, max_q=max_q, **kw)
+    small = torch.from_numpy(abs(want) < 60000)
+    assert small[19].all() and small[21].all() and (top > 1e9 or small.all())
+    compare(got.cpu()[small], want[small], off[small])
+    assert (got.cpu()[torch.from_numpy(abs(want) > 66000)].isinf()).all()
