@@ -586,8 +586,9 @@ __global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wav
         const int s = base + lane < n_steps ? base + lane : n_steps - 1;
         my_lin = fp8_block(c, c.page_ids, seq.first, g, runs.block(n_begin + wk + s * WK));
         const int at = my_lin >= 0 ? my_lin : 0;
-        my_ks = c.k_scale[at];
-        my_vs = c.v_scale[at];
+        const float ks = c.k_scale[at], vs = c.v_scale[at];
+        my_ks = my_lin >= 0 ? ks : 1.0f;  // (a page that is none holds zeros, and zero times what another block has may not be that)
+        my_vs = my_lin >= 0 ? vs : 1.0f;
     };
     const auto place_of = [&](int s) { return __builtin_amdgcn_readlane(my_lin, s & 63); };
 

@@ -121,8 +121,9 @@ __global__ __launch_bounds__(kFp8TileThreads) __attribute__((amdgpu_waves_per_eu
         if (first < mine) {
             const int s = first + lane < mine ? first + lane : mine - 1;
             const int at = fp8_block(c, c.page_ids, seq.first, g, block_of(s));
-            ks = c.k_scale[at >= 0 ? at : 0];
-            vs = c.v_scale[at >= 0 ? at : 0];
+            const float k_at = c.k_scale[at >= 0 ? at : 0], v_at = c.v_scale[at >= 0 ? at : 0];
+            ks = at >= 0 ? k_at : 1.0f;  // (a page that is none: zeros, see the other kernel)
+            vs = at >= 0 ? v_at : 1.0f;
             lin = first + lane < mine ? at : -1;
         }
     };

@@ -109,3 +109,16 @@ def test_candidates_past_fp16(dim, max_q, dtype, top):
     assert small[19].all() and small[21].all() and (top > 1e9 or small.all())
     compare(got.cpu()[small], want[small], off[small])
     assert (got.cpu()[torch.from_numpy(abs(want) > 66000)].isinf()).all()
+
+
+@TYPES
+@KERNELS
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), 2.0**100], ids=str)
+def test_pages_that_are_none_whatever_page_0_holds(lens, counts, dim, kw, dtype, scale):
+    """Page 0 is nobody's and holds anything; rows of pages that are not there count as zeros, their keys' weights as nothing."""
+    seed = next(i for i in range(1000) if 0 in R.make(lens, dim=32, heads_k=1, page=64, seed=i, spare=2)["free"])
+    c = cache(lens, dim, seed=seed)
+    c["k_scale"][0], c["v_scale"][0] = scale, scale
+    c["page_ids"][1], c["page_ids"][-1] = -1, 1 << 30
+    got = check(lens, counts, dim=dim, dtype=dtype, cache=c, seed=1, **kw)
+    assert got.isfinite().all()
