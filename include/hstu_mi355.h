@@ -334,8 +334,8 @@ HSTU_API const char* hstu_paged_fp8_fwd_kernel_name(const hstu_paged_fp8_fwd_par
 /*
  * Rows seq_offset[b] : seq_offset[b + 1] of k and v go to the positions cache_len[b], cache_len[b] + 1, ... of sequence b (cache_len is
  * not changed; rows that its pages have no room for are dropped).  Every block touched gets a new scale, the smallest power of two
- * that brings its largest finite magnitude, old rows included, to at most 448; codes round to nearest even, values that are not
- * finite become NaN.  The rows of a touched block behind the new end are cleared; weights of new rows and of those become 0.
+ * that brings its largest finite magnitude, old rows included, to at most 448; codes round to nearest even (but to 240 * 2^120, not 256 * 2^120,
+ * which no float holds), values that are not finite become NaN.  The rows of a touched block behind the new end are cleared; weights of new rows and of those become 0.
  */
 typedef struct hstu_paged_fp8_append_params {
     uint32_t struct_size; /* sizeof(hstu_paged_fp8_append_params) */

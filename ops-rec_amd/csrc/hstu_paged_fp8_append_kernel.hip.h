@@ -136,6 +136,15 @@ __global__ __launch_bounds__(kFp8AppendThreads) void hstu_paged_fp8_append_kerne
                 }
             }
         }
+        if (field == kFp8TopField) {
+#pragma unroll
+            for (int i = 0; i < KP; ++i) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    w[i][j] = fp8_below_infinity(w[i][j]);
+                }
+            }
+        }
         if (lin >= 0) {  // (otherwise there is no such page: the rows have no place)
 #pragma unroll
             for (int i = 0; i < KP; ++i) {
@@ -250,6 +259,18 @@ __global__ __launch_bounds__(kFp8AppendThreads) void hstu_paged_fp8_append_kerne
                     const uint32_t cd = fp8_codes2<Tag, true>(raw[u][4 * j + 3], scale, fp8_codes2<Tag, false>(raw[u][4 * j + 2], scale, 0u));
                     w[u][0][j] = __builtin_amdgcn_perm(cd, ab, 0x06040200u);
                     w[u][1][j] = __builtin_amdgcn_perm(cd, ab, 0x07050301u);
+                }
+            }
+        }
+        if (field == kFp8TopField) {
+#pragma unroll
+            for (int u = 0; u < VP; ++u) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        w[u][e][j] = fp8_below_infinity(w[u][e][j]);
+                    }
                 }
             }
         }

@@ -79,6 +79,14 @@ __device__ __forceinline__ float fp8_scale_of(uint32_t field) { return __builtin
 // 1 / scale, exactly: fields 1 .. 247 have the reciprocals 253 .. 7
 __device__ __forceinline__ float fp8_inverse_of(uint32_t field) { return __builtin_bit_cast(float, (254u - field) << 23); }
 
+// Four codes over the largest scale, 2^120: 256 of it is no float any more (a value that is finite rounds to it from 248 on), so 256 becomes 240.
+constexpr uint32_t kFp8TopField = 247;
+__device__ __forceinline__ uint32_t fp8_below_infinity(uint32_t codes)
+{
+    const uint32_t other = (codes & 0x7f7f7f7fu) ^ 0x78787878u;  // of a code of +-256: zero
+    return codes - ((0x80808080u - other & 0x80808080u) >> 7);
+}
+
 // bits of the magnitude of a finite value, 0 of any other
 __device__ __forceinline__ uint32_t finite_bits(float x)
 {

@@ -189,7 +189,8 @@ def hstu_paged_fp8_append(k, v, k_cache, v_cache, k_scale, v_scale, seq_offset, 
     it is.  Rows that the sequence's pages have no room for, and rows past ``max_seq_len``, are dropped.
 
     Each block of 32 tokens that is written to gets a new scale: the smallest power of two that brings its largest finite
-    magnitude, old rows included, to at most 448.  Codes round to nearest even; values that are not finite become NaN.  The rows of a
+    magnitude, old rows included, to at most 448.  Codes round to nearest even, but never to what no float holds (256 times the largest scale,
+    2^120); values that are not finite become NaN.  The rows of a
     written block behind the new end are cleared, and the ``weights`` of new rows and of those, where given, become 0."""
     _check(k.dim() == 3 and v.dim() == 3, "The k and v should be 3D in jagged layout")
     _check(k.dtype in (torch.bfloat16, torch.float16) and v.dtype == k.dtype, f"k and v must both be bfloat16 or float16, but they are {k.dtype} and {v.dtype}")

@@ -122,3 +122,50 @@ def test_pages_that_are_none_whatever_page_0_holds(lens, counts, dim, kw, dtype,
     c["page_ids"][1], c["page_ids"][-1] = -1, 1 << 30
     got = check(lens, counts, dim=dim, dtype=dtype, cache=c, seed=1, **kw)
     assert got.isfinite().all()
+
+
+@pytest.mark.parametrize("old", [0, 3], ids=["new-block", "older-rows"])
+def test_rows_at_the_top_of_bf16(old):
+    """The largest values of bf16 lie nearer to 256 * 2^120, which no float holds, than to 240 * 2^120, which they become: finite in the cache, after another
+    append and after an eviction, and no row has anything of what it does not see."""
+    top, n, dim = 3.3895313892515355e38, 40, 64
+    c = R.make([old], room=[100], page=64, heads_k=2, dim=dim, seed=2, spare=3, device=DEV, poison=False)
+    tensors = c["k_cache"], c["v_cache"], c["k_scale"], c["v_scale"]
+    k, v = (torch.zeros(n, 2, dim, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    k[1, 0, :6] = v[1, 0, :6] = torch.tensor([top, -top, 248 * 2.0**120, 247 * 2.0**120, -232 * 2.0**120, float("inf")], device=DEV)
+    v[35, 1, 7] = top
+    want = torch.tensor([240.0, -240.0, 240.0, 240.0, -224.0, float("nan")], device=DEV)  # (232 is a tie)
+
+    def row(t, i, head):
+        block = t[int(c["page_ids"][i // 64]), head, i % 64 // 32].float()
+        return block[i % 32] if block.shape[0] == 32 else block[:, i % 32]
+
+    def check_rows():
+        for t, s in ((tensors[0], tensors[2]), (tensors[1].transpose(3, 4).contiguous(), tensors[3])):
+            torch.testing.assert_close(row(t, old + 1, 0)[:6], want, rtol=0, atol=0, equal_nan=True)
+            assert s[int(c["page_ids"][0]), 0, 0] == 2.0**120
+        assert row(tensors[1].transpose(3, 4).contiguous(), old + 35, 1)[7] == 240
+
+    def add(rows, at):
+        OPS.hstu_paged_fp8_append(rows[0], rows[1], *tensors, R.offsets([len(rows[0])], device=DEV), torch.tensor([at], dtype=torch.int32, device=DEV),
+                                  c["page_offsets"], c["page_ids"], n, c["weights"])  # fmt: skip
+
+    add((k, v), old)
+    check_rows()
+    add((k[:1], v[:1]), old + 2)  # (into the same block, which is put together again)
+    check_rows()
+    add((k[2:], v[2:]), old + 2)
+    check_rows()
+    c["cache_len"] = torch.tensor([old + n], dtype=torch.int32, device=DEV)
+    tensors[1].view(torch.uint8)[int(c["page_ids"][0]), 0, 0, 5, old + 1] = 0  # (the value that was infinite)
+    tensors[0].view(torch.uint8)[int(c["page_ids"][0]), 0, 0, old + 1, 5] = 0
+    q, offs = queries([n], 2, dim, torch.bfloat16), R.offsets([n], device=DEV)
+    tgt = torch.tensor([n], dtype=torch.int32, device=DEV)
+    got = call(c, q, offs, [n], num_target=tgt, group=1, alpha=2.0**-126, silu_scale=1.0)
+    others = [i for i in range(n) if i != 1]  # (scores of the row 1, sums of five products of some 3e38, are past fp32)
+    assert got[others].isfinite().all()
+    new = torch.tensor(c["free"][:2], dtype=torch.int32, device=DEV)
+    before = [tensors[2][int(c["page_ids"][0]), 0, 0].clone(), row(tensors[0], old + 1, 0).clone()]
+    OPS.hstu_paged_fp8_evict(*tensors, c["weights"], c["cache_len"], c["page_offsets"], c["page_ids"], torch.tensor([0, 2], dtype=torch.int32, device=DEV), new, 100, 100)
+    c["page_ids"] = new
+    assert torch.equal(before[1], row(tensors[0], old + 1, 0)) and tensors[2][int(new[0]), 0, 0] == before[0]
