@@ -355,7 +355,7 @@ HSTU_API int hstu_paged_fp8_append(const hstu_paged_fp8_append_params* params, v
 /*
  * Of each sequence at most `keep` rows stay (no more than the new pages hold): the first `sinks`, the last `recent`, and of the others
  * those with the largest scores, ties to the lower index; a score is the fp32 sum of a row's weights over the key heads, in
- * their order.  cache_len is cut at max_seq_len_k.  The rows that stay are moved in order to the new pages (new_page_ids[new_page_offsets[b] : ...]), with new
+ * their order, NaN counting as -infinity.  cache_len is cut at max_seq_len_k.  The rows that stay are moved in order to the new pages (new_page_ids[new_page_offsets[b] : ...]), with new
  * scales and their weights; new_cache_len[b] is their number, kept[b] their old indices, -1 behind them.
  */
 typedef struct hstu_paged_fp8_evict_params {

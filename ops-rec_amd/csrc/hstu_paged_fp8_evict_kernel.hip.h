@@ -5,13 +5,10 @@
 
 namespace hstu {
 
-// A score as an integer that compares as the score does (larger is larger): NaN below everything, the two zeros the same.
+// A score as an integer that compares as the score does (larger is larger): NaN as -infinity, the two zeros the same.
 __device__ __forceinline__ uint32_t score_key(float s)
 {
-    if (s != s) {
-        return 0u;
-    }
-    const uint32_t bits = __builtin_bit_cast(uint32_t, s + 0.0f);
+    const uint32_t bits = __builtin_bit_cast(uint32_t, s == s ? s + 0.0f : -__builtin_inff());
     return (bits & 0x80000000u) != 0 ? ~bits : bits | 0x80000000u;
 }
 

@@ -224,7 +224,7 @@ def hstu_paged_fp8_evict(k_cache, v_cache, k_scale, v_scale, weights, cache_len,
                          max_seq_len_k, keep, sinks=0, recent=0):  # fmt: skip
     """Moves the rows worth keeping to other pages, ``new_page_ids[new_page_offsets[b] : new_page_offsets[b + 1]]`` of sequence ``b``: at
     most ``keep`` rows each (and no more than those pages hold) -- the first ``sinks``, the last ``recent``, and of the others those
-    with the largest sums of ``weights`` over the key heads, ties to the lower index -- in the order they were in, with scales of
+    with the largest sums of ``weights`` over the key heads, NaN counting as minus infinity, ties to the lower index -- in the order they were in, with scales of
     their new blocks and with their weights.  A sequence of no more than ``keep`` rows moves whole.  The old pages are only read: once
     the call is done (in the stream's order) they are the program's to hand out again.  New pages must be no pages that the call reads.
 

@@ -236,3 +236,18 @@ def test_sessions_on_two_streams():
             got.append(serve(c, steps, keep, 600))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for w, g in zip(want, got) for a, b in zip(w, g))
+
+
+@pytest.mark.parametrize("keep", [60, 100, 140, 180, 230])
+def test_scores_of_nan_rank_as_minus_infinity(keep):
+    """200 of 250 rows score NaN or -infinity, in turn: of those the first stay, whichever they are."""
+
+    def lowest(c, _):
+        pages = c["page_ids"].long()
+        for i in range(250):
+            if i % 5:
+                c["weights"][pages[i // 64], :, i % 64] = float("nan") if i % 2 else float("-inf")
+
+    _, _, kept, _, _ = check([250], keep, dim=16, change=lowest, seed=2)
+    lowest_kept = [i for i in kept[0].tolist() if i % 5]
+    assert lowest_kept == [i for i in range(250) if i % 5][: keep - 50]
