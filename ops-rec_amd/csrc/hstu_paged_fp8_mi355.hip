@@ -280,8 +280,10 @@ int check_evict(const hstu_paged_fp8_evict_params* p)
     return HSTU_OK;
 }
 
-// scores of the longest sequence allowed, in whole fours and where its first may be rounded down; none where LDS holds them
-int64_t evict_pitch(const hstu_paged_fp8_evict_params* p) { return p->max_seq_len_k + 8 <= kFp8SelectKeys ? 0 : ceil_div(p->max_seq_len_k, 4) * 4 + 8; }
+// rows that a sequence has at most: as many as are allowed, or as all the pages hold
+int64_t evict_rows(const hstu_paged_fp8_evict_params* p) { return std::min(p->max_seq_len_k, p->cache.n_page_ids * p->cache.page_size); }
+// scores of the longest sequence, in whole fours and where its first may be rounded down; none where LDS holds them
+int64_t evict_pitch(const hstu_paged_fp8_evict_params* p) { return evict_rows(p) + 8 <= kFp8SelectKeys ? 0 : ceil_div(evict_rows(p), 4) * 4 + 8; }
 uint64_t evict_workspace(const hstu_paged_fp8_evict_params* p) { return static_cast<uint64_t>(p->cache.n_offsets - 1) * evict_pitch(p) * 4; }
 
 }  // namespace
@@ -432,7 +434,7 @@ HSTU_API int hstu_paged_fp8_evict(const hstu_paged_fp8_evict_params* p, void* wo
     a.keys = static_cast<uint32_t*>(workspace);
     a.key_pitch = evict_pitch(p);
     a.n_new_page_ids = static_cast<int>(p->n_new_page_ids);
-    a.max_k = static_cast<int>(p->max_seq_len_k);
+    a.max_k = static_cast<int>(evict_rows(p));
     a.keep = static_cast<int>(p->keep);
     a.sinks = static_cast<int>(std::min<int64_t>(p->sinks, p->keep));
     a.recent = static_cast<int>(std::min<int64_t>(p->recent, p->keep));
@@ -440,10 +442,12 @@ HSTU_API int hstu_paged_fp8_evict(const hstu_paged_fp8_evict_params* p, void* wo
     const bool few = a.max_k <= kFp8SelectFew;
     const EvictKernel select = few ? kSelectFew : kSelect;
     hipLaunchKernelGGL(select, dim3(static_cast<unsigned>(a.c.n_batch)), dim3(few ? 256 : 1024), 0, s, a);
-    const int64_t most = std::min(p->keep, p->max_seq_len_k);
-    hipLaunchKernelGGL(kMove[dim_slot(a.c.dim)],
-                       dim3(static_cast<unsigned>(ceil_div(most, kBlock)), 2u * static_cast<unsigned>(a.c.n_heads), static_cast<unsigned>(a.c.n_batch)),
-                       dim3(kFp8AppendThreads), 0, s, a);
+    const int64_t most = std::min({p->keep, evict_rows(p), p->n_new_page_ids * p->cache.page_size});
+    if (most > 0) {
+        hipLaunchKernelGGL(kMove[dim_slot(a.c.dim)],
+                           dim3(static_cast<unsigned>(ceil_div(most, kBlock)), 2u * static_cast<unsigned>(a.c.n_heads), static_cast<unsigned>(a.c.n_batch)),
+                           dim3(kFp8AppendThreads), 0, s, a);
+    }
     return launched("hstu_paged_fp8_move_kernel");
 }
 

@@ -251,3 +251,10 @@ def test_scores_of_nan_rank_as_minus_infinity(keep):
     _, _, kept, _, _ = check([250], keep, dim=16, change=lowest, seed=2)
     lowest_kept = [i for i in kept[0].tolist() if i % 5]
     assert lowest_kept == [i for i in range(250) if i % 5][: keep - 50]
+
+
+@pytest.mark.parametrize("keep", [70, 100_000])
+def test_a_longest_length_without_a_limit(keep):
+    """(launches and workspace go by what the pages hold)"""
+    check([300, 77, 1100], keep, sinks=3, recent=20, seed=keep, max_k=1 << 24)
+    check([40001, 33], 10_000, sinks=3, recent=20, heads_k=1, dim=16, page=256, seed=keep, max_k=1 << 24)

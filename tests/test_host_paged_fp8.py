@@ -254,3 +254,14 @@ def test_the_attention_is_the_paged_oracle_s_on_the_same_values():
                                            seq_offset_k=R.offsets([70, 33]), num_target=targets, target_group_size=2, alpha=0.2, out_dtype=torch.float32)  # fmt: skip
     got, *_ = b.attend(q, R.offsets(counts), c["cache_len"], 12, 0.0, targets, 2, 0.2)
     np.testing.assert_allclose(got, want.double().numpy(), rtol=1e-4, atol=1e-4 * np.abs(got).max())
+
+
+def test_an_eviction_s_workspace_goes_by_what_the_pages_hold():
+    """A longest length without a limit asks for nothing that four pages of 64 rows cannot fill: scores that LDS holds need no workspace."""
+    lib, size = _native.load(), ctypes.c_uint64(1)
+    p = block(_native.PagedFp8EvictParams, max_seq_len_k=1 << 24, keep=1 << 24, n_offsets=2049)
+    assert lib.hstu_paged_fp8_evict_workspace_size(ctypes.byref(p), ctypes.byref(size)) == 0 and size.value == 0
+    p = block(_native.PagedFp8EvictParams, max_seq_len_k=1 << 24, n_page_ids=1000)
+    assert lib.hstu_paged_fp8_evict_workspace_size(ctypes.byref(p), ctypes.byref(size)) == 0 and 2 * 64000 * 4 <= size.value <= 2 * 64100 * 4
+    p = block(_native.PagedFp8EvictParams, max_seq_len_k=50000, n_page_ids=1000)
+    assert lib.hstu_paged_fp8_evict_workspace_size(ctypes.byref(p), ctypes.byref(size)) == 0 and 2 * 50000 * 4 <= size.value <= 2 * 50100 * 4
