@@ -169,3 +169,28 @@ def test_rows_at_the_top_of_bf16(old):
     OPS.hstu_paged_fp8_evict(*tensors, c["weights"], c["cache_len"], c["page_offsets"], c["page_ids"], torch.tensor([0, 2], dtype=torch.int32, device=DEV), new, 100, 100)
     c["page_ids"] = new
     assert torch.equal(before[1], row(tensors[0], old + 1, 0)) and tensors[2][int(new[0]), 0, 0] == before[0]
+
+
+def test_every_block_appended_past_32_bits():
+    """Blocks, scales and weights of pages beyond 4 GiB of the cache, the last block, which is written in part, among them; and nothing beside them."""
+    page, heads, dim = 256, 8, 128
+    n = (1 << 32) // (page * heads * dim) + 40
+    c = R.make([600], page=page, heads_k=heads, dim=dim, seed=1, device=DEV)
+    names, where = ("k_cache", "v_cache", "k_scale", "v_scale", "weights"), torch.tensor([n - 1, 3, n - 5], device=DEV)
+    raw = lambda t: t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t  # noqa: E731
+    big = dict(c, page_ids=where.to(torch.int32))
+    for name in names:
+        small = raw(c[name])
+        big[name] = torch.full((n, *small.shape[1:]), 7, dtype=small.dtype, device=DEV)
+        big[name][where] = small[c["page_ids"].long()]
+        big[name] = big[name].view(c[name].dtype)
+    k, v = (torch.randn(50, heads, dim, device=DEV).to(torch.bfloat16) for _ in range(2))
+    for t in (c, big):
+        OPS.hstu_paged_fp8_append(k, v, *(t[name] for name in names[:4]), R.offsets([50], device=DEV), t["cache_len"], t["page_offsets"], t["page_ids"], 50, t["weights"])
+    for name in names:
+        a, b = raw(c[name])[c["page_ids"].long()], raw(big[name])[where]
+        assert torch.equal(a.nan_to_num(-1.0) if a.is_floating_point() else a, b.nan_to_num(-1.0) if b.is_floating_point() else b)
+        for beside in (0, 2, 4, n - 6, n - 4, n - 2):
+            assert (raw(big[name])[beside] == 7).all()
+    book = R.book(dict(c, cache_len=torch.tensor([650])))
+    assert all(torch.from_numpy(book.rows(w, 0, h, 650)).isfinite().all() for w in (0, 1) for h in range(heads))
