@@ -40,9 +40,12 @@ _VGPR_FORM = ("-mllvm", "-amdgpu-mfma-vgpr-form=1")
 SOURCE_FLAGS = {"hstu_kernels_bwd_fused.hip": _VGPR_FORM, "hstu_kernels_fwd_pinned.hip": _VGPR_FORM}
 # The same where it is operands that stay in accumulators (the compiler knows of those: none is named).
 OPERAND_SOURCE_FLAGS = {"in_linear_silu_kernels_rows.hip": _VGPR_FORM}
-# And where nothing is pinned, but two columns of scores and outputs of up to 128 dims leave no register over for a score's way out
-# of an accumulator: without the form these kernels keep up to 220 bytes a lane in scratch memory, with it none.
-SCORE_SOURCE_FLAGS = {"hstu_paged_fp8_kernels_bf16.hip": _VGPR_FORM, "hstu_paged_fp8_kernels_f16.hip": _VGPR_FORM}
+# The attention kernels over the 8-bit paged cache pin nothing.  With rows of fp16, whose sums the vector unit scales, those of more than 128
+# dims have up to 112 bytes a lane in scratch memory and some 15000 moves from and to accumulators without the form, none and 2000 with it (8
+# sequences of 256 .. 512 rows on 2048 .. 8192 keys, d 256: 252 us without, 213 with it; d 192 184 and 154; 3 single rows on 30011 .. 120011 keys,
+# d 256, 59 and 57).  With rows of bf16 nothing is in scratch memory either way, and the same are faster without it (196 and 208, 146 and 153, 54.8
+# and 57.5); up to 128 dims it changes no register count.
+SCORE_SOURCE_FLAGS = {"hstu_paged_fp8_kernels_bf16.hip": (), "hstu_paged_fp8_kernels_f16.hip": _VGPR_FORM}
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
     "-O3",
