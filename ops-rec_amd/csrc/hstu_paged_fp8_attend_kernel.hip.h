@@ -108,7 +108,19 @@ struct Fp8Unit {
     {
         const bool other = sees & (static_cast<uint32_t>(up + by - own + 8) > 12u);
         if (__any(other)) {
-            const int change = other ? own - by - up : 0;
+            // (the sums stay below 2^100, of which a smaller unit for a block of far smaller scales would leave nothing finite)
+            float sum = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float x = acc[n][i];
+                    sum = __builtin_fmaxf(sum, __builtin_fabsf(x));
+                }
+            }
+            sum = __builtin_bit_cast(float, of_row(__builtin_bit_cast(uint32_t, sum)));
+            const int left = 100 - __builtin_amdgcn_frexp_expf(sum), room = sum > 0.0f ? (left > 0 ? left : 0) : 4096;
+            const int wanted = own - by - up, change = other ? (wanted < room ? wanted : room) : 0;
             up += change;
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
@@ -119,8 +131,8 @@ struct Fp8Unit {
             }
         }
     }
-    // What the denominators of a block's weights are multiplied by.  (For a row that sees a key of the block it is between 2^-30 and 2^25; one that
-    // does not has scores of zero.)
+    // What the denominators of a block's weights are multiplied by.  (One over it is at most 2^25 for a row that sees a key of the block, others have
+    // scores of zero; and of scores, below 2^33, 2^-64 leaves nothing in fp16.)
     __device__ __forceinline__ float denominator(int by) const
     {
         const int n = up + by;
@@ -759,7 +771,7 @@ __global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wav
         unit.undo<NC>(acc);
     }
     // ---- the sum over the wavefronts that shared the keys, and the store ----
-    const int lane_e = lane_here(), tid_e = 64 * wk + lane_e, half_e = lane_e >> 5;
+    const int lane_e = lane_here(), tid_e = 64 * wk + lane_e, half_e = lane_e >> 5, ratio = here(a.ratio);
     const bool partial = parts_used > 1 && deal.parts > 1;
     float* const to_partial = a.partial + (static_cast<int64_t>(deal.slot * c.n_heads + g) * a.row_tiles + tile) * TILE * dim;
 #pragma unroll
@@ -784,8 +796,8 @@ __global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wav
                 if (partial) {
                     *reinterpret_cast<f32x4_t*>(to_partial + static_cast<int64_t>(row) * dim + d) = x;
                 } else {
-                    const int ir = div_small(mr, a.ratio);
-                    const int64_t at = ((q0 + ir) * a.n_heads_q + g * a.ratio + (mr - ir * a.ratio)) * static_cast<int64_t>(dim) + d;
+                    const int ir = div_small(mr, ratio);
+                    const int64_t at = ((q0 + ir) * a.n_heads_q + g * ratio + (mr - ir * ratio)) * static_cast<int64_t>(dim) + d;
                     *reinterpret_cast<u32x2_t*>(out + at) = u32x2_t{pack2<Tag>(x[0] * a.c_out, x[1] * a.c_out), pack2<Tag>(x[2] * a.c_out, x[3] * a.c_out)};
                 }
             }

@@ -194,3 +194,16 @@ def test_every_block_appended_past_32_bits():
             assert (raw(big[name])[beside] == 7).all()
     book = R.book(dict(c, cache_len=torch.tensor([650])))
     assert all(torch.from_numpy(book.rows(w, 0, h, 650)).isfinite().all() for w in (0, 1) for h in range(heads))
+
+
+@TYPES
+@KERNELS
+@pytest.mark.parametrize("k_shift,v_shift", [(-66, -66), (-100, -100), (0, -110), (20, 60)], ids=str)
+def test_blocks_of_very_different_scales(lens, counts, dim, kw, dtype, k_shift, v_shift):
+    """Every third block nearly nothing (a cache written in bf16 holds it), or so large that an output is it: what the other blocks add stays."""
+    c = cache(lens, dim)
+    for name, shift in (("k_scale", k_shift), ("v_scale", v_shift)):
+        c[name].view(-1)[1::3] *= 2.0**shift
+    kw = dict(kw, silu_scale=2.0**-80) if v_shift > 0 and dtype == torch.float16 else kw
+    got = check(lens, counts, dim=dim, dtype=dtype, cache=c, seed=1, **kw)
+    assert got.isfinite().all() and (dtype == torch.bfloat16 or v_shift > 0 or got[1:].any())
