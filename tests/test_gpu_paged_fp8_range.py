@@ -207,3 +207,18 @@ def test_blocks_of_very_different_scales(lens, counts, dim, kw, dtype, k_shift, 
     kw = dict(kw, silu_scale=2.0**-80) if v_shift > 0 and dtype == torch.float16 else kw
     got = check(lens, counts, dim=dim, dtype=dtype, cache=c, seed=1, **kw)
     assert got.isfinite().all() and (dtype == torch.bfloat16 or v_shift > 0 or got[1:].any())
+
+
+@TYPES
+@pytest.mark.parametrize("dim,max_q", [(64, None), (128, MOST), (256, None)], ids=["keys", "tile", "d256"])
+def test_rows_that_are_not_finite_leave_the_others_alone(dim, max_q, dtype):
+    lens, counts = [200, 140, 77, 40], [40, 7, 77, 1]
+    c = cache(lens, dim)
+    q, offs = queries(counts, 2, dim, dtype), R.offsets(counts, device=DEV)
+    want = call(c, q, offs, counts, max_q=max_q)
+    q[7, 1, 3], q[9, 0], q[60, 0, dim - 1] = float("inf"), float("nan"), -float("inf")
+    got = call(c, q, offs, counts, max_q=max_q)
+    for at in ((7, 1), (9, 0), (60, 0)):
+        assert not got[at].isfinite().any()
+        got[at] = want[at]
+    assert torch.equal(got, want)
