@@ -273,11 +273,11 @@ HSTU_API int hstu_paged_fwd(const hstu_paged_fwd_params* params, void* workspace
  *   k_scale, v_scale  fp32 [num_pages, num_heads_k, page_size / 32]        a scale per block and head, a power of two
  *   weights  fp32 [num_pages, num_heads_k, page_size]                      accumulated attention weights; may be NULL
  *
- * The rows of sequence b are those of its pages page_ids[page_offsets[b] : page_offsets[b + 1]] in order, the first cache_len[b] of
- * them live.  Page ids outside [0, num_pages) stand for pages that are not there: nothing is read from them (their rows count as
- * zeros) or written to them.  A page that a call writes to must stand in it once, and nowhere else in the call; a page that is
- * only read may be shared by sequences.  head_dim is a multiple of 16 in [16, 256], page_size a multiple of 32; a sequence ends at
- * 2^24 rows, whatever its pages hold; pointers to caches, weights, q, k, v and out are 16-byte aligned.
+ * The rows of sequence b are those of its pages page_ids[page_offsets[b] : page_offsets[b + 1]] in order, the first cache_len[b] of them live.
+ * Page ids outside [0, num_pages) stand for pages that are not there: nothing is read from them (their rows count as zeros) or written to them. A
+ * page that a call writes to must stand in it once, and nowhere else in the call; a page that is only read may be shared by sequences. head_dim
+ * is a multiple of 16 in [16, 256], page_size a multiple of 32; a sequence ends at 2^24 rows, whatever its pages hold; the cache has no type, so
+ * rows of bf16 and of fp16 may write and read the same one; pointers to caches, weights, q, k, v and out are 16-byte aligned.
  */
 #define HSTU_PAGED_FP8_MAX_SEQ_LEN_K 16777216
 #define HSTU_PAGED_FP8_MAX_HEAD_DIM 256
@@ -332,10 +332,11 @@ HSTU_API int hstu_paged_fp8_fwd(const hstu_paged_fp8_fwd_params* params, void* w
 HSTU_API const char* hstu_paged_fp8_fwd_kernel_name(const hstu_paged_fp8_fwd_params* params);
 
 /*
- * Rows seq_offset[b] : seq_offset[b + 1] of k and v go to the positions cache_len[b], cache_len[b] + 1, ... of sequence b (cache_len is
- * not changed; rows that its pages have no room for are dropped).  Every block touched gets a new scale, the smallest power of two
- * that brings its largest finite magnitude, old rows included, to at most 448; codes round to nearest even (but to 240 * 2^120, not 256 * 2^120,
- * which no float holds), values that are not finite become NaN.  The rows of a touched block behind the new end are cleared; weights of new rows and of those become 0.
+ * Rows seq_offset[b] : seq_offset[b + 1] of k and v go to the positions cache_len[b], cache_len[b] + 1, ... of sequence b (cache_len is not
+ * changed; rows that its pages have no room for are dropped). Every block touched gets a new scale, the smallest power of two that brings its
+ * largest finite magnitude, old rows included, to at most 448; codes round to nearest even (but to 240 * 2^120, not 256 * 2^120, which no float
+ * holds), values that are not finite become NaN. The rows of a touched block behind the new end are cleared; weights of new rows and of those
+ * become 0.
  */
 typedef struct hstu_paged_fp8_append_params {
     uint32_t struct_size; /* sizeof(hstu_paged_fp8_append_params) */
@@ -353,10 +354,10 @@ typedef struct hstu_paged_fp8_append_params {
 HSTU_API int hstu_paged_fp8_append(const hstu_paged_fp8_append_params* params, void* stream);
 
 /*
- * Of each sequence at most `keep` rows stay (no more than the new pages hold): the first `sinks`, the last `recent`, and of the others
- * those with the largest scores, ties to the lower index; a score is the fp32 sum of a row's weights over the key heads, in
- * their order, NaN counting as -infinity.  cache_len is cut at max_seq_len_k.  The rows that stay are moved in order to the new pages (new_page_ids[new_page_offsets[b] : ...]), with new
- * scales and their weights; new_cache_len[b] is their number, kept[b] their old indices, -1 behind them.
+ * Of each sequence at most `keep` rows stay (no more than the new pages hold): the first `sinks`, the last `recent`, and of the others those with
+ * the largest scores, ties to the lower index; a score is the fp32 sum of a row's weights over the key heads, in their order, NaN counting as
+ * -infinity. cache_len is cut at max_seq_len_k. The rows that stay are moved in order to the new pages (new_page_ids[new_page_offsets[b] : ...]),
+ * with new scales and their weights; new_cache_len[b] is their number, kept[b] their old indices, -1 behind them.
  */
 typedef struct hstu_paged_fp8_evict_params {
     uint32_t struct_size; /* sizeof(hstu_paged_fp8_evict_params) */

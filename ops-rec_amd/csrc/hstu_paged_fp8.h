@@ -7,7 +7,9 @@ namespace hstu {
 constexpr int kFp8Block = 32;         // tokens that share a scale, and keys of one step of the attention kernel
 constexpr int kFp8MostKeys = 1 << 24; // rows of a sequence in the cache, at most (what places are found by is exact up to there)
 constexpr int kFp8MostSlots = 1 << 22;  // workgroups of an attention launch, of up to 512 threads: a grid has less than 2^32 threads
-constexpr int64_t kFp8WeightBytes = int64_t{512} << 20;  // of partial sums of weights in the workspace of a call, at most (but for one row tile)
+// Of partial sums of weights in the workspace of a call, at most.  Where a row tile's take more than half of it a launch takes one tile, which
+// keeps none; the parts of its keys are still those for all tiles at once.
+constexpr int64_t kFp8WeightBytes = int64_t{512} << 20;
 constexpr int kFp8JoinEnough = 1024;  // workgroups of the joins that fill the machine
 constexpr int kFp8AppendThreads = 128;
 constexpr int kFp8SelectKeys = 32768;   // scores that the selecting kernel holds in LDS
@@ -54,7 +56,7 @@ struct Fp8AttendArgs {
     int total_parts;  // the keys of the sequences are dealt to so many parts in all; 0: a sequence is one part
     int parts;        // of each sequence, where they are not dealt by length (more than 64 sequences)
     int chunk;        // blocks of a part: at least (dealt by length), or exactly
-    int most_blocks;  // that a row tile sweeps, at most
+    int most_blocks;  // that a row tile sweeps, but for targets behind a window, which may see more (the last part of a tile takes what is left)
     int max_blocks;  // pitch of weight_partial, in blocks
     float c_exp;     // -alpha * log2(e): silu(alpha s) = alpha * s / (1 + 2^(c_exp s))
     float c_out;     // alpha * silu_scale

@@ -3,8 +3,8 @@
 //   S = Q K^T,  P = silu(alpha S) * silu_scale * M,  O = P V,  with K and V the codes of the cache times their blocks' scales
 //
 // A step is one block of 32 keys, which lies in one page and has one scale for K and one for V.  Both products run on
-// v_mfma_f32_32x32x16 in the type of q, which holds an e4m3 value exactly; bf16 also holds it times the scale, a power of two, which
-// v_cvt_scalef32_pk multiplies by while it converts, so that scales cost nothing.  fp16 does not: see Fp8Unit.
+// v_mfma_f32_32x32x16 in the type of q, which holds an e4m3 value exactly; bf16 also holds it times the scale, a power of two (below
+// 2^-126 not all of its bits), which v_cvt_scalef32_pk multiplies by while it converts, so that scales cost nothing.  fp16 does not: see Fp8Unit.
 //   S^T[key][row] = K . Q^T     A = K: lane l % 32 takes key pi(l % 32) of the block, 16 dims of its half at a time; B = Q, in
 //                               registers from the start, the same dims
 //   O^T[dim][row] += V^T . P^T  A = V^T: lane l % 32 takes dim pi(l % 32) of a group of 32, the 16 keys of its half; B = P
@@ -19,7 +19,7 @@
 // A workgroup's wavefronts take the blocks of its 32 columns in turn, each converting what it reads, one block ahead in registers, and add
 // their outputs through LDS at the end: no barrier until then.  Bound by the bytes of the codes where columns are few (64 x 4 key heads of
 // one row on 2048 .. 8192 keys, d 128, 339 MB in 75 us, 4.5 TB/s; 3 x 2 of 30011 .. 120011, d 256, 231 MB in 51), else by a wavefront's chain
-// from load to product (about 1 us a step, 4 us before the first: 32 x 4 of 49 .. 64 rows on 501 .. 4001, d 64, 22 us).
+// from load to product (about 1 us a step, 4 us before the first: 32 x 4 of 49 .. 64 rows on 501 .. 4001, d 64, 24 us).
 #pragma once
 #include "hstu_paged_fp8_common.hip.h"
 #include "hstu_paged_fp8_variants.h"
@@ -644,8 +644,8 @@ __global__ __launch_bounds__(64 * WK) __attribute__((amdgpu_waves_per_eu(fp8_wav
         const int end = c0 + kFp8Block;
         // P goes into the second product rounded to the type of q.  What that leaves of half the keys (0 .. 7 and 16 .. 23 of a block) goes into a
         // product of its own, so that P adds less to the error than the output's rounding: bf16 outputs of few rows would else be 1.4 to
-        // 1.5 times as far off as rounding them alone, and are 1.2 times.  (64 rows of one query 74 us without, 77; 32 x 4 pairs of 49 .. 64 rows
-        // 22 and 24; both halves 78 and 26.5.)
+        // 1.5 times as far off as rounding them alone, and are 1.2 times.  (64 rows of one query 74 us without and 75 with it, 32 x 4 pairs of 49 .. 64
+        // rows 20 and 22; the other half as well would be 2 more.)
         u32x4_t p[2], rest;
         float w[16];
 #pragma unroll

@@ -155,7 +155,8 @@ Plan plan(const hstu_paged_fp8_fwd_params* p)
     // or half as many where there are more tiles than places for whole ones, so that one starts while another works (64 x 4 pairs of
     // 33 .. 40 rows on 200 .. 400 keys 14 us and 20 in whole ones, on 1500 .. 3000 38 and 45; of 8 .. 16 on 1500 .. 3000, as many tiles as
     // places, 31 and 32; 32 x 4 of them on 500 .. 1500 21 and 17).  Where tiles of 128 rows fill the machine their wavefronts share the
-    // conversion (16 x 4 of 1024 rows on 2000 .. 8000 keys 221 us, 241 in tiles of 32; 24 x 4 of 512 190 and 184): at 97 .. 128 dims and
+    // conversion (16 x 4 of 1024 rows on 2048 .. 8192 keys 237 us, 272 in tiles of 32; 24 x 4 of 512 on 2000 .. 8000 207 and 207, 64 x 4
+    // on 1000 .. 3000 232 and 258; fp16 252 and 287, 219 and 219, 255 and 270): at 97 .. 128 dims and
     // without weights only, elsewhere it is the other way round (d 96 191 and 189, d 64 165 and 139, with weights 329 and 307).
     const bool narrow = groups < 2;  // up to 64 dims a CU's registers take two workgroups
     const bool weights = p->cache.weights != nullptr, by_tile = groups == 3 && !weights && pairs * (rows / kFp8TileRows) >= 512;

@@ -8,10 +8,12 @@
 // bytes per lane, so that reads have no bank conflicts; two buffers for K and three for V, one barrier a step.  The products of K(t)
 // and of V(t - 1) go together, a chain of eight that wait for each other between four pairs that do not.  Three workgroups fit a CU,
 // and what one leaves of a SIMD's units another, which is nowhere in step with it, takes.  Bound by the vector and the matrix unit, which
-// overlap little: 16 x 4 key heads of 1024 rows on 2048 .. 8192 keys, d 128, 235 us (775 TFLOP/s), 64 such sequences of 5120 keys 850
-// TFLOP/s.  P is rounded to the type of q, once: what that adds to the error, as much as the output's rounding, is even over so many
-// outputs.  (Eight wavefronts half a step apart, one half multiplying while the other weighs, changing places at every barrier, took 10 %
-// longer; two shares of the keys for tiles of 64 rows lost to wavefronts alone.)
+// overlap little: 16 x 4 key heads of 1024 rows on 2048 .. 8192 keys, d 128, 237 us (770 TFLOP/s; fp16, with its units, 252), 64 such sequences
+// of 5120 keys 850 TFLOP/s.  P is rounded to the type of q, once, as in the 16-bit forward kernels: outputs are 1.4 times as far off as their
+// own rounding leaves them (0.0023 of their size in bf16; 0.0020 from the other kernel, which calls of fewer rows take).  A product for what that
+// rounding leaves of half the keys makes this 272 us, which is what the other kernel, with such a product, takes.  (Eight wavefronts half a step
+// apart, one half multiplying while the other weighs, changing places at every barrier, took 10 % longer; two shares of the keys for tiles of 64 rows
+// lost to wavefronts alone.)
 //   step t : S = K(t) Q and O += V(t - 1) P; convert K, V (t + 1) to LDS, request those of t + 3; P = silu(S) masked
 #pragma once
 #include "hstu_paged_fp8_attend_kernel.hip.h"

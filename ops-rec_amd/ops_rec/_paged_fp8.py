@@ -10,7 +10,9 @@ The cache of one layer, tensors that the program allocates and keeps::
     weights          fp32 [num_pages, heads_k, page_size]                  accumulated attention weights (optional)
 
 Sequence ``b`` has the pages ``page_ids[page_offsets[b] : page_offsets[b + 1]]``, and its first ``cache_len[b]`` rows in them are
-live; what lies behind them may hold anything.  A serving step appends the new rows (and the candidates to be ranked) behind
+live; what lies behind them may hold anything.  A cache has no type: rows of bf16 and of fp16 write it and read it.
+
+A serving step appends the new rows (and the candidates to be ranked) behind
 ``cache_len``, attends with the lengths that include them, and goes on from the length that it wants to keep: the next append
 overwrites the rest.
 
@@ -224,8 +226,8 @@ def hstu_paged_fp8_evict(k_cache, v_cache, k_scale, v_scale, weights, cache_len,
                          max_seq_len_k, keep, sinks=0, recent=0):  # fmt: skip
     """Moves the rows worth keeping to other pages, ``new_page_ids[new_page_offsets[b] : new_page_offsets[b + 1]]`` of sequence ``b``: at
     most ``keep`` rows each (and no more than those pages hold) -- the first ``sinks``, the last ``recent``, and of the others those
-    with the largest sums of ``weights`` over the key heads, NaN counting as minus infinity, ties to the lower index -- in the order they were in, with scales of
-    their new blocks and with their weights.  A sequence of no more than ``keep`` rows moves whole.  The old pages are only read: once
+    with the largest sums of ``weights`` over the key heads, NaN counting as minus infinity, ties to the lower index -- in the order they
+    were in, with scales of their new blocks and with their weights.  A sequence of no more than ``keep`` rows moves whole.  The old pages are only read: once
     the call is done (in the stream's order) they are the program's to hand out again.  New pages must be no pages that the call reads.
 
     Returns ``new_cache_len`` [batch] and ``kept`` [batch, keep]: the old indices of the rows that stay, -1 behind them (for what a
