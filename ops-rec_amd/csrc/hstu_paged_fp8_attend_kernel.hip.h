@@ -60,21 +60,25 @@ __device__ __forceinline__ Fp8Pair fp8_widen(u32x4_t codes, float scale)
     return r;
 }
 
-// A cache has no type, and fp16 does not hold what a code times its scale may be (from 65520 on it would be infinite, and zero times that NaN
-// in rows that do not see the key; below 2^-14 it would be rounded), nor what a weight may be before alpha and silu_scale.  So for rows of fp16
-// the products run on the codes themselves, which fp16 holds exactly.  A block's scale of K goes into the exponent of silu, and the weights go
-// into the second product times both scales, in units of their row's own.  Of a row of dim values up to m a score in units of K's scale is at most
-// 448 dim m; the unit is a power of two that puts this bound, times the scales of a block that the row has seen a key of, below 2^11, and is
-// changed, the row's sums with it, by a block whose scales' product is 2^5 times that block's or more, or less than 2^-8 of it.  Weights are then rounded to
-// multiples of 2^-24 of a unit at worst, 2^-25 of what the bound says for their block; a score's own sum in fp32 is good to 2^-24 of it.  (A row is a column
-// of the result: a lane holds of its own row only, and so does the lane of the same row in the other half.  Nothing that a row does not see changes
-// its unit, and a block that holds one value of 1e30 leaves the sums of other blocks as they are.)  It costs no instruction an
-// element: x / (1 + e) * 2^n is x / (e 2^-n + 2^-n).  bf16 reaches as far as fp32 and needs none of this.
+// A cache has no type, and fp16 does not hold what a code times its scale may be (from 65520 on it would be infinite, and zero times that
+// NaN in rows that do not see the key; below 2^-14 it would be rounded), nor what a weight may be before alpha and silu_scale. So for
+// rows of fp16 the products run on the codes themselves, which fp16 holds exactly. A block's scale of K goes into the exponent of silu,
+// and the weights go into the second product times both scales, in units of their row's own. Of a row of dim values up to m a score in
+// units of K's scale is at most 448 dim m; the unit is a power of two that puts this bound, times the scales of a block that the row has
+// seen a key of, below 2^11, and is changed, the row's sums with it, by a block whose scales' product is 2^5 times that block's or more,
+// or less than 2^-8 of it. Weights are then rounded to multiples of 2^-24 of a unit at worst, 2^-25 of what the bound says for their
+// block; a score's own sum in fp32 is good to 2^-24 of it. (A row is a column of the result: a lane holds of its own row only, and so
+// does the lane of the same row in the other half. Nothing that a row does not see changes its unit, and a block that holds one value of
+// 1e30 leaves the sums of other blocks as they are.) It costs no instruction an element: x / (1 + e) * 2^n is x / (e 2^-n + 2^-n). bf16
+// reaches as far as fp32 and needs none of this.
 struct Fp8Unit {
     int own;      // exponent of the unit's reciprocal for a block with scales of 1
     int up;       // and as it is: the unit is 2^-up; ahead of the first block one that none fits
     bool finite;  // the row
-    static __device__ __forceinline__ int exponent(float power_of_two) { return static_cast<int>(__builtin_bit_cast(uint32_t, power_of_two) >> 23 & 0xffu) - 127; }
+    static __device__ __forceinline__ int exponent(float power_of_two)
+    {
+        return static_cast<int>(__builtin_bit_cast(uint32_t, power_of_two) >> 23 & 0xffu) - 127;
+    }
     // what `x` is in the two lanes of this lane's row, the larger of them
     static __device__ __forceinline__ uint32_t of_row(uint32_t x)
     {
