@@ -1,0 +1,57 @@
+// Arguments of the gated projections' kernels.
+#pragma once
+#include <stdint.h>
+
+namespace hstu {
+
+constexpr int kActSilu = 0, kActGelu = 1, kActSigmoid = 2;
+
+// gated_gemm_kernel (gated_linear_gemm.hip.h): out[rows, cols] = a . b over `depth`
+struct GatedGemmArgs {
+    const void* n_side;  // forward: the weight [2 inner, depth]; x gradient: the weight [depth, cols]; weight gradient: x [depth, cols]
+    const void* m_side;  // forward: x [rows, depth]; x gradient: d_mixed [rows, depth]; weight gradient: d_mixed [depth, rows]
+    const void* bias;    // forward: [2 cols], 16-bit, or nullptr
+    void* out;           // forward: hidden [rows, cols], or nullptr; gradients: [rows, cols]
+    void* mixed;         // forward: [rows, 2 cols], or nullptr
+    float* partial;      // gradients in several chunks of the depth: [chunks][rows][cols]
+    int64_t rows;
+    int64_t depth;
+    int64_t chunk;  // of the depth, per workgroup: a multiple of 32, or the whole of it
+    int cols;       // of the output
+    int chunks;
+    int activation;
+    int tiles_m, tiles_n;
+};
+
+// gated_few_rows_kernel (gated_linear_few_rows.hip.h)
+struct GatedFewRowsArgs {
+    const void* x;       // [rows, depth]
+    const void* weight;  // [2 inner, depth]
+    const void* bias;    // [2 inner], 16-bit, or nullptr
+    void* hidden;        // [rows, inner], or nullptr
+    void* mixed;         // [rows, 2 inner], or nullptr
+    int64_t rows;
+    int depth;
+    int inner;
+    int activation;
+};
+
+// gated_stage_kernel and gated_sum_kernel (gated_linear_bwd_kernel.hip.h)
+struct GatedStageArgs {
+    const void* grad;   // [rows, inner]
+    const void* mixed;  // [rows, 2 inner]
+    void* d_mixed;      // [rows, 2 inner]
+    float* partial;     // [slices][2 inner] column sums, or nullptr
+    int64_t rows;
+    int inner;
+    int slices;
+    int activation;
+};
+struct GatedSumArgs {
+    const float* partial;  // [chunks][n]
+    void* out;             // [n], 16-bit
+    int64_t n;             // a multiple of 8
+    int chunks;
+};
+
+}  // namespace hstu

@@ -1,0 +1,324 @@
+// C ABI of gated_linear, forward and backward: argument checks, choice of kernels, launches.
+#include "../../include/ops_rec_layer_mi355.h"
+
+#include <hip/hip_runtime.h>
+
+#include "gated_linear_variants.h"
+#include "hstu_error.h"
+#include "layer_args.h"
+
+namespace {
+
+using hstu::GatedGemmArgs;
+using hstu::GatedTile;
+using hstu::set_error;
+
+static_assert(OPS_REC_ACT_SILU == hstu::kActSilu && OPS_REC_ACT_GELU == hstu::kActGelu && OPS_REC_ACT_SIGMOID == hstu::kActSigmoid, "one numbering");
+
+constexpr int64_t kStep = 32;          // of a product's depth
+constexpr int64_t kFewRows = 64;       // of a workgroup of the kernel for few rows
+constexpr int64_t kMostCols = 1 << 22; // (128 rows of twice as many columns lie behind one descriptor)
+constexpr int64_t kMostBytes = int64_t{1} << 31;  // behind one descriptor
+
+const hstu::GatedKernels& kernels_of(int dtype) { return dtype == HSTU_DT_BF16 ? hstu::gated_kernels_bf16() : hstu::gated_kernels_f16(); }
+
+int compute_units_or_256()  // (a size asked for where there is no device)
+{
+    int cus = 0;
+    return hstu::compute_units(&cus) == HSTU_OK ? cus : 256;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
+
+int validate(const gated_linear_params* p)
+{
+    if (p->struct_size != sizeof(gated_linear_params)) {
+        return set_error(HSTU_ERR_INVALID, "struct_size %u does not match this library (%zu)", p->struct_size, sizeof(gated_linear_params));
+    }
+    if (p->x == nullptr || p->weight == nullptr || (p->hidden == nullptr && p->mixed == nullptr)) {
+        return set_error(HSTU_ERR_NULLPTR, "x, weight, and hidden or mixed must be given");
+    }
+    if (p->dtype != HSTU_DT_BF16 && p->dtype != HSTU_DT_FP16) {
+        return set_error(HSTU_ERR_INVALID, "dtype %d is not one of bf16, fp16", p->dtype);
+    }
+    if (p->activation < 0 || p->activation > OPS_REC_ACT_SIGMOID) {
+        return set_error(HSTU_ERR_INVALID, "activation %d is none", p->activation);
+    }
+    if (p->rows < 1 || p->rows > 0x7fffffff) {
+        return set_error(HSTU_ERR_INVALID, "rows must be in [1, 2^31) (got %lld)", static_cast<long long>(p->rows));
+    }
+    if (p->cols < 8 || p->cols % 8 != 0 || p->inner < 8 || p->inner % 8 != 0 || p->cols > kMostCols || p->inner > kMostCols ||
+        p->inner * p->cols >= (int64_t{1} << 29)) {
+        return set_error(HSTU_ERR_INVALID, "the columns of x and hidden must be multiples of 8, at most 2^22, with a product below 2^29 (got %lld and %lld)",
+                         static_cast<long long>(p->cols), static_cast<long long>(p->inner));
+    }
+    for (const void* t : {p->x, p->weight, p->bias, static_cast<const void*>(p->hidden), static_cast<const void*>(p->mixed)}) {
+        if (!aligned16(t)) {
+            return set_error(HSTU_ERR_INVALID, "tensors must be 16-byte aligned");
+        }
+    }
+    return HSTU_OK;
+}
+
+int launched(const char* what)
+{
+    const hipError_t err = hipGetLastError();
+    return err == hipSuccess ? HSTU_OK : set_error(HSTU_ERR_RUNTIME, "launch of %s failed: %s", what, hipGetErrorString(err));
+}
+
+// Up to so many rows the kernel that streams the weight takes the call, in blocks of 64 rows.
+bool few_rows(const gated_linear_params* p) { return p->rows <= kFewRows; }
+
+// The tile: wide while its workgroups, two to a compute unit, fill the machine; square while those do; low for what is left.
+int tile_for(const GatedTile* tiles, int n, int64_t rows, int64_t cols)
+{
+    const int64_t cus = compute_units_or_256();
+    for (int i = 0; i < n - 1; ++i) {
+        if (ceil_div(rows, tiles[i].rows) * ceil_div(cols, tiles[i].cols) >= cus) {
+            return i;
+        }
+    }
+    return n - 1;
+}
+
+int launch_tiles(const GatedTile& t, GatedGemmArgs a, void* stream, const char* what)
+{
+    a.tiles_m = static_cast<int>(ceil_div(a.rows, t.rows));
+    a.tiles_n = static_cast<int>(ceil_div(a.cols, t.cols));
+    const int64_t all = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.chunks;
+    if (all > 0x70000000) {
+        return set_error(HSTU_ERR_INVALID, "%s would take %lld workgroups", what, static_cast<long long>(all));
+    }
+    hipLaunchKernelGGL(t.kernel, dim3(static_cast<uint32_t>(ceil_div(all, 8) * 8)), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    return launched(what);
+}
+
+// A gradient's product: its tile, and the chunks its depth is cut into so that short grids fill the machine -- two workgroups to a compute unit --,
+// each of 256 values at least: a chunk costs the traffic of its fp32 partial output.
+struct Product {
+    const GatedTile* tile;
+    int64_t chunk;
+    int64_t chunks;
+};
+Product plan(const GatedTile* tiles, int n, int64_t rows, int64_t cols, int64_t depth, int64_t depth_row_bytes)
+{
+    const int64_t cus = compute_units_or_256();
+    Product p;
+    p.tile = &tiles[tile_for(tiles, n, rows, cols)];
+    if (n == 2 && ceil_div(rows, tiles[0].rows) * ceil_div(cols, tiles[0].cols) * ceil_div(depth, 256) >= 2 * cus && cols > tiles[1].cols) {
+        p.tile = &tiles[0];  // (a depth long enough to fill the machine by its chunks)
+    }
+    const int64_t count = ceil_div(rows, p.tile->rows) * ceil_div(cols, p.tile->cols);
+    int64_t chunks = count >= cus ? 1 : 2 * cus / count;
+    chunks = chunks < ceil_div(depth, 256) ? chunks : ceil_div(depth, 256);
+    const int64_t fit = ceil_div(depth * depth_row_bytes, kMostBytes - kStep * depth_row_bytes);  // (a chunk lies behind one descriptor)
+    chunks = chunks > fit ? chunks : fit;
+    p.chunk = ceil_div(ceil_div(depth, chunks), kStep) * kStep;
+    p.chunks = ceil_div(depth, p.chunk);
+    return p;
+}
+
+uint64_t rounded(uint64_t bytes) { return (bytes + 255u) & ~uint64_t{255}; }
+
+struct BackwardPlan {
+    Product x, w;
+    int slices;
+    uint64_t d_mixed, sums, x_partial, w_partial;  // bytes, in this order
+    uint64_t total() const { return d_mixed + sums + (x_partial > w_partial ? x_partial : w_partial); }
+};
+
+BackwardPlan plan_backward(const gated_linear_bwd_params* p)
+{
+    const gated_linear_params& f = p->fwd;
+    const hstu::GatedKernels& k = kernels_of(f.dtype);
+    BackwardPlan b{};
+    // workgroups of the element-wise stage: eight per compute unit over all column blocks, a slice of at least 32 rows each
+    const int64_t blocks = ceil_div(f.inner, 256), places = 8 * static_cast<int64_t>(compute_units_or_256()) / blocks, useful = ceil_div(f.rows, 32);
+    const int64_t most = places > 1 ? places : 1;
+    b.slices = static_cast<int>(useful < most ? useful : most);
+    b.d_mixed = rounded(static_cast<uint64_t>(f.rows) * static_cast<uint64_t>(f.inner) * 4u);
+    b.sums = p->bias_grad != nullptr ? rounded(static_cast<uint64_t>(b.slices) * static_cast<uint64_t>(f.inner) * 8u) : 0;
+    if (p->x_grad != nullptr) {
+        b.x = plan(k.x_grad, hstu::kGatedTiles, f.rows, f.cols, 2 * f.inner, f.cols * 2);
+        b.x_partial = b.x.chunks > 1 ? static_cast<uint64_t>(b.x.chunks) * static_cast<uint64_t>(f.rows) * static_cast<uint64_t>(f.cols) * 4u : 0;
+    }
+    if (p->weight_grad != nullptr) {
+        b.w = plan(k.weight_grad, 2, 2 * f.inner, f.cols, f.rows, (2 * f.inner > f.cols ? 2 * f.inner : f.cols) * 2);
+        b.w_partial = b.w.chunks > 1 ? static_cast<uint64_t>(b.w.chunks) * static_cast<uint64_t>(2 * f.inner) * static_cast<uint64_t>(f.cols) * 4u : 0;
+    }
+    return b;
+}
+
+int validate(const gated_linear_bwd_params* p)
+{
+    if (p == nullptr) {
+        return set_error(HSTU_ERR_NULLPTR, "params is NULL");
+    }
+    if (p->struct_size != sizeof(gated_linear_bwd_params)) {
+        return set_error(HSTU_ERR_INVALID, "struct_size %u does not match this library (%zu)", p->struct_size, sizeof(gated_linear_bwd_params));
+    }
+    const int rc = validate(&p->fwd);
+    if (rc != HSTU_OK) {
+        return rc;
+    }
+    if (p->fwd.mixed == nullptr || p->grad == nullptr) {
+        return set_error(HSTU_ERR_NULLPTR, "mixed and grad must be given");
+    }
+    for (const void* t : {p->grad, static_cast<const void*>(p->x_grad), static_cast<const void*>(p->weight_grad), static_cast<const void*>(p->bias_grad)}) {
+        if (!aligned16(t)) {
+            return set_error(HSTU_ERR_INVALID, "tensors must be 16-byte aligned");
+        }
+    }
+    return HSTU_OK;
+}
+
+int launch_product(const hstu::GatedKernels& k, const Product& plan, GatedGemmArgs a, float* partial, void* stream, const char* what)
+{
+    a.chunk = plan.chunk;
+    a.chunks = static_cast<int>(plan.chunks);
+    a.partial = plan.chunks > 1 ? partial : nullptr;
+    const int rc = launch_tiles(*plan.tile, a, stream, what);
+    if (rc != HSTU_OK || a.partial == nullptr) {
+        return rc;
+    }
+    hstu::GatedSumArgs s{};
+    s.partial = partial;
+    s.out = a.out;
+    s.n = a.rows * a.cols;
+    s.chunks = a.chunks;
+    const int64_t blocks = ceil_div(s.n / 8, 256), most = 16 * static_cast<int64_t>(compute_units_or_256());
+    hipLaunchKernelGGL(k.sum, dim3(static_cast<uint32_t>(blocks < most ? blocks : most)), dim3(256), 0, static_cast<hipStream_t>(stream), s);
+    return launched("gated_sum_kernel");
+}
+
+}  // namespace
+
+extern "C" {
+
+HSTU_API const char* gated_linear_fwd_kernel_name(const gated_linear_params* p)
+{
+    if (p == nullptr || validate(p) != HSTU_OK) {
+        return nullptr;
+    }
+    static const char* const tiles[hstu::kGatedTiles] = {"gated_gemm_128x128", "gated_gemm_128x64", "gated_gemm_64x64"};
+    return few_rows(p) ? "gated_few_rows" : tiles[tile_for(kernels_of(p->dtype).forward, hstu::kGatedTiles, p->rows, p->inner)];
+}
+
+HSTU_API int gated_linear_fwd(const gated_linear_params* p, void* stream)
+{
+    if (p == nullptr) {
+        return set_error(HSTU_ERR_NULLPTR, "params is NULL");
+    }
+    const int rc = validate(p);
+    if (rc != HSTU_OK) {
+        return rc;
+    }
+    const hstu::GatedKernels& k = kernels_of(p->dtype);
+    if (few_rows(p)) {
+        hstu::GatedFewRowsArgs a{};
+        a.x = p->x;
+        a.weight = p->weight;
+        a.bias = p->bias;
+        a.hidden = p->hidden;
+        a.mixed = p->mixed;
+        a.rows = p->rows;
+        a.depth = static_cast<int>(p->cols);
+        a.inner = static_cast<int>(p->inner);
+        a.activation = p->activation;
+        const int size = p->rows <= 16 ? 0 : (p->rows <= 32 ? 1 : 2), block = 16 << size;
+        const bool sixteen = p->inner >= 16 * static_cast<int64_t>(compute_units_or_256());
+        hipLaunchKernelGGL(k.few_rows[size][sixteen ? 1 : 0],
+                           dim3(static_cast<uint32_t>(ceil_div(p->inner, sixteen ? 16 : 8)), static_cast<uint32_t>(ceil_div(p->rows, block))), dim3(512), 0,
+                           static_cast<hipStream_t>(stream), a);
+        return launched("gated_few_rows_kernel");
+    }
+    GatedGemmArgs a{};
+    a.n_side = p->weight;
+    a.m_side = p->x;
+    a.bias = p->bias;
+    a.out = p->hidden;
+    a.mixed = p->mixed;
+    a.rows = p->rows;
+    a.depth = a.chunk = p->cols;
+    a.cols = static_cast<int>(p->inner);
+    a.chunks = 1;
+    a.activation = p->activation;
+    return launch_tiles(k.forward[tile_for(k.forward, hstu::kGatedTiles, p->rows, p->inner)], a, stream, "gated_gemm_kernel (forward)");
+}
+
+HSTU_API int gated_linear_bwd_workspace_size(const gated_linear_bwd_params* p, uint64_t* workspace_bytes)
+{
+    const int rc = validate(p);
+    if (rc != HSTU_OK) {
+        return rc;
+    }
+    if (workspace_bytes == nullptr) {
+        return set_error(HSTU_ERR_NULLPTR, "workspace_bytes is NULL");
+    }
+    *workspace_bytes = plan_backward(p).total();
+    return HSTU_OK;
+}
+
+HSTU_API int gated_linear_bwd(const gated_linear_bwd_params* p, void* workspace, uint64_t workspace_bytes, void* stream)
+{
+    int rc = validate(p);
+    if (rc != HSTU_OK) {
+        return rc;
+    }
+    const BackwardPlan b = plan_backward(p);
+    if (workspace == nullptr || workspace_bytes < b.total() || !aligned16(workspace)) {
+        return set_error(HSTU_ERR_WORKSPACE, "gated_linear_bwd needs %llu bytes of workspace, 16-byte aligned (got %llu)", static_cast<unsigned long long>(b.total()),
+                         static_cast<unsigned long long>(workspace_bytes));
+    }
+    const gated_linear_params& f = p->fwd;
+    const hstu::GatedKernels& k = kernels_of(f.dtype);
+    uint8_t* const ws = static_cast<uint8_t*>(workspace);
+    float* const partial = reinterpret_cast<float*>(ws + b.d_mixed + b.sums);
+
+    hstu::GatedStageArgs s{};
+    s.grad = p->grad;
+    s.mixed = f.mixed;
+    s.d_mixed = ws;
+    s.partial = p->bias_grad != nullptr ? reinterpret_cast<float*>(ws + b.d_mixed) : nullptr;
+    s.rows = f.rows;
+    s.inner = static_cast<int>(f.inner);
+    s.slices = b.slices;
+    s.activation = f.activation;
+    hipLaunchKernelGGL(k.stage, dim3(static_cast<uint32_t>(b.slices * ceil_div(f.inner, 256))), dim3(256), 0, static_cast<hipStream_t>(stream), s);
+    rc = launched("gated_stage_kernel");
+    if (rc == HSTU_OK && p->bias_grad != nullptr) {
+        hstu::NormSumsArgs n{};
+        n.partial = s.partial;
+        n.out[0] = p->bias_grad;
+        n.kinds = 1;
+        n.slices = b.slices;
+        n.cols = static_cast<int>(2 * f.inner);
+        n.out_dtype = f.dtype;
+        rc = hstu::launch_column_sums(n, stream);
+    }
+    if (rc == HSTU_OK && p->x_grad != nullptr) {
+        GatedGemmArgs a{};
+        a.n_side = f.weight;
+        a.m_side = ws;
+        a.out = p->x_grad;
+        a.rows = f.rows;
+        a.depth = 2 * f.inner;
+        a.cols = static_cast<int>(f.cols);
+        rc = launch_product(k, b.x, a, partial, stream, "gated_gemm_kernel (x gradient)");
+    }
+    if (rc == HSTU_OK && p->weight_grad != nullptr) {
+        GatedGemmArgs a{};
+        a.n_side = f.x;
+        a.m_side = ws;
+        a.out = p->weight_grad;
+        a.rows = 2 * f.inner;
+        a.depth = f.rows;
+        a.cols = static_cast<int>(f.cols);
+        rc = launch_product(k, b.w, a, partial, stream, "gated_gemm_kernel (weight gradient)");
+    }
+    return rc;
+}
+
+}  // extern "C"

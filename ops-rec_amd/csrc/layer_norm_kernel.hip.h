@@ -1,0 +1,612 @@
+// Norms around a block of a layer, forward and backward, gfx950.
+//
+//   in front of a block:  s = residual + scale * x;  r = s rounded to the stream's type;  y = norm(s) * gamma + beta
+//   behind a block:       m = norm(x) * gamma + beta per part of a row;  out = [residual + residual_scale *] m * act(gate)
+//   norm(s) = (s - mean) * rstd, or s * rstd (root mean square);  rstd = 1 / sqrt(mean of the squares + eps)
+//
+// y is the norm of the sum before it is rounded, and the backward starts from what has all its bits: from the stream that was
+// written where that is fp32, from x and the residual that went in where it is 16-bit.  (From the rounded sum the gradients of
+// gamma and scale, fp32 sums over all rows, would be off by 2^-9 each row.)  Nothing is saved per row: a row is in registers in the
+// backward as well, where its mean and rstd cost two reductions and no memory.
+//
+//   backward, with n = norm(s), g = (gradient of m or y) * gamma, means over the part of a row:
+//     d s = rstd * (g - mean(g) - n * mean(g * n))       (root mean square: without mean(g))
+//     d gamma = sum over rows of (gradient of m or y) * n,  d beta = sum of it,  d scale = sum of d s * x
+//     d gate = d m * m * act'(gate)
+//
+// A dozen flops per value: bound by HBM.  A row (or part) belongs to G lanes -- a slice of a wavefront, a wavefront or a workgroup --
+// which hold it in registers as NV pieces of 8 values per lane; all loads of a row are in flight before the first use, and sums
+// over a wavefront go through DPP and lane swaps (10 instructions, no LDS).  Pieces start anywhere: the 16-byte accesses of this
+// machine need no alignment, so odd widths and strides take the same path, and only a last piece of fewer than 8 values goes value by value.
+//
+// The backward is persistent: a workgroup keeps one part of the columns and walks over rows, its lanes adding up the gradients of
+// gamma, beta and scale in registers; the sums of a workgroup's lane groups meet in LDS, one row of partial sums per workgroup goes to the
+// workspace, and a second kernel adds those in a fixed order: the same bits every launch.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "layer_args.h"
+#include "ln_mul_kernel.hip.h"
+
+namespace hstu {
+
+constexpr int kNormFront = 0, kNormBehind = 1;
+
+constexpr int norm_fwd_threads(int g) { return g > 256 ? g : 256; }
+constexpr int norm_bwd_threads(int g) { return g > 64 ? g : 512; }  // (barriers inside a row: one row at a time)
+
+// ---- 8 values of a row, as they lie in memory ----
+template <typename Tag>
+struct norm_piece {
+    typedef uint32_t words_t __attribute__((ext_vector_type(4), aligned(2)));
+    words_t w[ln_traits<Tag>::kPerChunk == 8 ? 1 : 2];
+};
+
+// piece c of a row of n values: all 8 where the row has them (c is clamped to the last whole piece, whose values the caller drops), the
+// values there are in the row's last, part-filled piece
+template <typename Tag>
+__device__ __forceinline__ norm_piece<Tag> norm_load(const typename ln_traits<Tag>::elem_t* row, int c, int n)
+{
+    using E = typename ln_traits<Tag>::elem_t;
+    norm_piece<Tag> p;
+    const int whole = n >> 3, rest = n & 7;
+    if (whole > 0) {
+        const typename norm_piece<Tag>::words_t* at =
+            reinterpret_cast<const typename norm_piece<Tag>::words_t*>(row + 8 * static_cast<int64_t>(min(c, whole - 1)));
+        p.w[0] = __builtin_nontemporal_load(at);
+        if constexpr (sizeof(E) == 4) {
+            p.w[1] = __builtin_nontemporal_load(at + 1);
+        }
+    }
+    if (rest != 0) {
+        if (c == whole) {
+            E e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                e[i] = i < rest ? row[8 * static_cast<int64_t>(whole) + i] : static_cast<E>(0.0f);
+            }
+            __builtin_memcpy(&p, e, sizeof e);
+        }
+    }
+    return p;
+}
+
+template <typename Tag>
+__device__ __forceinline__ void norm_unpack(const norm_piece<Tag>& p, float (&f)[8])
+{
+    using T = ln_traits<Tag>;
+#pragma unroll
+    for (int i = 0; i < 8 / T::kPerChunk; ++i) {
+        T::unpack(p.w[i], f + T::kPerChunk * i);
+    }
+}
+
+template <typename Tag>
+__device__ __forceinline__ void norm_store(typename ln_traits<Tag>::elem_t* row, int c, int n, const float (&f)[8])
+{
+    using T = ln_traits<Tag>;
+    using E = typename T::elem_t;
+    const int first = 8 * c;
+    if (first + 8 <= n) {
+        typename norm_piece<Tag>::words_t* at = reinterpret_cast<typename norm_piece<Tag>::words_t*>(row + first);
+#pragma unroll
+        for (int i = 0; i < 8 / T::kPerChunk; ++i) {
+            const typename norm_piece<Tag>::words_t w = T::pack(f + T::kPerChunk * i);
+            __builtin_nontemporal_store(w, at + i);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (first + i < n) {
+                row[first + i] = static_cast<E>(f[i]);
+            }
+        }
+    }
+}
+
+// 8 values per column (gamma, beta, scale), 0 past the end
+template <typename Tag>
+__device__ __forceinline__ void norm_columns(const void* p, bool f32, int64_t offset, int c, int n, float (&f)[8])
+{
+    if (f32) {
+        norm_unpack<ln_f32_tag>(norm_load<ln_f32_tag>(static_cast<const float*>(p) + offset, c, n), f);
+    } else {
+        norm_unpack<Tag>(norm_load<Tag>(static_cast<const typename ln_traits<Tag>::elem_t*>(p) + offset, c, n), f);
+    }
+}
+
+// ---- sums over the G lanes of a row ----
+template <int CTRL>
+__device__ __forceinline__ float dpp_of(float v)
+{
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+
+// (the elements are taken out first: this compiler casts element 0 for every element of a vector)
+typedef uint32_t lane_pair_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float swapped_sum(lane_pair_t s)
+{
+    const uint32_t a = s[0], b = s[1];
+    return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+
+template <int G>
+__device__ __forceinline__ float wave_sum(float v)
+{
+    v += dpp_of<0xB1>(v);   // lanes 1, 0, 3, 2 of a quad
+    v += dpp_of<0x4E>(v);   // 2, 3, 0, 1
+    v += dpp_of<0x141>(v);  // the other quad of 8 lanes
+    if constexpr (G >= 16) {
+        v += dpp_of<0x140>(v);  // the other 8 of 16 lanes
+    }
+    if constexpr (G >= 32) {
+        v = swapped_sum(__builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false));
+    }
+    if constexpr (G >= 64) {
+        v = swapped_sum(__builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false));
+    }
+    return v;
+}
+
+// K sums at once.  G > 64: through LDS, a slot of K * 16 floats per call, two slots in turn: a wavefront writes a slot again only
+// past the barrier of the call between, which every wavefront reaches after it has read the slot.
+constexpr int kNormSlots = 2;
+template <int G, int K>
+__device__ __forceinline__ void row_sums(float (&v)[K], float* s_part, int& slot)
+{
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        v[k] = wave_sum<G>(v[k]);
+    }
+    if constexpr (G > 64) {
+        constexpr int kWaves = G / 64;
+        float* const part = s_part + slot * 2 * 16;
+        slot ^= 1;
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                part[16 * k + (threadIdx.x % G) / 64] = v[k];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float t = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                t += part[16 * k + w];
+            }
+            v[k] = t;
+        }
+    }
+}
+
+// ---- act(z) and its slope: the hardware's exp2 and reciprocal where the result is rounded to 16 bits, library functions for fp32 ----
+template <typename Tag>
+__device__ __forceinline__ float norm_sigmoid(float z)
+{
+    if constexpr (ln_traits<Tag>::kPerChunk == 4) {
+        return 1.0f / (1.0f + expf(-z));
+    } else {
+        return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
+    }
+}
+
+// s (a lane's NV pieces, 0 outside the row) -> norm(s) in place; returns rstd.  Two passes over registers; the mean's own rounding is
+// taken out by the sum of the centred values, which is 0 for an exact mean.
+template <int G, int NV>
+__device__ __forceinline__ float normalise(float (&s)[NV][8], int lane, int len, bool rms, float epsilon, float* s_part, int& slot)
+{
+    const float inv_n = 1.0f / static_cast<float>(len);
+    float mean = 0.0f;
+    if (!rms) {
+        float sum[1] = {0.0f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                sum[0] += s[i][j];
+            }
+        }
+        row_sums<G>(sum, s_part, slot);
+        mean = sum[0] * inv_n;
+    }
+    float sq[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int left = len - 8 * (lane + i * G);  // columns of the row from this piece on
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            s[i][j] = j < left ? s[i][j] - mean : 0.0f;
+            sq[0] = __builtin_fmaf(s[i][j], s[i][j], sq[0]);
+            sq[1] += s[i][j];
+        }
+    }
+    row_sums<G>(sq, s_part, slot);
+    const float shift = rms ? 0.0f : sq[1] * inv_n;
+    const float rstd = 1.0f / sqrtf(fmaxf(sq[0] * inv_n - shift * shift, 0.0f) + epsilon);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            s[i][j] = (s[i][j] - shift) * rstd;
+        }
+    }
+    return rstd;
+}
+
+// values of pieces past the row's end -> 0
+template <int NV>
+__device__ __forceinline__ void drop_outside(float (&f)[NV][8], int lane, int g, int len)
+{
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int left = len - 8 * (lane + i * g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            f[i][j] = j < left ? f[i][j] : 0.0f;
+        }
+    }
+}
+
+// T = type of x (and of y, gate), R = type of the stream
+template <typename T, typename R, int MODE, int G, int NV>
+__global__ __launch_bounds__(norm_fwd_threads(G)) void norm_fwd_kernel(const NormArgs a)
+{
+    using TE = typename ln_traits<T>::elem_t;
+    using RE = typename ln_traits<R>::elem_t;
+    __shared__ float s_part[G > 64 ? kNormSlots * 2 * 16 : 1];
+    const uint32_t unit = (blockIdx.x * static_cast<uint32_t>(norm_fwd_threads(G)) + threadIdx.x) / G;
+    const int lane = threadIdx.x % G;
+    if (unit >= a.units) {  // (G > 64: a workgroup per unit, so that lanes that share barriers leave together)
+        return;
+    }
+    const uint32_t row = a.groups == 1 ? unit : unit / static_cast<uint32_t>(a.groups);
+    const int len = a.len;
+    const int64_t col0 = a.groups == 1 ? 0 : static_cast<int64_t>(unit - row * static_cast<uint32_t>(a.groups)) * len;
+    const int64_t dense = static_cast<int64_t>(row) * len * a.groups + col0;
+    const TE* const x = static_cast<const TE*>(a.x) + static_cast<int64_t>(row) * a.x_stride + col0;
+    const RE* const res = static_cast<const RE*>(a.residual) + static_cast<int64_t>(row) * a.residual_stride + col0;
+    const TE* const gate = static_cast<const TE*>(a.gate) + static_cast<int64_t>(row) * a.gate_stride + col0;
+    const bool f32 = a.affine_f32 != 0;
+    int slot = 0;
+
+    norm_piece<T> xp[NV], gp[NV];
+    norm_piece<R> rp[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        xp[i] = norm_load<T>(x, lane + i * G, len);
+    }
+    if (MODE == kNormFront || a.residual != nullptr) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            rp[i] = norm_load<R>(res, lane + i * G, len);
+        }
+    }
+    if (MODE == kNormBehind && a.gate != nullptr) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            gp[i] = norm_load<T>(gate, lane + i * G, len);
+        }
+    }
+    float s[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        norm_unpack<T>(xp[i], s[i]);
+    }
+    if constexpr (MODE == kNormFront) {
+        if (a.scale != nullptr) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float c[8], f[8];
+                norm_columns<T>(a.scale, f32, col0, lane + i * G, len, c);
+                norm_unpack<R>(rp[i], f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    s[i][j] = __builtin_fmaf(c[j], s[i][j], f[j]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float f[8];
+                norm_unpack<R>(rp[i], f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    s[i][j] += f[j];
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            norm_store<R>(static_cast<RE*>(a.sum) + dense, lane + i * G, len, s[i]);
+        }
+    }
+    drop_outside<NV>(s, lane, G, len);
+    normalise<G, NV>(s, lane, len, a.rms != 0, a.epsilon, s_part, slot);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float c[8], y[8];
+        norm_columns<T>(a.gamma, f32, col0, lane + i * G, len, c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            y[j] = s[i][j] * c[j];
+        }
+        if (a.beta != nullptr) {
+            norm_columns<T>(a.beta, f32, col0, lane + i * G, len, c);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                y[j] += c[j];
+            }
+        }
+        if constexpr (MODE == kNormBehind) {
+            if (a.gate != nullptr) {
+                float u[8];
+                norm_unpack<T>(gp[i], u);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    y[j] *= a.silu ? u[j] * norm_sigmoid<T>(u[j]) : u[j];
+                }
+            }
+            if (a.residual != nullptr) {
+                float f[8];
+                norm_unpack<R>(rp[i], f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    y[j] = __builtin_fmaf(a.residual_scale, y[j], f[j]);
+                }
+            }
+            norm_store<R>(static_cast<RE*>(a.out) + dense, lane + i * G, len, y);
+        } else {
+            norm_store<T>(static_cast<TE*>(a.out) + dense, lane + i * G, len, y);
+        }
+    }
+}
+
+template <typename T, typename R, int MODE, int G, int NV>
+__global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const NormBwdArgs a)
+{
+    using TE = typename ln_traits<T>::elem_t;
+    using RE = typename ln_traits<R>::elem_t;
+    constexpr int kThreads = norm_bwd_threads(G);
+    constexpr int kRows = kThreads / G;                          // rows of a workgroup at a time
+    constexpr bool kFromSum = MODE == kNormFront && ln_traits<R>::kPerChunk == 4;
+    constexpr bool kGradR = MODE == kNormBehind;                 // the gradient of the result has the stream's type
+    __shared__ float s_part[G > 64 ? kNormSlots * 2 * 16 : 1];
+    __shared__ __attribute__((aligned(16))) float s_sums[kRows > 1 ? kThreads * NV * 8 : 1];
+    const NormArgs& f = a.f;
+    const int sub = threadIdx.x / G, lane = threadIdx.x % G;
+    const int part = static_cast<int>(blockIdx.x % static_cast<uint32_t>(f.groups));
+    const uint32_t slice = blockIdx.x / static_cast<uint32_t>(f.groups);
+    const int len = f.len, cols = f.len * f.groups;
+    const int64_t col0 = static_cast<int64_t>(part) * len;
+    const uint32_t rows = f.units / static_cast<uint32_t>(f.groups);
+    const bool f32 = f.affine_f32 != 0;
+    const bool need_x = !kFromSum || f.scale != nullptr;
+    int slot = 0;
+
+    float gamma[NV][8], beta[NV][8], scale[NV][8];
+    float d_gamma[NV][8], d_beta[NV][8], d_scale[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        norm_columns<T>(f.gamma, f32, col0, lane + i * G, len, gamma[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            beta[i][j] = 0.0f;
+            scale[i][j] = 1.0f;
+            d_gamma[i][j] = d_beta[i][j] = d_scale[i][j] = 0.0f;
+        }
+        if (MODE == kNormBehind && f.beta != nullptr) {
+            norm_columns<T>(f.beta, f32, col0, lane + i * G, len, beta[i]);
+        }
+        if (MODE == kNormFront && f.scale != nullptr) {
+            norm_columns<T>(f.scale, f32, col0, lane + i * G, len, scale[i]);
+        }
+    }
+
+    drop_outside<NV>(gamma, lane, G, len);  // (what lies past the row's end must not reach its sums, NaN least of all)
+
+    for (uint32_t row0 = slice * kRows; row0 < rows; row0 += static_cast<uint32_t>(a.slices) * kRows) {
+        const uint32_t row = row0 + sub;
+        if (kRows > 1 && row >= rows) {  // (the lanes of a row leave together; no barrier in this loop for G <= 64)
+            break;
+        }
+        const int64_t dense = static_cast<int64_t>(row) * cols + col0;
+        const TE* const x = static_cast<const TE*>(f.x) + static_cast<int64_t>(row) * f.x_stride + col0;
+        norm_piece<T> xp[NV], yp[NV], gp[NV];
+        norm_piece<R> sp[NV], dp[NV];
+        if (need_x) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                xp[i] = norm_load<T>(x, lane + i * G, len);
+            }
+        }
+        if constexpr (MODE == kNormFront) {
+            const RE* const from = kFromSum ? static_cast<const RE*>(a.sum) + dense
+                                            : static_cast<const RE*>(f.residual) + static_cast<int64_t>(row) * f.residual_stride + col0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                sp[i] = norm_load<R>(from, lane + i * G, len);
+            }
+            if (a.sum_grad != nullptr) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    dp[i] = norm_load<R>(static_cast<const RE*>(a.sum_grad) + dense, lane + i * G, len);
+                }
+            }
+            if (a.grad != nullptr) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    yp[i] = norm_load<T>(static_cast<const TE*>(a.grad) + dense, lane + i * G, len);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                dp[i] = norm_load<R>(static_cast<const RE*>(a.grad) + dense, lane + i * G, len);
+            }
+            if (f.gate != nullptr) {
+                const TE* const gate = static_cast<const TE*>(f.gate) + static_cast<int64_t>(row) * f.gate_stride + col0;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    gp[i] = norm_load<T>(gate, lane + i * G, len);
+                }
+            }
+        }
+        float n[NV][8];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if constexpr (MODE == kNormFront) {
+                norm_unpack<R>(sp[i], n[i]);
+                if constexpr (!kFromSum) {
+                    float v[8];
+                    norm_unpack<T>(xp[i], v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        n[i][j] = __builtin_fmaf(scale[i][j], v[j], n[i][j]);
+                    }
+                }
+            } else {
+                norm_unpack<T>(xp[i], n[i]);
+            }
+        }
+        drop_outside<NV>(n, lane, G, len);
+        const float rstd = normalise<G, NV>(n, lane, len, f.rms != 0, f.epsilon, s_part, slot);
+
+        // g = (gradient of m or y) * gamma; the gradient itself goes into the sums
+        float g[NV][8];
+        float means[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int left = len - 8 * (lane + i * G);
+            float d[8];
+            if constexpr (kGradR) {
+                norm_unpack<R>(dp[i], d);
+                float u[8], dg[8];
+                if (f.gate != nullptr) {
+                    norm_unpack<T>(gp[i], u);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float dz = d[j] * f.residual_scale;
+                    float act = 1.0f, slope = 1.0f;
+                    if (f.gate != nullptr) {
+                        act = u[j];
+                        if (f.silu) {
+                            const float sg = norm_sigmoid<T>(u[j]);
+                            act = u[j] * sg;
+                            slope = sg * __builtin_fmaf(u[j], 1.0f - sg, 1.0f);
+                        }
+                    }
+                    dg[j] = dz * __builtin_fmaf(n[i][j], gamma[i][j], beta[i][j]) * slope;
+                    d[j] = dz * act;
+                }
+                if (f.gate != nullptr && a.gate_grad != nullptr) {
+                    norm_store<T>(static_cast<TE*>(a.gate_grad) + dense, lane + i * G, len, dg);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    d[j] = 0.0f;
+                }
+                if (a.grad != nullptr) {
+                    norm_unpack<T>(yp[i], d);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                d[j] = j < left ? d[j] : 0.0f;
+                d_gamma[i][j] = __builtin_fmaf(d[j], n[i][j], d_gamma[i][j]);
+                d_beta[i][j] += d[j];
+                g[i][j] = d[j] * gamma[i][j];
+                means[0] = __builtin_fmaf(g[i][j], n[i][j], means[0]);
+                means[1] += g[i][j];
+            }
+        }
+        row_sums<G>(means, s_part, slot);
+        const float inv_n = 1.0f / static_cast<float>(len);
+        const float along = means[0] * inv_n, level = f.rms ? 0.0f : means[1] * inv_n;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float d[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                d[j] = rstd * (g[i][j] - __builtin_fmaf(n[i][j], along, level));
+            }
+            if constexpr (MODE == kNormFront) {
+                if (a.sum_grad != nullptr) {
+                    float v[8];
+                    norm_unpack<R>(dp[i], v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        d[j] += v[j];
+                    }
+                }
+                norm_store<R>(static_cast<RE*>(a.residual_grad) + dense, lane + i * G, len, d);
+                if (a.want_scale) {
+                    const int left = len - 8 * (lane + i * G);
+                    float v[8];
+                    norm_unpack<T>(xp[i], v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        d_scale[i][j] += j < left ? d[j] * v[j] : 0.0f;
+                    }
+                }
+                if (a.x_grad != nullptr) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        d[j] *= scale[i][j];
+                    }
+                    norm_store<T>(static_cast<TE*>(a.x_grad) + dense, lane + i * G, len, d);
+                }
+            } else if (a.x_grad != nullptr) {
+                norm_store<T>(static_cast<TE*>(a.x_grad) + dense, lane + i * G, len, d);
+            }
+        }
+    }
+
+    // the sums over this workgroup's rows, kind by kind
+    const auto put = [&](const float (&v)[NV][8], int kind) {
+        float* const out = a.partial + (static_cast<int64_t>(kind) * a.slices + slice) * cols + col0;
+        if constexpr (kRows > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    s_sums[(sub * NV * G + i * G + lane) * 8 + j] = v[i][j];
+                }
+            }
+            __syncthreads();
+            for (int c = threadIdx.x; c < len; c += kThreads) {
+                float t = 0.0f;
+#pragma unroll
+                for (int s = 0; s < kRows; ++s) {
+                    t += s_sums[s * NV * G * 8 + c];
+                }
+                out[c] = t;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = 8 * (lane + i * G);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (c + j < len) {
+                        out[c + j] = v[i][j];
+                    }
+                }
+            }
+        }
+    };
+    put(d_gamma, 0);
+    if (a.want_beta) {
+        put(d_beta, 1);
+    }
+    if (MODE == kNormFront && a.want_scale) {
+        put(d_scale, 1 + a.want_beta);
+    }
+}
+
+}  // namespace hstu

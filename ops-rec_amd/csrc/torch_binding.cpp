@@ -7,32 +7,15 @@
 // Every other call (something to convert, an argument to refuse, an empty output) goes to the Python implementation, which
 // holds the checks, their messages and the conversions; so nothing is accepted or refused here that is not there.
 
-#include <ATen/Context.h>
-#include <ATen/hip/EmptyTensor.h>
-#include <ATen/native/TensorFactories.h>
 #include <ATen/ops/mm.h>
-#include <ATen/ops/zeros.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/utils/pybind.h>
-#include <torch/library.h>
 
-#include <cstring>
-#include <optional>
-#include <tuple>
+#include "torch_binding.h"
 
-#include "../../include/hstu_mi355.h"
 #include "../../include/ops_rec_activation_mi355.h"
-
-namespace py = pybind11;
 
 namespace {
 
-using at::Tensor;
-using OptTensor = std::optional<Tensor>;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
+using namespace ops_rec_binding;
 
 // The Python implementations by name, set once by set_fallbacks(); never released (calls may come during interpreter exit).
 struct Fallbacks {
@@ -47,54 +30,6 @@ struct Fallbacks {
     PyObject* paged_fp8_evict = nullptr;   // _paged_fp8.hstu_paged_fp8_evict
 } fallbacks;
 
-template <typename R, typename... A>
-R in_python(PyObject* fn, const A&... args)
-{
-    py::gil_scoped_acquire gil;
-    TORCH_CHECK(fn != nullptr, "ops_rec: the Python implementations have not been attached");
-    return py::reinterpret_borrow<py::object>(fn)(args...).template cast<R>();
-}
-
-int dtype_code(at::ScalarType t)
-{
-    switch (t) {
-    case at::kBFloat16: return HSTU_DT_BF16;
-    case at::kHalf: return HSTU_DT_FP16;
-    case at::kFloat: return HSTU_DT_FP32;
-    case at::kFloat8_e4m3fn: return HSTU_DT_FP8_E4M3;
-    default: return -1;
-    }
-}
-
-// torch.empty without its way through the dispatcher: memory nobody has written yet holds NaN (all ones) when the program has asked
-// for that (torch.use_deterministic_algorithms with torch.utils.deterministic.fill_uninitialized_memory)
-Tensor empty(at::IntArrayRef size, at::ScalarType dtype, const at::Device& device)
-{
-    Tensor t(at::detail::empty_cuda(size, dtype, device, std::nullopt));
-    const at::Context& context = at::globalContext();
-    if (context.deterministicAlgorithms() && context.deterministicFillUninitializedMemory()) {
-        at::native::fill_empty_deterministic_(t);
-    }
-    return t;
-}
-
-// A workspace a call can do without: none (undefined) when the allocator has no room for it.
-Tensor empty_or_none(uint64_t bytes, const at::Device& device)
-{
-    if (bytes != 0) {
-        try {
-            return empty({static_cast<int64_t>(bytes)}, at::kByte, device);
-        } catch (const c10::OutOfMemoryError&) {
-        }
-    }
-    return Tensor();
-}
-
-void* ptr(const Tensor& t) { return t.defined() && t.numel() != 0 ? t.data_ptr() : nullptr; }
-void* ptr(const OptTensor& t) { return t.has_value() ? ptr(*t) : nullptr; }
-
-bool is_set(const OptTensor& t) { return t.has_value() && t->defined(); }
-
 // an optional tensor as the library reads it: absent, or on the device, contiguous and of the type and 1-D size given
 bool absent_or_vector(const OptTensor& t, at::ScalarType dtype, int64_t n, const at::Device& device)
 {
@@ -106,8 +41,6 @@ bool absent_or_plane(const OptTensor& t, const Tensor& q, int64_t batch, int64_t
     return !is_set(t) || (t->device() == q.device() && t->scalar_type() == q.scalar_type() && t->dim() == 4 && t->size(0) == batch &&
                           t->size(1) == q.size(1) && t->size(2) == max_q && t->size(3) == max_k && t->is_contiguous());
 }
-
-hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
 // The arguments of one attention call, in the order of the operators' schemas.
 struct Call {
@@ -273,9 +206,6 @@ Gradients backward(const Tensor& grad_in, const Call& c)
                                                                             c.group, c.alpha);
     return {std::get<0>(r), std::get<1>(r), std::get<2>(r), std::get<3>(r).value_or(Tensor())};
 }
-
-// q, k, v as the kernels read them (a view that is not contiguous is copied, as the Python implementation does)
-const Tensor contiguous(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
 
 Tensor jagged_equal(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask, const OptTensor& bias, int64_t mask_type,
                     int64_t max_seq_len, double silu_scale, const Tensor& offs, const OptTensor& ctx, const OptTensor& tgt,
@@ -711,18 +641,6 @@ Gradients in_linear_silu_backward(const Tensor& x, const Tensor& weight, const O
 // inputs get gradients are the same (ascendc/attention/hstu_v1/torch_extension/hstu_v1_autograd.py:53-374).  Both directions go
 // through the dispatcher below autograd, so tracing and functionalisation see the operators.
 
-template <typename F>
-auto operator_handle(const char* name, const char* overload)
-{
-    return c10::Dispatcher::singleton().findSchemaOrThrow(name, overload).typed<F>();
-}
-
-bool needs_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
-bool needs_grad(const OptTensor& t) { return t.has_value() && needs_grad(*t); }
-
-Tensor unwrap(const OptTensor& t) { return t.value_or(Tensor()); }
-OptTensor wrap(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
-
 template <bool DELTA>
 Tensor call_forward(const Call& c, bool deterministic)
 {
@@ -883,4 +801,5 @@ PYBIND11_MODULE(_torch_binding, m)
         fallbacks.paged_fp8_evict = fp8_evict.release().ptr();
     });
     m.def("fp8_forward", &fp8_forward, py::call_guard<py::gil_scoped_release>());
+    define_layer(m);
 }

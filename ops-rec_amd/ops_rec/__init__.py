@@ -16,12 +16,14 @@ import logging
 from . import _ops  # noqa: F401  (defines the attention operators)
 from . import _paged_fp8  # noqa: F401  (defines the operators of the 8-bit paged cache)
 from . import _activation  # noqa: F401  (defines ln_mul)
+from . import _layer  # noqa: F401  (defines the norms around a block, rotary positions and the gated projections)
 from . import _dispatch  # noqa: F401  (the native kernels of both, where they are built)
 from . import ascendc  # noqa: F401
 from . import autograd  # noqa: F401  (registers the autograd formulas)
+from ._layer import rotary_frequencies  # noqa: F401  (extension: the frequencies of rotary)
 from ._ops import hstu_jagged_fp8  # noqa: F401  (extension: fp8 inputs with per-head scales)
 
 logger = logging.getLogger(__name__)
 
 __version__ = "0.1.0"
-__all__ = ["ascendc", "autograd", "hstu_jagged_fp8", "__version__"]
+__all__ = ["ascendc", "autograd", "hstu_jagged_fp8", "rotary_frequencies", "__version__"]

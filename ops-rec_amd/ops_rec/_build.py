@@ -33,7 +33,17 @@ SOURCES = [
     "hstu_paged_fp8_mi355.hip",
     "hstu_paged_fp8_kernels_bf16.hip",
     "hstu_paged_fp8_kernels_f16.hip",
+    "layer_norm_mi355.hip",
+    "layer_norm_kernels_bf16.hip",
+    "layer_norm_kernels_f16.hip",
+    "layer_norm_kernels_f32.hip",
+    "rotary_mi355.hip",
+    "gated_linear_mi355.hip",
+    "gated_linear_kernels_bf16.hip",
+    "gated_linear_kernels_f16.hip",
 ]
+# the dispatcher kernels: host code, one library of its own
+BINDING_SOURCES = ["torch_binding.cpp", "torch_binding_layer.cpp"]
 # These kernels name the accumulator registers they keep their sums in (hstu_pinned_acc.hip.h); every other matrix result belongs in
 # vector registers, where the compiler would otherwise keep it in accumulators as well and copy each element out.
 _VGPR_FORM = ("-mllvm", "-amdgpu-mfma-vgpr-form=1")
@@ -78,7 +88,7 @@ def _run(cmd: list[str], verbose: bool) -> None:
 
 
 def _binding_command(output: str) -> list[str]:
-    """The dispatcher kernels (``csrc/torch_binding.cpp``): host code only, against torch's headers and the HIP library next to it."""
+    """The dispatcher kernels (``csrc/torch_binding*.cpp``): host code only, against torch's headers and the HIP library next to it."""
     import torch
 
     root = os.path.dirname(torch.__file__)
@@ -88,7 +98,7 @@ def _binding_command(output: str) -> list[str]:
     return [
         os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(a for i in includes for a in ("-isystem", i)),
-        os.path.join(CSRC, "torch_binding.cpp"), "-o", output, f"-L{os.path.join(root, 'lib')}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu",
+        *(os.path.join(CSRC, source) for source in BINDING_SOURCES), "-o", output, f"-L{os.path.join(root, 'lib')}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu",
         "-ltorch_hip", "-ltorch_python", f"-L{LIB_DIR}", f"-l:{os.path.basename(LIB_PATH)}", "-Wl,-rpath,$ORIGIN",
     ]  # fmt: skip
 

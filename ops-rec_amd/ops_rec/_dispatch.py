@@ -1,5 +1,5 @@
-"""Registers what runs for device tensors: the native dispatcher kernels (``csrc/torch_binding.cpp``), or the Python
-implementations of ``_ops`` and ``_activation``.
+"""Registers what runs for device tensors: the native dispatcher kernels (``csrc/torch_binding*.cpp``), or the Python
+implementations of ``_ops``, ``_paged_fp8``, ``_activation`` and ``_layer``.
 
 With the native kernels a call in canonical form never enters Python; any other call is handed to the Python implementation, which
 holds the checks and conversions.  Where the binding has not been built, or does not load (built for another torch), the Python
@@ -15,7 +15,7 @@ import os
 
 import torch
 
-from . import _activation, _build, _ops, _paged_fp8
+from . import _activation, _build, _layer, _ops, _paged_fp8
 
 logger = logging.getLogger(__name__)
 
@@ -31,6 +31,8 @@ def _load():
     module.set_fallbacks(_ops._forward_impl, _ops._backward_impl, _ops.hstu_paged, _activation.ln_mul,
                          _activation.distance_in_linear_silu, _activation.in_linear_silu_backward, _paged_fp8.hstu_paged_fp8,
                          _paged_fp8.hstu_paged_fp8_append, _paged_fp8.hstu_paged_fp8_evict)  # fmt: skip
+    module.set_layer_fallbacks(_layer.residual_norm, _layer.residual_norm_backward, _layer.norm_gate, _layer.norm_gate_backward, _layer.rotary,
+                                _layer.gated_linear, _layer.gated_linear_backward)  # fmt: skip
     return module
 
 

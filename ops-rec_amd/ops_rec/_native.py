@@ -48,6 +48,21 @@ EXPORTED_SYMBOLS = (
     "in_linear_silu_bwd_weight",
 )
 
+# declared in include/ops_rec_layer_mi355.h
+LAYER_SYMBOLS = (
+    "residual_norm_fwd",
+    "residual_norm_bwd_workspace_size",
+    "residual_norm_bwd",
+    "norm_gate_fwd",
+    "norm_gate_bwd_workspace_size",
+    "norm_gate_bwd",
+    "rotary_fwd",
+    "gated_linear_fwd",
+    "gated_linear_fwd_kernel_name",
+    "gated_linear_bwd_workspace_size",
+    "gated_linear_bwd",
+)
+
 
 class FwdParams(ctypes.Structure):
     """Mirror of ``hstu_jagged_fwd_params``."""
@@ -247,6 +262,95 @@ class InLinearSiluBwdWeightParams(ctypes.Structure):
     ]
 
 
+class ResidualNormParams(ctypes.Structure):
+    """Mirror of ``residual_norm_params`` (include/ops_rec_layer_mi355.h)."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("rms", ctypes.c_int32),
+        *((name, ctypes.c_void_p) for name in ("x", "residual", "gamma", "beta", "scale", "y", "sum")),
+        *((name, ctypes.c_int64) for name in ("rows", "cols", "x_stride", "residual_stride")),
+        *((name, ctypes.c_int32) for name in ("dtype", "stream_dtype", "affine_dtype")),
+        ("epsilon", ctypes.c_float),
+    ]
+
+
+class ResidualNormBwdParams(ctypes.Structure):
+    """Mirror of ``residual_norm_bwd_params``."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("reserved0", ctypes.c_uint32),
+        ("fwd", ResidualNormParams),
+        *((name, ctypes.c_void_p) for name in ("sum", "y_grad", "sum_grad", "x_grad", "residual_grad", "gamma_grad", "beta_grad", "scale_grad")),
+    ]
+
+
+class NormGateParams(ctypes.Structure):
+    """Mirror of ``norm_gate_params``."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("rms", ctypes.c_int32),
+        *((name, ctypes.c_void_p) for name in ("x", "gate", "gamma", "beta", "residual", "out")),
+        *((name, ctypes.c_int64) for name in ("rows", "cols", "x_stride", "gate_stride", "residual_stride")),
+        *((name, ctypes.c_int32) for name in ("groups", "silu", "dtype", "stream_dtype", "affine_dtype")),
+        ("epsilon", ctypes.c_float),
+        ("residual_scale", ctypes.c_float),
+        ("reserved0", ctypes.c_uint32),
+    ]
+
+
+class NormGateBwdParams(ctypes.Structure):
+    """Mirror of ``norm_gate_bwd_params``."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("reserved0", ctypes.c_uint32),
+        ("fwd", NormGateParams),
+        *((name, ctypes.c_void_p) for name in ("out_grad", "x_grad", "gate_grad", "gamma_grad", "beta_grad")),
+    ]
+
+
+class RotaryParams(ctypes.Structure):
+    """Mirror of ``rotary_params``."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32),
+        *((name, ctypes.c_void_p) for name in ("q", "k", "q_out", "k_out", "frequencies", "positions", "seq_offset", "start")),
+        *((name, ctypes.c_int64) for name in ("rows", "heads_q", "heads_k", "dim", "pairs", "n_offsets", "q_stride_row", "q_stride_head",
+                                              "k_stride_row", "k_stride_head")),  # fmt: skip
+        ("magnitude", ctypes.c_double),
+        *((name, ctypes.c_int32) for name in ("positions_dtype", "seq_offset_dtype", "start_dtype", "interleaved", "inverse")),
+        ("reserved0", ctypes.c_uint32),
+    ]
+
+
+class GatedLinearParams(ctypes.Structure):
+    """Mirror of ``gated_linear_params``."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("activation", ctypes.c_int32),
+        *((name, ctypes.c_void_p) for name in ("x", "weight", "bias", "hidden", "mixed")),
+        *((name, ctypes.c_int64) for name in ("rows", "cols", "inner")),
+        ("dtype", ctypes.c_int32),
+        ("reserved0", ctypes.c_uint32),
+    ]
+
+
+class GatedLinearBwdParams(ctypes.Structure):
+    """Mirror of ``gated_linear_bwd_params``."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("reserved0", ctypes.c_uint32),
+        ("fwd", GatedLinearParams),
+        *((name, ctypes.c_void_p) for name in ("grad", "x_grad", "weight_grad", "bias_grad")),
+    ]
+
+
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -303,7 +407,10 @@ def load() -> ctypes.CDLL:
     lib.hstu_paged_fwd_kernel_name.restype = ctypes.c_char_p
     lib.hstu_paged_fwd_kernel_name.argtypes = [ctypes.POINTER(PagedParams)]
     for name, params, workspace in (("hstu_paged_fp8_fwd", PagedFp8FwdParams, True), ("hstu_paged_fp8_append", PagedFp8AppendParams, False),
-                                    ("hstu_paged_fp8_evict", PagedFp8EvictParams, True)):  # fmt: skip
+                                    ("hstu_paged_fp8_evict", PagedFp8EvictParams, True), ("residual_norm_fwd", ResidualNormParams, False),
+                                    ("residual_norm_bwd", ResidualNormBwdParams, True), ("norm_gate_fwd", NormGateParams, False),
+                                    ("norm_gate_bwd", NormGateBwdParams, True), ("rotary_fwd", RotaryParams, False),
+                                    ("gated_linear_fwd", GatedLinearParams, False), ("gated_linear_bwd", GatedLinearBwdParams, True)):  # fmt: skip
         call = getattr(lib, name)
         call.restype = ctypes.c_int
         call.argtypes = [ctypes.POINTER(params), *((ctypes.c_void_p, ctypes.c_uint64) if workspace else ()), ctypes.c_void_p]
@@ -313,6 +420,8 @@ def load() -> ctypes.CDLL:
             size.argtypes = [ctypes.POINTER(params), ctypes.POINTER(ctypes.c_uint64)]
     lib.hstu_paged_fp8_fwd_kernel_name.restype = ctypes.c_char_p
     lib.hstu_paged_fp8_fwd_kernel_name.argtypes = [ctypes.POINTER(PagedFp8FwdParams)]
+    lib.gated_linear_fwd_kernel_name.restype = ctypes.c_char_p
+    lib.gated_linear_fwd_kernel_name.argtypes = [ctypes.POINTER(GatedLinearParams)]
     lib.ln_mul_fwd.restype = ctypes.c_int
     lib.ln_mul_fwd.argtypes = [ctypes.POINTER(LnMulParams), ctypes.c_void_p]
     lib.ln_mul_fwd_kernel_name.restype = ctypes.c_char_p

@@ -2,13 +2,15 @@
 
 Same surface as the reference module (ops_rec/ascendc/activation/__init__.py:30-55): both
 ``ops_rec.ascendc.activation.ln_mul(...)`` and ``from ops_rec.ascendc.activation import ln_mul`` work, and an
-unknown name raises ``AttributeError`` listing what exists.
+unknown name raises ``AttributeError`` listing what exists.  ``residual_norm``, ``norm_gate`` and ``gated_linear`` (each with its backward) are extensions:
+the reference has none of the kind.
 """
 
 import torch
 
 _NS = torch.ops.ops_rec
-_OPS = ("ln_mul", "distance_in_linear_silu", "in_linear_silu_backward")
+_OPS = ("ln_mul", "distance_in_linear_silu", "in_linear_silu_backward", "residual_norm", "residual_norm_backward", "norm_gate",
+        "norm_gate_backward", "gated_linear", "gated_linear_backward")  # fmt: skip
 
 __all__ = [name for name in _OPS if hasattr(_NS, name)]
 for _name in __all__:
