@@ -30,34 +30,37 @@ __global__ __launch_bounds__(kStageThreads) void gated_stage_kernel(const GatedS
     }
     const int64_t step = static_cast<int64_t>(a.slices) * kStageRows;
     if (have) {
-        for (int64_t row = static_cast<int64_t>(slice) * kStageRows + sub; row < a.rows; row += step) {
-            const u32x4_t d4 = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(a.grad) + row * a.inner + col));
-            const uint16_t* const m = static_cast<const uint16_t*>(a.mixed) + row * 2 * a.inner + col;
-            const u32x4_t g4 = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(m));
-            const u32x4_t u4 = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(m + a.inner));
-            u32x4_t og, ou;
+        with_activation(a.activation, [&](auto chosen) {
+            constexpr int kind = decltype(chosen)::value;
+            for (int64_t row = static_cast<int64_t>(slice) * kStageRows + sub; row < a.rows; row += step) {
+                const u32x4_t d4 = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(a.grad) + row * a.inner + col));
+                const uint16_t* const m = static_cast<const uint16_t*>(a.mixed) + row * 2 * a.inner + col;
+                const u32x4_t g4 = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(m));
+                const u32x4_t u4 = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(m + a.inner));
+                u32x4_t og, ou;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float d[2], g[2], u[2], x[2], y[2];
-                ils_unpack2<Tag>(d4[e], d[0], d[1]);
-                ils_unpack2<Tag>(g4[e], g[0], g[1]);
-                ils_unpack2<Tag>(u4[e], u[0], u[1]);
+                for (int e = 0; e < 4; ++e) {
+                    float d[2], g[2], u[2], x[2], y[2];
+                    ils_unpack2<Tag>(d4[e], d[0], d[1]);
+                    ils_unpack2<Tag>(g4[e], g[0], g[1]);
+                    ils_unpack2<Tag>(u4[e], u[0], u[1]);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float act, slope;
-                    gated_act_slope(a.activation, g[h], act, slope);
-                    x[h] = d[h] * u[h] * slope;
-                    y[h] = d[h] * act;
-                    dg[2 * e + h] += x[h];
-                    du[2 * e + h] += y[h];
+                    for (int h = 0; h < 2; ++h) {
+                        float act, slope;
+                        gated_act_slope<kind>(g[h], act, slope);
+                        x[h] = d[h] * u[h] * slope;
+                        y[h] = d[h] * act;
+                        dg[2 * e + h] += x[h];
+                        du[2 * e + h] += y[h];
+                    }
+                    og[e] = pack2<Tag>(x[0], x[1]);
+                    ou[e] = pack2<Tag>(y[0], y[1]);
                 }
-                og[e] = pack2<Tag>(x[0], x[1]);
-                ou[e] = pack2<Tag>(y[0], y[1]);
+                uint16_t* const to = static_cast<uint16_t*>(a.d_mixed) + row * 2 * a.inner + col;
+                *reinterpret_cast<u32x4_t*>(to) = og;
+                *reinterpret_cast<u32x4_t*>(to + a.inner) = ou;
             }
-            uint16_t* const to = static_cast<uint16_t*>(a.d_mixed) + row * 2 * a.inner + col;
-            *reinterpret_cast<u32x4_t*>(to) = og;
-            *reinterpret_cast<u32x4_t*>(to + a.inner) = ou;
-        }
+        });
     }
     if (a.partial == nullptr) {
         return;

@@ -131,7 +131,9 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
         }
         const int64_t to = m0 + row;
         if (a.hidden != nullptr) {
-            static_cast<uint16_t*>(a.hidden)[to * a.inner + n0 + c] = static_cast<uint16_t>(pack2<Tag>(gated_act(a.activation, sum[0]) * sum[1], 0.0f));
+            float act = 0.0f;
+            with_activation(a.activation, [&](auto chosen) { act = gated_act<decltype(chosen)::value>(sum[0]); });
+            static_cast<uint16_t*>(a.hidden)[to * a.inner + n0 + c] = static_cast<uint16_t>(pack2<Tag>(act * sum[1], 0.0f));
         }
         if (a.mixed != nullptr) {
             uint16_t* const m = static_cast<uint16_t*>(a.mixed) + to * 2 * a.inner + n0 + c;

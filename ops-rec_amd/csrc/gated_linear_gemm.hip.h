@@ -33,25 +33,40 @@ __device__ __forceinline__ float gated_sigmoid(float z) { return __builtin_amdgc
 // act(z): silu, gelu by its tanh form -- z * sigmoid(2 sqrt(2 / pi) (z + 0.044715 z^3)) --, or the sigmoid.  (hardware exp2 and reciprocal, 1 ulp
 // each: the results are rounded to 8 or 11 bits.  Past |z| = 30 gelu's cube could make infinity times 0: its argument is bounded there, where the
 // sigmoid is 0 or 1 to all bits.)
-__device__ __forceinline__ float gated_act(int kind, float z)
+template <int ACT>
+__device__ __forceinline__ float gated_act(float z)
 {
-    if (kind == kActSilu) {
+    if constexpr (ACT == kActSilu) {
         return z * gated_sigmoid(z);
-    }
-    if (kind == kActGelu) {
+    } else if constexpr (ACT == kActGelu) {
         const float t = fminf(fmaxf(z, -30.0f), 30.0f);
         return z * gated_sigmoid(1.5957691216057308f * t * __builtin_fmaf(0.044715f * t, t, 1.0f));
+    } else {
+        return gated_sigmoid(z);
     }
-    return gated_sigmoid(z);
 }
 
-__device__ __forceinline__ void gated_act_slope(int kind, float z, float& act, float& slope)
+// `f` called with the activation as a constant: one choice for all of a kernel's values (a branch at each made 5000 instructions of an epilogue)
+template <typename F>
+__device__ __forceinline__ void with_activation(int kind, const F& f)
 {
     if (kind == kActSilu) {
+        f(std::integral_constant<int, kActSilu>{});
+    } else if (kind == kActGelu) {
+        f(std::integral_constant<int, kActGelu>{});
+    } else {
+        f(std::integral_constant<int, kActSigmoid>{});
+    }
+}
+
+template <int ACT>
+__device__ __forceinline__ void gated_act_slope(float z, float& act, float& slope)
+{
+    if constexpr (ACT == kActSilu) {
         const float s = gated_sigmoid(z);
         act = z * s;
         slope = s * __builtin_fmaf(z, 1.0f - s, 1.0f);
-    } else if (kind == kActGelu) {
+    } else if constexpr (ACT == kActGelu) {
         const float t = fminf(fmaxf(z, -30.0f), 30.0f);
         const float s = gated_sigmoid(1.5957691216057308f * t * __builtin_fmaf(0.044715f * t, t, 1.0f));
         act = z * s;
@@ -323,50 +338,53 @@ __global__ __launch_bounds__(kGemmThreads, gemm_workgroups_per_cu(BN, BM)) void 
                 }
             }
         }
+        with_activation(a.activation, [&](auto chosen) {
+            constexpr int kind = decltype(chosen)::value;
 #pragma unroll
-        for (int j = 0; j < MB; ++j) {
+            for (int j = 0; j < MB; ++j) {
 #pragma unroll
-            for (int i = 0; i < HB; ++i) {
+                for (int i = 0; i < HB; ++i) {
 #pragma unroll
-                for (int run = 0; run < 2; ++run) {
-                    u32x4_t hw, gw, uw;
+                    for (int run = 0; run < 2; ++run) {
+                        u32x4_t hw, gw, uw;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float g0 = acc[i][j][8 * run + 2 * e] + bias[0][i][run][2 * e], g1 = acc[i][j][8 * run + 2 * e + 1] + bias[0][i][run][2 * e + 1];
-                        const float u0 = acc[HB + i][j][8 * run + 2 * e] + bias[1][i][run][2 * e],
-                                    u1 = acc[HB + i][j][8 * run + 2 * e + 1] + bias[1][i][run][2 * e + 1];
-                        // (hidden is taken of the sums as they are, before mixed is rounded for the backward)
-                        hw[e] = pack2<Tag>(gated_act(a.activation, g0) * u0, gated_act(a.activation, g1) * u1);
-                        gw[e] = pack2<Tag>(g0, g1);
-                        uw[e] = pack2<Tag>(u0, u1);
-                    }
-                    uint16_t* const to = staged + r * kEpiRow + 32 * i + 16 * run + 8 * half;
-                    *reinterpret_cast<u32x4_t*>(to) = hw;
-                    *reinterpret_cast<u32x4_t*>(to + 32 * kEpiRow) = gw;
-                    *reinterpret_cast<u32x4_t*>(to + 64 * kEpiRow) = uw;
-                }
-            }
-            settle();
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int in_block = 8 * q + out_row;
-                const int64_t row = m0 + BM / 2 * wm + 32 * j + in_block;
-                const int col = col0 + 8 * out_chunk;
-                const uint16_t* const from = staged + in_block * kEpiRow + 8 * out_chunk;
-                if (row < a.rows && 8 * out_chunk < kRound && col < a.cols) {
-                    if (a.out != nullptr) {
-                        __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from),
-                                                    reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.out) + row * a.cols + col));
-                    }
-                    if (a.mixed != nullptr) {
-                        uint16_t* const to = static_cast<uint16_t*>(a.mixed) + row * 2 * a.cols + col;
-                        __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from + 32 * kEpiRow), reinterpret_cast<u32x4_t*>(to));
-                        __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from + 64 * kEpiRow), reinterpret_cast<u32x4_t*>(to + a.cols));
+                        for (int e = 0; e < 4; ++e) {
+                            const float g0 = acc[i][j][8 * run + 2 * e] + bias[0][i][run][2 * e], g1 = acc[i][j][8 * run + 2 * e + 1] + bias[0][i][run][2 * e + 1];
+                            const float u0 = acc[HB + i][j][8 * run + 2 * e] + bias[1][i][run][2 * e],
+                                        u1 = acc[HB + i][j][8 * run + 2 * e + 1] + bias[1][i][run][2 * e + 1];
+                            // (hidden is taken of the sums as they are, before mixed is rounded for the backward)
+                            hw[e] = pack2<Tag>(gated_act<kind>(g0) * u0, gated_act<kind>(g1) * u1);
+                            gw[e] = pack2<Tag>(g0, g1);
+                            uw[e] = pack2<Tag>(u0, u1);
+                        }
+                        uint16_t* const to = staged + r * kEpiRow + 32 * i + 16 * run + 8 * half;
+                        *reinterpret_cast<u32x4_t*>(to) = hw;
+                        *reinterpret_cast<u32x4_t*>(to + 32 * kEpiRow) = gw;
+                        *reinterpret_cast<u32x4_t*>(to + 64 * kEpiRow) = uw;
                     }
                 }
+                settle();
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int in_block = 8 * q + out_row;
+                    const int64_t row = m0 + BM / 2 * wm + 32 * j + in_block;
+                    const int col = col0 + 8 * out_chunk;
+                    const uint16_t* const from = staged + in_block * kEpiRow + 8 * out_chunk;
+                    if (row < a.rows && 8 * out_chunk < kRound && col < a.cols) {
+                        if (a.out != nullptr) {
+                            __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from),
+                                                        reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.out) + row * a.cols + col));
+                        }
+                        if (a.mixed != nullptr) {
+                            uint16_t* const to = static_cast<uint16_t*>(a.mixed) + row * 2 * a.cols + col;
+                            __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from + 32 * kEpiRow), reinterpret_cast<u32x4_t*>(to));
+                            __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from + 64 * kEpiRow), reinterpret_cast<u32x4_t*>(to + a.cols));
+                        }
+                    }
+                }
+                settle();
             }
-            settle();
-        }
+        });
     } else {
         static_assert(MODE == kGemmForward || NB % 2 == 0, "rounds of 64 columns");
 #pragma unroll
