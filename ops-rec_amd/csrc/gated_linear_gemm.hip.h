@@ -81,17 +81,38 @@ __device__ __forceinline__ void gated_act_slope(float z, float& act, float& slop
 // columns into the order of ils_column_of_mfma_row
 __device__ __forceinline__ int gemm_tr_col(int lane) { return 16 * ((lane >> 4) & 1) + 4 * (((lane & 1) << 1) | ((lane >> 1) & 1)); }
 
-constexpr int gemm_workgroups_per_cu(int bn, int bm) { return bn * bm >= 256 * 128 ? 2 : (bn * bm >= 128 * 128 ? 3 : 4); }
-
-template <typename Tag, int MODE, int BN, int BM, int STAGES>
-__global__ __launch_bounds__(kGemmThreads, gemm_workgroups_per_cu(BN, BM)) void gated_gemm_kernel(const GatedGemmArgs a)
+// A direct-to-LDS request: each lane's 16 bytes land at lds_byte_address + 16 * lane; out-of-range sources write zeros.  In assembly, and waited for by
+// count: behind the builtin the compiler lets no transposing LDS read pass before every request under way has arrived.
+__device__ __forceinline__ void gemm_request(uint32_t lds_byte_address, uint32_t voffset, u32x4_t rsrc, uint32_t soffset)
 {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :
+                 : "s"(lds_byte_address), "v"(voffset), "s"(rsrc), "s"(soffset)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ u32x4_t gemm_rsrc(const void* base, uint32_t bytes)
+{
+    const uint64_t at = reinterpret_cast<uint64_t>(base);
+    const u32x4_t r = {static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32) & 0xffffu, bytes, kBufferFlags};
+    return r;
+}
+
+// s_waitcnt: at most `vm` memory requests and `lgkm` LDS accesses under way
+constexpr int gemm_wait(int vm, int lgkm) { return (vm & 15) | (7 << 4) | (lgkm << 8) | ((vm >> 4) << 14); }
+
+// WM x WN wavefronts, each with MB x NB blocks of 32 x 32; STAGES tiles of LDS
+template <typename Tag, int MODE, int WM, int WN, int MB, int NB, int STAGES, int PER_CU>
+__global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const GatedGemmArgs a)
+{
+    static_assert(WM * WN == 4, "four wavefronts");
+    constexpr int BM = 32 * WM * MB, BN = 32 * WN * NB;  // of the tile
+    constexpr int kWaveN = 32 * NB, kWaveM = 32 * MB;
     constexpr bool NT = MODE != kGemmForward;     // the columns' side is read transposed
     constexpr bool MT = MODE == kGemmWeightGrad;  // the rows' side is
     constexpr int kReqsN = BN / 64, kReqsM = BM / 64, kReqs = kReqsN + kReqsM;  // direct-to-LDS instructions per wavefront and stage
+    static_assert(BM % 64 == 0 && BN % 64 == 0, "a stage's instructions are dealt evenly");
     constexpr int kNElems = BN * kGemmStep, kStage = (BN + BM) * kGemmStep;
-    constexpr int NB = BN / 64, MB = BM / 64;  // 32 x 32 blocks of a wavefront
-    constexpr int kEpiRow = 64 + 8;            // staged rows of 64 columns
+    constexpr int kEpiRow = (MODE == kGemmForward ? kWaveN / 2 : 64) + 8;  // staged rows of up to 64 columns
     constexpr int kEpiPlanes = MODE == kGemmForward ? 3 : 1;
     constexpr int kEpiWave = kEpiPlanes * 32 * kEpiRow;
     constexpr int kLds = STAGES * kStage > 4 * kEpiWave ? STAGES * kStage : 4 * kEpiWave;
@@ -99,7 +120,7 @@ __global__ __launch_bounds__(kGemmThreads, gemm_workgroups_per_cu(BN, BM)) void 
 
     const int lane = threadIdx.x & 63;
     const int wave = uniform(threadIdx.x >> 6);
-    const int wm = wave >> 1, wn = wave & 1;
+    const int wm = wave / WN, wn = wave % WN;
 
     // ---- the workgroup's tile
     const uint32_t tiles = static_cast<uint32_t>(a.tiles_m) * static_cast<uint32_t>(a.tiles_n);
@@ -124,22 +145,22 @@ __global__ __launch_bounds__(kGemmThreads, gemm_workgroups_per_cu(BN, BM)) void 
     // ---- sources.  Rows and depth past the end read as zeros on both sides (out-of-range bytes of a descriptor)
     const uint32_t n_row_bytes = static_cast<uint32_t>(NT ? a.cols : static_cast<int>(a.depth)) * 2u;
     const uint32_t m_row_bytes = MT ? static_cast<uint32_t>(a.rows) * 2u : static_cast<uint32_t>(a.depth) * 2u;
-    __amdgpu_buffer_rsrc_t n_rsrc, u_rsrc, m_rsrc;
+    u32x4_t n_rsrc, u_rsrc, m_rsrc;
     if constexpr (NT) {
-        n_rsrc = make_rsrc(static_cast<const uint8_t*>(a.n_side) + depth0 * n_row_bytes, static_cast<uint32_t>(depth) * n_row_bytes);
+        n_rsrc = gemm_rsrc(static_cast<const uint8_t*>(a.n_side) + depth0 * n_row_bytes, static_cast<uint32_t>(depth) * n_row_bytes);
         u_rsrc = n_rsrc;
     } else {
         const int rows_w = min(kOutCols, a.cols - n0);
         const uint8_t* const w = static_cast<const uint8_t*>(a.n_side);
-        n_rsrc = make_rsrc(w + static_cast<int64_t>(n0) * n_row_bytes, static_cast<uint32_t>(rows_w) * n_row_bytes);
-        u_rsrc = make_rsrc(w + (static_cast<int64_t>(a.cols) + n0) * n_row_bytes, static_cast<uint32_t>(rows_w) * n_row_bytes);
+        n_rsrc = gemm_rsrc(w + static_cast<int64_t>(n0) * n_row_bytes, static_cast<uint32_t>(rows_w) * n_row_bytes);
+        u_rsrc = gemm_rsrc(w + (static_cast<int64_t>(a.cols) + n0) * n_row_bytes, static_cast<uint32_t>(rows_w) * n_row_bytes);
     }
     if constexpr (MT) {
-        m_rsrc = make_rsrc(static_cast<const uint8_t*>(a.m_side) + depth0 * m_row_bytes, static_cast<uint32_t>(depth) * m_row_bytes);
+        m_rsrc = gemm_rsrc(static_cast<const uint8_t*>(a.m_side) + depth0 * m_row_bytes, static_cast<uint32_t>(depth) * m_row_bytes);
     } else {
         const int rows_m = a.rows - m0 < BM ? static_cast<int>(a.rows - m0) : BM;
         const uint32_t skipped = static_cast<uint32_t>(depth0) * 2u;
-        m_rsrc = make_rsrc(static_cast<const uint8_t*>(a.m_side) + m0 * m_row_bytes + skipped, static_cast<uint32_t>(rows_m) * m_row_bytes - skipped);
+        m_rsrc = gemm_rsrc(static_cast<const uint8_t*>(a.m_side) + m0 * m_row_bytes + skipped, static_cast<uint32_t>(rows_m) * m_row_bytes - skipped);
     }
 
     // ---- requests: byte offset of the lane's 16 bytes at depth 0, and (row-wise sides) where in the step they are
@@ -163,51 +184,67 @@ __global__ __launch_bounds__(kGemmThreads, gemm_workgroups_per_cu(BN, BM)) void 
             const int chunk = (lane & 3) ^ ((lds_row >> 2) & 3);
             int row = lds_row;
             if (n_part) {
-                // a wavefront's BN / 2 rows: BN / 4 of the gate, BN / 4 of the other projection
-                const int w = lds_row / (BN / 2), r = lds_row % (BN / 2) % (BN / 4);
-                row = w * (BN / 4) + (r & ~31) + ils_column_of_mfma_row(r & 31);
+                // a wavefront's rows: half of the gate, half of the other projection
+                const int w = lds_row / kWaveN, r = lds_row % kWaveN % (kWaveN / 2);
+                row = w * (kWaveN / 2) + (r & ~31) + ils_column_of_mfma_row(r & 31);
             }
             req_off[i] = static_cast<uint32_t>(row) * (n_part ? n_row_bytes : m_row_bytes) + chunk * 16u;
             req_depth[i] = 8 * chunk;
         }
     }
+    // A whole step's addresses are the lane's at depth 0 and a scalar; the depth's last, part-filled step and those past it are checked lane by
+    // lane (a scalar past a descriptor's end would not be).
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint16_t*)s_tiles));
     auto request = [&](int stage, int step) {
-        uint16_t* const base = s_tiles + stage * kStage;
         const int d0 = step * kGemmStep;
+        const auto each = [&](auto&& f) {
 #pragma unroll
-        for (int i = 0; i < kReqs; ++i) {
-            const bool n_part = i < kReqsN;
-            const int q = wave + 4 * (n_part ? i : i - kReqsN);
-            const bool across = n_part ? NT : MT;
-            const uint32_t along = across ? static_cast<uint32_t>(d0) * (n_part ? n_row_bytes : m_row_bytes) : static_cast<uint32_t>(d0) * 2u;
-            const uint32_t off = d0 + req_depth[i] < depth ? req_off[i] + along : kOutOfRange;
-            // (forward: 16 LDS rows of one projection per instruction)
-            const bool upper = MODE == kGemmForward && n_part && (16 * q) % (BN / 2) >= BN / 4;
-            load_to_lds_b128(n_part ? (upper ? u_rsrc : n_rsrc) : m_rsrc, base + (n_part ? 0 : kNElems) + q * 512, off);
+            for (int i = 0; i < kReqs; ++i) {
+                const bool n_part = i < kReqsN;
+                const int q = wave + 4 * (n_part ? i : i - kReqsN);
+                const uint32_t along = static_cast<uint32_t>(d0) * ((n_part ? NT : MT) ? (n_part ? n_row_bytes : m_row_bytes) : 2u);
+                // (forward: 16 LDS rows of one projection per instruction)
+                const bool upper = MODE == kGemmForward && n_part && (16 * q) % kWaveN >= kWaveN / 2;
+                f(i, lds0 + static_cast<uint32_t>(2 * (stage * kStage + (n_part ? 0 : kNElems) + q * 512)), n_part ? (upper ? u_rsrc : n_rsrc) : m_rsrc, along);
+            }
+        };
+        if (d0 + kGemmStep <= depth) {
+            each([&](int i, uint32_t to, u32x4_t rsrc, uint32_t along) { gemm_request(to, req_off[i], rsrc, along); });
+        } else {
+            each([&](int i, uint32_t to, u32x4_t rsrc, uint32_t along) {
+                gemm_request(to, d0 + req_depth[i] < depth ? req_off[i] + along : kOutOfRange, rsrc, 0u);
+            });
         }
     };
 
-    // ---- operand reads: wavefront (wm, wn) has rows BM / 2 wm .. and columns BN / 2 wn .. of the tile
-    int n_off[NB], m_off[MB];
+    // ---- operand reads: wavefront (wm, wn) has rows kWaveM wm .. and columns kWaveN wn .. of the tile.  Addresses within a stage: of a row-wise side,
+    // block 0 for each half of the step (further blocks are constants away); of the other, each block (whose 64-byte groups are XOR-ed)
     const int r = lane & 31, half = lane >> 5;
     const int swz = (r >> 2) & 3;
     const int tr_row = 8 * half + ((lane & 15) >> 2);
+    int n_at[NT ? NB : 2], m_at[MT ? MB : 2];
+    if constexpr (NT) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-        if constexpr (NT) {
-            const int c = BN / 2 * wn + 32 * i + gemm_tr_col(lane);
-            n_off[i] = tr_row * BN + v_chunk_swizzle<BN>(tr_row, c >> 3) * 8 + (c & 7);
-        } else {
-            n_off[i] = (BN / 2 * wn + 32 * i + r) * kGemmStep;
+        for (int i = 0; i < NB; ++i) {
+            const int c = kWaveN * wn + 32 * i + gemm_tr_col(lane);
+            n_at[i] = tr_row * BN + v_chunk_swizzle<BN>(tr_row, c >> 3) * 8 + (c & 7);
+        }
+    } else {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            n_at[kk] = (kWaveN * wn + r) * kGemmStep + ((2 * kk + half) ^ swz) * 8;
         }
     }
+    if constexpr (MT) {
 #pragma unroll
-    for (int j = 0; j < MB; ++j) {
-        if constexpr (MT) {
-            const int c = BM / 2 * wm + 32 * j + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-            m_off[j] = kNElems + tr_row * BM + v_chunk_swizzle<BM>(tr_row, c >> 3) * 8 + (c & 7);
-        } else {
-            m_off[j] = kNElems + (BM / 2 * wm + 32 * j + r) * kGemmStep;
+        for (int j = 0; j < MB; ++j) {
+            const int c = kWaveM * wm + 32 * j + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+            m_at[j] = kNElems + tr_row * BM + v_chunk_swizzle<BM>(tr_row, c >> 3) * 8 + (c & 7);
+        }
+    } else {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            m_at[kk] = kNElems + (kWaveM * wm + r) * kGemmStep + ((2 * kk + half) ^ swz) * 8;
         }
     }
     auto read_across = [&](const uint16_t* p, int width) -> u32x4_t {
@@ -229,61 +266,80 @@ __global__ __launch_bounds__(kGemmThreads, gemm_workgroups_per_cu(BN, BM)) void 
         }
     }
 
+    // A step is two halves of 16.  While the products of one half run, the operands of the next are read, so that the matrix pipe finds them
+    // there; the barrier that hands a stage over stands between the halves, when every wavefront has read all of the step before it:
+    // its stage is free and is asked for again at once, STAGES steps ahead.  (Past the end the requests go on, out of range, so that their count
+    // stays what the wait expects.)
     const int n_steps = (depth + kGemmStep - 1) / kGemmStep;
-    constexpr int kAhead = STAGES - 1;
-    for (int s = 0; s < kAhead && s < n_steps; ++s) {
-        request(s, s);
-    }
-    constexpr int kWait0 = 0 | (7 << 4) | (15 << 8);
-    constexpr int kWait1 = kReqs | (7 << 4) | (15 << 8);
-    static_assert(STAGES <= 3 && kReqs <= 15, "the count must fit the low bits of the wait instruction");
-    for (int t = 0; t < n_steps; ++t) {
-        // requests issued after step t's own: those of step t + 1 with three stages
-        __builtin_amdgcn_sched_barrier(0);
-        if (STAGES == 3 && t + 1 < n_steps) {
-            __builtin_amdgcn_s_waitcnt(kWait1);
-        } else {
-            __builtin_amdgcn_s_waitcnt(kWait0);
-        }
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        // every wavefront is past step t - 1: its stage may be overwritten
-        if (t + kAhead < n_steps) {
-            request((t + kAhead) % STAGES, t + kAhead);
-        }
-        const uint16_t* const st = s_tiles + (t % STAGES) * kStage;
+    u32x4_t nv[2][NB], mv[2][MB];
+    auto read = [&](int set, const uint16_t* st, int kk) {
+        const uint16_t* const n_from = st + n_at[NT ? 0 : kk];
+        const uint16_t* const m_from = st + m_at[MT ? 0 : kk];
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            const int chunk = ((2 * kk + half) ^ swz) * 8;
-            u32x4_t nv[NB], mv[MB];
-#pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                if constexpr (NT) {
-                    nv[i] = read_across(st + n_off[i] + 16 * kk * BN, BN);
-                } else {
-                    nv[i] = *reinterpret_cast<const u32x4_t*>(st + n_off[i] + chunk);
-                }
+        for (int i = 0; i < NB; ++i) {
+            if constexpr (NT) {
+                nv[set][i] = read_across(st + n_at[i] + 16 * kk * BN, BN);
+            } else {
+                nv[set][i] = *reinterpret_cast<const u32x4_t*>(n_from + 32 * i * kGemmStep);
             }
+        }
+#pragma unroll
+        for (int j = 0; j < MB; ++j) {
+            if constexpr (MT) {
+                mv[set][j] = read_across(st + m_at[j] + 16 * kk * BM, BM);
+            } else {
+                mv[set][j] = *reinterpret_cast<const u32x4_t*>(m_from + 32 * j * kGemmStep);
+            }
+        }
+    };
+    auto multiply = [&](int set) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
 #pragma unroll
             for (int j = 0; j < MB; ++j) {
-                if constexpr (MT) {
-                    mv[j] = read_across(st + m_off[j] + 16 * kk * BM, BM);
-                } else {
-                    mv[j] = *reinterpret_cast<const u32x4_t*>(st + m_off[j] + chunk);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < NB; ++i) {
-#pragma unroll
-                for (int j = 0; j < MB; ++j) {
-                    acc[i][j] = mfma32<Tag>(nv[i], mv[j], acc[i][j]);
-                }
+                acc[i][j] = mfma32<Tag>(nv[set][i], mv[set][j], acc[i][j]);
             }
         }
+    };
+    // the order asked of the scheduler: a read of the next operands behind each of the first products
+    constexpr int kReads = NB * (NT ? 2 : 1) + MB * (MT ? 2 : 1);
+    auto order = [] {
+        constexpr int kProducts = NB * MB, kEach = (kReads + kProducts - 1) / kProducts;
+#pragma unroll
+        for (int u = 0; u < kProducts; ++u) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);      // an MFMA
+            __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);  // LDS reads
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) {
+        request(s, s);
     }
+    __builtin_amdgcn_s_waitcnt(gemm_wait((STAGES - 1) * kReqs, 15));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    read(0, s_tiles, 0);
+    int stage = 0;
+    for (int t = 0; t < n_steps; ++t) {
+        __builtin_amdgcn_sched_barrier(0);
+        const uint16_t* const st = s_tiles + stage * kStage;
+        read(1, st, 1);
+        multiply(0);
+        order();
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(gemm_wait((STAGES - 2) * kReqs, 0));
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        request(stage, t + STAGES);
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        read(0, s_tiles + stage * kStage, 0);
+        multiply(1);
+        order();
+    }
+    __builtin_amdgcn_s_waitcnt(gemm_wait(0, 0));  // (the last requests write LDS that is used otherwise below)
 
     // ---- gradients in chunks of the depth: fp32 partial outputs, runs of 8 columns
-    const int64_t row_of_lane = m0 + BM / 2 * wm + r;
+    const int64_t row_of_lane = m0 + kWaveM * wm + r;
     if (MODE != kGemmForward && a.partial != nullptr) {
         float* const out = a.partial + static_cast<int64_t>(part) * a.rows * a.cols;
 #pragma unroll
@@ -293,7 +349,7 @@ __global__ __launch_bounds__(kGemmThreads, gemm_workgroups_per_cu(BN, BM)) void 
                 const int64_t row = row_of_lane + 32 * j;
 #pragma unroll
                 for (int run = 0; run < 2; ++run) {
-                    const int col = n0 + BN / 2 * wn + 32 * i + 16 * run + 8 * half;
+                    const int col = n0 + kWaveN * wn + 32 * i + 16 * run + 8 * half;
                     if (row < a.rows && col < a.cols) {
                         float4* const to = reinterpret_cast<float4*>(out + row * a.cols + col);
                         to[0] = make_float4(acc[i][j][8 * run], acc[i][j][8 * run + 1], acc[i][j][8 * run + 2], acc[i][j][8 * run + 3]);
@@ -315,10 +371,10 @@ __global__ __launch_bounds__(kGemmThreads, gemm_workgroups_per_cu(BN, BM)) void 
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     };
     if constexpr (MODE == kGemmForward) {
-        constexpr int kRound = BN / 4 < 64 ? BN / 4 : 64;  // columns of both projections a wavefront has: BN / 4, by up to 64
-        static_assert(BN / 4 == kRound, "one round");
+        constexpr int kRound = kWaveN / 2;  // columns of both projections a wavefront has
+        static_assert(kRound <= 64 && NB % 2 == 0, "one round");
         constexpr int HB = NB / 2;  // blocks of each projection
-        const int col0 = n0 + BN / 4 * wn;
+        const int col0 = n0 + kRound * wn;
         float bias[2][HB][2][8];
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
@@ -367,7 +423,7 @@ __global__ __launch_bounds__(kGemmThreads, gemm_workgroups_per_cu(BN, BM)) void 
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int in_block = 8 * q + out_row;
-                    const int64_t row = m0 + BM / 2 * wm + 32 * j + in_block;
+                    const int64_t row = m0 + kWaveM * wm + 32 * j + in_block;
                     const int col = col0 + 8 * out_chunk;
                     const uint16_t* const from = staged + in_block * kEpiRow + 8 * out_chunk;
                     if (row < a.rows && 8 * out_chunk < kRound && col < a.cols) {
@@ -407,8 +463,8 @@ __global__ __launch_bounds__(kGemmThreads, gemm_workgroups_per_cu(BN, BM)) void 
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int in_block = 8 * q + out_row;
-                    const int64_t row = m0 + BM / 2 * wm + 32 * j + in_block;
-                    const int col = n0 + BN / 2 * wn + 64 * c + 8 * out_chunk;
+                    const int64_t row = m0 + kWaveM * wm + 32 * j + in_block;
+                    const int col = n0 + kWaveN * wn + 64 * c + 8 * out_chunk;
                     if (row < a.rows && col < a.cols) {
                         __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(staged + in_block * kEpiRow + 8 * out_chunk),
                                                     reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.out) + row * a.cols + col));

@@ -71,9 +71,12 @@ int launched(const char* what)
 // Up to so many rows the kernel that streams the weight takes the call, in blocks of 64 rows.
 bool few_rows(const gated_linear_params* p) { return p->rows <= kFewRows; }
 
-// The tile: wide while its workgroups, two to a compute unit, fill the machine; square while those do; low for what is left.
+// The tile whose launch takes the fewest steps of the matrix units: rounds of workgroups times what a workgroup has to do, the larger
+// tiles' steps counted for less, as they need fewer bytes from LDS and memory for the same products.
 int tile_for(const GatedTile* tiles, int n, int64_t rows, int64_t cols)
 {
+    static const int forced = getenv("GATED_TILE") ? atoi(getenv("GATED_TILE")) : -1;
+    if (forced >= 0) return forced < n ? forced : n - 1;
     const int64_t cus = compute_units_or_256();
     for (int i = 0; i < n - 1; ++i) {
         if (ceil_div(rows, tiles[i].rows) * ceil_div(cols, tiles[i].cols) >= cus) {
@@ -107,11 +110,9 @@ Product plan(const GatedTile* tiles, int n, int64_t rows, int64_t cols, int64_t 
     const int64_t cus = compute_units_or_256();
     Product p;
     p.tile = &tiles[tile_for(tiles, n, rows, cols)];
-    if (n == 2 && ceil_div(rows, tiles[0].rows) * ceil_div(cols, tiles[0].cols) * ceil_div(depth, 256) >= 2 * cus && cols > tiles[1].cols) {
-        p.tile = &tiles[0];  // (a depth long enough to fill the machine by its chunks)
-    }
     const int64_t count = ceil_div(rows, p.tile->rows) * ceil_div(cols, p.tile->cols);
-    int64_t chunks = count >= cus ? 1 : 2 * cus / count;
+    int64_t chunks = count >= cus ? 1 : p.tile->per_cu * cus / count;
+    chunks = chunks > 1 ? chunks : 1;
     chunks = chunks < ceil_div(depth, 256) ? chunks : ceil_div(depth, 256);
     const int64_t fit = ceil_div(depth * depth_row_bytes, kMostBytes - kStep * depth_row_bytes);  // (a chunk lies behind one descriptor)
     chunks = chunks > fit ? chunks : fit;
@@ -141,11 +142,11 @@ BackwardPlan plan_backward(const gated_linear_bwd_params* p)
     b.d_mixed = rounded(static_cast<uint64_t>(f.rows) * static_cast<uint64_t>(f.inner) * 4u);
     b.sums = p->bias_grad != nullptr ? rounded(static_cast<uint64_t>(b.slices) * static_cast<uint64_t>(f.inner) * 8u) : 0;
     if (p->x_grad != nullptr) {
-        b.x = plan(k.x_grad, hstu::kGatedTiles, f.rows, f.cols, 2 * f.inner, f.cols * 2);
+        b.x = plan(k.x_grad, hstu::kGatedXGradTiles, f.rows, f.cols, 2 * f.inner, f.cols * 2);
         b.x_partial = b.x.chunks > 1 ? static_cast<uint64_t>(b.x.chunks) * static_cast<uint64_t>(f.rows) * static_cast<uint64_t>(f.cols) * 4u : 0;
     }
     if (p->weight_grad != nullptr) {
-        b.w = plan(k.weight_grad, 2, 2 * f.inner, f.cols, f.rows, (2 * f.inner > f.cols ? 2 * f.inner : f.cols) * 2);
+        b.w = plan(k.weight_grad, hstu::kGatedWeightTiles, 2 * f.inner, f.cols, f.rows, (2 * f.inner > f.cols ? 2 * f.inner : f.cols) * 2);
         b.w_partial = b.w.chunks > 1 ? static_cast<uint64_t>(b.w.chunks) * static_cast<uint64_t>(2 * f.inner) * static_cast<uint64_t>(f.cols) * 4u : 0;
     }
     return b;
@@ -202,8 +203,8 @@ HSTU_API const char* gated_linear_fwd_kernel_name(const gated_linear_params* p)
     if (p == nullptr || validate(p) != HSTU_OK) {
         return nullptr;
     }
-    static const char* const tiles[hstu::kGatedTiles] = {"gated_gemm_128x128", "gated_gemm_128x64", "gated_gemm_64x64"};
-    return few_rows(p) ? "gated_few_rows" : tiles[tile_for(kernels_of(p->dtype).forward, hstu::kGatedTiles, p->rows, p->inner)];
+    static const char* const tiles[hstu::kGatedForwardTiles] = {"gated_gemm_256x128", "gated_gemm_128x128", "gated_gemm_128x64", "gated_gemm_64x64"};
+    return few_rows(p) ? "gated_few_rows" : tiles[tile_for(kernels_of(p->dtype).forward, hstu::kGatedForwardTiles, p->rows, p->inner)];
 }
 
 HSTU_API int gated_linear_fwd(const gated_linear_params* p, void* stream)
@@ -245,7 +246,7 @@ HSTU_API int gated_linear_fwd(const gated_linear_params* p, void* stream)
     a.cols = static_cast<int>(p->inner);
     a.chunks = 1;
     a.activation = p->activation;
-    return launch_tiles(k.forward[tile_for(k.forward, hstu::kGatedTiles, p->rows, p->inner)], a, stream, "gated_gemm_kernel (forward)");
+    return launch_tiles(k.forward[tile_for(k.forward, hstu::kGatedForwardTiles, p->rows, p->inner)], a, stream, "gated_gemm_kernel (forward)");
 }
 
 HSTU_API int gated_linear_bwd_workspace_size(const gated_linear_bwd_params* p, uint64_t* workspace_bytes)

@@ -7,19 +7,22 @@
 
 namespace hstu {
 
-template <typename Tag, int MODE, int BN, int BM, int STAGES>
+template <typename Tag, int MODE, int WM, int WN, int MB, int NB, int STAGES, int PER_CU>
 constexpr GatedTile gated_tile()
 {
-    return {gated_gemm_kernel<Tag, MODE, BN, BM, STAGES>, MODE == kGemmForward ? BN / 2 : BN, BM};
+    return {gated_gemm_kernel<Tag, MODE, WM, WN, MB, NB, STAGES, PER_CU>, 32 * WN * NB / (MODE == kGemmForward ? 2 : 1), 32 * WM * MB, PER_CU};
 }
 
 template <typename Tag>
 const GatedKernels& gated_table()
 {
     static const GatedKernels table = {
-        {gated_tile<Tag, kGemmForward, 256, 128, 3>(), gated_tile<Tag, kGemmForward, 128, 128, 3>(), gated_tile<Tag, kGemmForward, 128, 64, 3>()},
-        {gated_tile<Tag, kGemmXGrad, 256, 128, 3>(), gated_tile<Tag, kGemmXGrad, 128, 128, 3>(), gated_tile<Tag, kGemmXGrad, 128, 64, 3>()},
-        {gated_tile<Tag, kGemmWeightGrad, 256, 128, 3>(), gated_tile<Tag, kGemmWeightGrad, 128, 128, 3>()},
+        {gated_tile<Tag, kGemmForward, 2, 2, 4, 4, 4, 1>(), gated_tile<Tag, kGemmForward, 2, 2, 2, 4, 3, 2>(), gated_tile<Tag, kGemmForward, 2, 2, 2, 2, 3, 3>(),
+         gated_tile<Tag, kGemmForward, 2, 2, 1, 2, 3, 4>()},
+        {gated_tile<Tag, kGemmXGrad, 2, 2, 4, 4, 4, 1>(), gated_tile<Tag, kGemmXGrad, 2, 2, 3, 4, 4, 1>(), gated_tile<Tag, kGemmXGrad, 2, 2, 2, 4, 3, 2>(),
+         gated_tile<Tag, kGemmXGrad, 2, 2, 2, 2, 3, 3>(), gated_tile<Tag, kGemmXGrad, 2, 2, 1, 2, 3, 4>()},
+        {gated_tile<Tag, kGemmWeightGrad, 2, 2, 4, 4, 4, 1>(), gated_tile<Tag, kGemmWeightGrad, 2, 2, 2, 4, 3, 2>(),
+         gated_tile<Tag, kGemmWeightGrad, 2, 2, 2, 2, 3, 3>()},
         {{gated_few_rows_kernel<Tag, 1, 8>, gated_few_rows_kernel<Tag, 1, 16>},
          {gated_few_rows_kernel<Tag, 2, 8>, gated_few_rows_kernel<Tag, 2, 16>},
          {gated_few_rows_kernel<Tag, 4, 8>, gated_few_rows_kernel<Tag, 4, 16>}},

@@ -8,14 +8,15 @@ struct GatedTile {
     void (*kernel)(const GatedGemmArgs);
     int cols;  // of the output, per workgroup (in the forward: of hidden)
     int rows;
+    int per_cu;  // workgroups that a compute unit holds
 };
 
-enum { kGatedTileWide, kGatedTileSquare, kGatedTileLow, kGatedTiles };
+constexpr int kGatedForwardTiles = 4, kGatedXGradTiles = 5, kGatedWeightTiles = 3;  // by falling size
 
 struct GatedKernels {
-    GatedTile forward[kGatedTiles];
-    GatedTile x_grad[kGatedTiles];
-    GatedTile weight_grad[2];  // wide, square
+    GatedTile forward[kGatedForwardTiles];
+    GatedTile x_grad[kGatedXGradTiles];
+    GatedTile weight_grad[kGatedWeightTiles];
     void (*few_rows[3][2])(const GatedFewRowsArgs);  // up to 16, 32, 64 rows; 8 or 16 columns of hidden per workgroup
     void (*stage)(const GatedStageArgs);
     void (*sum)(const GatedSumArgs);
