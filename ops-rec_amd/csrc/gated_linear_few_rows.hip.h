@@ -1,6 +1,6 @@
 // The gated projections for few rows, gfx950: hidden = act(x Wg^T + bg) * (x Wu^T + bu) for single tokens and small batches.
 //
-// Bound by the bytes of the weight, each read once per block of up to 64 rows, and for small layers by latency.  A workgroup has C columns of
+// Bound by the bytes of the weight, each read once, and for small layers by latency.  A workgroup has C columns of
 // hidden: C rows of the gate's weight and the C of the other projection, straight from memory into v_mfma_f32_16x16x32 operands (a lane's 16
 // bytes are 8 values of one weight row; nothing of the weight is read twice, so LDS would only add a trip).  Its eight wavefronts share
 // the depth: each takes every eighth run of 64 values, whose loads are all in flight before the first product, and the partial sums meet in LDS.
@@ -31,28 +31,29 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
 {
     constexpr int AB = C == 16 ? 2 : 1;  // 16-row weight operands
     constexpr int kRows = 16 * MB;
-    // partial sums [wavefront][operand][row of x][16 weight rows], rows padded by 4 so that 16 rows at 16 bytes spread over the banks
-    constexpr int kPitch = 16 + 4;
-    __shared__ __attribute__((aligned(16))) float s_part[kFewWaves * AB * kRows * kPitch];
+    // partial sums of half the wavefronts [wavefront][operand][row of x][16 weight rows], rows padded by 4 so that 16 rows at 16 bytes spread over
+    // the banks.  (Of all of them, 64 rows would leave room for one workgroup to a compute unit: 48 rows, 2048 -> 5632, 22 us.)
+    constexpr int kPitch = 16 + 4, kHalf = kFewWaves / 2;
+    __shared__ __attribute__((aligned(16))) float s_part[kHalf * AB * kRows * kPitch];
 
     const int lane = threadIdx.x & 63;
     const int wave = uniform(threadIdx.x >> 6);
     const int n0 = static_cast<int>(blockIdx.x) * C;
-    const int64_t m0 = static_cast<int64_t>(blockIdx.y) * kRows;
-    const int rows = a.rows - m0 < kRows ? static_cast<int>(a.rows - m0) : kRows;
+    const int rows = static_cast<int>(a.rows);  // (at most kRows)
     const int cols = min(C, a.inner - n0);
     const uint32_t row_bytes = static_cast<uint32_t>(a.depth) * 2u;
     // rows past the end read as zeros
     const __amdgpu_buffer_rsrc_t g_rsrc = make_rsrc(static_cast<const uint8_t*>(a.weight) + static_cast<int64_t>(n0) * row_bytes, static_cast<uint32_t>(cols) * row_bytes);
     const __amdgpu_buffer_rsrc_t u_rsrc =
         make_rsrc(static_cast<const uint8_t*>(a.weight) + (static_cast<int64_t>(a.inner) + n0) * row_bytes, static_cast<uint32_t>(cols) * row_bytes);
-    const __amdgpu_buffer_rsrc_t x_rsrc = make_rsrc(static_cast<const uint8_t*>(a.x) + m0 * row_bytes, static_cast<uint32_t>(rows) * row_bytes);
+    const __amdgpu_buffer_rsrc_t x_rsrc = make_rsrc(a.x, static_cast<uint32_t>(rows) * row_bytes);
 
     const int r = lane & 15, quarter = lane >> 4;
-    auto load = [&](__amdgpu_buffer_rsrc_t rsrc, int row, int d) -> u32x4_t {
-        const uint32_t off = d < a.depth ? static_cast<uint32_t>(row) * row_bytes + static_cast<uint32_t>(d) * 2u : kOutOfRange;
-        return __builtin_amdgcn_raw_buffer_load_b128(rsrc, static_cast<int>(off), 0, 0);
+    auto offset = [&](int row, int d) -> int {
+        return static_cast<int>(d < a.depth ? static_cast<uint32_t>(row) * row_bytes + static_cast<uint32_t>(d) * 2u : kOutOfRange);
     };
+    // (the weight is read once: non-temporal, so that x stays in the caches)
+    auto load_weight = [&](__amdgpu_buffer_rsrc_t rsrc, int row, int d) -> u32x4_t { return __builtin_amdgcn_raw_buffer_load_b128(rsrc, offset(row, d), 0, 2); };
     f32x4_t acc[AB][MB];
 #pragma unroll
     for (int i = 0; i < AB; ++i) {
@@ -70,21 +71,21 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
             for (int k = 0; k < 2; ++k) {
                 const int d = d0 + s * kFewWaves * kFewStep + 32 * k + 8 * quarter;
                 if constexpr (C == 16) {
-                    w[s][k][0] = load(g_rsrc, r, d);
-                    w[s][k][1] = load(u_rsrc, r, d);
+                    w[s][k][0] = load_weight(g_rsrc, r, d);
+                    w[s][k][1] = load_weight(u_rsrc, r, d);
                 } else {
                     // (rows 0 .. 7 the gate's, 8 .. 15 the other projection's, by lane)
                     const uint32_t in_row = d < a.depth && (r & 7) < cols ? static_cast<uint32_t>(d) * 2u : kOutOfRange;
                     const int64_t row = static_cast<int64_t>(n0) + (r & 7) + (r >= 8 ? a.inner : 0);
                     u32x4_t v = {0u, 0u, 0u, 0u};
                     if (in_row != kOutOfRange) {
-                        v = *reinterpret_cast<const u32x4_t*>(static_cast<const uint8_t*>(a.weight) + row * row_bytes + in_row);
+                        v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(static_cast<const uint8_t*>(a.weight) + row * row_bytes + in_row));
                     }
                     w[s][k][0] = v;
                 }
 #pragma unroll
                 for (int j = 0; j < MB; ++j) {
-                    x[s][k][j] = load(x_rsrc, 16 * j + r, d);
+                    x[s][k][j] = __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, offset(16 * j + r, d), 0, 0);
                 }
             }
         }
@@ -102,12 +103,25 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
             }
         }
     }
-    // a lane has weight rows 4 quarter .. + 3 of row r of x
+    // a lane has weight rows 4 quarter .. + 3 of row r of x; the second half of the wavefronts hands its sums to the first
+    auto place = [&](int w, int i, int j) { return reinterpret_cast<f32x4_t*>(s_part + ((w * AB + i) * kRows + 16 * j + r) * kPitch + 4 * quarter); };
+    if (wave >= kHalf) {
 #pragma unroll
-    for (int i = 0; i < AB; ++i) {
+        for (int i = 0; i < AB; ++i) {
 #pragma unroll
-        for (int j = 0; j < MB; ++j) {
-            *reinterpret_cast<f32x4_t*>(s_part + ((wave * AB + i) * kRows + 16 * j + r) * kPitch + 4 * quarter) = acc[i][j];
+            for (int j = 0; j < MB; ++j) {
+                *place(wave - kHalf, i, j) = acc[i][j];
+            }
+        }
+    }
+    __syncthreads();
+    if (wave < kHalf) {
+#pragma unroll
+        for (int i = 0; i < AB; ++i) {
+#pragma unroll
+            for (int j = 0; j < MB; ++j) {
+                *place(wave, i, j) += acc[i][j];
+            }
         }
     }
     __syncthreads();
@@ -120,7 +134,7 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
 #pragma unroll
-            for (int w = 0; w < kFewWaves; ++w) {
+            for (int w = 0; w < kHalf; ++w) {
                 const int i = C == 16 ? p : 0, col = C == 16 ? c : c + 8 * p;
                 sum[p] += s_part[((w * AB + i) * kRows + row) * kPitch + col];
             }
@@ -129,7 +143,7 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
                 sum[p] += lo_to_float<Tag>(b);
             }
         }
-        const int64_t to = m0 + row;
+        const int64_t to = row;
         if (a.hidden != nullptr) {
             float act = 0.0f;
             with_activation(a.activation, [&](auto chosen) { act = gated_act<decltype(chosen)::value>(sum[0]); });

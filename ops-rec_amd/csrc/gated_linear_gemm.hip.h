@@ -114,7 +114,9 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
     constexpr int kNElems = BN * kGemmStep, kStage = (BN + BM) * kGemmStep;
     constexpr int kEpiRow = (MODE == kGemmForward ? kWaveN / 2 : 64) + 8;  // staged rows of up to 64 columns
     constexpr int kEpiPlanes = MODE == kGemmForward ? 3 : 1;
-    constexpr int kEpiWave = kEpiPlanes * 32 * kEpiRow;
+    // (a second piece where the stages' LDS has room for it)
+    constexpr int kEpiPieces = MODE == kGemmForward && 2 * 4 * kEpiPlanes * 32 * kEpiRow <= STAGES * kStage ? 2 : 1;
+    constexpr int kEpiWave = kEpiPieces * kEpiPlanes * 32 * kEpiRow;
     constexpr int kLds = STAGES * kStage > 4 * kEpiWave ? STAGES * kStage : 4 * kEpiWave;
     __shared__ __attribute__((aligned(1024))) uint16_t s_tiles[kLds];
 
@@ -254,14 +256,36 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
         return v;
     };
 
+    // the sums start from the bias: nothing is left to add behind the products
     f32x16_t acc[NB][MB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
+        float first[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            first[e] = 0.0f;
+        }
+        if constexpr (MODE == kGemmForward) {
+            if (a.bias != nullptr) {
+#pragma unroll
+                for (int run = 0; run < 2; ++run) {
+                    const int upper = i / (NB / 2), col = n0 + kWaveN / 2 * wn + 32 * (i % (NB / 2)) + 16 * run + 8 * half;
+                    u32x4_t w = {0u, 0u, 0u, 0u};
+                    if (col < a.cols) {
+                        w = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(a.bias) + static_cast<int64_t>(upper) * a.cols + col);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        ils_unpack2<Tag>(w[e], first[8 * run + 2 * e], first[8 * run + 2 * e + 1]);
+                    }
+                }
+            }
+        }
 #pragma unroll
         for (int j = 0; j < MB; ++j) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                acc[i][j][e] = 0.0f;
+                acc[i][j][e] = first[e];
             }
         }
     }
@@ -361,10 +385,10 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
         return;
     }
 
-    // ---- 16-bit outputs, through LDS in pieces of 32 rows by 64 columns per wavefront, so that every store writes whole 128-byte runs
+    // ---- 16-bit outputs, through LDS in pieces of 32 rows by up to 64 columns per wavefront, so that every store writes whole 128-byte runs.  Pieces
+    // alternate between two places: the values of the next are worked out while the last goes out.
     __builtin_amdgcn_s_barrier();  // every wavefront is done reading the last stage
     uint16_t* const staged = s_tiles + wave * kEpiWave;
-    const int out_row = lane >> 3, out_chunk = lane & 7;
     auto settle = [] {  // (a wavefront's own LDS accesses stay in order; the compiler must keep them so)
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -374,30 +398,15 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
         constexpr int kRound = kWaveN / 2;  // columns of both projections a wavefront has
         static_assert(kRound <= 64 && NB % 2 == 0, "one round");
         constexpr int HB = NB / 2;  // blocks of each projection
-        const int col0 = n0 + kRound * wn;
-        float bias[2][HB][2][8];
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-#pragma unroll
-            for (int i = 0; i < HB; ++i) {
-#pragma unroll
-                for (int run = 0; run < 2; ++run) {
-                    const int col = col0 + 32 * i + 16 * run + 8 * half;
-                    u32x4_t w = {0u, 0u, 0u, 0u};
-                    if (a.bias != nullptr && col < a.cols) {
-                        w = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(a.bias) + static_cast<int64_t>(p) * a.cols + col);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        ils_unpack2<Tag>(w[e], bias[p][i][run][2 * e], bias[p][i][run][2 * e + 1]);
-                    }
-                }
-            }
-        }
-        with_activation(a.activation, [&](auto chosen) {
+        constexpr int kPerRow = kRound / 8, kRowsAtOnce = 64 / kPerRow;  // lanes to a row of 16-byte pieces, rows of a store
+        const int col = n0 + kRound * wn + 8 * (lane % kPerRow);
+        const auto finish = [&](auto chosen, auto kept) {
             constexpr int kind = decltype(chosen)::value;
+            constexpr bool keep = decltype(kept)::value;
+            constexpr int kPlane = 32 * kEpiRow;
 #pragma unroll
             for (int j = 0; j < MB; ++j) {
+                uint16_t* const piece = staged + (j % kEpiPieces) * kEpiPlanes * kPlane;
 #pragma unroll
                 for (int i = 0; i < HB; ++i) {
 #pragma unroll
@@ -405,44 +414,56 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
                         u32x4_t hw, gw, uw;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const float g0 = acc[i][j][8 * run + 2 * e] + bias[0][i][run][2 * e], g1 = acc[i][j][8 * run + 2 * e + 1] + bias[0][i][run][2 * e + 1];
-                            const float u0 = acc[HB + i][j][8 * run + 2 * e] + bias[1][i][run][2 * e],
-                                        u1 = acc[HB + i][j][8 * run + 2 * e + 1] + bias[1][i][run][2 * e + 1];
+                            const float g0 = acc[i][j][8 * run + 2 * e], g1 = acc[i][j][8 * run + 2 * e + 1];
+                            const float u0 = acc[HB + i][j][8 * run + 2 * e], u1 = acc[HB + i][j][8 * run + 2 * e + 1];
                             // (hidden is taken of the sums as they are, before mixed is rounded for the backward)
                             hw[e] = pack2<Tag>(gated_act<kind>(g0) * u0, gated_act<kind>(g1) * u1);
-                            gw[e] = pack2<Tag>(g0, g1);
-                            uw[e] = pack2<Tag>(u0, u1);
+                            if constexpr (keep) {
+                                gw[e] = pack2<Tag>(g0, g1);
+                                uw[e] = pack2<Tag>(u0, u1);
+                            }
                         }
-                        uint16_t* const to = staged + r * kEpiRow + 32 * i + 16 * run + 8 * half;
+                        uint16_t* const to = piece + r * kEpiRow + 32 * i + 16 * run + 8 * half;
                         *reinterpret_cast<u32x4_t*>(to) = hw;
-                        *reinterpret_cast<u32x4_t*>(to + 32 * kEpiRow) = gw;
-                        *reinterpret_cast<u32x4_t*>(to + 64 * kEpiRow) = uw;
+                        if constexpr (keep) {
+                            *reinterpret_cast<u32x4_t*>(to + kPlane) = gw;
+                            *reinterpret_cast<u32x4_t*>(to + 2 * kPlane) = uw;
+                        }
                     }
                 }
                 settle();
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int in_block = 8 * q + out_row;
+                for (int q = 0; q < 32 / kRowsAtOnce; ++q) {
+                    const int in_block = kRowsAtOnce * q + lane / kPerRow;
                     const int64_t row = m0 + kWaveM * wm + 32 * j + in_block;
-                    const int col = col0 + 8 * out_chunk;
-                    const uint16_t* const from = staged + in_block * kEpiRow + 8 * out_chunk;
-                    if (row < a.rows && 8 * out_chunk < kRound && col < a.cols) {
-                        if (a.out != nullptr) {
+                    const uint16_t* const from = piece + in_block * kEpiRow + 8 * (lane % kPerRow);
+                    if (row < a.rows && col < a.cols) {
+                        if (!keep || a.out != nullptr) {
                             __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from),
                                                         reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.out) + row * a.cols + col));
                         }
-                        if (a.mixed != nullptr) {
+                        if constexpr (keep) {
                             uint16_t* const to = static_cast<uint16_t*>(a.mixed) + row * 2 * a.cols + col;
-                            __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from + 32 * kEpiRow), reinterpret_cast<u32x4_t*>(to));
-                            __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from + 64 * kEpiRow), reinterpret_cast<u32x4_t*>(to + a.cols));
+                            __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from + kPlane), reinterpret_cast<u32x4_t*>(to));
+                            __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from + 2 * kPlane), reinterpret_cast<u32x4_t*>(to + a.cols));
                         }
                     }
                 }
-                settle();
+                if constexpr (kEpiPieces == 1) {
+                    settle();
+                }
+            }
+        };
+        with_activation(a.activation, [&](auto chosen) {
+            if (a.mixed != nullptr) {
+                finish(chosen, std::true_type{});
+            } else {
+                finish(chosen, std::false_type{});
             }
         });
     } else {
         static_assert(MODE == kGemmForward || NB % 2 == 0, "rounds of 64 columns");
+        const int out_row = lane >> 3, out_chunk = lane & 7;
 #pragma unroll
         for (int j = 0; j < MB; ++j) {
 #pragma unroll

@@ -68,22 +68,29 @@ int launched(const char* what)
     return err == hipSuccess ? HSTU_OK : set_error(HSTU_ERR_RUNTIME, "launch of %s failed: %s", what, hipGetErrorString(err));
 }
 
-// Up to so many rows the kernel that streams the weight takes the call, in blocks of 64 rows.
+// Up to so many rows the kernel that streams the weight takes the call.
 bool few_rows(const gated_linear_params* p) { return p->rows <= kFewRows; }
 
-// The tile whose launch takes the fewest steps of the matrix units: rounds of workgroups times what a workgroup has to do, the larger
-// tiles' steps counted for less, as they need fewer bytes from LDS and memory for the same products.
-int tile_for(const GatedTile* tiles, int n, int64_t rows, int64_t cols)
+// What a product is estimated to take, in us: rounds of workgroups, one per compute unit each, and with several chunks of the depth the traffic of
+// their fp32 partial outputs and the launch that adds them.
+double cost_of(const GatedTile& t, int64_t rows, int64_t cols, int64_t depth, int64_t chunks)
 {
-    static const int forced = getenv("GATED_TILE") ? atoi(getenv("GATED_TILE")) : -1;
-    if (forced >= 0) return forced < n ? forced : n - 1;
-    const int64_t cus = compute_units_or_256();
-    for (int i = 0; i < n - 1; ++i) {
-        if (ceil_div(rows, tiles[i].rows) * ceil_div(cols, tiles[i].cols) >= cus) {
-            return i;
+    const int64_t all = ceil_div(rows, t.rows) * ceil_div(cols, t.cols) * chunks, rounds = ceil_div(all, compute_units_or_256());
+    const double steps = static_cast<double>(ceil_div(ceil_div(depth, chunks), kStep));
+    const double products = static_cast<double>(rounds) * (steps * (rounds == 1 ? t.alone : t.step) + t.fixed);
+    return chunks == 1 ? products : products + 4.0 + static_cast<double>(rows) * static_cast<double>(cols) * static_cast<double>(chunks) * 1.1e-6;
+}
+
+const GatedTile& forward_tile(const gated_linear_params* p)
+{
+    const GatedTile* const tiles = kernels_of(p->dtype).forward;
+    const GatedTile* best = &tiles[0];
+    for (int i = 1; i < hstu::kGatedForwardTiles; ++i) {
+        if (cost_of(tiles[i], p->rows, p->inner, p->cols, 1) < cost_of(*best, p->rows, p->inner, p->cols, 1)) {
+            best = &tiles[i];
         }
     }
-    return n - 1;
+    return *best;
 }
 
 int launch_tiles(const GatedTile& t, GatedGemmArgs a, void* stream, const char* what)
@@ -98,8 +105,8 @@ int launch_tiles(const GatedTile& t, GatedGemmArgs a, void* stream, const char* 
     return launched(what);
 }
 
-// A gradient's product: its tile, and the chunks its depth is cut into so that short grids fill the machine -- two workgroups to a compute unit --,
-// each of 256 values at least: a chunk costs the traffic of its fp32 partial output.
+// A gradient's product: its tile, and the chunks its depth is cut into where the tiles are too few for the machine -- one or two workgroups to a compute
+// unit then, of 256 values of the depth at least.
 struct Product {
     const GatedTile* tile;
     int64_t chunk;
@@ -107,16 +114,22 @@ struct Product {
 };
 Product plan(const GatedTile* tiles, int n, int64_t rows, int64_t cols, int64_t depth, int64_t depth_row_bytes)
 {
-    const int64_t cus = compute_units_or_256();
-    Product p;
-    p.tile = &tiles[tile_for(tiles, n, rows, cols)];
-    const int64_t count = ceil_div(rows, p.tile->rows) * ceil_div(cols, p.tile->cols);
-    int64_t chunks = count >= cus ? 1 : p.tile->per_cu * cus / count;
-    chunks = chunks > 1 ? chunks : 1;
-    chunks = chunks < ceil_div(depth, 256) ? chunks : ceil_div(depth, 256);
-    const int64_t fit = ceil_div(depth * depth_row_bytes, kMostBytes - kStep * depth_row_bytes);  // (a chunk lies behind one descriptor)
-    chunks = chunks > fit ? chunks : fit;
-    p.chunk = ceil_div(ceil_div(depth, chunks), kStep) * kStep;
+    const int64_t cus = compute_units_or_256(), fit = ceil_div(depth * depth_row_bytes, kMostBytes - kStep * depth_row_bytes);  // (a chunk lies behind one descriptor)
+    const GatedTile* tile = nullptr;
+    int64_t chunks = 0;
+    double cost = 0.0;
+    for (int i = 0; i < n; ++i) {
+        const int64_t count = ceil_div(rows, tiles[i].rows) * ceil_div(cols, tiles[i].cols);
+        for (const int64_t wanted : {int64_t{1}, cus / count, 2 * cus / count}) {
+            int64_t c = wanted < ceil_div(depth, 256) ? wanted : ceil_div(depth, 256);
+            c = c > fit ? c : fit;
+            const double each = cost_of(tiles[i], rows, cols, depth, c);
+            if (tile == nullptr || each < cost) {
+                tile = &tiles[i], chunks = c, cost = each;
+            }
+        }
+    }
+    Product p{tile, ceil_div(ceil_div(depth, chunks), kStep) * kStep, 0};
     p.chunks = ceil_div(depth, p.chunk);
     return p;
 }
@@ -203,8 +216,7 @@ HSTU_API const char* gated_linear_fwd_kernel_name(const gated_linear_params* p)
     if (p == nullptr || validate(p) != HSTU_OK) {
         return nullptr;
     }
-    static const char* const tiles[hstu::kGatedForwardTiles] = {"gated_gemm_256x128", "gated_gemm_128x128", "gated_gemm_128x64", "gated_gemm_64x64"};
-    return few_rows(p) ? "gated_few_rows" : tiles[tile_for(kernels_of(p->dtype).forward, hstu::kGatedForwardTiles, p->rows, p->inner)];
+    return few_rows(p) ? "gated_few_rows" : forward_tile(p).name;
 }
 
 HSTU_API int gated_linear_fwd(const gated_linear_params* p, void* stream)
@@ -228,10 +240,9 @@ HSTU_API int gated_linear_fwd(const gated_linear_params* p, void* stream)
         a.depth = static_cast<int>(p->cols);
         a.inner = static_cast<int>(p->inner);
         a.activation = p->activation;
-        const int size = p->rows <= 16 ? 0 : (p->rows <= 32 ? 1 : 2), block = 16 << size;
+        const int blocks = static_cast<int>(ceil_div(p->rows, 16));  // of 16 rows: at most four
         const bool sixteen = p->inner >= 16 * static_cast<int64_t>(compute_units_or_256());
-        hipLaunchKernelGGL(k.few_rows[size][sixteen ? 1 : 0],
-                           dim3(static_cast<uint32_t>(ceil_div(p->inner, sixteen ? 16 : 8)), static_cast<uint32_t>(ceil_div(p->rows, block))), dim3(512), 0,
+        hipLaunchKernelGGL(k.few_rows[blocks - 1][sixteen ? 1 : 0], dim3(static_cast<uint32_t>(ceil_div(p->inner, sixteen ? 16 : 8))), dim3(512), 0,
                            static_cast<hipStream_t>(stream), a);
         return launched("gated_few_rows_kernel");
     }
@@ -246,7 +257,7 @@ HSTU_API int gated_linear_fwd(const gated_linear_params* p, void* stream)
     a.cols = static_cast<int>(p->inner);
     a.chunks = 1;
     a.activation = p->activation;
-    return launch_tiles(k.forward[tile_for(k.forward, hstu::kGatedForwardTiles, p->rows, p->inner)], a, stream, "gated_gemm_kernel (forward)");
+    return launch_tiles(forward_tile(p), a, stream, "gated_gemm_kernel (forward)");
 }
 
 HSTU_API int gated_linear_bwd_workspace_size(const gated_linear_bwd_params* p, uint64_t* workspace_bytes)

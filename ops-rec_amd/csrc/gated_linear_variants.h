@@ -6,9 +6,12 @@ namespace hstu {
 
 struct GatedTile {
     void (*kernel)(const GatedGemmArgs);
+    const char* name;
     int cols;  // of the output, per workgroup (in the forward: of hidden)
     int rows;
-    int per_cu;  // workgroups that a compute unit holds
+    // what a workgroup takes, in us (measured at 512 .. 4096 deep products; only their ratios matter): a step of the depth with a compute unit to itself, its
+    // share of a step where the units are full, and everything before the first and behind the last step
+    float alone, step, fixed;
 };
 
 constexpr int kGatedForwardTiles = 4, kGatedXGradTiles = 5, kGatedWeightTiles = 3;  // by falling size
@@ -17,7 +20,7 @@ struct GatedKernels {
     GatedTile forward[kGatedForwardTiles];
     GatedTile x_grad[kGatedXGradTiles];
     GatedTile weight_grad[kGatedWeightTiles];
-    void (*few_rows[3][2])(const GatedFewRowsArgs);  // up to 16, 32, 64 rows; 8 or 16 columns of hidden per workgroup
+    void (*few_rows[4][2])(const GatedFewRowsArgs);  // up to 16, 32, 48, 64 rows; 8 or 16 columns of hidden per workgroup
     void (*stage)(const GatedStageArgs);
     void (*sum)(const GatedSumArgs);
 };

@@ -112,11 +112,11 @@ def name(rows, cols, inner):
 
 def test_every_tile_of_the_forward():
     seen = set()
-    for rows, cols, inner in ((64, 64, 64), (200, 64, 256), (1300, 64, 2048), (8300, 72, 2056)):
+    for rows, cols, inner in ((64, 64, 64), (200, 64, 256), (700, 64, 2048), (8300, 72, 2056), (4096, 2056, 2048)):
         seen.add(name(rows, cols, inner))
         check(rows, cols, inner, BF16, backward=False, seed=3)
         check(rows, cols, inner, FP16, "gelu", backward=False, bias=False, seed=4)
-    assert len(seen) == 4, seen
+    assert len(seen) == 5, seen
 
 
 def test_values_far_out():
