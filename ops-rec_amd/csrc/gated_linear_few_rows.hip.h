@@ -1,10 +1,11 @@
 // The gated projections for few rows, gfx950: hidden = act(x Wg^T + bg) * (x Wu^T + bu) for single tokens and small batches.
 //
-// Bound by the bytes of the weight, each read once, and for small layers by latency.  A workgroup has C columns of
-// hidden: C rows of the gate's weight and the C of the other projection, straight from memory into v_mfma_f32_16x16x32 operands (a lane's 16
-// bytes are 8 values of one weight row; nothing of the weight is read twice, so LDS would only add a trip).  Its eight wavefronts share
-// the depth: each takes every eighth run of 64 values, whose loads are all in flight before the first product, and the partial sums meet in LDS.
-// C is 8 (gate and other projection are the two halves of one operand) where 16 would leave compute units without a workgroup.
+// Bound by the bytes of the weight, each read once, by those of x, which every workgroup reads, and for small layers by latency.  A workgroup has C columns
+// of hidden: C rows of the gate's weight and the C of the other projection, straight from memory into v_mfma_f32_16x16x32 operands (a lane's 16 bytes are
+// 8 values of one weight row; nothing of the weight is read twice, so LDS would only add a trip).  Its eight wavefronts share the depth: each takes every
+// eighth run of 64 values, whose loads are all in flight before the first product, and the partial sums meet in LDS.
+// C is 8, 16, 24 or 32, whichever leaves the fullest compute unit the least to read: rounds of workgroups times 2 C + rows.  (48 rows,
+// 2048 -> 5632: 352 workgroups of 16 columns, two on some compute units, took 25 us; 235 of 24, one on each, 15.)
 #pragma once
 #include "gated_linear_gemm.hip.h"
 
@@ -25,14 +26,14 @@ __device__ __forceinline__ f32x4_t gated_mfma16(u32x4_t a, u32x4_t b, f32x4_t c)
     }
 }
 
-// MB = blocks of 16 rows, C = columns of hidden per workgroup (8 or 16)
-template <typename Tag, int MB, int C>
+// MB = blocks of 16 rows, AB = blocks of 16 weight rows (C = 8 AB)
+template <typename Tag, int MB, int AB>
 __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const GatedFewRowsArgs a)
 {
-    constexpr int AB = C == 16 ? 2 : 1;  // 16-row weight operands
+    constexpr int C = 8 * AB;
     constexpr int kRows = 16 * MB;
     // partial sums of half the wavefronts [wavefront][operand][row of x][16 weight rows], rows padded by 4 so that 16 rows at 16 bytes spread over
-    // the banks.  (Of all of them, 64 rows would leave room for one workgroup to a compute unit: 48 rows, 2048 -> 5632, 22 us.)
+    // the banks
     constexpr int kPitch = 16 + 4, kHalf = kFewWaves / 2;
     __shared__ __attribute__((aligned(16))) float s_part[kHalf * AB * kRows * kPitch];
 
@@ -42,18 +43,18 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
     const int rows = static_cast<int>(a.rows);  // (at most kRows)
     const int cols = min(C, a.inner - n0);
     const uint32_t row_bytes = static_cast<uint32_t>(a.depth) * 2u;
-    // rows past the end read as zeros
-    const __amdgpu_buffer_rsrc_t g_rsrc = make_rsrc(static_cast<const uint8_t*>(a.weight) + static_cast<int64_t>(n0) * row_bytes, static_cast<uint32_t>(cols) * row_bytes);
-    const __amdgpu_buffer_rsrc_t u_rsrc =
-        make_rsrc(static_cast<const uint8_t*>(a.weight) + (static_cast<int64_t>(a.inner) + n0) * row_bytes, static_cast<uint32_t>(cols) * row_bytes);
+    // rows and columns past the end read as zeros
+    const __amdgpu_buffer_rsrc_t w_rsrc = make_rsrc(a.weight, static_cast<uint32_t>(2 * a.inner) * row_bytes);
     const __amdgpu_buffer_rsrc_t x_rsrc = make_rsrc(a.x, static_cast<uint32_t>(rows) * row_bytes);
 
     const int r = lane & 15, quarter = lane >> 4;
-    auto offset = [&](int row, int d) -> int {
-        return static_cast<int>(d < a.depth ? static_cast<uint32_t>(row) * row_bytes + static_cast<uint32_t>(d) * 2u : kOutOfRange);
-    };
-    // (the weight is read once: non-temporal, so that x stays in the caches)
-    auto load_weight = [&](__amdgpu_buffer_rsrc_t rsrc, int row, int d) -> u32x4_t { return __builtin_amdgcn_raw_buffer_load_b128(rsrc, offset(row, d), 0, 2); };
+    // the lane's weight rows, the gate's C ahead of the other projection's
+    uint32_t w_row[AB];
+#pragma unroll
+    for (int i = 0; i < AB; ++i) {
+        const int at = 16 * i + r, c = at < C ? at : at - C;
+        w_row[i] = c < cols ? static_cast<uint32_t>((at < C ? 0 : a.inner) + n0 + c) * row_bytes : kOutOfRange;
+    }
     f32x4_t acc[AB][MB];
 #pragma unroll
     for (int i = 0; i < AB; ++i) {
@@ -62,35 +63,34 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
             acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         }
     }
-    constexpr int kUnroll = MB <= 2 ? 4 : 2;
-    for (int d0 = wave * kFewStep; d0 < a.depth; d0 += kFewWaves * kFewStep * kUnroll) {
-        u32x4_t w[kUnroll][2][AB], x[kUnroll][2][MB];
+    constexpr int kUnroll = AB + MB <= 4 ? 4 : 2;
+    // Workgroups begin at different runs of the depth: rows a multiple of 4 KB apart lie in one channel of the L2, which all would ask at once.
+    const int runs = (a.depth + kFewStep - 1) / kFewStep, turn = static_cast<int>(blockIdx.x * 5u % static_cast<uint32_t>(runs));
+    const auto batch = [&](auto count, int run0) {  // so many runs, every eighth from run0 on
+        constexpr int kCount = decltype(count)::value;
+        u32x4_t w[kCount][2][AB], x[kCount][2][MB];
 #pragma unroll
-        for (int s = 0; s < kUnroll; ++s) {
+        for (int s = 0; s < kCount; ++s) {
+            const int run = run0 + s * kFewWaves + turn;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const int d = d0 + s * kFewWaves * kFewStep + 32 * k + 8 * quarter;
-                if constexpr (C == 16) {
-                    w[s][k][0] = load_weight(g_rsrc, r, d);
-                    w[s][k][1] = load_weight(u_rsrc, r, d);
-                } else {
-                    // (rows 0 .. 7 the gate's, 8 .. 15 the other projection's, by lane)
-                    const uint32_t in_row = d < a.depth && (r & 7) < cols ? static_cast<uint32_t>(d) * 2u : kOutOfRange;
-                    const int64_t row = static_cast<int64_t>(n0) + (r & 7) + (r >= 8 ? a.inner : 0);
-                    u32x4_t v = {0u, 0u, 0u, 0u};
-                    if (in_row != kOutOfRange) {
-                        v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(static_cast<const uint8_t*>(a.weight) + row * row_bytes + in_row));
-                    }
-                    w[s][k][0] = v;
+                const int d = (run < runs ? run : run - runs) * kFewStep + 32 * k + 8 * quarter;
+                const uint32_t along = static_cast<uint32_t>(d) * 2u;
+#pragma unroll
+                for (int i = 0; i < AB; ++i) {  // (the weight is read once: non-temporal, so that x stays in the caches)
+                    const uint32_t off = d < a.depth && w_row[i] != kOutOfRange ? w_row[i] + along : kOutOfRange;
+                    w[s][k][i] = __builtin_amdgcn_raw_buffer_load_b128(w_rsrc, static_cast<int>(off), 0, 2);
                 }
 #pragma unroll
                 for (int j = 0; j < MB; ++j) {
-                    x[s][k][j] = __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, offset(16 * j + r, d), 0, 0);
+                    const uint32_t off = d < a.depth ? static_cast<uint32_t>(16 * j + r) * row_bytes + along : kOutOfRange;
+                    x[s][k][j] = __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, static_cast<int>(off), 0, 0);
                 }
             }
         }
+        __builtin_amdgcn_sched_barrier(0);  // (the compiler would move each load to its product, to save registers that are there)
 #pragma unroll
-        for (int s = 0; s < kUnroll; ++s) {
+        for (int s = 0; s < kCount; ++s) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
 #pragma unroll
@@ -102,6 +102,13 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
                 }
             }
         }
+    };
+    int run0 = wave;
+    for (; run0 + kFewWaves * (kUnroll - 1) < runs; run0 += kFewWaves * kUnroll) {
+        batch(std::integral_constant<int, kUnroll>{}, run0);
+    }
+    for (; run0 < runs; run0 += kFewWaves) {
+        batch(std::integral_constant<int, 1>{}, run0);
     }
     // a lane has weight rows 4 quarter .. + 3 of row r of x; the second half of the wavefronts hands its sums to the first
     auto place = [&](int w, int i, int j) { return reinterpret_cast<f32x4_t*>(s_part + ((w * AB + i) * kRows + 16 * j + r) * kPitch + 4 * quarter); };
@@ -125,8 +132,8 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
         }
     }
     __syncthreads();
-    for (int at = threadIdx.x; at < kRows * C; at += kFewThreads) {
-        const int row = at / C, c = at % C;
+    for (int one = threadIdx.x; one < kRows * C; one += kFewThreads) {
+        const int row = one / C, c = one % C;
         if (row >= rows || c >= cols) {
             continue;
         }
@@ -135,8 +142,8 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
         for (int p = 0; p < 2; ++p) {
 #pragma unroll
             for (int w = 0; w < kHalf; ++w) {
-                const int i = C == 16 ? p : 0, col = C == 16 ? c : c + 8 * p;
-                sum[p] += s_part[((w * AB + i) * kRows + row) * kPitch + col];
+                const int at = c + p * C;
+                sum[p] += s_part[((w * AB + at / 16) * kRows + row) * kPitch + at % 16];
             }
             if (a.bias != nullptr) {
                 const uint32_t b = static_cast<const uint16_t*>(a.bias)[static_cast<int64_t>(p) * a.inner + n0 + c];

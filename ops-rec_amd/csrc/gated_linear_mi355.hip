@@ -68,8 +68,19 @@ int launched(const char* what)
     return err == hipSuccess ? HSTU_OK : set_error(HSTU_ERR_RUNTIME, "launch of %s failed: %s", what, hipGetErrorString(err));
 }
 
-// Up to so many rows the kernel that streams the weight takes the call.
-bool few_rows(const gated_linear_params* p) { return p->rows <= kFewRows; }
+// The kernel for few rows: its columns of hidden per workgroup, in eights -- the fullest compute unit's weight rows and rows of x are what it waits for.
+int64_t few_rows_read(const gated_linear_params* p, int wide)
+{
+    return ceil_div(ceil_div(p->inner, 8 * wide), compute_units_or_256()) * (16 * wide + p->rows);
+}
+int few_rows_columns(const gated_linear_params* p)
+{
+    int best = 1;
+    for (int wide = 2; wide <= 4; ++wide) {
+        best = few_rows_read(p, wide) < few_rows_read(p, best) ? wide : best;
+    }
+    return best;
+}
 
 // What a product is estimated to take, in us: rounds of workgroups, one per compute unit each, and with several chunks of the depth the traffic of
 // their fp32 partial outputs and the launch that adds them.
@@ -91,6 +102,17 @@ const GatedTile& forward_tile(const gated_linear_params* p)
         }
     }
     return *best;
+}
+
+// Up to 64 rows the kernel that streams the weight, unless the tiles are estimated faster: a compute unit reads 27 GB/s there (measured at 1 .. 64 rows of
+// 2048 x 5632 and 4096 x 11264; the latter's 33 .. 64 rows took 55 .. 74 us, 56 in tiles), and both take some 5 us besides.
+bool few_rows(const gated_linear_params* p)
+{
+    if (p->rows > kFewRows) {
+        return false;
+    }
+    const double read = static_cast<double>(few_rows_read(p, few_rows_columns(p))) * static_cast<double>(p->cols) * 2.0 / 27e3;
+    return read <= 1.25 * cost_of(forward_tile(p), p->rows, p->inner, p->cols, 1);  // (whose steps were measured with weights in the caches)
 }
 
 int launch_tiles(const GatedTile& t, GatedGemmArgs a, void* stream, const char* what)
@@ -240,9 +262,8 @@ HSTU_API int gated_linear_fwd(const gated_linear_params* p, void* stream)
         a.depth = static_cast<int>(p->cols);
         a.inner = static_cast<int>(p->inner);
         a.activation = p->activation;
-        const int blocks = static_cast<int>(ceil_div(p->rows, 16));  // of 16 rows: at most four
-        const bool sixteen = p->inner >= 16 * static_cast<int64_t>(compute_units_or_256());
-        hipLaunchKernelGGL(k.few_rows[blocks - 1][sixteen ? 1 : 0], dim3(static_cast<uint32_t>(ceil_div(p->inner, sixteen ? 16 : 8))), dim3(512), 0,
+        const int blocks = static_cast<int>(ceil_div(p->rows, 16)), wide = few_rows_columns(p);
+        hipLaunchKernelGGL(k.few_rows[blocks - 1][wide - 1], dim3(static_cast<uint32_t>(ceil_div(p->inner, 8 * wide))), dim3(512), 0,
                            static_cast<hipStream_t>(stream), a);
         return launched("gated_few_rows_kernel");
     }

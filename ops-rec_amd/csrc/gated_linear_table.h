@@ -25,10 +25,10 @@ const GatedKernels& gated_table()
          gated_tile<Tag, kGemmXGrad, 1, 2, 3, 4>("gated_gemm_64x128", 0.25f, 0.17f, 1.5f)},
         {gated_tile<Tag, kGemmWeightGrad, 4, 4, 4, 1>("gated_gemm_256x256", 0.85f, 0.85f, 5.0f), gated_tile<Tag, kGemmWeightGrad, 2, 4, 3, 2>("gated_gemm_128x256", 0.45f, 0.41f, 3.0f),
          gated_tile<Tag, kGemmWeightGrad, 2, 2, 3, 3>("gated_gemm_128x128", 0.30f, 0.23f, 2.0f)},
-        {{gated_few_rows_kernel<Tag, 1, 8>, gated_few_rows_kernel<Tag, 1, 16>},
-         {gated_few_rows_kernel<Tag, 2, 8>, gated_few_rows_kernel<Tag, 2, 16>},
-         {gated_few_rows_kernel<Tag, 3, 8>, gated_few_rows_kernel<Tag, 3, 16>},
-         {gated_few_rows_kernel<Tag, 4, 8>, gated_few_rows_kernel<Tag, 4, 16>}},
+        {{gated_few_rows_kernel<Tag, 1, 1>, gated_few_rows_kernel<Tag, 1, 2>, gated_few_rows_kernel<Tag, 1, 3>, gated_few_rows_kernel<Tag, 1, 4>},
+         {gated_few_rows_kernel<Tag, 2, 1>, gated_few_rows_kernel<Tag, 2, 2>, gated_few_rows_kernel<Tag, 2, 3>, gated_few_rows_kernel<Tag, 2, 4>},
+         {gated_few_rows_kernel<Tag, 3, 1>, gated_few_rows_kernel<Tag, 3, 2>, gated_few_rows_kernel<Tag, 3, 3>, gated_few_rows_kernel<Tag, 3, 4>},
+         {gated_few_rows_kernel<Tag, 4, 1>, gated_few_rows_kernel<Tag, 4, 2>, gated_few_rows_kernel<Tag, 4, 3>, gated_few_rows_kernel<Tag, 4, 4>}},
         gated_stage_kernel<Tag>,
         gated_sum_kernel<Tag>};
     return table;

@@ -72,8 +72,8 @@ struct RotaryArgs {
     int dim, pairs;
     int n_offsets;
     int heads_each;   // heads a thread turns
-    int head_blocks;  // threads that share a row and eight pairs
-    int turned, items;  // pieces of a head: of eight pairs, and with those that are copied
+    int head_blocks;  // threads that share a row and its pairs
+    int turned, items;  // threads of a head: with pairs to turn, and with those that copy
     int positions64, offsets64, start64;
     float magnitude;
     float sign;  // of sin

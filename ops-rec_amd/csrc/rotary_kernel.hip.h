@@ -4,10 +4,11 @@
 //
 // The angle is formed in 64 bits and cut to a fraction of a turn before it goes to 32: at position 10^6 an angle of 32 bits is off by 0.06.
 //
-// Bound by HBM: every value is read and written once.  A thread has 8 pairs of a row (two 16-byte pieces of a head, whichever layout)
-// and turns them in several heads of q and k, so that a sine and a cosine serve them all; short batches give each thread fewer heads, down
-// to one, and pay the sines again for more threads.  Values of a head past its pairs are copied by threads of their own, 8 each.  Pieces start
-// anywhere (16-byte accesses need no alignment here); a part-filled last piece goes value by value.
+// Bound by HBM: every value is read and written once.  A thread has two 16-byte pieces of a head -- the same piece of both halves, or two
+// pieces of pairs that lie side by side, half of the turned values apart, so that neighbouring threads have neighbouring pieces either way -- and turns them in
+// several heads of q and k: a sine and a cosine serve them all.  Short batches give each thread fewer heads, down to one, and pay the sines again for more
+// threads.  Values of a head past its pairs are copied by threads of their own, two pieces each.  Pieces start anywhere (16-byte accesses need no
+// alignment here); a part-filled last piece goes value by value.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -18,6 +19,46 @@ namespace hstu {
 
 constexpr int kRotaryThreads = 256;
 constexpr int kRotaryAtOnce = 4;  // heads whose loads are in flight together
+
+// ---- 16 bytes of a row of n values: those that are there, the others undefined ----
+template <typename Tag>
+struct rotary_piece {
+    typedef uint32_t words_t __attribute__((ext_vector_type(4), aligned(2)));
+    static constexpr int kValues = ln_traits<Tag>::kPerChunk;
+    using elem_t = typename ln_traits<Tag>::elem_t;
+    words_t w;
+
+    __device__ __forceinline__ void load(const elem_t* row, int c, int n)
+    {
+        const int first = c * kValues;
+        if (first + kValues <= n) {
+            w = __builtin_nontemporal_load(reinterpret_cast<const words_t*>(row + first));
+        } else {
+            elem_t e[kValues];
+#pragma unroll
+            for (int i = 0; i < kValues; ++i) {
+                e[i] = first + i < n ? row[first + i] : static_cast<elem_t>(0.0f);
+            }
+            __builtin_memcpy(&w, e, sizeof w);
+        }
+    }
+    __device__ __forceinline__ void unpack(float (&f)[kValues]) const { ln_traits<Tag>::unpack(w, f); }
+    static __device__ __forceinline__ void store(elem_t* row, int c, int n, const float (&f)[kValues])
+    {
+        const int first = c * kValues;
+        if (first + kValues <= n) {
+            const words_t packed = ln_traits<Tag>::pack(f);
+            __builtin_nontemporal_store(packed, reinterpret_cast<words_t*>(row + first));
+        } else {
+#pragma unroll
+            for (int i = 0; i < kValues; ++i) {
+                if (first + i < n) {
+                    row[first + i] = static_cast<elem_t>(f[i]);
+                }
+            }
+        }
+    }
+};
 
 __device__ __forceinline__ int64_t rotary_index(const void* p, int64_t i, int idx64)
 {
@@ -97,76 +138,81 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
                              : static_cast<E*>(a.k_out) + (static_cast<int64_t>(row) * (a.heads - a.heads_q) + (h - a.heads_q)) * a.dim;
     };
 
+    constexpr int kValues = rotary_piece<T>::kValues;
     if (item >= a.turned) {  // values that are not turned
-        const int c = item - a.turned, begin = 2 * a.pairs, n = a.dim - begin;
+        const int begin = 2 * a.pairs, n = a.dim - begin;
+        const int c0 = item - a.turned, c1 = c0 + a.items - a.turned;
         for (int h0 = first; h0 < last; h0 += kRotaryAtOnce) {
-            norm_piece<T> p[kRotaryAtOnce];
+            rotary_piece<T> p[kRotaryAtOnce][2];
 #pragma unroll
             for (int i = 0; i < kRotaryAtOnce; ++i) {
                 if (h0 + i < last) {
-                    p[i] = norm_load<T>(from(h0 + i) + begin, c, n);
+                    p[i][0].load(from(h0 + i) + begin, c0, n);
+                    p[i][1].load(from(h0 + i) + begin, c1, n);
                 }
             }
 #pragma unroll
             for (int i = 0; i < kRotaryAtOnce; ++i) {
                 if (h0 + i < last) {
-                    float f[8];
-                    norm_unpack<T>(p[i], f);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        f[j] = inside ? f[j] : 0.0f;
+                    for (int part = 0; part < 2; ++part) {
+                        float f[kValues];
+                        p[i][part].unpack(f);
+#pragma unroll
+                        for (int j = 0; j < kValues; ++j) {
+                            f[j] = inside ? f[j] : 0.0f;
+                        }
+                        rotary_piece<T>::store(to(h0 + i) + begin, part == 0 ? c0 : c1, n, f);
                     }
-                    norm_store<T>(to(h0 + i) + begin, c, n, f);
                 }
             }
         }
         return;
     }
 
-    float cs[8], sn[8];
+    // side by side: pieces `item` and `item + turned` of all the turned values; halves: piece `item` of each
+    const int n = INTERLEAVED ? 2 * a.pairs : a.pairs;
+    const int c0 = item, c1 = INTERLEAVED ? item + a.turned : item;
+    const int half = INTERLEAVED ? 0 : a.pairs;
+    float cs[kValues], sn[kValues];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int pair = min(8 * item + j, a.pairs - 1);
-        double turns = position * a.frequencies[pair] * 0.15915494309189533577;  // 1 / (2 pi)
+    for (int j = 0; j < kValues; ++j) {
+        const int at = INTERLEAVED ? (j < kValues / 2 ? c0 : c1) * (kValues / 2) + j % (kValues / 2) : c0 * kValues + j;
+        double turns = position * a.frequencies[min(at, a.pairs - 1)] * 0.15915494309189533577;  // 1 / (2 pi)
         turns -= rint(turns);
         rotary_turn<T>(static_cast<float>(turns), cs[j], sn[j]);
-        cs[j] = inside ? cs[j] * a.magnitude : 0.0f;
-        sn[j] = inside ? sn[j] * a.magnitude * a.sign : 0.0f;
+        cs[j] *= a.magnitude;
+        sn[j] *= a.magnitude * a.sign;
     }
-    // side by side: 16 values from 16 item on, as two pieces; halves: piece `item` of each
-    constexpr int kSecond = INTERLEAVED ? 1 : 0;
-    const int n = INTERLEAVED ? 2 * a.pairs : a.pairs;
-    const int c0 = INTERLEAVED ? 2 * item : item, c1 = c0 + kSecond;
-    const int half = INTERLEAVED ? 0 : a.pairs;
-    const bool two = 8 * c1 < n;
     for (int h0 = first; h0 < last; h0 += kRotaryAtOnce) {
-        norm_piece<T> lo[kRotaryAtOnce], hi[kRotaryAtOnce];
+        rotary_piece<T> lo[kRotaryAtOnce], hi[kRotaryAtOnce];
 #pragma unroll
         for (int i = 0; i < kRotaryAtOnce; ++i) {
             if (h0 + i < last) {
                 const E* const p = from(h0 + i);
-                lo[i] = norm_load<T>(p, c0, n);
-                hi[i] = norm_load<T>(p + half, c1, n);
+                lo[i].load(p, c0, n);
+                hi[i].load(p + half, c1, n);
             }
         }
 #pragma unroll
         for (int i = 0; i < kRotaryAtOnce; ++i) {
             if (h0 + i < last) {
-                float u[8], v[8];
-                norm_unpack<T>(lo[i], u);
-                norm_unpack<T>(hi[i], v);
+                float u[kValues], v[kValues];
+                lo[i].unpack(u);
+                hi[i].unpack(v);
                 if constexpr (INTERLEAVED) {
+                    constexpr int kPairs = kValues / 2;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < kPairs; ++j) {
                         const float a0 = u[2 * j], b0 = u[2 * j + 1], a1 = v[2 * j], b1 = v[2 * j + 1];
                         u[2 * j] = a0 * cs[j] - b0 * sn[j];
                         u[2 * j + 1] = b0 * cs[j] + a0 * sn[j];
-                        v[2 * j] = a1 * cs[4 + j] - b1 * sn[4 + j];
-                        v[2 * j + 1] = b1 * cs[4 + j] + a1 * sn[4 + j];
+                        v[2 * j] = a1 * cs[kPairs + j] - b1 * sn[kPairs + j];
+                        v[2 * j + 1] = b1 * cs[kPairs + j] + a1 * sn[kPairs + j];
                     }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
+                    for (int j = 0; j < kValues; ++j) {
                         const float a0 = u[j], b0 = v[j];
                         u[j] = a0 * cs[j] - b0 * sn[j];
                         v[j] = b0 * cs[j] + a0 * sn[j];
@@ -174,16 +220,14 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
                 }
                 if (!inside) {  // (zeros, whatever the values: a product with 0 would keep NaN)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
+                    for (int j = 0; j < kValues; ++j) {
                         u[j] = 0.0f;
                         v[j] = 0.0f;
                     }
                 }
                 E* const p = to(h0 + i);
-                norm_store<T>(p, c0, n, u);
-                if (two) {
-                    norm_store<T>(p + half, c1, n, v);
-                }
+                rotary_piece<T>::store(p, c0, n, u);
+                rotary_piece<T>::store(p + half, c1, n, v);
             }
         }
     }

@@ -92,18 +92,21 @@ extern "C" HSTU_API int rotary_fwd(const rotary_params* p, void* stream)
     a.dim = static_cast<int>(p->dim);
     a.pairs = static_cast<int>(p->pairs);
     a.n_offsets = static_cast<int>(p->n_offsets);
-    a.turned = (a.pairs + 7) / 8;
-    a.items = a.turned + (a.dim - 2 * a.pairs + 7) / 8;
+    // threads of a head: two 16-byte pieces each.  Halves have their own last pieces; pairs that lie side by side fill theirs together
+    const int values = static_cast<int>(16 / size);
+    a.turned = p->interleaved ? ((2 * a.pairs + values - 1) / values + 1) / 2 : (a.pairs + values - 1) / values;
+    a.items = a.turned + ((a.dim - 2 * a.pairs + values - 1) / values + 1) / 2;
     a.positions64 = p->positions_dtype == HSTU_IDX_I64;
     a.offsets64 = p->seq_offset_dtype == HSTU_IDX_I64;
     a.start64 = p->start_dtype == HSTU_IDX_I64;
     a.magnitude = static_cast<float>(p->magnitude);
     a.sign = p->inverse ? -1.0f : 1.0f;
-    // heads per thread: up to 8, fewer while the threads would not give every SIMD two wavefronts
-    a.heads_each = heads < 8 ? heads : 8;
-    while (a.heads_each > 1 && p->rows * a.items * ((heads + a.heads_each - 1) / a.heads_each) < static_cast<int64_t>(cus) * 512) {
-        a.heads_each = (a.heads_each + 1) / 2;
+    // Threads that share a row's pairs, each with as many heads as the others: one while the threads give every SIMD four wavefronts, more until they do
+    a.head_blocks = 1;
+    while (a.head_blocks < heads && p->rows * a.items * a.head_blocks < static_cast<int64_t>(cus) * 1024) {
+        ++a.head_blocks;
     }
+    a.heads_each = (heads + a.head_blocks - 1) / a.head_blocks;
     a.head_blocks = (heads + a.heads_each - 1) / a.heads_each;
     const kernel_t kernel = kernel_for(p->dtype, p->interleaved != 0);
     // (a launch numbers its threads in 32 bits)
