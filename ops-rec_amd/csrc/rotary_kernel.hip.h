@@ -18,7 +18,7 @@
 namespace hstu {
 
 constexpr int kRotaryThreads = 256;
-constexpr int kRotaryAtOnce = 4;  // heads whose loads are in flight together
+constexpr int kRotaryHeads = 8;  // heads of a thread, at most: their loads are all in flight while the row's place and its sines are worked out
 
 // ---- 16 bytes of a row of n values: those that are there, the others undefined ----
 template <typename Tag>
@@ -113,6 +113,33 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
     const int first = static_cast<int>(rest - row * static_cast<uint32_t>(a.head_blocks)) * a.heads_each;
     const int last = min(first + a.heads_each, a.heads);
 
+    const auto from = [&](int h) -> const E* {
+        return h < a.heads_q ? static_cast<const E*>(a.q) + row * a.q_stride_row + h * a.q_stride_head
+                             : static_cast<const E*>(a.k) + row * a.k_stride_row + (h - a.heads_q) * a.k_stride_head;
+    };
+    const auto to = [&](int h) -> E* {
+        return h < a.heads_q ? static_cast<E*>(a.q_out) + (static_cast<int64_t>(row) * a.heads_q + h) * a.dim
+                             : static_cast<E*>(a.k_out) + (static_cast<int64_t>(row) * (a.heads - a.heads_q) + (h - a.heads_q)) * a.dim;
+    };
+
+    constexpr int kValues = rotary_piece<T>::kValues;
+    // turned values: side by side pieces `item` and `item + turned` of all of them, halves piece `item` of each; copied values: two pieces of the rest
+    const bool copied = item >= a.turned;
+    const int rest0 = item - a.turned;
+    const int begin = copied ? 2 * a.pairs : 0, n = copied ? a.dim - begin : INTERLEAVED ? 2 * a.pairs : a.pairs;
+    const int c0 = copied ? rest0 : item, c1 = copied ? rest0 + a.items - a.turned : INTERLEAVED ? item + a.turned : item;
+    const int apart = copied || INTERLEAVED ? 0 : a.pairs;
+    rotary_piece<T> lo[kRotaryHeads], hi[kRotaryHeads];
+#pragma unroll
+    for (int i = 0; i < kRotaryHeads; ++i) {
+        if (first + i < last) {
+            const E* const p = from(first + i) + begin;
+            lo[i].load(p, c0, n);
+            hi[i].load(p + apart, c1, n);
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
     bool inside = true;
     double position = 0.0;
     if (a.positions != nullptr) {
@@ -129,77 +156,25 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
             position = static_cast<double>(p);
         }
     }
-    const auto from = [&](int h) -> const E* {
-        return h < a.heads_q ? static_cast<const E*>(a.q) + row * a.q_stride_row + h * a.q_stride_head
-                             : static_cast<const E*>(a.k) + row * a.k_stride_row + (h - a.heads_q) * a.k_stride_head;
-    };
-    const auto to = [&](int h) -> E* {
-        return h < a.heads_q ? static_cast<E*>(a.q_out) + (static_cast<int64_t>(row) * a.heads_q + h) * a.dim
-                             : static_cast<E*>(a.k_out) + (static_cast<int64_t>(row) * (a.heads - a.heads_q) + (h - a.heads_q)) * a.dim;
-    };
-
-    constexpr int kValues = rotary_piece<T>::kValues;
-    if (item >= a.turned) {  // values that are not turned
-        const int begin = 2 * a.pairs, n = a.dim - begin;
-        const int c0 = item - a.turned, c1 = c0 + a.items - a.turned;
-        for (int h0 = first; h0 < last; h0 += kRotaryAtOnce) {
-            rotary_piece<T> p[kRotaryAtOnce][2];
-#pragma unroll
-            for (int i = 0; i < kRotaryAtOnce; ++i) {
-                if (h0 + i < last) {
-                    p[i][0].load(from(h0 + i) + begin, c0, n);
-                    p[i][1].load(from(h0 + i) + begin, c1, n);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < kRotaryAtOnce; ++i) {
-                if (h0 + i < last) {
-#pragma unroll
-                    for (int part = 0; part < 2; ++part) {
-                        float f[kValues];
-                        p[i][part].unpack(f);
-#pragma unroll
-                        for (int j = 0; j < kValues; ++j) {
-                            f[j] = inside ? f[j] : 0.0f;
-                        }
-                        rotary_piece<T>::store(to(h0 + i) + begin, part == 0 ? c0 : c1, n, f);
-                    }
-                }
-            }
-        }
-        return;
-    }
-
-    // side by side: pieces `item` and `item + turned` of all the turned values; halves: piece `item` of each
-    const int n = INTERLEAVED ? 2 * a.pairs : a.pairs;
-    const int c0 = item, c1 = INTERLEAVED ? item + a.turned : item;
-    const int half = INTERLEAVED ? 0 : a.pairs;
     float cs[kValues], sn[kValues];
+    if (!copied) {
 #pragma unroll
-    for (int j = 0; j < kValues; ++j) {
-        const int at = INTERLEAVED ? (j < kValues / 2 ? c0 : c1) * (kValues / 2) + j % (kValues / 2) : c0 * kValues + j;
-        double turns = position * a.frequencies[min(at, a.pairs - 1)] * 0.15915494309189533577;  // 1 / (2 pi)
-        turns -= rint(turns);
-        rotary_turn<T>(static_cast<float>(turns), cs[j], sn[j]);
-        cs[j] *= a.magnitude;
-        sn[j] *= a.magnitude * a.sign;
-    }
-    for (int h0 = first; h0 < last; h0 += kRotaryAtOnce) {
-        rotary_piece<T> lo[kRotaryAtOnce], hi[kRotaryAtOnce];
-#pragma unroll
-        for (int i = 0; i < kRotaryAtOnce; ++i) {
-            if (h0 + i < last) {
-                const E* const p = from(h0 + i);
-                lo[i].load(p, c0, n);
-                hi[i].load(p + half, c1, n);
-            }
+        for (int j = 0; j < kValues; ++j) {
+            const int at = INTERLEAVED ? (j < kValues / 2 ? c0 : c1) * (kValues / 2) + j % (kValues / 2) : c0 * kValues + j;
+            double turns = position * a.frequencies[min(at, a.pairs - 1)] * 0.15915494309189533577;  // 1 / (2 pi)
+            turns -= rint(turns);
+            rotary_turn<T>(static_cast<float>(turns), cs[j], sn[j]);
+            cs[j] *= a.magnitude;
+            sn[j] *= a.magnitude * a.sign;
         }
+    }
 #pragma unroll
-        for (int i = 0; i < kRotaryAtOnce; ++i) {
-            if (h0 + i < last) {
-                float u[kValues], v[kValues];
-                lo[i].unpack(u);
-                hi[i].unpack(v);
+    for (int i = 0; i < kRotaryHeads; ++i) {
+        if (first + i < last) {
+            float u[kValues], v[kValues];
+            lo[i].unpack(u);
+            hi[i].unpack(v);
+            if (!copied) {
                 if constexpr (INTERLEAVED) {
                     constexpr int kPairs = kValues / 2;
 #pragma unroll
@@ -218,17 +193,17 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
                         v[j] = b0 * cs[j] + a0 * sn[j];
                     }
                 }
-                if (!inside) {  // (zeros, whatever the values: a product with 0 would keep NaN)
-#pragma unroll
-                    for (int j = 0; j < kValues; ++j) {
-                        u[j] = 0.0f;
-                        v[j] = 0.0f;
-                    }
-                }
-                E* const p = to(h0 + i);
-                rotary_piece<T>::store(p, c0, n, u);
-                rotary_piece<T>::store(p + half, c1, n, v);
             }
+            if (!inside) {  // (zeros, whatever the values: a product with 0 would keep NaN)
+#pragma unroll
+                for (int j = 0; j < kValues; ++j) {
+                    u[j] = 0.0f;
+                    v[j] = 0.0f;
+                }
+            }
+            E* const p = to(first + i) + begin;
+            rotary_piece<T>::store(p, c0, n, u);
+            rotary_piece<T>::store(p + apart, c1, n, v);
         }
     }
 }

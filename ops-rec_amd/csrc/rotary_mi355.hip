@@ -101,9 +101,10 @@ extern "C" HSTU_API int rotary_fwd(const rotary_params* p, void* stream)
     a.start64 = p->start_dtype == HSTU_IDX_I64;
     a.magnitude = static_cast<float>(p->magnitude);
     a.sign = p->inverse ? -1.0f : 1.0f;
-    // Threads that share a row's pairs, each with as many heads as the others: one while the threads give every SIMD four wavefronts, more until they do
-    a.head_blocks = 1;
-    while (a.head_blocks < heads && p->rows * a.items * a.head_blocks < static_cast<int64_t>(cus) * 1024) {
+    // Threads that share a row's pairs, each with as many heads as the others, at most 8; more of them until they give every SIMD two wavefronts (with four, 20292
+    // rows of 4 + 4 heads of 128 took 22 us, 18 with two: the sines are paid for again)
+    a.head_blocks = (heads + hstu::kRotaryHeads - 1) / hstu::kRotaryHeads;
+    while (a.head_blocks < heads && p->rows * a.items * a.head_blocks < static_cast<int64_t>(cus) * 512) {
         ++a.head_blocks;
     }
     a.heads_each = (heads + a.head_blocks - 1) / a.head_blocks;
