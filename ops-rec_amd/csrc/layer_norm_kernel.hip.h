@@ -193,6 +193,23 @@ __device__ __forceinline__ float norm_sigmoid(float z)
     }
 }
 
+// values of pieces past the row's end -> 0 (rows that fill the lanes have none)
+template <int G, int NV>
+__device__ __forceinline__ void drop_outside(float (&f)[NV][8], int lane, int len)
+{
+    if (len == 8 * G * NV) {
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int left = len - 8 * (lane + i * G);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            f[i][j] = j < left ? f[i][j] : 0.0f;
+        }
+    }
+}
+
 // s (a lane's NV pieces, 0 outside the row) -> norm(s) in place; returns rstd.  Two passes over registers; the mean's own rounding is
 // taken out by the sum of the centred values, which is 0 for an exact mean.
 template <int G, int NV>
@@ -215,10 +232,16 @@ __device__ __forceinline__ float normalise(float (&s)[NV][8], int lane, int len,
     float sq[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int left = len - 8 * (lane + i * G);  // columns of the row from this piece on
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            s[i][j] = j < left ? s[i][j] - mean : 0.0f;
+            s[i][j] -= mean;
+        }
+    }
+    drop_outside<G, NV>(s, lane, len);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
             sq[0] = __builtin_fmaf(s[i][j], s[i][j], sq[0]);
             sq[1] += s[i][j];
         }
@@ -226,140 +249,153 @@ __device__ __forceinline__ float normalise(float (&s)[NV][8], int lane, int len,
     row_sums<G>(sq, s_part, slot);
     const float shift = rms ? 0.0f : sq[1] * inv_n;
     const float rstd = 1.0f / sqrtf(fmaxf(sq[0] * inv_n - shift * shift, 0.0f) + epsilon);
+    const float away = -shift * rstd;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            s[i][j] = (s[i][j] - shift) * rstd;
+            s[i][j] = __builtin_fmaf(s[i][j], rstd, away);
         }
     }
     return rstd;
 }
 
-// values of pieces past the row's end -> 0
-template <int NV>
-__device__ __forceinline__ void drop_outside(float (&f)[NV][8], int lane, int g, int len)
-{
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int left = len - 8 * (lane + i * g);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            f[i][j] = j < left ? f[i][j] : 0.0f;
-        }
-    }
-}
-
-// T = type of x (and of y, gate), R = type of the stream
-template <typename T, typename R, int MODE, int G, int NV>
+// T = type of x (and of y, gate), R = type of the stream; U = parts of rows whose loads are in flight together.  Lanes stay with their columns: from part to
+// part they move on by the lanes of the whole grid, a multiple of the parts of a row, and hold gamma, beta and scale in registers.  (Loaded for every row
+// again they were half of the kernel's requests: 65536 x 1024 with a gate 99 us, 76 so.)
+template <typename T, typename R, int MODE, int G, int NV, int U>
 __global__ __launch_bounds__(norm_fwd_threads(G)) void norm_fwd_kernel(const NormArgs a)
 {
+    static_assert(G <= 64 || U == 1, "lanes that share barriers have one row");
     using TE = typename ln_traits<T>::elem_t;
     using RE = typename ln_traits<R>::elem_t;
+    constexpr uint32_t kPerWg = norm_fwd_threads(G) / G;
     __shared__ float s_part[G > 64 ? kNormSlots * 2 * 16 : 1];
-    const uint32_t unit = (blockIdx.x * static_cast<uint32_t>(norm_fwd_threads(G)) + threadIdx.x) / G;
     const int lane = threadIdx.x % G;
-    if (unit >= a.units) {  // (G > 64: a workgroup per unit, so that lanes that share barriers leave together)
-        return;
-    }
-    const uint32_t row = a.groups == 1 ? unit : unit / static_cast<uint32_t>(a.groups);
     const int len = a.len;
-    const int64_t col0 = a.groups == 1 ? 0 : static_cast<int64_t>(unit - row * static_cast<uint32_t>(a.groups)) * len;
-    const int64_t dense = static_cast<int64_t>(row) * len * a.groups + col0;
-    const TE* const x = static_cast<const TE*>(a.x) + static_cast<int64_t>(row) * a.x_stride + col0;
-    const RE* const res = static_cast<const RE*>(a.residual) + static_cast<int64_t>(row) * a.residual_stride + col0;
-    const TE* const gate = static_cast<const TE*>(a.gate) + static_cast<int64_t>(row) * a.gate_stride + col0;
     const bool f32 = a.affine_f32 != 0;
+    const uint32_t first = blockIdx.x * kPerWg + threadIdx.x / G, step = gridDim.x * kPerWg;
+    const uint32_t groups = static_cast<uint32_t>(a.groups);
+    const int64_t col0 = groups == 1 ? 0 : static_cast<int64_t>(first % groups) * len;
     int slot = 0;
 
-    norm_piece<T> xp[NV], gp[NV];
-    norm_piece<R> rp[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        xp[i] = norm_load<T>(x, lane + i * G, len);
-    }
-    if (MODE == kNormFront || a.residual != nullptr) {
+    float gamma[NV][8], beta[NV][8], scale[NV][8];
+    const auto hold = [&] {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            rp[i] = norm_load<R>(res, lane + i * G, len);
-        }
-    }
-    if (MODE == kNormBehind && a.gate != nullptr) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            gp[i] = norm_load<T>(gate, lane + i * G, len);
-        }
-    }
-    float s[NV][8];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        norm_unpack<T>(xp[i], s[i]);
-    }
-    if constexpr (MODE == kNormFront) {
-        if (a.scale != nullptr) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                float c[8], f[8];
-                norm_columns<T>(a.scale, f32, col0, lane + i * G, len, c);
-                norm_unpack<R>(rp[i], f);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    s[i][j] = __builtin_fmaf(c[j], s[i][j], f[j]);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                float f[8];
-                norm_unpack<R>(rp[i], f);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    s[i][j] += f[j];
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            norm_store<R>(static_cast<RE*>(a.sum) + dense, lane + i * G, len, s[i]);
-        }
-    }
-    drop_outside<NV>(s, lane, G, len);
-    normalise<G, NV>(s, lane, len, a.rms != 0, a.epsilon, s_part, slot);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        float c[8], y[8];
-        norm_columns<T>(a.gamma, f32, col0, lane + i * G, len, c);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            y[j] = s[i][j] * c[j];
-        }
-        if (a.beta != nullptr) {
-            norm_columns<T>(a.beta, f32, col0, lane + i * G, len, c);
+            const int c = lane + i * G;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                y[j] += c[j];
+                beta[i][j] = 0.0f;
+                scale[i][j] = 1.0f;
+            }
+            norm_columns<T>(a.gamma, f32, col0, c, len, gamma[i]);
+            if (a.beta != nullptr) {
+                norm_columns<T>(a.beta, f32, col0, c, len, beta[i]);
+            }
+            if (MODE == kNormFront && a.scale != nullptr) {
+                norm_columns<T>(a.scale, f32, col0, c, len, scale[i]);
             }
         }
-        if constexpr (MODE == kNormBehind) {
-            if (a.gate != nullptr) {
-                float u[8];
-                norm_unpack<T>(gp[i], u);
+    };
+
+    bool held = false;
+    for (uint64_t unit0 = first; unit0 < a.units; unit0 += static_cast<uint64_t>(step) * U) {  // (G > 64: all of a workgroup's lanes go round as often)
+        norm_piece<T> xp[U][NV], gp[U][NV];
+        norm_piece<R> rp[U][NV];
+        int64_t dense[U];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    y[j] *= a.silu ? u[j] * norm_sigmoid<T>(u[j]) : u[j];
+        for (int t = 0; t < U; ++t) {
+            const uint64_t unit = unit0 + static_cast<uint64_t>(t) * step;
+            dense[t] = -1;
+            if (unit < a.units) {
+                const uint32_t row = groups == 1 ? static_cast<uint32_t>(unit) : static_cast<uint32_t>(unit) / groups;
+                dense[t] = static_cast<int64_t>(row) * len * a.groups + col0;
+                const TE* const x = static_cast<const TE*>(a.x) + static_cast<int64_t>(row) * a.x_stride + col0;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    xp[t][i] = norm_load<T>(x, lane + i * G, len);
+                }
+                if (MODE == kNormFront || a.residual != nullptr) {
+                    const RE* const res = static_cast<const RE*>(a.residual) + static_cast<int64_t>(row) * a.residual_stride + col0;
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) {
+                        rp[t][i] = norm_load<R>(res, lane + i * G, len);
+                    }
+                }
+                if (MODE == kNormBehind && a.gate != nullptr) {
+                    const TE* const gate = static_cast<const TE*>(a.gate) + static_cast<int64_t>(row) * a.gate_stride + col0;
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) {
+                        gp[t][i] = norm_load<T>(gate, lane + i * G, len);
+                    }
                 }
             }
-            if (a.residual != nullptr) {
-                float f[8];
-                norm_unpack<R>(rp[i], f);
+        }
+        if (!held) {  // (behind the first rows' loads)
+            held = true;
+            hold();
+        }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    y[j] = __builtin_fmaf(a.residual_scale, y[j], f[j]);
+        for (int t = 0; t < U; ++t) {
+            if (dense[t] < 0) {
+                continue;
+            }
+            float s[NV][8];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                norm_unpack<T>(xp[t][i], s[i]);
+            }
+            if constexpr (MODE == kNormFront) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    float f[8];
+                    norm_unpack<R>(rp[t][i], f);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        s[i][j] = __builtin_fmaf(scale[i][j], s[i][j], f[j]);
+                    }
+                    norm_store<R>(static_cast<RE*>(a.sum) + dense[t], lane + i * G, len, s[i]);
                 }
             }
-            norm_store<R>(static_cast<RE*>(a.out) + dense, lane + i * G, len, y);
-        } else {
-            norm_store<T>(static_cast<TE*>(a.out) + dense, lane + i * G, len, y);
+            drop_outside<G, NV>(s, lane, len);
+            normalise<G, NV>(s, lane, len, a.rms != 0, a.epsilon, s_part, slot);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    y[j] = __builtin_fmaf(s[i][j], gamma[i][j], beta[i][j]);
+                }
+                if constexpr (MODE == kNormBehind) {
+                    if (a.gate != nullptr) {
+                        float u[8];
+                        norm_unpack<T>(gp[t][i], u);
+                        if (a.silu) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                y[j] *= u[j] * norm_sigmoid<T>(u[j]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                y[j] *= u[j];
+                            }
+                        }
+                    }
+                    if (a.residual != nullptr) {
+                        float f[8];
+                        norm_unpack<R>(rp[t][i], f);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            y[j] = __builtin_fmaf(a.residual_scale, y[j], f[j]);
+                        }
+                    }
+                    norm_store<R>(static_cast<RE*>(a.out) + dense[t], lane + i * G, len, y);
+                } else {
+                    norm_store<T>(static_cast<TE*>(a.out) + dense[t], lane + i * G, len, y);
+                }
+            }
         }
     }
 }
@@ -405,21 +441,20 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
         }
     }
 
-    drop_outside<NV>(gamma, lane, G, len);  // (what lies past the row's end must not reach its sums, NaN least of all)
+    drop_outside<G, NV>(gamma, lane, len);  // (what lies past the row's end must not reach its sums, NaN least of all)
 
-    for (uint32_t row0 = slice * kRows; row0 < rows; row0 += static_cast<uint32_t>(a.slices) * kRows) {
-        const uint32_t row = row0 + sub;
-        if (kRows > 1 && row >= rows) {  // (the lanes of a row leave together; no barrier in this loop for G <= 64)
-            break;
-        }
+    // a row's values as they lie in memory; those of the next row are on their way while one is worked on
+    struct Row {
+        norm_piece<T> x[NV], y[NV], gate[NV];
+        norm_piece<R> s[NV], d[NV];
+    };
+    const auto load = [&](uint32_t row, Row& w) {
         const int64_t dense = static_cast<int64_t>(row) * cols + col0;
-        const TE* const x = static_cast<const TE*>(f.x) + static_cast<int64_t>(row) * f.x_stride + col0;
-        norm_piece<T> xp[NV], yp[NV], gp[NV];
-        norm_piece<R> sp[NV], dp[NV];
         if (need_x) {
+            const TE* const x = static_cast<const TE*>(f.x) + static_cast<int64_t>(row) * f.x_stride + col0;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                xp[i] = norm_load<T>(x, lane + i * G, len);
+                w.x[i] = norm_load<T>(x, lane + i * G, len);
             }
         }
         if constexpr (MODE == kNormFront) {
@@ -427,51 +462,66 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
                                             : static_cast<const RE*>(f.residual) + static_cast<int64_t>(row) * f.residual_stride + col0;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                sp[i] = norm_load<R>(from, lane + i * G, len);
+                w.s[i] = norm_load<R>(from, lane + i * G, len);
             }
             if (a.sum_grad != nullptr) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    dp[i] = norm_load<R>(static_cast<const RE*>(a.sum_grad) + dense, lane + i * G, len);
+                    w.d[i] = norm_load<R>(static_cast<const RE*>(a.sum_grad) + dense, lane + i * G, len);
                 }
             }
             if (a.grad != nullptr) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    yp[i] = norm_load<T>(static_cast<const TE*>(a.grad) + dense, lane + i * G, len);
+                    w.y[i] = norm_load<T>(static_cast<const TE*>(a.grad) + dense, lane + i * G, len);
                 }
             }
         } else {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                dp[i] = norm_load<R>(static_cast<const RE*>(a.grad) + dense, lane + i * G, len);
+                w.d[i] = norm_load<R>(static_cast<const RE*>(a.grad) + dense, lane + i * G, len);
             }
             if (f.gate != nullptr) {
                 const TE* const gate = static_cast<const TE*>(f.gate) + static_cast<int64_t>(row) * f.gate_stride + col0;
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    gp[i] = norm_load<T>(gate, lane + i * G, len);
+                    w.gate[i] = norm_load<T>(gate, lane + i * G, len);
                 }
             }
+        }
+    };
+    Row next;
+    if (slice * kRows + sub < rows) {
+        load(slice * kRows + sub, next);
+    }
+    for (uint64_t row0 = static_cast<uint64_t>(slice) * kRows; row0 < rows; row0 += static_cast<uint64_t>(a.slices) * kRows) {
+        const uint64_t row = row0 + sub, after = row + static_cast<uint64_t>(a.slices) * kRows;
+        if (kRows > 1 && row >= rows) {  // (the lanes of a row leave together; no barrier in this loop for G <= 64)
+            break;
+        }
+        const int64_t dense = static_cast<int64_t>(row) * cols + col0;
+        const Row now = next;
+        if (after < rows) {
+            load(static_cast<uint32_t>(after), next);
         }
         float n[NV][8];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if constexpr (MODE == kNormFront) {
-                norm_unpack<R>(sp[i], n[i]);
+                norm_unpack<R>(now.s[i], n[i]);
                 if constexpr (!kFromSum) {
                     float v[8];
-                    norm_unpack<T>(xp[i], v);
+                    norm_unpack<T>(now.x[i], v);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         n[i][j] = __builtin_fmaf(scale[i][j], v[j], n[i][j]);
                     }
                 }
             } else {
-                norm_unpack<T>(xp[i], n[i]);
+                norm_unpack<T>(now.x[i], n[i]);
             }
         }
-        drop_outside<NV>(n, lane, G, len);
+        drop_outside<G, NV>(n, lane, len);
         const float rstd = normalise<G, NV>(n, lane, len, f.rms != 0, f.epsilon, s_part, slot);
 
         // g = (gradient of m or y) * gamma; the gradient itself goes into the sums
@@ -482,10 +532,10 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
             const int left = len - 8 * (lane + i * G);
             float d[8];
             if constexpr (kGradR) {
-                norm_unpack<R>(dp[i], d);
+                norm_unpack<R>(now.d[i], d);
                 float u[8], dg[8];
                 if (f.gate != nullptr) {
-                    norm_unpack<T>(gp[i], u);
+                    norm_unpack<T>(now.gate[i], u);
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -511,12 +561,17 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
                     d[j] = 0.0f;
                 }
                 if (a.grad != nullptr) {
-                    norm_unpack<T>(yp[i], d);
+                    norm_unpack<T>(now.y[i], d);
+                }
+            }
+            if (len != 8 * G * NV) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    d[j] = j < left ? d[j] : 0.0f;
                 }
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                d[j] = j < left ? d[j] : 0.0f;
                 d_gamma[i][j] = __builtin_fmaf(d[j], n[i][j], d_gamma[i][j]);
                 d_beta[i][j] += d[j];
                 g[i][j] = d[j] * gamma[i][j];
@@ -537,7 +592,7 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
             if constexpr (MODE == kNormFront) {
                 if (a.sum_grad != nullptr) {
                     float v[8];
-                    norm_unpack<R>(dp[i], v);
+                    norm_unpack<R>(now.d[i], v);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         d[j] += v[j];
@@ -547,7 +602,7 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
                 if (a.want_scale) {
                     const int left = len - 8 * (lane + i * G);
                     float v[8];
-                    norm_unpack<T>(xp[i], v);
+                    norm_unpack<T>(now.x[i], v);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         d_scale[i][j] += j < left ? d[j] * v[j] : 0.0f;

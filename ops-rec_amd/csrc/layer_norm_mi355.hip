@@ -181,9 +181,15 @@ int describe(const norm_gate_params* p, NormArgs* a)
 int launch_fwd(const NormArgs& a, int dtype, int stream_dtype, int mode, void* stream, const char* what)
 {
     const NormVariant* v = variant_for(dtype, stream_dtype, a.len);
-    const uint32_t per_wg = static_cast<uint32_t>(v->fwd_threads / v->fwd_lanes);
-    const uint32_t grid = a.units / per_wg + (a.units % per_wg != 0 ? 1u : 0u);
-    hipLaunchKernelGGL(v->fwd[mode], dim3(grid), dim3(v->fwd_threads), 0, static_cast<hipStream_t>(stream), a);
+    int cus = 0;
+    if (const int rc = hstu::compute_units(&cus); rc != HSTU_OK) {
+        return rc;
+    }
+    // workgroups for eight wavefronts per SIMD at most, as many as have equal shares, and a multiple of the parts of a row (lanes keep their columns)
+    const int64_t per_wg = v->fwd_threads / v->lanes, wanted = (static_cast<int64_t>(a.units) + per_wg - 1) / per_wg;
+    const int64_t places = static_cast<int64_t>(cus) * (2048 / v->fwd_threads), rounds = (wanted + places - 1) / places;
+    const int64_t even = (wanted + rounds - 1) / rounds, grid = (even + a.groups - 1) / a.groups * a.groups;
+    hipLaunchKernelGGL(v->fwd[mode], dim3(static_cast<uint32_t>(grid)), dim3(v->fwd_threads), 0, static_cast<hipStream_t>(stream), a);
     return finish(hipGetLastError(), what);
 }
 
@@ -195,7 +201,7 @@ int slices_of(const NormArgs& a, const NormVariant* v)
     if (hstu::compute_units(&cus) != HSTU_OK) {
         cus = 256;
     }
-    const int64_t per_wg = v->bwd_threads / v->bwd_lanes, rows = a.units / static_cast<uint32_t>(a.groups);
+    const int64_t per_wg = v->bwd_threads / v->lanes, rows = a.units / static_cast<uint32_t>(a.groups);
     const int64_t useful = (rows + per_wg - 1) / per_wg, places = static_cast<int64_t>(cus) * (1024 / v->bwd_threads) / a.groups;
     const int64_t most = places > 1 ? places : 1;
     return static_cast<int>(useful < most ? useful : most);

@@ -5,28 +5,28 @@
 
 namespace hstu {
 
-// The forward and the backward kernel of a capacity: the backward holds three sums per column beside the row and takes more lanes
-// with fewer pieces each (4 pieces a lane would put 60 to 400 registers into scratch memory).
-template <typename T, typename R, int G, int NV, int BG, int BNV>
+// parts of rows whose loads are in flight together: two where a lane has one piece of each
+constexpr int norm_units(int g, int nv) { return g <= 64 && nv == 1 ? 2 : 1; }
+
+// G lanes with NV pieces of 8 columns each.  (One piece a lane where there are lanes enough: 2048 columns on 64 lanes with four took 34 us for 8192 rows, on 256
+// 27; with two the backward holds 200 registers, with four 60 to 400 of them would be in scratch memory.)
+template <typename T, typename R, int G, int NV>
 constexpr NormVariant norm_variant()
 {
-    static_assert(G * NV == BG * BNV, "both hold the same rows");
     return {8 * G * NV,
             G,
             norm_fwd_threads(G),
-            BG,
-            norm_bwd_threads(BG),
-            {norm_fwd_kernel<T, R, kNormFront, G, NV>, norm_fwd_kernel<T, R, kNormBehind, G, NV>},
-            {norm_bwd_kernel<T, R, kNormFront, BG, BNV>, norm_bwd_kernel<T, R, kNormBehind, BG, BNV>}};
+            norm_bwd_threads(G),
+            {norm_fwd_kernel<T, R, kNormFront, G, NV, norm_units(G, NV)>, norm_fwd_kernel<T, R, kNormBehind, G, NV, norm_units(G, NV)>},
+            {norm_bwd_kernel<T, R, kNormFront, G, NV>, norm_bwd_kernel<T, R, kNormBehind, G, NV>}};
 }
 
 template <typename T, typename R>
 const NormVariant* norm_table()
 {
-    static const NormVariant table[kNormVariants] = {
-        norm_variant<T, R, 8, 1, 8, 1>(),    norm_variant<T, R, 16, 1, 16, 1>(),   norm_variant<T, R, 32, 1, 32, 1>(),
-        norm_variant<T, R, 64, 1, 64, 1>(),  norm_variant<T, R, 64, 2, 64, 2>(),   norm_variant<T, R, 64, 4, 256, 1>(),
-        norm_variant<T, R, 256, 2, 256, 2>(), norm_variant<T, R, 256, 4, 512, 2>(), norm_variant<T, R, 1024, 2, 1024, 2>()};
+    static const NormVariant table[kNormVariants] = {norm_variant<T, R, 8, 1>(),   norm_variant<T, R, 16, 1>(),  norm_variant<T, R, 32, 1>(),
+                                                     norm_variant<T, R, 64, 1>(),  norm_variant<T, R, 64, 2>(),  norm_variant<T, R, 256, 1>(),
+                                                     norm_variant<T, R, 512, 1>(), norm_variant<T, R, 1024, 1>(), norm_variant<T, R, 1024, 2>()};
     return table;
 }
 

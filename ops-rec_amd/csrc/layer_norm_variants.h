@@ -9,8 +9,8 @@ constexpr int kNormMaxLen = 16384;  // columns that share a mean, at most: the l
 
 struct NormVariant {
     int capacity;                    // columns that share a mean, at most
-    int fwd_lanes, fwd_threads;      // lanes that share a row, and of a workgroup
-    int bwd_lanes, bwd_threads;
+    int lanes;                       // that share a row
+    int fwd_threads, bwd_threads;    // of a workgroup
     void (*fwd[2])(const NormArgs);  // in front of a block, behind one
     void (*bwd[2])(const NormBwdArgs);
 };
