@@ -202,7 +202,7 @@ int slices_of(const NormArgs& a, const NormVariant* v)
         cus = 256;
     }
     const int64_t per_wg = v->bwd_threads / v->lanes, rows = a.units / static_cast<uint32_t>(a.groups);
-    const int64_t useful = (rows + per_wg - 1) / per_wg, places = static_cast<int64_t>(cus) * (1024 / v->bwd_threads) / a.groups;
+    const int64_t useful = (rows + per_wg - 1) / per_wg, places = static_cast<int64_t>(cus) * (v->lanes > 64 ? (512 / v->bwd_threads > 1 ? 512 / v->bwd_threads : 1) : 1024 / v->bwd_threads) / a.groups;
     const int64_t most = places > 1 ? places : 1;
     return static_cast<int>(useful < most ? useful : most);
 }
