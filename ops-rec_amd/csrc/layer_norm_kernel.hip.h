@@ -43,31 +43,36 @@ struct norm_piece {
     words_t w[ln_traits<Tag>::kPerChunk == 8 ? 1 : 2];
 };
 
-// piece c of a row of n values: all 8 where the row has them (c is clamped to the last whole piece, whose values the caller drops), the
-// values there are in the row's last, part-filled piece
+// Piece c of a row of n values is columns 8 c .. + 7; the row's last piece, where it is not whole, is its last 8 columns, some of which the piece before has
+// too: every lane's access is one of 16 bytes, and what two lanes hold is stored twice, the same bits, and counted once (norm_own).  (A last
+// piece taken value by value cost rows of 1002 columns a quarter of the bandwidth.)  Rows of fewer than 8 values are such a piece that starts
+// ahead of the row, and do go value by value.  Pieces past the row repeat its last one, and count nowhere.
+__device__ __forceinline__ int norm_base(int c, int n) { return 8 * c + 8 <= n ? 8 * c : n - 8; }
+// the first of a piece's values that is its own: 0 of a whole piece, 8 of a piece past the row
+__device__ __forceinline__ int norm_own(int c, int n)
+{
+    const int left = n - 8 * c;
+    return left >= 8 ? 0 : 8 - (left > 0 ? left : 0);
+}
+
 template <typename Tag>
 __device__ __forceinline__ norm_piece<Tag> norm_load(const typename ln_traits<Tag>::elem_t* row, int c, int n)
 {
     using E = typename ln_traits<Tag>::elem_t;
     norm_piece<Tag> p;
-    const int whole = n >> 3, rest = n & 7;
-    if (whole > 0) {
-        const typename norm_piece<Tag>::words_t* at =
-            reinterpret_cast<const typename norm_piece<Tag>::words_t*>(row + 8 * static_cast<int64_t>(min(c, whole - 1)));
+    if (n >= 8) {
+        const typename norm_piece<Tag>::words_t* at = reinterpret_cast<const typename norm_piece<Tag>::words_t*>(row + norm_base(c, n));
         p.w[0] = __builtin_nontemporal_load(at);
         if constexpr (sizeof(E) == 4) {
             p.w[1] = __builtin_nontemporal_load(at + 1);
         }
-    }
-    if (rest != 0) {
-        if (c == whole) {
-            E e[8];
+    } else {
+        E e[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                e[i] = i < rest ? row[8 * static_cast<int64_t>(whole) + i] : static_cast<E>(0.0f);
-            }
-            __builtin_memcpy(&p, e, sizeof e);
+        for (int i = 0; i < 8; ++i) {
+            e[i] = i >= 8 - n ? row[i - (8 - n)] : static_cast<E>(0.0f);
         }
+        __builtin_memcpy(&p, e, sizeof e);
     }
     return p;
 }
@@ -87,9 +92,11 @@ __device__ __forceinline__ void norm_store(typename ln_traits<Tag>::elem_t* row,
 {
     using T = ln_traits<Tag>;
     using E = typename T::elem_t;
-    const int first = 8 * c;
-    if (first + 8 <= n) {
-        typename norm_piece<Tag>::words_t* at = reinterpret_cast<typename norm_piece<Tag>::words_t*>(row + first);
+    if (8 * c >= n) {
+        return;
+    }
+    if (n >= 8) {
+        typename norm_piece<Tag>::words_t* at = reinterpret_cast<typename norm_piece<Tag>::words_t*>(row + norm_base(c, n));
 #pragma unroll
         for (int i = 0; i < 8 / T::kPerChunk; ++i) {
             const typename norm_piece<Tag>::words_t w = T::pack(f + T::kPerChunk * i);
@@ -98,14 +105,14 @@ __device__ __forceinline__ void norm_store(typename ln_traits<Tag>::elem_t* row,
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            if (first + i < n) {
-                row[first + i] = static_cast<E>(f[i]);
+            if (i >= 8 - n) {
+                row[i - (8 - n)] = static_cast<E>(f[i]);
             }
         }
     }
 }
 
-// 8 values per column (gamma, beta, scale), 0 past the end
+// 8 values per column (gamma, beta, scale)
 template <typename Tag>
 __device__ __forceinline__ void norm_columns(const void* p, bool f32, int64_t offset, int c, int n, float (&f)[8])
 {
@@ -193,59 +200,49 @@ __device__ __forceinline__ float norm_sigmoid(float z)
     }
 }
 
-// values of pieces past the row's end -> 0 (rows that fill the lanes have none)
+// s (a lane's NV pieces) -> norm(s) in place; returns rstd.  Two passes over registers; the mean's own rounding is taken out by the sum of the centred
+// values, which is 0 for an exact mean.  `full`: rows that fill the lanes, whose values are all their own.
 template <int G, int NV>
-__device__ __forceinline__ void drop_outside(float (&f)[NV][8], int lane, int len)
-{
-    if (len == 8 * G * NV) {
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int left = len - 8 * (lane + i * G);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            f[i][j] = j < left ? f[i][j] : 0.0f;
-        }
-    }
-}
-
-// s (a lane's NV pieces, 0 outside the row) -> norm(s) in place; returns rstd.  Two passes over registers; the mean's own rounding is
-// taken out by the sum of the centred values, which is 0 for an exact mean.
-template <int G, int NV>
-__device__ __forceinline__ float normalise(float (&s)[NV][8], int lane, int len, bool rms, float epsilon, float* s_part, int& slot)
+__device__ __forceinline__ float normalise(float (&s)[NV][8], const int (&own)[NV], bool full, int len, bool rms, float epsilon, float* s_part, int& slot)
 {
     const float inv_n = 1.0f / static_cast<float>(len);
-    float mean = 0.0f;
+    const auto each = [&](auto&& f) {  // over the values that are the lane's own
+        if (full) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    f(s[i][j]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    f(j >= own[i] ? s[i][j] : 0.0f);
+                }
+            }
+        }
+    };
     if (!rms) {
         float sum[1] = {0.0f};
+        each([&](float v) { sum[0] += v; });
+        row_sums<G>(sum, s_part, slot);
+        const float mean = sum[0] * inv_n;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                sum[0] += s[i][j];
+                s[i][j] -= mean;
             }
         }
-        row_sums<G>(sum, s_part, slot);
-        mean = sum[0] * inv_n;
     }
     float sq[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            s[i][j] -= mean;
-        }
-    }
-    drop_outside<G, NV>(s, lane, len);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            sq[0] = __builtin_fmaf(s[i][j], s[i][j], sq[0]);
-            sq[1] += s[i][j];
-        }
-    }
+    each([&](float v) {
+        sq[0] = __builtin_fmaf(v, v, sq[0]);
+        sq[1] += v;
+    });
     row_sums<G>(sq, s_part, slot);
     const float shift = rms ? 0.0f : sq[1] * inv_n;
     const float rstd = 1.0f / sqrtf(fmaxf(sq[0] * inv_n - shift * shift, 0.0f) + epsilon);
@@ -273,6 +270,12 @@ __global__ __launch_bounds__(norm_fwd_threads(G)) void norm_fwd_kernel(const Nor
     __shared__ float s_part[G > 64 ? kNormSlots * 2 * 16 : 1];
     const int lane = threadIdx.x % G;
     const int len = a.len;
+    const bool full = len == 8 * G * NV;
+    int own[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        own[i] = norm_own(lane + i * G, len);
+    }
     const bool f32 = a.affine_f32 != 0;
     const uint32_t first = blockIdx.x * kPerWg + threadIdx.x / G, step = gridDim.x * kPerWg;
     const uint32_t groups = static_cast<uint32_t>(a.groups);
@@ -358,8 +361,7 @@ __global__ __launch_bounds__(norm_fwd_threads(G)) void norm_fwd_kernel(const Nor
                     norm_store<R>(static_cast<RE*>(a.sum) + dense[t], lane + i * G, len, s[i]);
                 }
             }
-            drop_outside<G, NV>(s, lane, len);
-            normalise<G, NV>(s, lane, len, a.rms != 0, a.epsilon, s_part, slot);
+            normalise<G, NV>(s, own, full, len, a.rms != 0, a.epsilon, s_part, slot);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 float y[8];
@@ -416,6 +418,12 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
     const int part = static_cast<int>(blockIdx.x % static_cast<uint32_t>(f.groups));
     const uint32_t slice = blockIdx.x / static_cast<uint32_t>(f.groups);
     const int len = f.len, cols = f.len * f.groups;
+    const bool full = len == 8 * G * NV;
+    int own[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        own[i] = norm_own(lane + i * G, len);
+    }
     const int64_t col0 = static_cast<int64_t>(part) * len;
     const uint32_t rows = f.units / static_cast<uint32_t>(f.groups);
     const bool f32 = f.affine_f32 != 0;
@@ -440,8 +448,6 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
             norm_columns<T>(f.scale, f32, col0, lane + i * G, len, scale[i]);
         }
     }
-
-    drop_outside<G, NV>(gamma, lane, len);  // (what lies past the row's end must not reach its sums, NaN least of all)
 
     // a row's values as they lie in memory; those of the next row are on their way while one is worked on
     struct Row {
@@ -521,15 +527,13 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
                 norm_unpack<T>(now.x[i], n[i]);
             }
         }
-        drop_outside<G, NV>(n, lane, len);
-        const float rstd = normalise<G, NV>(n, lane, len, f.rms != 0, f.epsilon, s_part, slot);
+        const float rstd = normalise<G, NV>(n, own, full, len, f.rms != 0, f.epsilon, s_part, slot);
 
         // g = (gradient of m or y) * gamma; the gradient itself goes into the sums
         float g[NV][8];
         float means[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int left = len - 8 * (lane + i * G);
             float d[8];
             if constexpr (kGradR) {
                 norm_unpack<R>(now.d[i], d);
@@ -564,19 +568,28 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
                     norm_unpack<T>(now.y[i], d);
                 }
             }
-            if (len != 8 * G * NV) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    d[j] = j < left ? d[j] : 0.0f;
-                }
-            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                d_gamma[i][j] = __builtin_fmaf(d[j], n[i][j], d_gamma[i][j]);
-                d_beta[i][j] += d[j];
                 g[i][j] = d[j] * gamma[i][j];
-                means[0] = __builtin_fmaf(g[i][j], n[i][j], means[0]);
-                means[1] += g[i][j];
+            }
+            // (sums take a lane's own values: what another lane has too, or lies past the row, must not reach them, NaN least of all)
+            if (full) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    d_gamma[i][j] = __builtin_fmaf(d[j], n[i][j], d_gamma[i][j]);
+                    d_beta[i][j] += d[j];
+                    means[0] = __builtin_fmaf(g[i][j], n[i][j], means[0]);
+                    means[1] += g[i][j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const bool mine = j >= own[i];
+                    d_gamma[i][j] = __builtin_fmaf(d[j], n[i][j], d_gamma[i][j]);
+                    d_beta[i][j] += d[j];
+                    means[0] += mine ? g[i][j] * n[i][j] : 0.0f;
+                    means[1] += mine ? g[i][j] : 0.0f;
+                }
             }
         }
         row_sums<G>(means, s_part, slot);
@@ -600,12 +613,11 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
                 }
                 norm_store<R>(static_cast<RE*>(a.residual_grad) + dense, lane + i * G, len, d);
                 if (a.want_scale) {
-                    const int left = len - 8 * (lane + i * G);
                     float v[8];
                     norm_unpack<T>(now.x[i], v);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        d_scale[i][j] += j < left ? d[j] * v[j] : 0.0f;
+                        d_scale[i][j] = __builtin_fmaf(d[j], v[j], d_scale[i][j]);
                     }
                 }
                 if (a.x_grad != nullptr) {
@@ -621,16 +633,19 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
         }
     }
 
-    // the sums over this workgroup's rows, kind by kind
+    // the sums over this workgroup's rows, kind by kind: a column from the lane whose own it is
     const auto put = [&](const float (&v)[NV][8], int kind) {
         float* const out = a.partial + (static_cast<int64_t>(kind) * a.slices + slice) * cols + col0;
         if constexpr (kRows > 1) {
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
+                const int base = norm_base(lane + i * G, len);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    s_sums[(sub * NV * G + i * G + lane) * 8 + j] = v[i][j];
+                    if (j >= own[i]) {
+                        s_sums[sub * NV * G * 8 + base + j] = v[i][j];
+                    }
                 }
             }
             __syncthreads();
@@ -645,11 +660,11 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
         } else {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c = 8 * (lane + i * G);
+                const int base = norm_base(lane + i * G, len);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    if (c + j < len) {
-                        out[c + j] = v[i][j];
+                    if (j >= own[i]) {
+                        out[base + j] = v[i][j];
                     }
                 }
             }
