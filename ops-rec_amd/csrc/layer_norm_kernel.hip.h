@@ -36,6 +36,15 @@ constexpr int kNormFront = 0, kNormBehind = 1;
 constexpr int norm_fwd_threads(int g) { return g > 256 ? g : 256; }
 constexpr int norm_bwd_threads(int g) { return g > 64 ? g : 512; }  // (barriers inside a row: one row at a time)
 
+// a lane's group within its workgroup: where a group is whole wavefronts, it and all that follows from it (rows, addresses) is the same in all lanes
+// and kept in scalar registers
+template <int G>
+__device__ __forceinline__ int norm_sub()
+{
+    const int sub = threadIdx.x / G;
+    return G >= 64 ? __builtin_amdgcn_readfirstlane(sub) : sub;
+}
+
 // ---- 8 values of a row, as they lie in memory ----
 template <typename Tag>
 struct norm_piece {
@@ -277,7 +286,7 @@ __global__ __launch_bounds__(norm_fwd_threads(G)) void norm_fwd_kernel(const Nor
         own[i] = norm_own(lane + i * G, len);
     }
     const bool f32 = a.affine_f32 != 0;
-    const uint32_t first = blockIdx.x * kPerWg + threadIdx.x / G, step = gridDim.x * kPerWg;
+    const uint32_t first = blockIdx.x * kPerWg + norm_sub<G>(), step = gridDim.x * kPerWg;
     const uint32_t groups = static_cast<uint32_t>(a.groups);
     const int64_t col0 = groups == 1 ? 0 : static_cast<int64_t>(first % groups) * len;
     int slot = 0;
@@ -414,7 +423,7 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
     __shared__ float s_part[G > 64 ? kNormSlots * 2 * 16 : 1];
     __shared__ __attribute__((aligned(16))) float s_sums[kRows > 1 ? kThreads * NV * 8 : 1];
     const NormArgs& f = a.f;
-    const int sub = threadIdx.x / G, lane = threadIdx.x % G;
+    const int sub = norm_sub<G>(), lane = threadIdx.x % G;
     const int part = static_cast<int>(blockIdx.x % static_cast<uint32_t>(f.groups));
     const uint32_t slice = blockIdx.x / static_cast<uint32_t>(f.groups);
     const int len = f.len, cols = f.len * f.groups;
@@ -496,8 +505,9 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
             }
         }
     };
+    constexpr bool kAhead = G < 1024;
     Row next;
-    if (slice * kRows + sub < rows) {
+    if (kAhead && slice * kRows + sub < rows) {
         load(slice * kRows + sub, next);
     }
     for (uint64_t row0 = static_cast<uint64_t>(slice) * kRows; row0 < rows; row0 += static_cast<uint64_t>(a.slices) * kRows) {
@@ -506,9 +516,14 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
             break;
         }
         const int64_t dense = static_cast<int64_t>(row) * cols + col0;
-        const Row now = next;
-        if (after < rows) {
-            load(static_cast<uint32_t>(after), next);
+        Row now;
+        if constexpr (kAhead) {
+            now = next;
+            if (after < rows) {
+                load(static_cast<uint32_t>(after), next);
+            }
+        } else {
+            load(static_cast<uint32_t>(row), now);
         }
         float n[NV][8];
 #pragma unroll
