@@ -153,7 +153,8 @@ HSTU_API int rotary_fwd(const rotary_params* params, void* stream);
 /*
  * gated_linear, both projections of a gated feed-forward block with activation and product:
  *   mixed = x weight^T + bias = (g, u);  hidden = act(g) * u
- * sums in fp32; hidden is taken of them before mixed, which a backward reads, is rounded.
+ * sums in fp32, of which hidden is taken.  A backward reads mixed: 24 bits of every sum, in 3 * inner words of 16 bits per row, in an order of this
+ * library's own.
  */
 typedef struct gated_linear_params {
     uint32_t struct_size; /* sizeof(gated_linear_params), checked */
@@ -162,7 +163,7 @@ typedef struct gated_linear_params {
     const void* weight; /* [2 * inner, cols], same type: the rows of g, then those of u */
     const void* bias;   /* [2 * inner], same type, or NULL for none */
     void* hidden;       /* [rows, inner], same type, or NULL */
-    void* mixed;        /* [rows, 2 * inner], same type, or NULL; one of the two must be given */
+    void* mixed;        /* [rows, 3 * inner] words of 16 bits, or NULL; one of the two must be given */
     int64_t rows;
     int64_t cols;  /* a multiple of 8, at most 2^22 */
     int64_t inner; /* a multiple of 8, at most 2^22; inner * cols below 2^29 */

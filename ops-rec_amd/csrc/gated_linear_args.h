@@ -12,7 +12,7 @@ struct GatedGemmArgs {
     const void* m_side;  // forward: x [rows, depth]; x gradient: d_mixed [rows, depth]; weight gradient: d_mixed [depth, rows]
     const void* bias;    // forward: [2 cols], 16-bit, or nullptr
     void* out;           // forward: hidden [rows, cols], or nullptr; gradients: [rows, cols]
-    void* mixed;         // forward: [rows, 2 cols], or nullptr
+    void* mixed;         // forward: [rows, 3 cols] (kept_high), or nullptr
     float* partial;      // gradients in several chunks of the depth: [chunks][rows][cols]
     int64_t rows;
     int64_t depth;
@@ -29,7 +29,7 @@ struct GatedFewRowsArgs {
     const void* weight;  // [2 inner, depth]
     const void* bias;    // [2 inner], 16-bit, or nullptr
     void* hidden;        // [rows, inner], or nullptr
-    void* mixed;         // [rows, 2 inner], or nullptr
+    void* mixed;         // [rows, 3 inner], or nullptr
     int64_t rows;
     int depth;
     int inner;
@@ -39,7 +39,7 @@ struct GatedFewRowsArgs {
 // gated_stage_kernel and gated_sum_kernel (gated_linear_bwd_kernel.hip.h)
 struct GatedStageArgs {
     const void* grad;   // [rows, inner]
-    const void* mixed;  // [rows, 2 inner]
+    const void* mixed;  // [rows, 3 inner]
     void* d_mixed;      // [rows, 2 inner]
     float* partial;     // [slices][2 inner] column sums, or nullptr
     int64_t rows;

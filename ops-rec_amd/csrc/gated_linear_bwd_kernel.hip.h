@@ -3,7 +3,8 @@
 //   mixed = (g, u), grad = gradient of hidden:   d g = grad * u * act'(g),   d u = grad * act(g),   d mixed = (d g, d u)
 //   d bias = column sums of d mixed, taken of the values before they are rounded
 //
-// Bound by HBM: three values read and two written per column of hidden.  A thread has 8 columns and walks over the rows of its slice; its
+// Bound by HBM: 8 bytes read and 4 written per column of hidden.  (d mixed is rounded to the type of x, half a step of it: what the matrix instructions of
+// the products behind it multiply.)  A thread has 8 columns and walks over the rows of its slice; its
 // sums stay in registers, those of a workgroup's eight rows of threads meet in LDS, and a row of partial sums per workgroup goes to the workspace.
 #pragma once
 #include "gated_linear_gemm.hip.h"
@@ -34,16 +35,20 @@ __global__ __launch_bounds__(kStageThreads) void gated_stage_kernel(const GatedS
             constexpr int kind = decltype(chosen)::value;
             for (int64_t row = static_cast<int64_t>(slice) * kStageRows + sub; row < a.rows; row += step) {
                 const u32x4_t d4 = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(a.grad) + row * a.inner + col));
-                const uint16_t* const m = static_cast<const uint16_t*>(a.mixed) + row * 2 * a.inner + col;
+                const uint16_t* const m = static_cast<const uint16_t*>(a.mixed) + row * 3 * a.inner + col;
                 const u32x4_t g4 = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(m));
                 const u32x4_t u4 = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(m + a.inner));
+                const u32x4_t low = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(m + 2 * a.inner));
                 u32x4_t og, ou;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float d[2], g[2], u[2], x[2], y[2];
+                    float d[2], x[2], y[2];
                     ils_unpack2<Tag>(d4[e], d[0], d[1]);
-                    ils_unpack2<Tag>(g4[e], g[0], g[1]);
-                    ils_unpack2<Tag>(u4[e], u[0], u[1]);
+                    const uint32_t gl = low[e / 2], ul = low[2 + e / 2];
+                    const float g[2] = {e % 2 == 0 ? kept_value<0, 0>(g4[e], gl) : kept_value<0, 2>(g4[e], gl),
+                                        e % 2 == 0 ? kept_value<1, 1>(g4[e], gl) : kept_value<1, 3>(g4[e], gl)};
+                    const float u[2] = {e % 2 == 0 ? kept_value<0, 0>(u4[e], ul) : kept_value<0, 2>(u4[e], ul),
+                                        e % 2 == 0 ? kept_value<1, 1>(u4[e], ul) : kept_value<1, 3>(u4[e], ul)};
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         float act, slope;

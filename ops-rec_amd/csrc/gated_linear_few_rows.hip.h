@@ -157,9 +157,14 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
             static_cast<uint16_t*>(a.hidden)[to * a.inner + n0 + c] = static_cast<uint16_t>(pack2<Tag>(act * sum[1], 0.0f));
         }
         if (a.mixed != nullptr) {
-            uint16_t* const m = static_cast<uint16_t*>(a.mixed) + to * 2 * a.inner + n0 + c;
-            m[0] = static_cast<uint16_t>(pack2<Tag>(sum[0], 0.0f));
-            m[a.inner] = static_cast<uint16_t>(pack2<Tag>(sum[1], 0.0f));
+            uint16_t* const m = static_cast<uint16_t*>(a.mixed) + to * 3 * a.inner;
+            uint8_t* const low = reinterpret_cast<uint8_t*>(m + 2 * a.inner) + 16 * ((n0 + c) / 8) + (n0 + c) % 8;
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const uint32_t bits = __builtin_bit_cast(uint32_t, sum[p]);
+                m[p * a.inner + n0 + c] = static_cast<uint16_t>(bits >> 16);
+                low[8 * p] = static_cast<uint8_t>(bits >> 8);
+            }
         }
     }
 }

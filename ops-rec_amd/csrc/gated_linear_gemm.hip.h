@@ -59,6 +59,25 @@ __device__ __forceinline__ void with_activation(int kind, const F& f)
     }
 }
 
+// What a backward needs of g and u, "mixed": the upper 24 bits of their fp32 sums, 2^-15 of them at most cut off, whatever the type of x.  Rounded to that type they
+// would add to the gradients as much as the rounding of d_mixed and that of the gradients themselves do; the third byte costs 17 us of writing and as much of
+// reading at 20292 rows of 2 x 2048.  A row is [g's upper 16 bits][u's upper 16 bits][for every 8 columns: g's 8 third bytes, u's 8].
+__device__ __forceinline__ uint32_t kept_high(float a, float b)
+{
+    return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302);
+}
+__device__ __forceinline__ uint32_t kept_low(float a, float b, float c, float d)
+{
+    return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x0c0c0501) |
+           __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, d), __builtin_bit_cast(uint32_t, c), 0x05010c0c);
+}
+// value H of the pair `high`, its third byte at K of `low`
+template <int H, int K>
+__device__ __forceinline__ float kept_value(uint32_t high, uint32_t low)
+{
+    return __builtin_bit_cast(float, __builtin_amdgcn_perm(high, low, (H == 0 ? 0x0504000cu : 0x0706000cu) | (K << 8)));
+}
+
 template <int ACT>
 __device__ __forceinline__ void gated_act_slope(float z, float& act, float& slope)
 {
@@ -112,8 +131,8 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
     constexpr int kReqsN = BN / 64, kReqsM = BM / 64, kReqs = kReqsN + kReqsM;  // direct-to-LDS instructions per wavefront and stage
     static_assert(BM % 64 == 0 && BN % 64 == 0, "a stage's instructions are dealt evenly");
     constexpr int kNElems = BN * kGemmStep, kStage = (BN + BM) * kGemmStep;
-    constexpr int kEpiRow = (MODE == kGemmForward ? kWaveN / 2 : 64) + 8;  // staged rows of up to 64 columns
-    constexpr int kEpiPlanes = MODE == kGemmForward ? 3 : 1;
+    constexpr int kEpiRow = MODE == kGemmForward ? kWaveN / 2 : 64 + 8;  // staged rows of up to 64 columns
+    constexpr int kEpiPlanes = MODE == kGemmForward ? 4 : 1;
     // (a second piece where the stages' LDS has room for it)
     constexpr int kEpiPieces = MODE == kGemmForward && 2 * 4 * kEpiPlanes * 32 * kEpiRow <= STAGES * kStage ? 2 : 1;
     constexpr int kEpiWave = kEpiPieces * kEpiPlanes * 32 * kEpiRow;
@@ -388,7 +407,6 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
     // ---- 16-bit outputs, through LDS in pieces of 32 rows by up to 64 columns per wavefront, so that every store writes whole 128-byte runs.  Pieces
     // alternate between two places: the values of the next are worked out while the last goes out.
     __builtin_amdgcn_s_barrier();  // every wavefront is done reading the last stage
-    uint16_t* const staged = s_tiles + wave * kEpiWave;
     auto settle = [] {  // (a wavefront's own LDS accesses stay in order; the compiler must keep them so)
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -400,34 +418,45 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
         constexpr int HB = NB / 2;  // blocks of each projection
         constexpr int kPerRow = kRound / 8, kRowsAtOnce = 64 / kPerRow;  // lanes to a row of 16-byte pieces, rows of a store
         const int col = n0 + kRound * wn + 8 * (lane % kPerRow);
+        // where a row's 16 bytes lie: rows are not padded, and the rows that share 256 bytes of banks take turns over the whole of them
+        const auto at = [](int row, int chunk) { return row * kRound + 8 * (chunk ^ (row / (128 / kRound) % kPerRow)); };
         const auto finish = [&](auto chosen, auto kept) {
             constexpr int kind = decltype(chosen)::value;
             constexpr bool keep = decltype(kept)::value;
-            constexpr int kPlane = 32 * kEpiRow;
+            constexpr int kPlane = 32 * kRound, kPlanes = keep ? kEpiPlanes : 1;
+            constexpr int kPieces = 2 * 4 * kPlanes * kPlane <= kLds ? 2 : 1;
+            uint16_t* const mine = s_tiles + wave * kPieces * kPlanes * kPlane;
 #pragma unroll
             for (int j = 0; j < MB; ++j) {
-                uint16_t* const piece = staged + (j % kEpiPieces) * kEpiPlanes * kPlane;
+                uint16_t* const piece = mine + (j % kPieces) * kPlanes * kPlane;
 #pragma unroll
                 for (int i = 0; i < HB; ++i) {
 #pragma unroll
                     for (int run = 0; run < 2; ++run) {
-                        u32x4_t hw, gw, uw;
+                        u32x4_t hw, gw, uw, low;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const float g0 = acc[i][j][8 * run + 2 * e], g1 = acc[i][j][8 * run + 2 * e + 1];
                             const float u0 = acc[HB + i][j][8 * run + 2 * e], u1 = acc[HB + i][j][8 * run + 2 * e + 1];
-                            // (hidden is taken of the sums as they are, before mixed is rounded for the backward)
+                            // (hidden is taken of the sums as they are)
                             hw[e] = pack2<Tag>(gated_act<kind>(g0) * u0, gated_act<kind>(g1) * u1);
                             if constexpr (keep) {
-                                gw[e] = pack2<Tag>(g0, g1);
-                                uw[e] = pack2<Tag>(u0, u1);
+                                gw[e] = kept_high(g0, g1);
+                                uw[e] = kept_high(u0, u1);
                             }
                         }
-                        uint16_t* const to = piece + r * kEpiRow + 32 * i + 16 * run + 8 * half;
+                        uint16_t* const to = piece + at(r, 4 * i + 2 * run + half);
                         *reinterpret_cast<u32x4_t*>(to) = hw;
                         if constexpr (keep) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                low[e] = kept_low(acc[i][j][8 * run + 4 * e], acc[i][j][8 * run + 4 * e + 1], acc[i][j][8 * run + 4 * e + 2], acc[i][j][8 * run + 4 * e + 3]);
+                                low[2 + e] = kept_low(acc[HB + i][j][8 * run + 4 * e], acc[HB + i][j][8 * run + 4 * e + 1], acc[HB + i][j][8 * run + 4 * e + 2],
+                                                      acc[HB + i][j][8 * run + 4 * e + 3]);
+                            }
                             *reinterpret_cast<u32x4_t*>(to + kPlane) = gw;
                             *reinterpret_cast<u32x4_t*>(to + 2 * kPlane) = uw;
+                            *reinterpret_cast<u32x4_t*>(to + 3 * kPlane) = low;
                         }
                     }
                 }
@@ -436,20 +465,22 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
                 for (int q = 0; q < 32 / kRowsAtOnce; ++q) {
                     const int in_block = kRowsAtOnce * q + lane / kPerRow;
                     const int64_t row = m0 + kWaveM * wm + 32 * j + in_block;
-                    const uint16_t* const from = piece + in_block * kEpiRow + 8 * (lane % kPerRow);
+                    const uint16_t* const from = piece + at(in_block, lane % kPerRow);
                     if (row < a.rows && col < a.cols) {
                         if (!keep || a.out != nullptr) {
                             __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from),
                                                         reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.out) + row * a.cols + col));
                         }
                         if constexpr (keep) {
-                            uint16_t* const to = static_cast<uint16_t*>(a.mixed) + row * 2 * a.cols + col;
-                            __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from + kPlane), reinterpret_cast<u32x4_t*>(to));
-                            __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from + 2 * kPlane), reinterpret_cast<u32x4_t*>(to + a.cols));
+                            uint16_t* const to = static_cast<uint16_t*>(a.mixed) + row * 3 * a.cols + col;
+#pragma unroll
+                            for (int p = 0; p < 3; ++p) {
+                                __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from + (1 + p) * kPlane), reinterpret_cast<u32x4_t*>(to + p * a.cols));
+                            }
                         }
                     }
                 }
-                if constexpr (kEpiPieces == 1) {
+                if constexpr (kPieces == 1) {
                     settle();
                 }
             }
@@ -463,6 +494,7 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
         });
     } else {
         static_assert(MODE == kGemmForward || NB % 2 == 0, "rounds of 64 columns");
+        uint16_t* const staged = s_tiles + wave * kEpiWave;
         const int out_row = lane >> 3, out_chunk = lane & 7;
 #pragma unroll
         for (int j = 0; j < MB; ++j) {

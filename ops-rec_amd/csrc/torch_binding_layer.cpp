@@ -447,7 +447,7 @@ Pair gated_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, 
     if (describe_gated_linear(x, weight, bias, activation, p)) {
         const c10::DeviceGuard guard(x.device());
         Tensor hidden = empty({p.rows, p.inner}, x.scalar_type(), x.device());
-        Tensor mixed = keep ? empty({p.rows, 2 * p.inner}, x.scalar_type(), x.device()) : empty({0}, x.scalar_type(), x.device());
+        Tensor mixed = keep ? empty({p.rows, 3 * p.inner}, at::kShort, x.device()) : empty({0}, at::kShort, x.device());
         p.hidden = hidden.data_ptr();
         p.mixed = ptr(mixed);
         const int rc = gated_linear_fwd(&p, stream_of(x));
@@ -466,18 +466,18 @@ Three gated_linear_backward(const Tensor& grad_in, const Tensor& x, const Tensor
 {
     const Tensor grad = contiguous(grad_in);
     gated_linear_bwd_params p;
-    const auto readable = [&](const Tensor& t, int64_t cols) {
-        return t.dim() == 2 && t.size(0) == x.size(0) && t.size(1) == cols && t.scalar_type() == x.scalar_type() && t.device() == x.device() &&
+    const auto readable = [&](const Tensor& t, int64_t cols, at::ScalarType dtype) {
+        return t.dim() == 2 && t.size(0) == x.size(0) && t.size(1) == cols && t.scalar_type() == dtype && t.device() == x.device() &&
                t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
     };
     if ((wanted[0] || wanted[1] || (wanted[2] && is_set(bias))) && describe_gated_linear(x, weight, bias, activation, p.fwd) &&
-        readable(grad, p.fwd.inner) && (mixed_in.numel() == 0 || readable(mixed_in, 2 * p.fwd.inner))) {
+        readable(grad, p.fwd.inner, x.scalar_type()) && (mixed_in.numel() == 0 || readable(mixed_in, 3 * p.fwd.inner, at::kShort))) {
         const c10::DeviceGuard guard(x.device());
         const auto make = [&](bool want, at::IntArrayRef size) { return want ? empty(size, x.scalar_type(), x.device()) : empty({0}, x.scalar_type(), x.device()); };
         Tensor mixed = mixed_in;
         int rc = HSTU_OK;
         if (mixed.numel() == 0) {
-            mixed = empty({p.fwd.rows, 2 * p.fwd.inner}, x.scalar_type(), x.device());
+            mixed = empty({p.fwd.rows, 3 * p.fwd.inner}, at::kShort, x.device());
             p.fwd.mixed = mixed.data_ptr();
             rc = gated_linear_fwd(&p.fwd, stream_of(x));
         }
@@ -506,6 +506,7 @@ struct GatedLinearFunction : torch::autograd::Function<GatedLinearFunction> {
         const at::AutoDispatchBelowADInplaceOrView below;
         const auto [hidden, mixed] = op.call(x, weight, bias, activation, keep);
         ctx->set_materialize_grads(false);
+        ctx->mark_non_differentiable({mixed});
         ctx->save_for_backward({x, weight, unwrap(bias), mixed});
         ctx->saved_data["activation"] = activation;
         return {hidden, mixed};
@@ -513,7 +514,6 @@ struct GatedLinearFunction : torch::autograd::Function<GatedLinearFunction> {
 
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
-        TORCH_CHECK(!grads[1].defined(), "gated_linear: no gradient flows through mixed, which is there for the backward pass");
         variable_list out(5);
         if (grads[0].defined()) {
             static const auto op = operator_handle<decltype(gated_linear_backward)>("ops_rec::gated_linear_backward", "");

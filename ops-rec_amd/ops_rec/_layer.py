@@ -400,17 +400,18 @@ def _describe_gated_linear(p, x, weight, bias, hidden, mixed, activation):
 
 
 def gated_linear(x, weight, bias=None, activation="silu", keep=False):
-    """``hidden = act(g) * u`` with ``(g, u) = mixed = x @ weight^T + bias``: both projections of a gated feed-forward block, its activation and the
+    """``hidden = act(g) * u`` with ``(g, u) = x @ weight^T + bias``: both projections of a gated feed-forward block, its activation and the
     product, for x [rows, cols] and weight [2 * inner, cols], the rows of g first.  Returns ``(hidden, mixed)``, mixed empty unless ``keep``.
 
-    A backward pass reads mixed: a call in training passes ``keep=True`` (without it, as a block that saves memory may prefer, the backward
-    multiplies again).  ``activation`` is "silu", "gelu" (by its tanh form) or "sigmoid".  x, weight and bias are all bf16 or all fp16; cols and inner are
-    multiples of 8.  Sums are fp32, and hidden is taken of them before mixed is rounded.  No gradient flows through mixed."""
+    Mixed is for the backward pass alone, which reads g and u out of it: 24 bits of each, as int16 [rows, 3 * inner] in an order of their own.
+    No gradient flows through it: it does not require one.  A call in training passes ``keep=True`` (without it, as a block that saves memory
+    may prefer, the backward multiplies again).  ``activation`` is "silu", "gelu" (by its tanh form) or "sigmoid".  x, weight and bias are all bf16
+    or all fp16; cols and inner are multiples of 8.  Sums are fp32, and hidden is taken of them."""
     _gated_linear_checks(x, weight, bias, activation)
     _on_device(x.device, (("x", x), ("weight", weight), ("bias", bias)))
     inner = weight.size(0) // 2
     hidden = torch.empty((x.size(0), inner), dtype=x.dtype, device=x.device)
-    mixed = torch.empty((x.size(0), 2 * inner) if keep else (0,), dtype=x.dtype, device=x.device)
+    mixed = torch.empty((x.size(0), 3 * inner) if keep else (0,), dtype=torch.int16, device=x.device)
     if x.size(0) != 0:
         xc, wc, bc = _aligned(x), _aligned(weight), None if bias is None else _aligned(bias)
         p = _native.GatedLinearParams()
@@ -422,7 +423,7 @@ def gated_linear(x, weight, bias=None, activation="silu", keep=False):
 def gated_linear_meta(x, weight, bias=None, activation="silu", keep=False):
     _check(x.dim() == 2, "The x should be 2D")
     _check(weight.dim() == 2, "The weight should be 2D")
-    return x.new_empty((x.size(0), weight.size(0) // 2)), x.new_empty((x.size(0), weight.size(0)) if keep else (0,))
+    return x.new_empty((x.size(0), weight.size(0) // 2)), x.new_empty((x.size(0), 3 * (weight.size(0) // 2)) if keep else (0,), dtype=torch.int16)
 
 
 def gated_linear_backward(grad, x, weight, bias, mixed, activation, wanted):
@@ -432,7 +433,8 @@ def gated_linear_backward(grad, x, weight, bias, mixed, activation, wanted):
     _check(len(wanted) == 3, "wanted must have three elements")
     rows, inner = x.size(0), weight.size(0) // 2
     _check(tuple(grad.shape) == (rows, inner) and grad.dtype == x.dtype, f"grad must be {[rows, inner]} of the dtype of x")
-    _check(mixed.numel() == 0 or (tuple(mixed.shape) == (rows, 2 * inner) and mixed.dtype == x.dtype), f"mixed must be empty or {[rows, 2 * inner]} of the dtype of x")
+    _check(mixed.numel() == 0 or (tuple(mixed.shape) == (rows, 3 * inner) and mixed.dtype == torch.int16),
+           f"mixed must be empty or {[rows, 3 * inner]} of int16")  # fmt: skip
     _on_device(x.device, (("x", x), ("grad", grad), ("weight", weight), ("bias", bias), ("mixed", mixed)))
     make = torch.zeros if rows == 0 else torch.empty
     shapes = ((rows, x.size(1)), tuple(weight.shape), (2 * inner,))
@@ -443,7 +445,7 @@ def gated_linear_backward(grad, x, weight, bias, mixed, activation, wanted):
         p = _native.GatedLinearBwdParams()
         p.struct_size = ctypes.sizeof(p)
         if mixed.numel() == 0:
-            mixed = torch.empty((rows, 2 * inner), dtype=x.dtype, device=x.device)
+            mixed = torch.empty((rows, 3 * inner), dtype=torch.int16, device=x.device)
             _describe_gated_linear(p.fwd, xc, wc, bc, None, mixed, activation)
             _call("gated_linear_fwd", p.fwd, x.device, workspace=False)
         mc = _aligned(mixed)
@@ -463,12 +465,12 @@ def gated_linear_backward_meta(grad, x, weight, bias, mixed, activation, wanted)
 def _gated_linear_setup(ctx, inputs, output):
     x, weight, bias, activation, _ = inputs
     ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(output[1])
     ctx.save_for_backward(x, weight, bias, output[1])
     ctx.activation = activation
 
 
-def _gated_linear_grad(ctx, grad, mixed_grad):
-    _check(mixed_grad is None, "gated_linear: no gradient flows through mixed, which is there for the backward pass")
+def _gated_linear_grad(ctx, grad, _):
     x, weight, bias, mixed = ctx.saved_tensors
     if grad is None:
         return (None,) * 5

@@ -43,7 +43,7 @@ def test_meta_inference():
     grads = OPS.residual_norm_backward(y, None, x, x, None, g, None, False, torch.bfloat16, 1e-5, False)
     assert [tuple(t.shape) for t in grads] == [(0,), (5, 24), (24,), (0,), (0,)]
     x, w = torch.empty(5, 24, device="meta", dtype=torch.float16), torch.empty(80, 24, device="meta", dtype=torch.float16)
-    assert [tuple(t.shape) for t in OPS.gated_linear(x, w, None, "gelu", True)] == [(5, 40), (5, 80)] and OPS.gated_linear(x, w)[1].shape == (0,)
+    assert [tuple(t.shape) for t in OPS.gated_linear(x, w, None, "gelu", True)] == [(5, 40), (5, 120)] and OPS.gated_linear(x, w)[1].shape == (0,)
     grads = OPS.gated_linear_backward(torch.empty(5, 40, device="meta"), x, w, None, x, "silu", [True, False, True])
     assert [tuple(t.shape) for t in grads] == [(5, 24), (0,), (0,)]
     q, k = torch.empty(7, 4, 16, device="meta"), torch.empty(7, 2, 16, device="meta")
@@ -68,6 +68,8 @@ def test_fake_tensors_that_record_gradients():
             OPS.rotary(q, q, f.requires_grad_(True), offs)
         with torch.no_grad():
             assert not OPS.rotary(q, q, f, offs)[0].requires_grad
+        hidden, mixed = OPS.gated_linear(x, torch.empty(32, 24, device="cuda", dtype=torch.bfloat16), None, "silu", True)
+        assert hidden.requires_grad and not mixed.requires_grad
 
 
 def test_refusals_of_the_norms():
