@@ -5,7 +5,8 @@
 // 8 values of one weight row; nothing of the weight is read twice, so LDS would only add a trip).  Its eight wavefronts share the depth: each takes every
 // eighth run of 64 values, whose loads are all in flight before the first product, and the partial sums meet in LDS.
 // C is 8, 16, 24 or 32, whichever leaves the fullest compute unit the least to read: rounds of workgroups times 2 C + rows.  (48 rows,
-// 2048 -> 5632: 352 workgroups of 16 columns, two on some compute units, took 25 us; 235 of 24, one on each, 15.)
+// 2048 -> 5632: 352 workgroups of 16 columns, two on some compute units, took 25 us; 235 of 24, one on each, 18.6; with one row 11.4: every
+// compute unit reads as much of x as of the weight there.  Loads of twice as many runs under way are no faster.)
 #pragma once
 #include "gated_linear_gemm.hip.h"
 

@@ -17,7 +17,7 @@
 // A dozen flops per value: bound by HBM.  A row (or part) belongs to G lanes -- a slice of a wavefront, a wavefront or a workgroup --
 // which hold it in registers as NV pieces of 8 values per lane; all loads of a row are in flight before the first use, and sums
 // over a wavefront go through DPP and lane swaps (10 instructions, no LDS).  Pieces start anywhere: the 16-byte accesses of this
-// machine need no alignment, so odd widths and strides take the same path, and only a last piece of fewer than 8 values goes value by value.
+// machine need no alignment, so odd widths and strides take the same path, and a row's last piece, where it is not whole, is its last 8 values (norm_base).
 //
 // The backward is persistent: a workgroup keeps one part of the columns and walks over rows, its lanes adding up the gradients of
 // gamma, beta and scale in registers; the sums of a workgroup's lane groups meet in LDS, one row of partial sums per workgroup goes to the
@@ -439,22 +439,66 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
     const bool need_x = !kFromSum || f.scale != nullptr;
     int slot = 0;
 
+    // The longest rows (2048 pieces) have no registers for gamma, beta and scale, which are loaded for every row, nor for the sums of gamma's and beta's
+    // gradients, which are kept in LDS, a lane's own in its own place.  (All in registers, which spill: 2048 x 16384 228 us with a gate, 230 in
+    // front; 150 and 127 so.)
+    constexpr bool kHold = NV * G < 2048;
+    __shared__ float4 s_acc[kHold ? 1 : 2 * NV * 2 * kThreads];
+    const auto acc_at = [&](int kind, int i, int h) { return s_acc + ((kind * NV + i) * 2 + h) * kThreads + threadIdx.x; };
+    const auto add = [&](float (&sums)[NV][8], int kind, int i, const float (&v)[8]) {
+        if constexpr (kHold) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                sums[i][j] += v[j];
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float4 t = *acc_at(kind, i, h);
+                t.x += v[4 * h], t.y += v[4 * h + 1], t.z += v[4 * h + 2], t.w += v[4 * h + 3];
+                *acc_at(kind, i, h) = t;
+            }
+        }
+    };
     float gamma[NV][8], beta[NV][8], scale[NV][8];
     float d_gamma[NV][8], d_beta[NV][8], d_scale[NV][8];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        norm_columns<T>(f.gamma, f32, col0, lane + i * G, len, gamma[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            d_gamma[i][j] = d_beta[i][j] = d_scale[i][j] = 0.0f;
+        }
+        if constexpr (!kHold) {
+#pragma unroll
+            for (int at = 0; at < 4; ++at) {
+                *acc_at(at / 2, i, at % 2) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+        }
+    }
+    const auto hold = [&](int i) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             beta[i][j] = 0.0f;
-            scale[i][j] = 1.0f;
-            d_gamma[i][j] = d_beta[i][j] = d_scale[i][j] = 0.0f;
         }
+        norm_columns<T>(f.gamma, f32, col0, lane + i * G, len, gamma[i]);
         if (MODE == kNormBehind && f.beta != nullptr) {
             norm_columns<T>(f.beta, f32, col0, lane + i * G, len, beta[i]);
         }
+    };
+    const auto hold_scale = [&](int i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            scale[i][j] = 1.0f;
+        }
         if (MODE == kNormFront && f.scale != nullptr) {
             norm_columns<T>(f.scale, f32, col0, lane + i * G, len, scale[i]);
+        }
+    };
+    if constexpr (kHold) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            hold(i);
+            hold_scale(i);
         }
     }
 
@@ -531,6 +575,9 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
             if constexpr (MODE == kNormFront) {
                 norm_unpack<R>(now.s[i], n[i]);
                 if constexpr (!kFromSum) {
+                    if constexpr (!kHold) {
+                        hold_scale(i);
+                    }
                     float v[8];
                     norm_unpack<T>(now.x[i], v);
 #pragma unroll
@@ -550,6 +597,9 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             float d[8];
+            if constexpr (!kHold) {
+                hold(i);
+            }
             if constexpr (kGradR) {
                 norm_unpack<R>(now.d[i], d);
                 float u[8], dg[8];
@@ -588,11 +638,16 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
                 g[i][j] = d[j] * gamma[i][j];
             }
             // (sums take a lane's own values: what another lane has too, or lies past the row, must not reach them, NaN least of all)
+            float dn[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                dn[j] = d[j] * n[i][j];
+            }
+            add(d_gamma, 0, i, dn);
+            add(d_beta, 1, i, d);
             if (full) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    d_gamma[i][j] = __builtin_fmaf(d[j], n[i][j], d_gamma[i][j]);
-                    d_beta[i][j] += d[j];
                     means[0] = __builtin_fmaf(g[i][j], n[i][j], means[0]);
                     means[1] += g[i][j];
                 }
@@ -600,8 +655,6 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const bool mine = j >= own[i];
-                    d_gamma[i][j] = __builtin_fmaf(d[j], n[i][j], d_gamma[i][j]);
-                    d_beta[i][j] += d[j];
                     means[0] += mine ? g[i][j] * n[i][j] : 0.0f;
                     means[1] += mine ? g[i][j] : 0.0f;
                 }
@@ -636,6 +689,9 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
                     }
                 }
                 if (a.x_grad != nullptr) {
+                    if constexpr (!kHold) {
+                        hold_scale(i);
+                    }
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         d[j] *= scale[i][j];
@@ -649,6 +705,17 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
     }
 
     // the sums over this workgroup's rows, kind by kind: a column from the lane whose own it is
+    if constexpr (!kHold) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float4 g4 = *acc_at(0, i, h), b4 = *acc_at(1, i, h);
+                d_gamma[i][4 * h] = g4.x, d_gamma[i][4 * h + 1] = g4.y, d_gamma[i][4 * h + 2] = g4.z, d_gamma[i][4 * h + 3] = g4.w;
+                d_beta[i][4 * h] = b4.x, d_beta[i][4 * h + 1] = b4.y, d_beta[i][4 * h + 2] = b4.z, d_beta[i][4 * h + 3] = b4.w;
+            }
+        }
+    }
     const auto put = [&](const float (&v)[NV][8], int kind) {
         float* const out = a.partial + (static_cast<int64_t>(kind) * a.slices + slice) * cols + col0;
         if constexpr (kRows > 1) {
