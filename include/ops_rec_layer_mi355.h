@@ -165,8 +165,8 @@ typedef struct gated_linear_params {
     void* hidden;       /* [rows, inner], same type, or NULL */
     void* mixed;        /* [rows, 3 * inner] words of 16 bits, or NULL; one of the two must be given */
     int64_t rows;
-    int64_t cols;  /* a multiple of 8, at most 2^22 */
-    int64_t inner; /* a multiple of 8, at most 2^22; inner * cols below 2^29 */
+    int64_t cols;  /* a multiple of 8, at most 2^21 */
+    int64_t inner; /* a multiple of 8, at most 2^21; inner * cols below 2^29 */
     int32_t dtype; /* HSTU_DT_BF16 or HSTU_DT_FP16 */
     uint32_t reserved0;
 } gated_linear_params;

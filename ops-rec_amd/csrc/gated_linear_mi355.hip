@@ -17,7 +17,7 @@ static_assert(OPS_REC_ACT_SILU == hstu::kActSilu && OPS_REC_ACT_GELU == hstu::kA
 
 constexpr int64_t kStep = 32;          // of a product's depth
 constexpr int64_t kFewRows = 64;       // of a workgroup of the kernel for few rows
-constexpr int64_t kMostCols = 1 << 22; // (128 rows of twice as many columns lie behind one descriptor)
+constexpr int64_t kMostCols = 1 << 21; // (256 rows of twice as many columns lie behind one descriptor of 2^31 bytes)
 constexpr int64_t kMostBytes = int64_t{1} << 31;  // behind one descriptor
 
 const hstu::GatedKernels& kernels_of(int dtype) { return dtype == HSTU_DT_BF16 ? hstu::gated_kernels_bf16() : hstu::gated_kernels_f16(); }
@@ -51,7 +51,7 @@ int validate(const gated_linear_params* p)
     }
     if (p->cols < 8 || p->cols % 8 != 0 || p->inner < 8 || p->inner % 8 != 0 || p->cols > kMostCols || p->inner > kMostCols ||
         p->inner * p->cols >= (int64_t{1} << 29)) {
-        return set_error(HSTU_ERR_INVALID, "the columns of x and hidden must be multiples of 8, at most 2^22, with a product below 2^29 (got %lld and %lld)",
+        return set_error(HSTU_ERR_INVALID, "the columns of x and hidden must be multiples of 8, at most 2^21, with a product below 2^29 (got %lld and %lld)",
                          static_cast<long long>(p->cols), static_cast<long long>(p->inner));
     }
     for (const void* t : {p->x, p->weight, p->bias, static_cast<const void*>(p->hidden), static_cast<const void*>(p->mixed)}) {

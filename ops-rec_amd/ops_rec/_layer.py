@@ -374,7 +374,7 @@ def _rotary_grad(ctx, q_grad, k_grad):
 # --------------------------------------------------------------------------------------- gated projections ----
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2}
-MAX_GATED_COLUMNS = 1 << 22
+MAX_GATED_COLUMNS = 1 << 21
 
 
 def _gated_linear_checks(x, weight, bias, activation) -> None:
@@ -386,7 +386,7 @@ def _gated_linear_checks(x, weight, bias, activation) -> None:
     cols, inner = x.size(1), weight.size(0) // 2
     _check(weight.size(0) % 2 == 0 and weight.size(1) == cols, f"weight must be [2 * inner, {cols}], but it is {list(weight.shape)}")
     _check(8 <= cols <= MAX_GATED_COLUMNS and cols % 8 == 0 and 8 <= inner <= MAX_GATED_COLUMNS and inner % 8 == 0 and inner * cols < 1 << 29,
-           f"the columns of x and of hidden must be multiples of 8, at most 2^22, with a product below 2^29, but they are {cols} and {inner}")  # fmt: skip
+           f"the columns of x and of hidden must be multiples of 8, at most 2^21, with a product below 2^29, but they are {cols} and {inner}")  # fmt: skip
     _check(x.size(0) < 1 << 31, f"at most 2^31 - 1 rows, but there are {x.size(0)}")
     if bias is not None:
         _check(bias.dim() == 1 and bias.numel() == 2 * inner, f"bias must have 2 * inner elements ({2 * inner}), but it is {list(bias.shape)}")

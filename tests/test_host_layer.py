@@ -145,6 +145,7 @@ def test_refusals_of_gated_linear():
         (lambda: call(x, w[:24]), "multiples of 8"),
         (lambda: call(odd, torch.zeros(32, 20).half()), "multiples of 8"),
         (lambda: call(x[:, :0], w[:, :0]), "multiples of 8"),
+        (lambda: call(torch.zeros(2, 8).half(), torch.zeros(2 * ((1 << 21) + 8), 8).half()), "at most 2\\^21"),
         (lambda: call(x, w, b[:31]), "bias must have 2 \\* inner elements"),
         (lambda: call(x, w, b.float()), "bias must have the dtype of x"),
         (lambda: call(x, w, b), "x must be a GPU tensor"),
@@ -215,7 +216,7 @@ def _gated_params():
     [
         ("gated_linear_fwd", _gated_params,
          [("struct_size", 4, 161002), ("x", None, 161001), ("weight", None, 161001), ("hidden", None, 161001), ("rows", 0, 161002), ("cols", 60, 161002),
-          ("inner", 0, 161002), ("inner", 1 << 23, 161002), ("cols", 1 << 23, 161002), ("dtype", _native.DT_FP32, 161002),
+          ("inner", 0, 161002), ("inner", (1 << 21) + 8, 161002), ("cols", (1 << 21) + 8, 161002), ("dtype", _native.DT_FP32, 161002),
           ("activation", 3, 161002), ("activation", -1, 161002), ("x", 0x1008, 161002), ("bias", 0x1002, 161002)]),
         ("residual_norm_fwd", _norm_params,
          [("struct_size", 4, 161002), ("x", None, 161001), ("residual", None, 161001), ("gamma", None, 161001), ("y", None, 161001), ("sum", None, 161001),
