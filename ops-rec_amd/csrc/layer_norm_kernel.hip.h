@@ -254,7 +254,8 @@ __device__ __forceinline__ float normalise(float (&s)[NV][8], const int (&own)[N
     });
     row_sums<G>(sq, s_part, slot);
     const float shift = rms ? 0.0f : sq[1] * inv_n;
-    const float rstd = 1.0f / sqrtf(fmaxf(sq[0] * inv_n - shift * shift, 0.0f) + epsilon);
+    const float size = sq[0] * inv_n - shift * shift;
+    const float rstd = 1.0f / sqrtf((size < 0.0f ? 0.0f : size) + epsilon);  // (NaN stays: a row with one has no root mean square)
     const float away = -shift * rstd;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {

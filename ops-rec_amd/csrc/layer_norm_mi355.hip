@@ -72,6 +72,8 @@ const NormVariant* variant_for(int dtype, int stream_dtype, int64_t len)
     return v;
 }
 
+constexpr int64_t kMostCols = 1 << 20;  // (a launch has less than 2^32 threads: a workgroup per part of a row, or per 16 columns of the sums)
+
 int check_common(int64_t rows, int64_t cols, int64_t groups, int dtype, int stream_dtype, int affine_dtype, float epsilon)
 {
     if (rows < 1 || cols < 1) {
@@ -92,8 +94,9 @@ int check_common(int64_t rows, int64_t cols, int64_t groups, int dtype, int stre
     if (cols / groups > hstu::kNormMaxLen) {
         return set_error(HSTU_ERR_INVALID, "at most %d columns share a mean (got %lld)", hstu::kNormMaxLen, static_cast<long long>(cols / groups));
     }
-    if (cols > 0x7fffffff || rows > 0x7fffffff / groups) {
-        return set_error(HSTU_ERR_INVALID, "rows * groups and columns must stay below 2^31");
+    if (cols > kMostCols || rows > 0x7fffffff / groups) {
+        return set_error(HSTU_ERR_INVALID, "at most 2^20 columns, and rows * groups below 2^31 (got %lld, and %lld rows)", static_cast<long long>(cols),
+                         static_cast<long long>(rows));
     }
     if (!(epsilon >= 0.0f)) {
         return set_error(HSTU_ERR_INVALID, "epsilon must not be negative");

@@ -24,6 +24,7 @@ from ._ops import _DTYPE_CODE, _PYTHON_KERNELS, _check, _lib_def, _lib_meta, _pt
 from ._paged_fp8 import _aligned, _call
 
 NORM_MAX_LEN = 16384  # columns that share a mean, at most
+MAX_NORM_COLUMNS = 1 << 20
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 _lib_def.define("residual_norm(Tensor x, Tensor residual, Tensor gamma, Tensor? beta=None, Tensor? scale=None, float epsilon=1e-5, bool rms=False) -> "
@@ -62,11 +63,12 @@ def _dense(t: Optional[torch.Tensor]):
 def _norm_shapes(x, gamma, beta, epsilon, groups, **planes) -> None:
     _check(x.dim() == 2, "The x should be 2D")
     _check(x.dtype in _FLOATS, f"unsupported dtype {x.dtype}")
-    _check(x.size(1) > 0, "x must have columns")
+    _check(0 < x.size(1) <= MAX_NORM_COLUMNS, f"x must have columns, at most 2^20, but it is {list(x.shape)}")
     for name, t in planes.items():
         _check(t is None or t.shape == x.shape, f"{name} must have the shape of x ({list(x.shape)}), but it is {list(getattr(t, 'shape', ()))}")
     _check(int(groups) >= 1 and x.size(1) % int(groups) == 0, f"the columns ({x.size(1)}) must be a multiple of groups, but groups is {groups}")
     _check(x.size(1) // int(groups) <= NORM_MAX_LEN, f"at most {NORM_MAX_LEN} columns share a mean, but there are {x.size(1) // int(groups)}")
+    _check(x.size(0) * int(groups) < 1 << 31, f"rows * groups must stay below 2^31, but there are {x.size(0)} rows and {groups} groups")
     _check(float(epsilon) >= 0.0, f"epsilon must not be negative, but it is {epsilon}")
 
 

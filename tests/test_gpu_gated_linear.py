@@ -128,6 +128,32 @@ def test_every_tile_of_the_forward():
     assert len(seen) == 5, seen
 
 
+def test_the_widest():
+    """2^21 columns, where a tile's rows of d_mixed fill a descriptor; a gradient on a few columns alone, so that these are what the sums are made of."""
+    rows, inner = 260, 1 << 21
+    g = torch.Generator().manual_seed(3)
+    x, weight = torch.randn(rows, 8, generator=g).to(BF16), torch.zeros(2 * inner, 8, dtype=BF16)
+    some = torch.tensor([0, 1, 255, 70000, inner // 2 - 1, inner // 2, inner - 256, inner - 1])
+    both = torch.cat([some, some + inner])
+    weight[both] = torch.randn(16, 8, generator=g).to(BF16)
+    dh = torch.randn(rows, 8, generator=g).to(BF16)
+    wide = torch.zeros(rows, inner, dtype=BF16, device=DEV)
+    wide[:, some.to(DEV)] = dh.to(DEV)
+    leaves = [x.to(DEV).requires_grad_(True), weight.to(DEV).requires_grad_(True)]
+    hidden = A.gated_linear(*leaves, None, "silu", True)[0]
+    dx, dw = torch.autograd.grad(hidden, leaves, wide)
+    x64, w64, dh64 = x.double(), weight[both].double(), dh.double()
+    gate, up = (x64 @ w64.t()).chunk(2, dim=1)
+    s = torch.sigmoid(gate)
+    compare(hidden.detach()[:, some.to(DEV)], gate * s * up, 2.0**-17 * (x64.abs() @ w64.abs().t()).max() * (gate.abs() + up.abs()), "hidden")
+    d = torch.cat([dh64 * up * s * (1 + gate * (1 - s)), dh64 * gate * s], dim=1)
+    room = 2.0**-8 * d.abs() + 2.0**-13 * d.abs().max()  # (its rounding; g and u are cut by 2^-15 of them at most, and off by their sums)
+    compare(dx, d @ w64, room @ w64.abs() + 2.0**-18 * (d.abs() @ w64.abs()), "x")
+    compare(dw[both.to(DEV)], d.t() @ x64, room.t() @ x64.abs() + 2.0**-18 * (d.t().abs() @ x64.abs()), "weight")
+    dw[both.to(DEV)] = 0
+    assert torch.count_nonzero(dw) == 0
+
+
 def test_values_far_out():
     # gates whose exponentials overflow and underflow, and that are not finite
     x = torch.eye(8, dtype=BF16, device=DEV)

@@ -165,6 +165,19 @@ def test_a_row_that_is_not_finite_stays_alone(cols):
         assert torch.equal(db[1][rest], back[1][rest]) and torch.isnan(db[1][4]).all()
 
 
+@pytest.mark.parametrize("cols", [7, 64, 1002, 8200])
+def test_a_row_with_nan_has_no_root_mean_square(cols):
+    g = torch.Generator().manual_seed(cols)
+    x, gamma = randn(g, 5, cols, dtype=BF16).to(DEV), randn(g, cols).to(DEV)
+    x[2, cols // 2] = float("nan")
+    y, total = A.residual_norm(x, x, gamma, rms=True)
+    assert torch.isnan(y[2]).all() and torch.isfinite(y[[0, 1, 3, 4]]).all() and int(torch.isnan(total).sum()) == 1
+    assert torch.isnan(A.norm_gate(x, None, gamma, rms=True)[2]).all()
+    x[2, cols // 2] = float("inf")
+    y = A.norm_gate(x, None, gamma, rms=True)
+    assert int(torch.isnan(y[2]).sum()) == 1 and torch.count_nonzero(y[2]) == 1  # inf / inf there, the others' share is 0
+
+
 def test_rows_of_equal_values():
     gamma, beta = torch.full((64,), 2.0, device=DEV), torch.full((64,), 0.5, device=DEV)
     x = torch.tensor([0.0, 1.0, -3.5, 1000.0], device=DEV)[:, None].repeat(1, 64)

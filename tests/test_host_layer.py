@@ -95,6 +95,8 @@ def test_refusals_of_the_norms():
         (lambda: gate(x, x.half(), g), "gate must have the dtype of x"),
         (lambda: gate(x, x, g, None, None, 1.0, 5), "multiple of groups"),
         (lambda: gate(x, x, g, None, None, 1.0, 0), "multiple of groups"),
+        (lambda: gate(torch.zeros(1, (1 << 20) + 8), None, g, None, None, 1.0, 128), "at most 2\\^20"),
+        (lambda: gate(torch.zeros(1, 1).expand(1 << 27, 16), None, g, None, None, 1.0, 16), "rows \\* groups must stay below"),
         (lambda: gate(x.half(), None, g, None, x.bfloat16()), "residual must be float32 or of the dtype of x"),
         (lambda: gate(x, None, g), "x must be a GPU tensor"),
         (lambda: _layer.norm_gate_backward(x, x.half(), None, g, None, False, 1.0, 1, 1e-5, False, False), "grad must have the dtype of x"),
@@ -223,7 +225,7 @@ def _gated_params():
           ("rows", 0, 161002), ("cols", 0, 161002), ("cols", 16385, 161002), ("rows", 1 << 31, 161002), ("x_stride", -1, 161002), ("dtype", 3, 161002),
           ("stream_dtype", _native.DT_FP16, 161002), ("affine_dtype", _native.DT_FP16, 161002), ("epsilon", -1.0, 161002), ("epsilon", math.nan, 161002)]),
         ("norm_gate_fwd", _gate_params,
-         [("struct_size", 4, 161002), ("x", None, 161001), ("gamma", None, 161001), ("out", None, 161001), ("groups", 0, 161002), ("groups", 5, 161002),
+         [("struct_size", 4, 161002), ("x", None, 161001), ("gamma", None, 161001), ("out", None, 161001), ("groups", 0, 161002), ("groups", 5, 161002), ("cols", 1 << 22, 161002),
           ("stream_dtype", _native.DT_FP32, 161002), ("gate_stride", -8, 161002), ("rows", 1 << 30, 161002)]),
         ("rotary_fwd", _rotary_params,
          [("struct_size", 4, 161002), ("q", None, 161001), ("frequencies", None, 161001), ("seq_offset", None, 161002), ("positions", 0x1000, 161002),
