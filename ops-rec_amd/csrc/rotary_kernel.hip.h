@@ -8,7 +8,7 @@
 // pieces of pairs that lie side by side, half of the turned values apart, so that neighbouring threads have neighbouring pieces either way -- and turns them in
 // several heads of q and k: a sine and a cosine serve them all.  Short batches give each thread fewer heads, down to one, and pay the sines again for more
 // threads.  Values of a head past its pairs are copied by threads of their own, two pieces each.  Pieces start anywhere (16-byte accesses need no
-// alignment here); a part-filled last piece goes value by value.
+// alignment here); a last piece that is not whole starts earlier.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -20,7 +20,7 @@ namespace hstu {
 constexpr int kRotaryThreads = 256;
 constexpr int kRotaryHeads = 8;  // heads of a thread, at most: their loads are all in flight while the row's place and its sines are worked out
 
-// ---- 16 bytes of a row of n values: those that are there, the others undefined ----
+// ---- 16 bytes of a row of n values, from `first` on; of a row of fewer values, those that are there, the others undefined ----
 template <typename Tag>
 struct rotary_piece {
     typedef uint32_t words_t __attribute__((ext_vector_type(4), aligned(2)));
@@ -28,10 +28,12 @@ struct rotary_piece {
     using elem_t = typename ln_traits<Tag>::elem_t;
     words_t w;
 
-    __device__ __forceinline__ void load(const elem_t* row, int c, int n)
+    // where piece c starts: the last, where it is not whole, is the row's last values, some of which the piece before has too (the same bits twice), and
+    // a piece past the row is that one again
+    static __device__ __forceinline__ int place(int c, int n) { return n >= kValues ? min(c * kValues, n - kValues) : c * kValues; }
+    __device__ __forceinline__ void load(const elem_t* row, int first, int n)
     {
-        const int first = c * kValues;
-        if (first + kValues <= n) {
+        if (n >= kValues) {
             w = __builtin_nontemporal_load(reinterpret_cast<const words_t*>(row + first));
         } else {
             elem_t e[kValues];
@@ -43,12 +45,15 @@ struct rotary_piece {
         }
     }
     __device__ __forceinline__ void unpack(float (&f)[kValues]) const { ln_traits<Tag>::unpack(w, f); }
-    static __device__ __forceinline__ void store(elem_t* row, int c, int n, const float (&f)[kValues])
+    static __device__ __forceinline__ void store(elem_t* row, int first, int n, const float (&f)[kValues], bool streamed)
     {
-        const int first = c * kValues;
-        if (first + kValues <= n) {
+        if (n >= kValues) {
             const words_t packed = ln_traits<Tag>::pack(f);
-            __builtin_nontemporal_store(packed, reinterpret_cast<words_t*>(row + first));
+            if (streamed) {
+                __builtin_nontemporal_store(packed, reinterpret_cast<words_t*>(row + first));
+            } else {
+                *reinterpret_cast<words_t*>(row + first) = packed;
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < kValues; ++i) {
@@ -127,7 +132,8 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
     const bool copied = item >= a.turned;
     const int rest0 = item - a.turned;
     const int begin = copied ? 2 * a.pairs : 0, n = copied ? a.dim - begin : INTERLEAVED ? 2 * a.pairs : a.pairs;
-    const int c0 = copied ? rest0 : item, c1 = copied ? rest0 + a.items - a.turned : INTERLEAVED ? item + a.turned : item;
+    const int c0 = rotary_piece<T>::place(copied ? rest0 : item, n);
+    const int c1 = rotary_piece<T>::place(copied ? rest0 + a.items - a.turned : INTERLEAVED ? item + a.turned : item, n);
     const int apart = copied || INTERLEAVED ? 0 : a.pairs;
     rotary_piece<T> lo[kRotaryHeads], hi[kRotaryHeads];
 #pragma unroll
@@ -160,7 +166,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
     if (!copied) {
 #pragma unroll
         for (int j = 0; j < kValues; ++j) {
-            const int at = INTERLEAVED ? (j < kValues / 2 ? c0 : c1) * (kValues / 2) + j % (kValues / 2) : c0 * kValues + j;
+            const int at = INTERLEAVED ? (j < kValues / 2 ? c0 : c1) / 2 + j % (kValues / 2) : c0 + j;
             double turns = position * a.frequencies[min(at, a.pairs - 1)] * 0.15915494309189533577;  // 1 / (2 pi)
             turns -= rint(turns);
             rotary_turn<T>(static_cast<float>(turns), cs[j], sn[j]);
@@ -202,8 +208,8 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
                 }
             }
             E* const p = to(first + i) + begin;
-            rotary_piece<T>::store(p, c0, n, u);
-            rotary_piece<T>::store(p + apart, c1, n, v);
+            rotary_piece<T>::store(p, c0, n, u, a.streamed);
+            rotary_piece<T>::store(p + apart, c1, n, v, a.streamed);
         }
     }
 }

@@ -12,6 +12,13 @@ DEV = "cuda:0"
 ACT, ATT = ops_rec.ascendc.activation, ops_rec.ascendc.attention
 
 
+@pytest.fixture(autouse=True)
+def _memory_goes_back():
+    """Cached blocks go back to the device after each test: tests that count what the allocator takes find it as they expect it."""
+    yield
+    torch.cuda.empty_cache()
+
+
 def weights(cols, heads, dim, inner, dtype, seed):
     g = torch.Generator().manual_seed(seed)
     hd = heads * dim

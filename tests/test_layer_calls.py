@@ -18,6 +18,13 @@ GRAPH = CHECKS + ("test_autograd_registration",)
 BACKENDS = ["aot_eager", "inductor"]
 
 
+@pytest.fixture(autouse=True)
+def _memory_goes_back():
+    """Cached blocks go back to the device after each test: tests that count what the allocator takes find it as they expect it."""
+    yield
+    torch.cuda.empty_cache()
+
+
 def randn(seed, *shape, dtype=FP32, std=1.0, mean=0.0):
     return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * std + mean).to(dtype).to(DEV)
 
