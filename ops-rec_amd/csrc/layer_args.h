@@ -75,7 +75,6 @@ struct RotaryArgs {
     int head_blocks;  // threads that share a row and its pairs
     int turned, items;  // threads of a head: with pairs to turn, and with those that copy
     int positions64, offsets64, start64;
-    int streamed;  // stores past the caches
     float magnitude;
     float sign;  // of sin
 };

@@ -20,8 +20,13 @@ namespace hstu {
 constexpr int kRotaryThreads = 256;
 constexpr int kRotaryHeads = 8;  // heads of a thread, at most: their loads are all in flight while the row's place and its sines are worked out
 
-// ---- 16 bytes of a row of n values, from `first` on; of a row of fewer values, those that are there, the others undefined ----
-template <typename Tag>
+// Stores that fill whole 128-byte lines go past the caches (kRotaryLines), others do not: there a line's parts meet before it is written (65536 rows of 8 + 8
+// heads of 96 values, 64 of them turned, bf16: 135 us past the caches, 103 through them; 20292 rows of 4 + 4 heads, halves of 64 values, 18.3 and 20.2).
+// Heads with runs of fewer values than a piece have (kRotaryShort) ask for them one by one.
+constexpr int kRotaryLines = 0, kRotaryPieces = 1, kRotaryShort = 2;
+
+// ---- 16 bytes of a run of n values, from `first` on; of a shorter run those that are there, the others undefined ----
+template <typename Tag, int KIND>
 struct rotary_piece {
     typedef uint32_t words_t __attribute__((ext_vector_type(4), aligned(2)));
     static constexpr int kValues = ln_traits<Tag>::kPerChunk;
@@ -30,35 +35,37 @@ struct rotary_piece {
 
     // where piece c starts: the last, where it is not whole, is the row's last values, some of which the piece before has too (the same bits twice), and
     // a piece past the row is that one again
-    static __device__ __forceinline__ int place(int c, int n) { return n >= kValues ? min(c * kValues, n - kValues) : c * kValues; }
-    __device__ __forceinline__ void load(const elem_t* row, int first, int n)
+    static __device__ __forceinline__ bool whole(int n) { return KIND != kRotaryShort || n >= kValues; }
+    static __device__ __forceinline__ int place(int c, int n) { return whole(n) ? min(c * kValues, n - kValues) : c * kValues; }
+    // `at`: where the piece starts in the head
+    __device__ __forceinline__ void load(const elem_t* head, int at, int first, int n)
     {
-        if (n >= kValues) {
-            w = __builtin_nontemporal_load(reinterpret_cast<const words_t*>(row + first));
+        if (whole(n)) {
+            w = __builtin_nontemporal_load(reinterpret_cast<const words_t*>(head + at));
         } else {
             elem_t e[kValues];
 #pragma unroll
             for (int i = 0; i < kValues; ++i) {
-                e[i] = first + i < n ? row[first + i] : static_cast<elem_t>(0.0f);
+                e[i] = first + i < n ? head[at + i] : static_cast<elem_t>(0.0f);
             }
             __builtin_memcpy(&w, e, sizeof w);
         }
     }
     __device__ __forceinline__ void unpack(float (&f)[kValues]) const { ln_traits<Tag>::unpack(w, f); }
-    static __device__ __forceinline__ void store(elem_t* row, int first, int n, const float (&f)[kValues], bool streamed)
+    static __device__ __forceinline__ void store(elem_t* head, int at, int first, int n, const float (&f)[kValues])
     {
-        if (n >= kValues) {
+        if (whole(n)) {
             const words_t packed = ln_traits<Tag>::pack(f);
-            if (streamed) {
-                __builtin_nontemporal_store(packed, reinterpret_cast<words_t*>(row + first));
+            if constexpr (KIND == kRotaryLines) {
+                __builtin_nontemporal_store(packed, reinterpret_cast<words_t*>(head + at));
             } else {
-                *reinterpret_cast<words_t*>(row + first) = packed;
+                *reinterpret_cast<words_t*>(head + at) = packed;
             }
         } else {
 #pragma unroll
             for (int i = 0; i < kValues; ++i) {
                 if (first + i < n) {
-                    row[first + i] = static_cast<elem_t>(f[i]);
+                    head[at + i] = static_cast<elem_t>(f[i]);
                 }
             }
         }
@@ -104,7 +111,7 @@ __device__ __forceinline__ void rotary_turn(float turns, float& c, float& s)
     }
 }
 
-template <typename T, bool INTERLEAVED>
+template <typename T, bool INTERLEAVED, int KIND>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs a)
 {
     using E = typename ln_traits<T>::elem_t;
@@ -127,21 +134,22 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
                              : static_cast<E*>(a.k_out) + (static_cast<int64_t>(row) * (a.heads - a.heads_q) + (h - a.heads_q)) * a.dim;
     };
 
-    constexpr int kValues = rotary_piece<T>::kValues;
+    using Piece = rotary_piece<T, KIND>;
+    constexpr int kValues = Piece::kValues;
     // turned values: side by side pieces `item` and `item + turned` of all of them, halves piece `item` of each; copied values: two pieces of the rest
     const bool copied = item >= a.turned;
     const int rest0 = item - a.turned;
     const int begin = copied ? 2 * a.pairs : 0, n = copied ? a.dim - begin : INTERLEAVED ? 2 * a.pairs : a.pairs;
-    const int c0 = rotary_piece<T>::place(copied ? rest0 : item, n);
-    const int c1 = rotary_piece<T>::place(copied ? rest0 + a.items - a.turned : INTERLEAVED ? item + a.turned : item, n);
-    const int apart = copied || INTERLEAVED ? 0 : a.pairs;
-    rotary_piece<T> lo[kRotaryHeads], hi[kRotaryHeads];
+    const int c0 = Piece::place(copied ? rest0 : item, n);
+    const int c1 = Piece::place(copied ? rest0 + a.items - a.turned : INTERLEAVED ? item + a.turned : item, n);
+    const int at0 = begin + c0, at1 = begin + c1 + (copied || INTERLEAVED ? 0 : a.pairs);
+    Piece lo[kRotaryHeads], hi[kRotaryHeads];
 #pragma unroll
     for (int i = 0; i < kRotaryHeads; ++i) {
         if (first + i < last) {
-            const E* const p = from(first + i) + begin;
-            lo[i].load(p, c0, n);
-            hi[i].load(p + apart, c1, n);
+            const E* const p = from(first + i);
+            lo[i].load(p, at0, c0, n);
+            hi[i].load(p, at1, c1, n);
         }
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -207,9 +215,9 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
                     v[j] = 0.0f;
                 }
             }
-            E* const p = to(first + i) + begin;
-            rotary_piece<T>::store(p, c0, n, u, a.streamed);
-            rotary_piece<T>::store(p + apart, c1, n, v, a.streamed);
+            E* const p = to(first + i);
+            Piece::store(p, at0, c0, n, u);
+            Piece::store(p, at1, c1, n, v);
         }
     }
 }

@@ -13,15 +13,20 @@ using hstu::set_error;
 
 typedef void (*kernel_t)(const RotaryArgs);
 
-kernel_t kernel_for(int dtype, bool interleaved)
+template <typename T>
+kernel_t kernel_for(bool interleaved, int kind)
 {
-    if (dtype == HSTU_DT_FP32) {
-        return interleaved ? hstu::rotary_kernel<hstu::ln_f32_tag, true> : hstu::rotary_kernel<hstu::ln_f32_tag, false>;
-    }
-    if (dtype == HSTU_DT_BF16) {
-        return interleaved ? hstu::rotary_kernel<hstu::ln_bf16_tag, true> : hstu::rotary_kernel<hstu::ln_bf16_tag, false>;
-    }
-    return interleaved ? hstu::rotary_kernel<hstu::ln_f16_tag, true> : hstu::rotary_kernel<hstu::ln_f16_tag, false>;
+    using namespace hstu;
+    static const kernel_t table[2][3] = {{rotary_kernel<T, false, kRotaryLines>, rotary_kernel<T, false, kRotaryPieces>, rotary_kernel<T, false, kRotaryShort>},
+                                         {rotary_kernel<T, true, kRotaryLines>, rotary_kernel<T, true, kRotaryPieces>, rotary_kernel<T, true, kRotaryShort>}};
+    return table[interleaved ? 1 : 0][kind];
+}
+
+kernel_t kernel_for(int dtype, bool interleaved, int kind)
+{
+    return dtype == HSTU_DT_FP32   ? kernel_for<hstu::ln_f32_tag>(interleaved, kind)
+           : dtype == HSTU_DT_BF16 ? kernel_for<hstu::ln_bf16_tag>(interleaved, kind)
+                                   : kernel_for<hstu::ln_f16_tag>(interleaved, kind);
 }
 
 int validate(const rotary_params* p)
@@ -96,10 +101,6 @@ extern "C" HSTU_API int rotary_fwd(const rotary_params* p, void* stream)
     const int values = static_cast<int>(16 / size);
     a.turned = p->interleaved ? ((2 * a.pairs + values - 1) / values + 1) / 2 : (a.pairs + values - 1) / values;
     a.items = a.turned + ((a.dim - 2 * a.pairs + values - 1) / values + 1) / 2;
-    // Stores that fill whole 128-byte lines go past the caches, others do not: there the line's parts meet before it is written (65536 rows of 8 + 8 heads,
-    // 96 values, 64 of them turned, bf16: 135 us past the caches, 103 through them; 64 of 128 values a half 18.3 and 20.2 for 20292 rows of 4 + 4)
-    const int64_t run = p->interleaved ? static_cast<int64_t>(a.turned) * 16 : a.pairs * size;
-    a.streamed = run % 128 == 0 && a.dim * size % 128 == 0 && reinterpret_cast<uintptr_t>(p->q_out) % 128 == 0 && reinterpret_cast<uintptr_t>(p->k_out) % 128 == 0;
     a.positions64 = p->positions_dtype == HSTU_IDX_I64;
     a.offsets64 = p->seq_offset_dtype == HSTU_IDX_I64;
     a.start64 = p->start_dtype == HSTU_IDX_I64;
@@ -113,7 +114,12 @@ extern "C" HSTU_API int rotary_fwd(const rotary_params* p, void* stream)
     }
     a.heads_each = (heads + a.head_blocks - 1) / a.head_blocks;
     a.head_blocks = (heads + a.heads_each - 1) / a.heads_each;
-    const kernel_t kernel = kernel_for(p->dtype, p->interleaved != 0);
+    // runs of values that are turned, and those that are copied; whether all stores of 16 bytes fill whole lines
+    const int64_t turned = p->interleaved ? 2 * p->pairs : p->pairs, copied = p->dim - 2 * p->pairs;
+    const int64_t run = p->interleaved ? static_cast<int64_t>(a.turned) * 16 : turned * size;
+    const bool lines = run % 128 == 0 && a.dim * size % 128 == 0 && reinterpret_cast<uintptr_t>(p->q_out) % 128 == 0 && reinterpret_cast<uintptr_t>(p->k_out) % 128 == 0;
+    const bool shorter = turned < values || (copied > 0 && copied < values);
+    const kernel_t kernel = kernel_for(p->dtype, p->interleaved != 0, shorter ? hstu::kRotaryShort : lines ? hstu::kRotaryLines : hstu::kRotaryPieces);
     // (a launch numbers its threads in 32 bits)
     const int64_t most = (int64_t{1} << 31) / (static_cast<int64_t>(a.items) * a.head_blocks);
     for (int64_t row0 = 0; row0 < p->rows; row0 += most) {
