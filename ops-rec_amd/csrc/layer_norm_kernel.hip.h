@@ -54,8 +54,8 @@ struct norm_piece {
 
 // Piece c of a row of n values is columns 8 c .. + 7; the row's last piece, where it is not whole, is its last 8 columns, some of which the piece before has
 // too: every lane's access is one of 16 bytes, and what two lanes hold is stored twice, the same bits, and counted once (norm_own).  (A last
-// piece taken value by value cost rows of 1002 columns a quarter of the bandwidth.)  Rows of fewer than 8 values are such a piece that starts
-// ahead of the row, and do go value by value.  Pieces past the row repeat its last one, and count nowhere.
+// piece taken value by value cost rows of 1002 columns a quarter of the bandwidth.)  Rows of fewer than 8 values (SHORT) are such a piece that
+// starts ahead of the row, and do go value by value, in kernels of their own: with the choice at each load 8192 x 4096 took 46 us, 40 so.  Pieces past the row repeat its last one, and count nowhere.
 __device__ __forceinline__ int norm_base(int c, int n) { return 8 * c + 8 <= n ? 8 * c : n - 8; }
 // the first of a piece's values that is its own: 0 of a whole piece, 8 of a piece past the row
 __device__ __forceinline__ int norm_own(int c, int n)
@@ -64,12 +64,12 @@ __device__ __forceinline__ int norm_own(int c, int n)
     return left >= 8 ? 0 : 8 - (left > 0 ? left : 0);
 }
 
-template <typename Tag>
+template <typename Tag, bool SHORT>
 __device__ __forceinline__ norm_piece<Tag> norm_load(const typename ln_traits<Tag>::elem_t* row, int c, int n)
 {
     using E = typename ln_traits<Tag>::elem_t;
     norm_piece<Tag> p;
-    if (n >= 8) {
+    if constexpr (!SHORT) {
         const typename norm_piece<Tag>::words_t* at = reinterpret_cast<const typename norm_piece<Tag>::words_t*>(row + norm_base(c, n));
         p.w[0] = __builtin_nontemporal_load(at);
         if constexpr (sizeof(E) == 4) {
@@ -96,7 +96,7 @@ __device__ __forceinline__ void norm_unpack(const norm_piece<Tag>& p, float (&f)
     }
 }
 
-template <typename Tag>
+template <typename Tag, bool SHORT>
 __device__ __forceinline__ void norm_store(typename ln_traits<Tag>::elem_t* row, int c, int n, const float (&f)[8])
 {
     using T = ln_traits<Tag>;
@@ -104,7 +104,7 @@ __device__ __forceinline__ void norm_store(typename ln_traits<Tag>::elem_t* row,
     if (8 * c >= n) {
         return;
     }
-    if (n >= 8) {
+    if constexpr (!SHORT) {
         typename norm_piece<Tag>::words_t* at = reinterpret_cast<typename norm_piece<Tag>::words_t*>(row + norm_base(c, n));
 #pragma unroll
         for (int i = 0; i < 8 / T::kPerChunk; ++i) {
@@ -122,13 +122,13 @@ __device__ __forceinline__ void norm_store(typename ln_traits<Tag>::elem_t* row,
 }
 
 // 8 values per column (gamma, beta, scale)
-template <typename Tag>
+template <typename Tag, bool SHORT>
 __device__ __forceinline__ void norm_columns(const void* p, bool f32, int64_t offset, int c, int n, float (&f)[8])
 {
     if (f32) {
-        norm_unpack<ln_f32_tag>(norm_load<ln_f32_tag>(static_cast<const float*>(p) + offset, c, n), f);
+        norm_unpack<ln_f32_tag>(norm_load<ln_f32_tag, SHORT>(static_cast<const float*>(p) + offset, c, n), f);
     } else {
-        norm_unpack<Tag>(norm_load<Tag>(static_cast<const typename ln_traits<Tag>::elem_t*>(p) + offset, c, n), f);
+        norm_unpack<Tag>(norm_load<Tag, SHORT>(static_cast<const typename ln_traits<Tag>::elem_t*>(p) + offset, c, n), f);
     }
 }
 
@@ -270,7 +270,7 @@ __device__ __forceinline__ float normalise(float (&s)[NV][8], const int (&own)[N
 // T = type of x (and of y, gate), R = type of the stream; U = parts of rows whose loads are in flight together.  Lanes stay with their columns: from part to
 // part they move on by the lanes of the whole grid, a multiple of the parts of a row, and hold gamma, beta and scale in registers.  (Loaded for every row
 // again they were half of the kernel's requests: 65536 x 1024 with a gate 99 us, 76 so.)
-template <typename T, typename R, int MODE, int G, int NV, int U>
+template <typename T, typename R, int MODE, int G, int NV, int U, bool SHORT>
 __global__ __launch_bounds__(norm_fwd_threads(G)) void norm_fwd_kernel(const NormArgs a)
 {
     static_assert(G <= 64 || U == 1, "lanes that share barriers have one row");
@@ -302,12 +302,12 @@ __global__ __launch_bounds__(norm_fwd_threads(G)) void norm_fwd_kernel(const Nor
                 beta[i][j] = 0.0f;
                 scale[i][j] = 1.0f;
             }
-            norm_columns<T>(a.gamma, f32, col0, c, len, gamma[i]);
+            norm_columns<T, SHORT>(a.gamma, f32, col0, c, len, gamma[i]);
             if (a.beta != nullptr) {
-                norm_columns<T>(a.beta, f32, col0, c, len, beta[i]);
+                norm_columns<T, SHORT>(a.beta, f32, col0, c, len, beta[i]);
             }
             if (MODE == kNormFront && a.scale != nullptr) {
-                norm_columns<T>(a.scale, f32, col0, c, len, scale[i]);
+                norm_columns<T, SHORT>(a.scale, f32, col0, c, len, scale[i]);
             }
         }
     };
@@ -327,20 +327,20 @@ __global__ __launch_bounds__(norm_fwd_threads(G)) void norm_fwd_kernel(const Nor
                 const TE* const x = static_cast<const TE*>(a.x) + static_cast<int64_t>(row) * a.x_stride + col0;
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    xp[t][i] = norm_load<T>(x, lane + i * G, len);
+                    xp[t][i] = norm_load<T, SHORT>(x, lane + i * G, len);
                 }
                 if (MODE == kNormFront || a.residual != nullptr) {
                     const RE* const res = static_cast<const RE*>(a.residual) + static_cast<int64_t>(row) * a.residual_stride + col0;
 #pragma unroll
                     for (int i = 0; i < NV; ++i) {
-                        rp[t][i] = norm_load<R>(res, lane + i * G, len);
+                        rp[t][i] = norm_load<R, SHORT>(res, lane + i * G, len);
                     }
                 }
                 if (MODE == kNormBehind && a.gate != nullptr) {
                     const TE* const gate = static_cast<const TE*>(a.gate) + static_cast<int64_t>(row) * a.gate_stride + col0;
 #pragma unroll
                     for (int i = 0; i < NV; ++i) {
-                        gp[t][i] = norm_load<T>(gate, lane + i * G, len);
+                        gp[t][i] = norm_load<T, SHORT>(gate, lane + i * G, len);
                     }
                 }
             }
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(norm_fwd_threads(G)) void norm_fwd_kernel(const Nor
                     for (int j = 0; j < 8; ++j) {
                         s[i][j] = __builtin_fmaf(scale[i][j], s[i][j], f[j]);
                     }
-                    norm_store<R>(static_cast<RE*>(a.sum) + dense[t], lane + i * G, len, s[i]);
+                    norm_store<R, SHORT>(static_cast<RE*>(a.sum) + dense[t], lane + i * G, len, s[i]);
                 }
             }
             normalise<G, NV>(s, own, full, len, a.rms != 0, a.epsilon, s_part, slot);
@@ -403,16 +403,16 @@ __global__ __launch_bounds__(norm_fwd_threads(G)) void norm_fwd_kernel(const Nor
                             y[j] = __builtin_fmaf(a.residual_scale, y[j], f[j]);
                         }
                     }
-                    norm_store<R>(static_cast<RE*>(a.out) + dense[t], lane + i * G, len, y);
+                    norm_store<R, SHORT>(static_cast<RE*>(a.out) + dense[t], lane + i * G, len, y);
                 } else {
-                    norm_store<T>(static_cast<TE*>(a.out) + dense[t], lane + i * G, len, y);
+                    norm_store<T, SHORT>(static_cast<TE*>(a.out) + dense[t], lane + i * G, len, y);
                 }
             }
         }
     }
 }
 
-template <typename T, typename R, int MODE, int G, int NV>
+template <typename T, typename R, int MODE, int G, int NV, bool SHORT>
 __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const NormBwdArgs a)
 {
     using TE = typename ln_traits<T>::elem_t;
@@ -481,9 +481,9 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
         for (int j = 0; j < 8; ++j) {
             beta[i][j] = 0.0f;
         }
-        norm_columns<T>(f.gamma, f32, col0, lane + i * G, len, gamma[i]);
+        norm_columns<T, SHORT>(f.gamma, f32, col0, lane + i * G, len, gamma[i]);
         if (MODE == kNormBehind && f.beta != nullptr) {
-            norm_columns<T>(f.beta, f32, col0, lane + i * G, len, beta[i]);
+            norm_columns<T, SHORT>(f.beta, f32, col0, lane + i * G, len, beta[i]);
         }
     };
     const auto hold_scale = [&](int i) {
@@ -492,7 +492,7 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
             scale[i][j] = 1.0f;
         }
         if (MODE == kNormFront && f.scale != nullptr) {
-            norm_columns<T>(f.scale, f32, col0, lane + i * G, len, scale[i]);
+            norm_columns<T, SHORT>(f.scale, f32, col0, lane + i * G, len, scale[i]);
         }
     };
     if constexpr (kHold) {
@@ -514,7 +514,7 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
             const TE* const x = static_cast<const TE*>(f.x) + static_cast<int64_t>(row) * f.x_stride + col0;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                w.x[i] = norm_load<T>(x, lane + i * G, len);
+                w.x[i] = norm_load<T, SHORT>(x, lane + i * G, len);
             }
         }
         if constexpr (MODE == kNormFront) {
@@ -522,30 +522,30 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
                                             : static_cast<const RE*>(f.residual) + static_cast<int64_t>(row) * f.residual_stride + col0;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                w.s[i] = norm_load<R>(from, lane + i * G, len);
+                w.s[i] = norm_load<R, SHORT>(from, lane + i * G, len);
             }
             if (a.sum_grad != nullptr) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    w.d[i] = norm_load<R>(static_cast<const RE*>(a.sum_grad) + dense, lane + i * G, len);
+                    w.d[i] = norm_load<R, SHORT>(static_cast<const RE*>(a.sum_grad) + dense, lane + i * G, len);
                 }
             }
             if (a.grad != nullptr) {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    w.y[i] = norm_load<T>(static_cast<const TE*>(a.grad) + dense, lane + i * G, len);
+                    w.y[i] = norm_load<T, SHORT>(static_cast<const TE*>(a.grad) + dense, lane + i * G, len);
                 }
             }
         } else {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                w.d[i] = norm_load<R>(static_cast<const RE*>(a.grad) + dense, lane + i * G, len);
+                w.d[i] = norm_load<R, SHORT>(static_cast<const RE*>(a.grad) + dense, lane + i * G, len);
             }
             if (f.gate != nullptr) {
                 const TE* const gate = static_cast<const TE*>(f.gate) + static_cast<int64_t>(row) * f.gate_stride + col0;
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    w.gate[i] = norm_load<T>(gate, lane + i * G, len);
+                    w.gate[i] = norm_load<T, SHORT>(gate, lane + i * G, len);
                 }
             }
         }
@@ -623,7 +623,7 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
                     d[j] = dz * act;
                 }
                 if (f.gate != nullptr && a.gate_grad != nullptr) {
-                    norm_store<T>(static_cast<TE*>(a.gate_grad) + dense, lane + i * G, len, dg);
+                    norm_store<T, SHORT>(static_cast<TE*>(a.gate_grad) + dense, lane + i * G, len, dg);
                 }
             } else {
 #pragma unroll
@@ -680,7 +680,7 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
                         d[j] += v[j];
                     }
                 }
-                norm_store<R>(static_cast<RE*>(a.residual_grad) + dense, lane + i * G, len, d);
+                norm_store<R, SHORT>(static_cast<RE*>(a.residual_grad) + dense, lane + i * G, len, d);
                 if (a.want_scale) {
                     float v[8];
                     norm_unpack<T>(now.x[i], v);
@@ -697,10 +697,10 @@ __global__ __launch_bounds__(norm_bwd_threads(G)) void norm_bwd_kernel(const Nor
                     for (int j = 0; j < 8; ++j) {
                         d[j] *= scale[i][j];
                     }
-                    norm_store<T>(static_cast<TE*>(a.x_grad) + dense, lane + i * G, len, d);
+                    norm_store<T, SHORT>(static_cast<TE*>(a.x_grad) + dense, lane + i * G, len, d);
                 }
             } else if (a.x_grad != nullptr) {
-                norm_store<T>(static_cast<TE*>(a.x_grad) + dense, lane + i * G, len, d);
+                norm_store<T, SHORT>(static_cast<TE*>(a.x_grad) + dense, lane + i * G, len, d);
             }
         }
     }

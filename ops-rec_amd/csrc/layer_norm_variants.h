@@ -4,7 +4,7 @@
 
 namespace hstu {
 
-constexpr int kNormVariants = 9;
+constexpr int kNormVariants = 10;
 constexpr int kNormMaxLen = 16384;  // columns that share a mean, at most: the last variant's capacity
 
 struct NormVariant {
