@@ -55,7 +55,8 @@ struct norm_piece {
 // Piece c of a row of n values is columns 8 c .. + 7; the row's last piece, where it is not whole, is its last 8 columns, some of which the piece before has
 // too: every lane's access is one of 16 bytes, and what two lanes hold is stored twice, the same bits, and counted once (norm_own).  (A last
 // piece taken value by value cost rows of 1002 columns a quarter of the bandwidth.)  Rows of fewer than 8 values (SHORT) are such a piece that
-// starts ahead of the row, and do go value by value, in kernels of their own: with the choice at each load 8192 x 4096 took 46 us, 40 so.  Pieces past the row repeat its last one, and count nowhere.
+// starts ahead of the row, and do go value by value, in kernels of their own: with the choice at each load 8192 x 4096 took 46 us, 40 so.  Pieces
+// past the row repeat its last one, and count nowhere.
 __device__ __forceinline__ int norm_base(int c, int n) { return 8 * c + 8 <= n ? 8 * c : n - 8; }
 // the first of a piece's values that is its own: 0 of a whole piece, 8 of a piece past the row
 __device__ __forceinline__ int norm_own(int c, int n)
