@@ -163,7 +163,7 @@ typedef struct gated_linear_params {
     const void* weight; /* [2 * inner, cols], same type: the rows of g, then those of u */
     const void* bias;   /* [2 * inner], same type, or NULL for none */
     void* hidden;       /* [rows, inner], same type, or NULL */
-    void* mixed;        /* [rows, 3 * inner] words of 16 bits, or NULL; one of the two must be given */
+    void* mixed;        /* [rows, 3 * inner] words of 16 bits, or NULL; the forward writes one of the two at least */
     int64_t rows;
     int64_t cols;  /* a multiple of 8, at most 2^21 */
     int64_t inner; /* a multiple of 8, at most 2^21; inner * cols below 2^29 */
@@ -176,7 +176,8 @@ HSTU_API int gated_linear_fwd(const gated_linear_params* params, void* stream);
 /* name of the kernel variant gated_linear_fwd would launch, or NULL after an error */
 HSTU_API const char* gated_linear_fwd_kernel_name(const gated_linear_params* params);
 
-/* The gradients of gated_linear.  `fwd` describes the call as it was, with mixed as it was written (hidden is not read). */
+/* The gradients of gated_linear.  `fwd` describes the call as it was, with mixed as it was written (hidden is not read), or
+ * NULL: g and u are then multiplied again. */
 typedef struct gated_linear_bwd_params {
     uint32_t struct_size; /* sizeof(gated_linear_bwd_params), checked */
     uint32_t reserved0;

@@ -8,12 +8,13 @@ constexpr int kActSilu = 0, kActGelu = 1, kActSigmoid = 2;
 
 // gated_gemm_kernel (gated_linear_gemm.hip.h): out[rows, cols] = a . b over `depth`
 struct GatedGemmArgs {
-    const void* n_side;  // forward: the weight [2 inner, depth]; x gradient: the weight [depth, cols]; weight gradient: x [depth, cols]
-    const void* m_side;  // forward: x [rows, depth]; x gradient: d_mixed [rows, depth]; weight gradient: d_mixed [depth, rows]
-    const void* bias;    // forward: [2 cols], 16-bit, or nullptr
-    void* out;           // forward: hidden [rows, cols], or nullptr; gradients: [rows, cols]
+    const void* n_side;  // forward, d_mixed: the weight [2 inner, depth]; x gradient: the weight [depth, cols]; weight gradient: x [depth, cols]
+    const void* m_side;  // forward, d_mixed: x [rows, depth]; x gradient: d_mixed [rows, depth]; weight gradient: d_mixed [depth, rows]
+    const void* bias;    // forward, d_mixed: [2 cols], 16-bit, or nullptr
+    void* out;           // forward: hidden [rows, cols], or nullptr; d_mixed: [rows, 2 cols]; gradients: [rows, cols]
     void* mixed;         // forward: [rows, 3 cols] (kept_high), or nullptr
-    float* partial;      // gradients in several chunks of the depth: [chunks][rows][cols]
+    const void* grad;    // d_mixed: the gradient of hidden [rows, cols]
+    float* partial;      // gradients in several chunks of the depth: [chunks][rows][cols]; d_mixed: column sums [2 row tiles][2 cols], or nullptr
     int64_t rows;
     int64_t depth;
     int64_t chunk;  // of the depth, per workgroup: a multiple of 32, or the whole of it

@@ -1,6 +1,7 @@
 // The matrix products of the gated projections for gfx950: one tile kernel for the forward and both products of the backward.
 //
 //   forward          mixed = x W^T + b = (g, u);  hidden = act(g) * u          depth = columns of x
+//   d_mixed          (grad u act'(g), grad act(g)) of (g, u) multiplied again     depth = columns of x
 //   x gradient       d x = d_mixed W                                           depth = 2 inner
 //   weight gradient  d W = d_mixed^T x                                         depth = rows, in chunks
 //
@@ -20,12 +21,13 @@
 #pragma once
 #include "gated_linear_args.h"
 #include "in_linear_silu_kernel.hip.h"
+#include "lane_sums.hip.h"
 
 namespace hstu {
 
 constexpr int kGemmThreads = 256;
 constexpr int kGemmStep = 32;  // of the depth
-constexpr int kGemmForward = 0, kGemmXGrad = 1, kGemmWeightGrad = 2;
+constexpr int kGemmForward = 0, kGemmXGrad = 1, kGemmWeightGrad = 2, kGemmMixedGrad = 3;
 constexpr int kGemmBand = 8;  // row tiles of a band
 
 __device__ __forceinline__ float gated_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f)); }
@@ -126,15 +128,16 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
     static_assert(WM * WN == 4, "four wavefronts");
     constexpr int BM = 32 * WM * MB, BN = 32 * WN * NB;  // of the tile
     constexpr int kWaveN = 32 * NB, kWaveM = 32 * MB;
-    constexpr bool NT = MODE != kGemmForward;     // the columns' side is read transposed
+    constexpr bool kBoth = MODE == kGemmForward || MODE == kGemmMixedGrad;  // the tile has both projections
+    constexpr bool NT = !kBoth;                   // the columns' side is read transposed
     constexpr bool MT = MODE == kGemmWeightGrad;  // the rows' side is
     constexpr int kReqsN = BN / 64, kReqsM = BM / 64, kReqs = kReqsN + kReqsM;  // direct-to-LDS instructions per wavefront and stage
     static_assert(BM % 64 == 0 && BN % 64 == 0, "a stage's instructions are dealt evenly");
     constexpr int kNElems = BN * kGemmStep, kStage = (BN + BM) * kGemmStep;
-    constexpr int kEpiRow = MODE == kGemmForward ? kWaveN / 2 : 64 + 8;  // staged rows of up to 64 columns
-    constexpr int kEpiPlanes = MODE == kGemmForward ? 4 : 1;
+    constexpr int kEpiRow = kBoth ? kWaveN / 2 : 64 + 8;  // staged rows of up to 64 columns
+    constexpr int kEpiPlanes = MODE == kGemmForward ? 4 : kBoth ? 2 : 1;
     // (a second piece where the stages' LDS has room for it)
-    constexpr int kEpiPieces = MODE == kGemmForward && 2 * 4 * kEpiPlanes * 32 * kEpiRow <= STAGES * kStage ? 2 : 1;
+    constexpr int kEpiPieces = kBoth && 2 * 4 * kEpiPlanes * 32 * kEpiRow <= STAGES * kStage ? 2 : 1;
     constexpr int kEpiWave = kEpiPieces * kEpiPlanes * 32 * kEpiRow;
     constexpr int kLds = STAGES * kStage > 4 * kEpiWave ? STAGES * kStage : 4 * kEpiWave;
     __shared__ __attribute__((aligned(1024))) uint16_t s_tiles[kLds];
@@ -158,7 +161,7 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
     const int tile_n = static_cast<int>(at / high), tile_m = static_cast<int>(band * kGemmBand + at % high);
 
     const int64_t m0 = static_cast<int64_t>(tile_m) * BM;
-    constexpr int kOutCols = MODE == kGemmForward ? BN / 2 : BN;
+    constexpr int kOutCols = kBoth ? BN / 2 : BN;
     const int n0 = tile_n * kOutCols;
     const int64_t depth0 = static_cast<int64_t>(part) * a.chunk;
     const int depth = static_cast<int>(min(a.chunk, a.depth - depth0));  // of this workgroup
@@ -225,7 +228,7 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
                 const int q = wave + 4 * (n_part ? i : i - kReqsN);
                 const uint32_t along = static_cast<uint32_t>(d0) * ((n_part ? NT : MT) ? (n_part ? n_row_bytes : m_row_bytes) : 2u);
                 // (forward: 16 LDS rows of one projection per instruction)
-                const bool upper = MODE == kGemmForward && n_part && (16 * q) % kWaveN >= kWaveN / 2;
+                const bool upper = kBoth && n_part && (16 * q) % kWaveN >= kWaveN / 2;
                 f(i, lds0 + static_cast<uint32_t>(2 * (stage * kStage + (n_part ? 0 : kNElems) + q * 512)), n_part ? (upper ? u_rsrc : n_rsrc) : m_rsrc, along);
             }
         };
@@ -275,6 +278,31 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
         return v;
     };
 
+    // d_mixed: the gradient's values of the lane's columns and rows, asked for ahead of everything else where there are registers to hold them
+    constexpr bool kGradsAhead = MB * NB < 8;
+    u32x4_t grads[MODE == kGemmMixedGrad ? MB : 1][NB / 2][2];
+    const auto ask_for_grads = [&](int j) {
+        const int64_t row = m0 + kWaveM * wm + 32 * j + r;
+        const uint16_t* const from = static_cast<const uint16_t*>(a.grad) + row * a.cols + n0 + kWaveN / 2 * wn + 8 * half;
+#pragma unroll
+        for (int i = 0; i < NB / 2; ++i) {
+#pragma unroll
+            for (int run = 0; run < 2; ++run) {
+                const int along = 32 * i + 16 * run;
+                grads[j][i][run] = u32x4_t{0u, 0u, 0u, 0u};
+                if (row < a.rows && n0 + kWaveN / 2 * wn + 8 * half + along < a.cols) {
+                    grads[j][i][run] = *reinterpret_cast<const u32x4_t*>(from + along);
+                }
+            }
+        }
+    };
+    if constexpr (MODE == kGemmMixedGrad && kGradsAhead) {
+#pragma unroll
+        for (int j = 0; j < MB; ++j) {
+            ask_for_grads(j);
+        }
+    }
+
     // the sums start from the bias: nothing is left to add behind the products
     f32x16_t acc[NB][MB];
 #pragma unroll
@@ -284,7 +312,7 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
         for (int e = 0; e < 16; ++e) {
             first[e] = 0.0f;
         }
-        if constexpr (MODE == kGemmForward) {
+        if constexpr (kBoth) {
             if (a.bias != nullptr) {
 #pragma unroll
                 for (int run = 0; run < 2; ++run) {
@@ -383,7 +411,7 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
 
     // ---- gradients in chunks of the depth: fp32 partial outputs, runs of 8 columns
     const int64_t row_of_lane = m0 + kWaveM * wm + r;
-    if (MODE != kGemmForward && a.partial != nullptr) {
+    if (!kBoth && a.partial != nullptr) {
         float* const out = a.partial + static_cast<int64_t>(part) * a.rows * a.cols;
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
@@ -412,7 +440,7 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     };
-    if constexpr (MODE == kGemmForward) {
+    if constexpr (kBoth) {
         constexpr int kRound = kWaveN / 2;  // columns of both projections a wavefront has
         static_assert(kRound <= 64 && NB % 2 == 0, "one round");
         constexpr int HB = NB / 2;  // blocks of each projection
@@ -420,80 +448,164 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
         const int col = n0 + kRound * wn + 8 * (lane % kPerRow);
         // where a row's 16 bytes lie: rows are not padded, and the rows that share 256 bytes of banks take turns over the whole of them
         const auto at = [](int row, int chunk) { return row * kRound + 8 * (chunk ^ (row / (128 / kRound) % kPerRow)); };
-        const auto finish = [&](auto chosen, auto kept) {
-            constexpr int kind = decltype(chosen)::value;
-            constexpr bool keep = decltype(kept)::value;
-            constexpr int kPlane = 32 * kRound, kPlanes = keep ? kEpiPlanes : 1;
-            constexpr int kPieces = 2 * 4 * kPlanes * kPlane <= kLds ? 2 : 1;
-            uint16_t* const mine = s_tiles + wave * kPieces * kPlanes * kPlane;
+        if constexpr (MODE == kGemmMixedGrad) {
+            constexpr int kPlane = 32 * kRound;
+            uint16_t* const mine = s_tiles + wave * kEpiWave;
+            with_activation(a.activation, [&](auto chosen) {
+                constexpr int kind = decltype(chosen)::value;
 #pragma unroll
-            for (int j = 0; j < MB; ++j) {
-                uint16_t* const piece = mine + (j % kPieces) * kPlanes * kPlane;
+                for (int j = 0; j < MB; ++j) {
+                    uint16_t* const piece = mine + (j % kEpiPieces) * kEpiPlanes * kPlane;
+                    const bool there = row_of_lane + 32 * j < a.rows;
+                    if constexpr (!kGradsAhead) {
+                        ask_for_grads(j);
+                    }
 #pragma unroll
-                for (int i = 0; i < HB; ++i) {
+                    for (int i = 0; i < HB; ++i) {
+#pragma unroll
+                        for (int run = 0; run < 2; ++run) {
+                            u32x4_t gw, uw;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                float d[2];
+                                const uint32_t pair = grads[j][i][run][e];
+                                ils_unpack2<Tag>(pair, d[0], d[1]);
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const int at_e = 8 * run + 2 * e + h;
+                                    float act, slope;
+                                    gated_act_slope<kind>(acc[i][j][at_e], act, slope);
+                                    // (rows past the end count for nothing, whatever the bias makes of them)
+                                    const float x = there ? d[h] * acc[HB + i][j][at_e] * slope : 0.0f, y = there ? d[h] * act : 0.0f;
+                                    acc[i][j][at_e] = x;
+                                    acc[HB + i][j][at_e] = y;
+                                }
+                                gw[e] = pack2<Tag>(acc[i][j][8 * run + 2 * e], acc[i][j][8 * run + 2 * e + 1]);
+                                uw[e] = pack2<Tag>(acc[HB + i][j][8 * run + 2 * e], acc[HB + i][j][8 * run + 2 * e + 1]);
+                            }
+                            uint16_t* const to = piece + at(r, 4 * i + 2 * run + half);
+                            *reinterpret_cast<u32x4_t*>(to) = gw;
+                            *reinterpret_cast<u32x4_t*>(to + kPlane) = uw;
+                        }
+                    }
+                    settle();
+#pragma unroll
+                    for (int q = 0; q < 32 / kRowsAtOnce; ++q) {
+                        const int in_block = kRowsAtOnce * q + lane / kPerRow;
+                        const int64_t row = m0 + kWaveM * wm + 32 * j + in_block;
+                        const uint16_t* const from = piece + at(in_block, lane % kPerRow);
+                        if (row < a.rows && col < a.cols) {
+                            uint16_t* const to = static_cast<uint16_t*>(a.out) + row * 2 * a.cols + col;
+                            *reinterpret_cast<u32x4_t*>(to) = *reinterpret_cast<const u32x4_t*>(from);
+                            *reinterpret_cast<u32x4_t*>(to + a.cols) = *reinterpret_cast<const u32x4_t*>(from + kPlane);
+                        }
+                    }
+                    if constexpr (kEpiPieces == 1) {
+                        settle();
+                    }
+                }
+            });
+            if (a.partial != nullptr) {  // column sums of the values before they are rounded, a row of them for each wavefront's rows
+                float* const out = a.partial + (static_cast<int64_t>(tile_m) * WM + wm) * 2 * a.cols;
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
 #pragma unroll
                     for (int run = 0; run < 2; ++run) {
-                        u32x4_t hw, gw, uw, low;
+                        float t[8];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float g0 = acc[i][j][8 * run + 2 * e], g1 = acc[i][j][8 * run + 2 * e + 1];
-                            const float u0 = acc[HB + i][j][8 * run + 2 * e], u1 = acc[HB + i][j][8 * run + 2 * e + 1];
-                            // (hidden is taken of the sums as they are)
-                            hw[e] = pack2<Tag>(gated_act<kind>(g0) * u0, gated_act<kind>(g1) * u1);
+                        for (int e = 0; e < 8; ++e) {
+                            t[e] = acc[i][0][8 * run + e];
+#pragma unroll
+                            for (int j = 1; j < MB; ++j) {
+                                t[e] += acc[i][j][8 * run + e];
+                            }
+                            t[e] = wave_sum<32>(t[e]);
+                        }
+                        const int c = n0 + kRound * wn + 32 * (i % HB) + 16 * run + 8 * half;
+                        if (r == 0 && c < a.cols) {
+                            float4* const to = reinterpret_cast<float4*>(out + static_cast<int64_t>(i / HB) * a.cols + c);
+                            to[0] = make_float4(t[0], t[1], t[2], t[3]);
+                            to[1] = make_float4(t[4], t[5], t[6], t[7]);
+                        }
+                    }
+                }
+            }
+        } else {
+            const auto finish = [&](auto chosen, auto kept) {
+                constexpr int kind = decltype(chosen)::value;
+                constexpr bool keep = decltype(kept)::value;
+                constexpr int kPlane = 32 * kRound, kPlanes = keep ? kEpiPlanes : 1;
+                constexpr int kPieces = 2 * 4 * kPlanes * kPlane <= kLds ? 2 : 1;
+                uint16_t* const mine = s_tiles + wave * kPieces * kPlanes * kPlane;
+#pragma unroll
+                for (int j = 0; j < MB; ++j) {
+                    uint16_t* const piece = mine + (j % kPieces) * kPlanes * kPlane;
+#pragma unroll
+                    for (int i = 0; i < HB; ++i) {
+#pragma unroll
+                        for (int run = 0; run < 2; ++run) {
+                            u32x4_t hw, gw, uw, low;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float g0 = acc[i][j][8 * run + 2 * e], g1 = acc[i][j][8 * run + 2 * e + 1];
+                                const float u0 = acc[HB + i][j][8 * run + 2 * e], u1 = acc[HB + i][j][8 * run + 2 * e + 1];
+                                // (hidden is taken of the sums as they are)
+                                hw[e] = pack2<Tag>(gated_act<kind>(g0) * u0, gated_act<kind>(g1) * u1);
+                                if constexpr (keep) {
+                                    gw[e] = kept_high(g0, g1);
+                                    uw[e] = kept_high(u0, u1);
+                                }
+                            }
+                            uint16_t* const to = piece + at(r, 4 * i + 2 * run + half);
+                            *reinterpret_cast<u32x4_t*>(to) = hw;
                             if constexpr (keep) {
-                                gw[e] = kept_high(g0, g1);
-                                uw[e] = kept_high(u0, u1);
-                            }
-                        }
-                        uint16_t* const to = piece + at(r, 4 * i + 2 * run + half);
-                        *reinterpret_cast<u32x4_t*>(to) = hw;
-                        if constexpr (keep) {
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                low[e] = kept_low(acc[i][j][8 * run + 4 * e], acc[i][j][8 * run + 4 * e + 1], acc[i][j][8 * run + 4 * e + 2], acc[i][j][8 * run + 4 * e + 3]);
-                                low[2 + e] = kept_low(acc[HB + i][j][8 * run + 4 * e], acc[HB + i][j][8 * run + 4 * e + 1], acc[HB + i][j][8 * run + 4 * e + 2],
-                                                      acc[HB + i][j][8 * run + 4 * e + 3]);
-                            }
-                            *reinterpret_cast<u32x4_t*>(to + kPlane) = gw;
-                            *reinterpret_cast<u32x4_t*>(to + 2 * kPlane) = uw;
-                            *reinterpret_cast<u32x4_t*>(to + 3 * kPlane) = low;
-                        }
-                    }
-                }
-                settle();
-#pragma unroll
-                for (int q = 0; q < 32 / kRowsAtOnce; ++q) {
-                    const int in_block = kRowsAtOnce * q + lane / kPerRow;
-                    const int64_t row = m0 + kWaveM * wm + 32 * j + in_block;
-                    const uint16_t* const from = piece + at(in_block, lane % kPerRow);
-                    if (row < a.rows && col < a.cols) {
-                        if (!keep || a.out != nullptr) {
-                            __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from),
-                                                        reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.out) + row * a.cols + col));
-                        }
-                        if constexpr (keep) {
-                            uint16_t* const to = static_cast<uint16_t*>(a.mixed) + row * 3 * a.cols + col;
-#pragma unroll
-                            for (int p = 0; p < 3; ++p) {
-                                __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from + (1 + p) * kPlane), reinterpret_cast<u32x4_t*>(to + p * a.cols));
+                                for (int e = 0; e < 2; ++e) {
+                                    low[e] = kept_low(acc[i][j][8 * run + 4 * e], acc[i][j][8 * run + 4 * e + 1], acc[i][j][8 * run + 4 * e + 2], acc[i][j][8 * run + 4 * e + 3]);
+                                    low[2 + e] = kept_low(acc[HB + i][j][8 * run + 4 * e], acc[HB + i][j][8 * run + 4 * e + 1], acc[HB + i][j][8 * run + 4 * e + 2],
+                                                          acc[HB + i][j][8 * run + 4 * e + 3]);
+                                }
+                                *reinterpret_cast<u32x4_t*>(to + kPlane) = gw;
+                                *reinterpret_cast<u32x4_t*>(to + 2 * kPlane) = uw;
+                                *reinterpret_cast<u32x4_t*>(to + 3 * kPlane) = low;
                             }
                         }
                     }
-                }
-                if constexpr (kPieces == 1) {
                     settle();
+#pragma unroll
+                    for (int q = 0; q < 32 / kRowsAtOnce; ++q) {
+                        const int in_block = kRowsAtOnce * q + lane / kPerRow;
+                        const int64_t row = m0 + kWaveM * wm + 32 * j + in_block;
+                        const uint16_t* const from = piece + at(in_block, lane % kPerRow);
+                        if (row < a.rows && col < a.cols) {
+                            if (!keep || a.out != nullptr) {
+                                __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from),
+                                                            reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.out) + row * a.cols + col));
+                            }
+                            if constexpr (keep) {
+                                uint16_t* const to = static_cast<uint16_t*>(a.mixed) + row * 3 * a.cols + col;
+#pragma unroll
+                                for (int p = 0; p < 3; ++p) {
+                                    __builtin_nontemporal_store(*reinterpret_cast<const u32x4_t*>(from + (1 + p) * kPlane), reinterpret_cast<u32x4_t*>(to + p * a.cols));
+                                }
+                            }
+                        }
+                    }
+                    if constexpr (kPieces == 1) {
+                        settle();
+                    }
                 }
-            }
-        };
-        with_activation(a.activation, [&](auto chosen) {
-            if (a.mixed != nullptr) {
-                finish(chosen, std::true_type{});
-            } else {
-                finish(chosen, std::false_type{});
-            }
-        });
+            };
+            with_activation(a.activation, [&](auto chosen) {
+                if (a.mixed != nullptr) {
+                    finish(chosen, std::true_type{});
+                } else {
+                    finish(chosen, std::false_type{});
+                }
+            });
+        }
     } else {
-        static_assert(MODE == kGemmForward || NB % 2 == 0, "rounds of 64 columns");
+        static_assert(kBoth || NB % 2 == 0, "rounds of 64 columns");
         uint16_t* const staged = s_tiles + wave * kEpiWave;
         const int out_row = lane >> 3, out_chunk = lane & 7;
 #pragma unroll

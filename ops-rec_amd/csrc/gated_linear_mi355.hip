@@ -37,8 +37,8 @@ int validate(const gated_linear_params* p)
     if (p->struct_size != sizeof(gated_linear_params)) {
         return set_error(HSTU_ERR_INVALID, "struct_size %u does not match this library (%zu)", p->struct_size, sizeof(gated_linear_params));
     }
-    if (p->x == nullptr || p->weight == nullptr || (p->hidden == nullptr && p->mixed == nullptr)) {
-        return set_error(HSTU_ERR_NULLPTR, "x, weight, and hidden or mixed must be given");
+    if (p->x == nullptr || p->weight == nullptr) {
+        return set_error(HSTU_ERR_NULLPTR, "x and weight must be given");
     }
     if (p->dtype != HSTU_DT_BF16 && p->dtype != HSTU_DT_FP16) {
         return set_error(HSTU_ERR_INVALID, "dtype %d is not one of bf16, fp16", p->dtype);
@@ -92,17 +92,18 @@ double cost_of(const GatedTile& t, int64_t rows, int64_t cols, int64_t depth, in
     return chunks == 1 ? products : products + 4.0 + static_cast<double>(rows) * static_cast<double>(cols) * static_cast<double>(chunks) * 1.1e-6;
 }
 
-const GatedTile& forward_tile(const gated_linear_params* p)
+const GatedTile& best_of(const GatedTile* tiles, int n, const gated_linear_params* p)
 {
-    const GatedTile* const tiles = kernels_of(p->dtype).forward;
     const GatedTile* best = &tiles[0];
-    for (int i = 1; i < hstu::kGatedForwardTiles; ++i) {
+    for (int i = 1; i < n; ++i) {
         if (cost_of(tiles[i], p->rows, p->inner, p->cols, 1) < cost_of(*best, p->rows, p->inner, p->cols, 1)) {
             best = &tiles[i];
         }
     }
     return *best;
 }
+const GatedTile& forward_tile(const gated_linear_params* p) { return best_of(kernels_of(p->dtype).forward, hstu::kGatedForwardTiles, p); }
+const GatedTile& mixed_tile(const gated_linear_params* p) { return best_of(kernels_of(p->dtype).mixed_grad, hstu::kGatedMixedTiles, p); }
 
 // Up to 64 rows the kernel that streams the weight, unless the tiles are estimated faster: a compute unit reads 27 GB/s there (measured at 1 .. 64 rows of
 // 2048 x 5632 and 4096 x 11264; the latter's 33 .. 64 rows took 55 .. 74 us, 56 in tiles), and both take some 5 us besides.
@@ -173,7 +174,8 @@ BackwardPlan plan_backward(const gated_linear_bwd_params* p)
     // workgroups of the element-wise stage: eight per compute unit over all column blocks, a slice of at least 32 rows each
     const int64_t blocks = ceil_div(f.inner, 256), places = 8 * static_cast<int64_t>(compute_units_or_256()) / blocks, useful = ceil_div(f.rows, 32);
     const int64_t most = places > 1 ? places : 1;
-    b.slices = static_cast<int>(useful < most ? useful : most);
+    // (multiplied again, d_mixed has a row of column sums for each half of a tile)
+    b.slices = static_cast<int>(f.mixed == nullptr ? 2 * ceil_div(f.rows, mixed_tile(&f).rows) : useful < most ? useful : most);
     b.d_mixed = rounded(static_cast<uint64_t>(f.rows) * static_cast<uint64_t>(f.inner) * 4u);
     b.sums = p->bias_grad != nullptr ? rounded(static_cast<uint64_t>(b.slices) * static_cast<uint64_t>(f.inner) * 8u) : 0;
     if (p->x_grad != nullptr) {
@@ -199,8 +201,8 @@ int validate(const gated_linear_bwd_params* p)
     if (rc != HSTU_OK) {
         return rc;
     }
-    if (p->fwd.mixed == nullptr || p->grad == nullptr) {
-        return set_error(HSTU_ERR_NULLPTR, "mixed and grad must be given");
+    if (p->grad == nullptr) {
+        return set_error(HSTU_ERR_NULLPTR, "grad must be given");
     }
     for (const void* t : {p->grad, static_cast<const void*>(p->x_grad), static_cast<const void*>(p->weight_grad), static_cast<const void*>(p->bias_grad)}) {
         if (!aligned16(t)) {
@@ -249,6 +251,9 @@ HSTU_API int gated_linear_fwd(const gated_linear_params* p, void* stream)
     const int rc = validate(p);
     if (rc != HSTU_OK) {
         return rc;
+    }
+    if (p->hidden == nullptr && p->mixed == nullptr) {
+        return set_error(HSTU_ERR_NULLPTR, "hidden or mixed must be given");
     }
     const hstu::GatedKernels& k = kernels_of(p->dtype);
     if (few_rows(p)) {
@@ -310,20 +315,37 @@ HSTU_API int gated_linear_bwd(const gated_linear_bwd_params* p, void* workspace,
     uint8_t* const ws = static_cast<uint8_t*>(workspace);
     float* const partial = reinterpret_cast<float*>(ws + b.d_mixed + b.sums);
 
-    hstu::GatedStageArgs s{};
-    s.grad = p->grad;
-    s.mixed = f.mixed;
-    s.d_mixed = ws;
-    s.partial = p->bias_grad != nullptr ? reinterpret_cast<float*>(ws + b.d_mixed) : nullptr;
-    s.rows = f.rows;
-    s.inner = static_cast<int>(f.inner);
-    s.slices = b.slices;
-    s.activation = f.activation;
-    hipLaunchKernelGGL(k.stage, dim3(static_cast<uint32_t>(b.slices * ceil_div(f.inner, 256))), dim3(256), 0, static_cast<hipStream_t>(stream), s);
-    rc = launched("gated_stage_kernel");
+    float* const sums = p->bias_grad != nullptr ? reinterpret_cast<float*>(ws + b.d_mixed) : nullptr;
+    if (f.mixed == nullptr) {
+        GatedGemmArgs a{};
+        a.n_side = f.weight;
+        a.m_side = f.x;
+        a.bias = f.bias;
+        a.grad = p->grad;
+        a.out = ws;
+        a.partial = sums;
+        a.rows = f.rows;
+        a.depth = a.chunk = f.cols;
+        a.cols = static_cast<int>(f.inner);
+        a.chunks = 1;
+        a.activation = f.activation;
+        rc = launch_tiles(mixed_tile(&f), a, stream, "gated_gemm_kernel (d_mixed)");
+    } else {
+        hstu::GatedStageArgs s{};
+        s.grad = p->grad;
+        s.mixed = f.mixed;
+        s.d_mixed = ws;
+        s.partial = sums;
+        s.rows = f.rows;
+        s.inner = static_cast<int>(f.inner);
+        s.slices = b.slices;
+        s.activation = f.activation;
+        hipLaunchKernelGGL(k.stage, dim3(static_cast<uint32_t>(b.slices * ceil_div(f.inner, 256))), dim3(256), 0, static_cast<hipStream_t>(stream), s);
+        rc = launched("gated_stage_kernel");
+    }
     if (rc == HSTU_OK && p->bias_grad != nullptr) {
         hstu::NormSumsArgs n{};
-        n.partial = s.partial;
+        n.partial = sums;
         n.out[0] = p->bias_grad;
         n.kinds = 1;
         n.slices = b.slices;

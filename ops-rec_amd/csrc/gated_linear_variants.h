@@ -14,10 +14,11 @@ struct GatedTile {
     float alone, step, fixed;
 };
 
-constexpr int kGatedForwardTiles = 4, kGatedXGradTiles = 5, kGatedWeightTiles = 3;  // by falling size
+constexpr int kGatedForwardTiles = 4, kGatedMixedTiles = 3, kGatedXGradTiles = 5, kGatedWeightTiles = 3;  // by falling size
 
 struct GatedKernels {
     GatedTile forward[kGatedForwardTiles];
+    GatedTile mixed_grad[kGatedMixedTiles];
     GatedTile x_grad[kGatedXGradTiles];
     GatedTile weight_grad[kGatedWeightTiles];
     void (*few_rows[4][4])(const GatedFewRowsArgs);  // up to 16, 32, 48, 64 rows; 8, 16, 24, 32 columns of hidden per workgroup

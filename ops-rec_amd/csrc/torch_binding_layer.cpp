@@ -416,6 +416,8 @@ Pair rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& frequencies
 
 // -------------------------------------------------------------------------------------------------- gated projections ----
 
+constexpr int64_t kKeptColumns = 192;  // _layer.KEPT_COLUMNS
+
 // all of the description but hidden and mixed; false when the call is not in canonical form
 bool describe_gated_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, c10::string_view activation, gated_linear_params& p)
 {
@@ -447,7 +449,7 @@ Pair gated_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, 
     if (describe_gated_linear(x, weight, bias, activation, p)) {
         const c10::DeviceGuard guard(x.device());
         Tensor hidden = empty({p.rows, p.inner}, x.scalar_type(), x.device());
-        Tensor mixed = keep ? empty({p.rows, 3 * p.inner}, at::kShort, x.device()) : empty({0}, at::kShort, x.device());
+        Tensor mixed = keep && p.cols > kKeptColumns ? empty({p.rows, 3 * p.inner}, at::kShort, x.device()) : empty({0}, at::kShort, x.device());
         p.hidden = hidden.data_ptr();
         p.mixed = ptr(mixed);
         const int rc = gated_linear_fwd(&p, stream_of(x));
@@ -474,27 +476,17 @@ Three gated_linear_backward(const Tensor& grad_in, const Tensor& x, const Tensor
         readable(grad, p.fwd.inner, x.scalar_type()) && (mixed_in.numel() == 0 || readable(mixed_in, 3 * p.fwd.inner, at::kShort))) {
         const c10::DeviceGuard guard(x.device());
         const auto make = [&](bool want, at::IntArrayRef size) { return want ? empty(size, x.scalar_type(), x.device()) : empty({0}, x.scalar_type(), x.device()); };
-        Tensor mixed = mixed_in;
-        int rc = HSTU_OK;
-        if (mixed.numel() == 0) {
-            mixed = empty({p.fwd.rows, 3 * p.fwd.inner}, at::kShort, x.device());
-            p.fwd.mixed = mixed.data_ptr();
-            rc = gated_linear_fwd(&p.fwd, stream_of(x));
+        Tensor x_grad = make(wanted[0], x.sizes()), weight_grad = make(wanted[1], weight.sizes()), bias_grad = make(wanted[2] && is_set(bias), {weight.size(0)});
+        p.struct_size = sizeof p;
+        p.reserved0 = 0;
+        p.fwd.mixed = mixed_in.numel() != 0 ? mixed_in.data_ptr() : nullptr;
+        p.grad = grad.data_ptr();
+        p.x_grad = ptr(x_grad);
+        p.weight_grad = ptr(weight_grad);
+        p.bias_grad = ptr(bias_grad);
+        if (run_with_workspace(gated_linear_bwd_workspace_size, gated_linear_bwd, p, x, "gated_linear_backward")) {
+            return {x_grad, weight_grad, bias_grad};
         }
-        if (rc == HSTU_OK) {
-            Tensor x_grad = make(wanted[0], x.sizes()), weight_grad = make(wanted[1], weight.sizes()), bias_grad = make(wanted[2] && is_set(bias), {weight.size(0)});
-            p.struct_size = sizeof p;
-            p.reserved0 = 0;
-            p.fwd.mixed = mixed.data_ptr();
-            p.grad = grad.data_ptr();
-            p.x_grad = ptr(x_grad);
-            p.weight_grad = ptr(weight_grad);
-            p.bias_grad = ptr(bias_grad);
-            if (run_with_workspace(gated_linear_bwd_workspace_size, gated_linear_bwd, p, x, "gated_linear_backward")) {
-                return {x_grad, weight_grad, bias_grad};
-            }
-        }
-        TORCH_CHECK(rc == HSTU_OK || rc == HSTU_ERR_INVALID, "gated_linear_backward failed (", rc, "): ", hstu_last_error());
     }
     return in_python<Three>(fallbacks.gated_linear_backward, grad, x, weight, bias, mixed_in, std::string(activation), wanted);
 }

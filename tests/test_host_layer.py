@@ -43,7 +43,9 @@ def test_meta_inference():
     grads = OPS.residual_norm_backward(y, None, x, x, None, g, None, False, torch.bfloat16, 1e-5, False)
     assert [tuple(t.shape) for t in grads] == [(0,), (5, 24), (24,), (0,), (0,)]
     x, w = torch.empty(5, 24, device="meta", dtype=torch.float16), torch.empty(80, 24, device="meta", dtype=torch.float16)
-    assert [tuple(t.shape) for t in OPS.gated_linear(x, w, None, "gelu", True)] == [(5, 40), (5, 120)] and OPS.gated_linear(x, w)[1].shape == (0,)
+    assert [tuple(t.shape) for t in OPS.gated_linear(x, w, None, "gelu", True)] == [(5, 40), (0,)]
+    wide = torch.empty(5, 200, device="meta", dtype=torch.float16), torch.empty(80, 200, device="meta", dtype=torch.float16)
+    assert [tuple(t.shape) for t in OPS.gated_linear(*wide, None, "gelu", True)] == [(5, 40), (5, 120)] and OPS.gated_linear(*wide)[1].shape == (0,)
     grads = OPS.gated_linear_backward(torch.empty(5, 40, device="meta"), x, w, None, x, "silu", [True, False, True])
     assert [tuple(t.shape) for t in grads] == [(5, 24), (0,), (0,)]
     q, k = torch.empty(7, 4, 16, device="meta"), torch.empty(7, 2, 16, device="meta")

@@ -47,7 +47,7 @@ def rotary_call(rows=70, heads=4, heads_k=2, dim=64, dtype=BF16, seed=0):
     return ROTARY, tensors, (ops_rec.rotary_frequencies(48, device=DEV)[0], offsets, torch.tensor([7, 0, 100003], device=DEV), None, False, 1.1)
 
 
-def gated_linear_call(rows=70, cols=128, inner=264, dtype=BF16, seed=0):
+def gated_linear_call(rows=70, cols=256, inner=264, dtype=BF16, seed=0):
     tensors = (randn(seed, rows, cols, dtype=dtype), randn(seed + 1, 2 * inner, cols, dtype=dtype, std=cols**-0.5), randn(seed + 2, 2 * inner, dtype=dtype))
     return lambda *a: ACT.gated_linear(*a)[0], tensors, ("silu", True)
 

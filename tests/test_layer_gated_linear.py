@@ -73,6 +73,7 @@ def check(rows, cols, inner, dtype, activation="silu", bias=True, keep=True, bac
     a = act(activation, g)
     dev = [None if t is None else t.to(DEV).requires_grad_(backward) for t in (x, w, b)]
     hidden, kept = A.gated_linear(*dev, activation, keep)
+    keep = keep and cols > 192  # (else a backward multiplies again)
     assert hidden.dtype == dtype and hidden.is_contiguous() and tuple(kept.shape) == ((rows, 3 * inner) if keep else (0,)) and kept.dtype == torch.int16
     # (slopes of the activations are at most 1.13)
     compare(hidden, a * u, 1.13 * eg * u.abs() + a.abs() * eu + 2.0**-20 * (a * u).abs(), "hidden")
@@ -210,21 +211,20 @@ def test_views_and_no_rows():
     for wanted in ([True, False, False], [False, True, False], [False, False, True], [False, False, False]):
         got = A.gated_linear_backward(torch.ones_like(hidden), x, w, b, mixed.detach(), "silu", wanted)
         assert all(torch.equal(a, g) if want_it else a.numel() == 0 for a, g, want_it in zip(got, want, wanted))
-    again = A.gated_linear_backward(torch.ones_like(hidden), x, w, b, mixed.detach()[:0, 0], "silu", [True, True, True])
-    assert all(torch.equal(a, g) for a, g in zip(again, want))  # (mixed computed again)
+    check(90, 72, 40, FP16, keep=False, seed=9)  # (g and u multiplied again)
     frozen = A.gated_linear(leaves[0], w, b, "silu", True)[0]
     (dx,) = torch.autograd.grad(frozen, leaves[0], dh)
     assert torch.equal(dx, A.gated_linear_backward(dh, x, w, b, mixed.detach(), "silu", [True, False, False])[0])
     assert frozen.requires_grad and not A.gated_linear(*leaves, "silu", True)[1].requires_grad  # (no gradient flows through mixed)
     none = torch.empty(0, 72, dtype=FP16, device=DEV, requires_grad=True)
     hidden, mixed = A.gated_linear(none, leaves[1], leaves[2], "silu", True)
-    assert hidden.shape == (0, 40) and mixed.shape == (0, 120)
+    assert hidden.shape == (0, 40) and mixed.shape == (0,)
     dx, dw = torch.autograd.grad(hidden, [none, leaves[1]], hidden.detach())
     assert dx.shape == (0, 72) and torch.count_nonzero(dw) == 0 and dw.shape == w.shape
 
 
 def test_the_same_bits_every_time_and_across_batches():
-    x, w, b, dh = (t.to(DEV) for t in inputs(1500, 128, 264, BF16, True, 5))
+    x, w, b, dh = (t.to(DEV) for t in inputs(1500, 256, 264, BF16, True, 5))
     hidden, mixed = A.gated_linear(x, w, b, "silu", True)
     grads = A.gated_linear_backward(dh, x, w, b, mixed, "silu", [True, True, True])
     for _ in range(3):
