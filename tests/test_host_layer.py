@@ -269,6 +269,12 @@ def test_c_abi_of_the_backward():
     assert lib.gated_linear_bwd_workspace_size(ctypes.byref(w), ctypes.byref(size)) == 0 and size.value >= 10 * 256 * 2
     assert lib.gated_linear_bwd(ctypes.byref(w), 0x1000, size.value - 1, None) == 161004
     assert lib.gated_linear_bwd(ctypes.byref(w), 0x1008, size.value, None) == 161004
+    kept = size.value
+    w.fwd.mixed = w.fwd.hidden = None  # g and u are multiplied again
+    assert lib.gated_linear_bwd_workspace_size(ctypes.byref(w), ctypes.byref(size)) == 0 and size.value == kept
+    w.bias_grad = 0x1000  # (two rows of column sums of both projections)
+    assert lib.gated_linear_bwd_workspace_size(ctypes.byref(w), ctypes.byref(size)) == 0 and size.value >= kept + 2 * 256 * 4
+    assert lib.gated_linear_fwd(ctypes.byref(w.fwd), None) == 161001  # (a forward writes one of the two)
     w.x_grad = 0x1004
     assert lib.gated_linear_bwd_workspace_size(ctypes.byref(w), ctypes.byref(size)) == 161002
     g = _native.NormGateBwdParams()

@@ -310,6 +310,41 @@ def test_past_31_bits_of_elements():
     assert torch.equal(got[picked], ACT.gated_linear(x[picked.repeat(300)], weight)[0][: len(picked)])
 
 
+def test_gradients_past_31_bits_of_elements():
+    """Gradients on a few rows of a large batch, zeros on the others: their rows come out as in a batch of their own, and columns as the sums over them."""
+    rows, cols = 2_100_000, 1024
+    picked = torch.tensor([0, 1, 2_097_150, 2_097_151, 2_097_152, 2_097_153, rows - 2, rows - 1], device=DEV)
+    few = [randn(i, len(picked), cols, dtype=BF16) for i in range(3)]
+    x, gate, grad = (torch.zeros(rows, cols, dtype=BF16, device=DEV) for _ in range(3))
+    for t, v in zip((x, gate, grad), few):
+        t[picked] = v
+    gamma, beta = randn(4, cols, mean=1.0), randn(5, cols)
+    rest = (False, 1.0, 1, 1e-5, False, True)
+    got, want = ACT.norm_gate_backward(grad, x, gate, gamma, beta, *rest), ACT.norm_gate_backward(few[2], few[0], few[1], gamma, beta, *rest)
+    assert all(torch.equal(a[picked], b) for a, b in zip(got[:2], want[:2]))
+    assert all(torch.allclose(a, b, rtol=0, atol=2.0**-18 * float(b.abs().max())) for a, b in zip(got[2:], want[2:]))
+    got = ACT.residual_norm_backward(grad, gate, x, x, None, gamma, None, True, BF16, 1e-5, False)
+    want = ACT.residual_norm_backward(few[2], few[1], few[0], few[0], None, gamma, None, True, BF16, 1e-5, False)
+    assert torch.equal(got[1][picked], want[1])
+    del x, gate, grad, got
+    # d_mixed of 8.6e9 elements
+    inner = 2048
+    x, grad = torch.zeros(rows, 8, dtype=BF16, device=DEV), torch.zeros(rows, inner, dtype=BF16, device=DEV)
+    xs, ds = randn(6, len(picked), 8, dtype=BF16), randn(7, len(picked), inner, dtype=BF16)
+    x[picked], grad[picked] = xs, ds
+    weight = randn(8, 2 * inner, 8, dtype=BF16, std=0.3)
+    dx, dw, _ = ACT.gated_linear_backward(grad, x, weight, None, torch.empty(0, dtype=torch.int16, device=DEV), "sigmoid", [True, True, False])
+    x64, w64, d64 = (t.double().cpu() for t in (xs, weight, ds))
+    g, u = (x64 @ w64.t()).chunk(2, dim=1)
+    a = torch.sigmoid(g)
+    d_mixed = torch.cat([d64 * u * a * (1 - a), d64 * a], dim=1)
+    # d_mixed is rounded by half a step of its values, 2^-8 of them, and the results by as much again
+    for got, want, room in ((dx[picked], d_mixed @ w64, d_mixed.abs() @ w64.abs()), (dw, d_mixed.t() @ x64, d_mixed.abs().t() @ x64.abs())):
+        assert bool(((got.double().cpu() - want).abs() <= 2.0**-8 * want.abs() * (1 + 2.0**-7) + (2.0**-8 + 2.0**-17) * room).all())
+    dx[picked] = 0
+    assert torch.count_nonzero(dx) == 0
+
+
 def test_second_derivatives_of_a_rotation():
     """A rotation is linear: the gradient of its gradient is a rotation again."""
     _, (q, k), rest = rotary_call(dtype=FP32)
