@@ -36,7 +36,12 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
     // partial sums of half the wavefronts [wavefront][operand][row of x][16 weight rows], rows padded by 4 so that 16 rows at 16 bytes spread over
     // the banks
     constexpr int kPitch = 16 + 4, kHalf = kFewWaves / 2;
-    __shared__ __attribute__((aligned(16))) float s_part[kHalf * AB * kRows * kPitch];
+    constexpr int kUnroll = AB + MB <= 4 && MB <= 2 ? 4 : 2;
+    // x of a wavefront's runs on their way to the operands: rows of 128 bytes, 16-byte chunks XOR-ed with (row / 2) % 8
+    constexpr int kXWave = kUnroll * kRows * kFewStep;  // values
+    constexpr int kPart = kHalf * AB * kRows * kPitch * 4, kX = kFewWaves * kXWave * 2;
+    __shared__ __attribute__((aligned(1024))) uint8_t s_all[kPart > kX ? kPart : kX];
+    float* const s_part = reinterpret_cast<float*>(s_all);
 
     const int lane = threadIdx.x & 63;
     const int wave = uniform(threadIdx.x >> 6);
@@ -64,45 +69,52 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
             acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         }
     }
-    constexpr int kUnroll = AB + MB <= 4 ? 4 : 2;
     // Workgroups begin at different runs of the depth: rows a multiple of 4 KB apart lie in one channel of the L2, which all would ask at once.
     const int runs = (a.depth + kFewStep - 1) / kFewStep, turn = static_cast<int>(blockIdx.x * 5u % static_cast<uint32_t>(runs));
+    uint16_t* const s_x = reinterpret_cast<uint16_t*>(s_all) + wave * kXWave;
     const auto batch = [&](auto count, int run0) {  // so many runs, every eighth from run0 on
         constexpr int kCount = decltype(count)::value;
-        u32x4_t w[kCount][2][AB], x[kCount][2][MB];
+        u32x4_t w[kCount][2][AB];
 #pragma unroll
         for (int s = 0; s < kCount; ++s) {
-            const int run = run0 + s * kFewWaves + turn;
+            const int run = run0 + s * kFewWaves + turn, d0 = (run < runs ? run : run - runs) * kFewStep;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const int d = (run < runs ? run : run - runs) * kFewStep + 32 * k + 8 * quarter;
+                const int d = d0 + 32 * k + 8 * quarter;
                 const uint32_t along = static_cast<uint32_t>(d) * 2u;
 #pragma unroll
                 for (int i = 0; i < AB; ++i) {  // (the weight is read once: non-temporal, so that x stays in the caches)
                     const uint32_t off = d < a.depth && w_row[i] != kOutOfRange ? w_row[i] + along : kOutOfRange;
                     w[s][k][i] = __builtin_amdgcn_raw_buffer_load_b128(w_rsrc, static_cast<int>(off), 0, 2);
                 }
+            }
 #pragma unroll
-                for (int j = 0; j < MB; ++j) {
-                    const uint32_t off = d < a.depth ? static_cast<uint32_t>(16 * j + r) * row_bytes + along : kOutOfRange;
-                    x[s][k][j] = __builtin_amdgcn_raw_buffer_load_b128(x_rsrc, static_cast<int>(off), 0, 0);
-                }
+            for (int g = 0; g < 2 * MB; ++g) {  // 8 rows, a whole line each
+                const int row = 8 * g + (lane >> 3), d = d0 + 8 * ((lane & 7) ^ ((row >> 1) & 7));
+                const uint32_t off = d < a.depth ? static_cast<uint32_t>(row) * row_bytes + static_cast<uint32_t>(d) * 2u : kOutOfRange;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(x_rsrc, (__attribute__((address_space(3))) void*)(s_x + (s * kRows + 8 * g) * kFewStep), 16,
+                                                         static_cast<int>(off), 0, 0, 0);
             }
         }
         __builtin_amdgcn_sched_barrier(0);  // (the compiler would move each load to its product, to save registers that are there)
+        __builtin_amdgcn_s_waitcnt(gemm_wait(0, 15));
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
         for (int s = 0; s < kCount; ++s) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
 #pragma unroll
-                for (int i = 0; i < AB; ++i) {
+                for (int j = 0; j < MB; ++j) {
+                    const u32x4_t x = *reinterpret_cast<const u32x4_t*>(s_x + (s * kRows + 16 * j + r) * kFewStep + 8 * ((4 * k + quarter) ^ ((r >> 1) & 7)));
 #pragma unroll
-                    for (int j = 0; j < MB; ++j) {
-                        acc[i][j] = gated_mfma16<Tag>(w[s][k][i], x[s][k][j], acc[i][j]);
+                    for (int i = 0; i < AB; ++i) {
+                        acc[i][j] = gated_mfma16<Tag>(w[s][k][i], x, acc[i][j]);
                     }
                 }
             }
         }
+        __builtin_amdgcn_s_waitcnt(gemm_wait(63, 0));  // (x is read before the next runs' is written)
+        __builtin_amdgcn_sched_barrier(0);
     };
     int run0 = wave;
     for (; run0 + kFewWaves * (kUnroll - 1) < runs; run0 += kFewWaves * kUnroll) {
@@ -111,6 +123,7 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
     for (; run0 < runs; run0 += kFewWaves) {
         batch(std::integral_constant<int, 1>{}, run0);
     }
+    __syncthreads();  // (sums go where other wavefronts' x was)
     // a lane has weight rows 4 quarter .. + 3 of row r of x; the second half of the wavefronts hands its sums to the first
     auto place = [&](int w, int i, int j) { return reinterpret_cast<f32x4_t*>(s_part + ((w * AB + i) * kRows + 16 * j + r) * kPitch + 4 * quarter); };
     if (wave >= kHalf) {
