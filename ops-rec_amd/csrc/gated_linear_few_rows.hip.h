@@ -1,12 +1,13 @@
 // The gated projections for few rows, gfx950: hidden = act(x Wg^T + bg) * (x Wu^T + bu) for single tokens and small batches.
 //
 // Bound by the bytes of the weight, each read once, by those of x, which every workgroup reads, and for small layers by latency.  A workgroup has C columns
-// of hidden: C rows of the gate's weight and the C of the other projection, straight from memory into v_mfma_f32_16x16x32 operands (a lane's 16 bytes are
-// 8 values of one weight row; nothing of the weight is read twice, so LDS would only add a trip).  Its eight wavefronts share the depth: each takes every
-// eighth run of 64 values, whose loads are all in flight before the first product, and the partial sums meet in LDS.
+// of hidden: C rows of the gate's weight, the C of the other projection, and all rows of x.  Its eight wavefronts share the depth: each takes every eighth
+// run of 64 values, brings in the run's whole 128-byte lines of all these rows by direct-to-LDS requests, reads them back as v_mfma_f32_16x16x32 operands (16-byte
+// chunks XOR-ed with (row / 2) % 8), and the partial sums meet in LDS.  (Operands straight from memory take half a line of 16 rows an instruction, and a compute unit
+// has only so many requests under way: 48 rows, 2048 -> 5632, 18.6 us, 12.7 so, of 9.3 that the bytes would take; one row, 4096 -> 11264, 39.7 and 30.0.)
 // C is 8, 16, 24 or 32, whichever leaves the fullest compute unit the least to read: rounds of workgroups times 2 C + rows.  (48 rows,
-// 2048 -> 5632: 352 workgroups of 16 columns, two on some compute units, took 25 us; 235 of 24, one on each, 18.6; with one row 11.4: every
-// compute unit reads as much of x as of the weight there.  Loads of twice as many runs under way are no faster.)
+// 2048 -> 5632, straight from memory: 352 workgroups of 16 columns, two on some compute units, took 25 us; 235 of 24, one on each, 18.6.)  Two to four runs of a
+// wavefront under way instead of one, in as much more LDS, are level or slower.
 #pragma once
 #include "gated_linear_gemm.hip.h"
 
@@ -14,7 +15,7 @@ namespace hstu {
 
 constexpr int kFewWaves = 8;
 constexpr int kFewThreads = 64 * kFewWaves;
-constexpr int kFewStep = 64;  // values of the depth a wavefront takes at a time: two operands' worth, a whole 128-byte line of a weight row
+constexpr int kFewStep = 64;  // values of the depth a wavefront takes at a time: two operands' worth, a whole 128-byte line of a row
 typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 
 template <typename Tag>
@@ -36,11 +37,10 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
     // partial sums of half the wavefronts [wavefront][operand][row of x][16 weight rows], rows padded by 4 so that 16 rows at 16 bytes spread over
     // the banks
     constexpr int kPitch = 16 + 4, kHalf = kFewWaves / 2;
-    constexpr int kUnroll = AB + MB <= 4 && MB <= 2 ? 4 : 2;
-    // x of a wavefront's runs on their way to the operands: rows of 128 bytes, 16-byte chunks XOR-ed with (row / 2) % 8
-    constexpr int kXWave = kUnroll * kRows * kFewStep;  // values
-    constexpr int kPart = kHalf * AB * kRows * kPitch * 4, kX = kFewWaves * kXWave * 2;
-    __shared__ __attribute__((aligned(1024))) uint8_t s_all[kPart > kX ? kPart : kX];
+    // a wavefront's run on its way to the operands: rows of x, then of the weight
+    constexpr int kRun = (kRows + 16 * AB) * kFewStep;  // values
+    constexpr int kPart = kHalf * AB * kRows * kPitch * 4, kRuns = kFewWaves * kRun * 2;
+    __shared__ __attribute__((aligned(1024))) uint8_t s_all[kPart > kRuns ? kPart : kRuns];
     float* const s_part = reinterpret_cast<float*>(s_all);
 
     const int lane = threadIdx.x & 63;
@@ -55,11 +55,11 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
 
     const int r = lane & 15, quarter = lane >> 4;
     // the lane's weight rows, the gate's C ahead of the other projection's
-    uint32_t w_row[AB];
+    uint32_t w_row[2 * AB];
 #pragma unroll
-    for (int i = 0; i < AB; ++i) {
-        const int at = 16 * i + r, c = at < C ? at : at - C;
-        w_row[i] = c < cols ? static_cast<uint32_t>((at < C ? 0 : a.inner) + n0 + c) * row_bytes : kOutOfRange;
+    for (int g = 0; g < 2 * AB; ++g) {
+        const int at = 8 * g + (lane >> 3), c = at < C ? at : at - C;
+        w_row[g] = c < cols ? static_cast<uint32_t>((at < C ? 0 : a.inner) + n0 + c) * row_bytes : kOutOfRange;
     }
     f32x4_t acc[AB][MB];
 #pragma unroll
@@ -71,57 +71,44 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_rows_kernel(const Gated
     }
     // Workgroups begin at different runs of the depth: rows a multiple of 4 KB apart lie in one channel of the L2, which all would ask at once.
     const int runs = (a.depth + kFewStep - 1) / kFewStep, turn = static_cast<int>(blockIdx.x * 5u % static_cast<uint32_t>(runs));
-    uint16_t* const s_x = reinterpret_cast<uint16_t*>(s_all) + wave * kXWave;
-    const auto batch = [&](auto count, int run0) {  // so many runs, every eighth from run0 on
-        constexpr int kCount = decltype(count)::value;
-        u32x4_t w[kCount][2][AB];
+    uint16_t* const s_x = reinterpret_cast<uint16_t*>(s_all) + wave * kRun;
+    uint16_t* const s_w = s_x + kRows * kFewStep;
+    typedef __attribute__((address_space(3))) void lds_t;
+    const auto operand = [&](const uint16_t* rows_at, int block, int k) {
+        return *reinterpret_cast<const u32x4_t*>(rows_at + (16 * block + r) * kFewStep + 8 * ((4 * k + quarter) ^ ((r >> 1) & 7)));
+    };
+    for (int run0 = wave; run0 < runs; run0 += kFewWaves) {
+        const int run = run0 + turn, d0 = (run < runs ? run : run - runs) * kFewStep;
+        // 8 rows a request, a whole line each
+        const auto along = [&](int row) { return d0 + 8 * ((lane & 7) ^ ((row >> 1) & 7)); };
 #pragma unroll
-        for (int s = 0; s < kCount; ++s) {
-            const int run = run0 + s * kFewWaves + turn, d0 = (run < runs ? run : run - runs) * kFewStep;
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int d = d0 + 32 * k + 8 * quarter;
-                const uint32_t along = static_cast<uint32_t>(d) * 2u;
-#pragma unroll
-                for (int i = 0; i < AB; ++i) {  // (the weight is read once: non-temporal, so that x stays in the caches)
-                    const uint32_t off = d < a.depth && w_row[i] != kOutOfRange ? w_row[i] + along : kOutOfRange;
-                    w[s][k][i] = __builtin_amdgcn_raw_buffer_load_b128(w_rsrc, static_cast<int>(off), 0, 2);
-                }
-            }
-#pragma unroll
-            for (int g = 0; g < 2 * MB; ++g) {  // 8 rows, a whole line each
-                const int row = 8 * g + (lane >> 3), d = d0 + 8 * ((lane & 7) ^ ((row >> 1) & 7));
-                const uint32_t off = d < a.depth ? static_cast<uint32_t>(row) * row_bytes + static_cast<uint32_t>(d) * 2u : kOutOfRange;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(x_rsrc, (__attribute__((address_space(3))) void*)(s_x + (s * kRows + 8 * g) * kFewStep), 16,
-                                                         static_cast<int>(off), 0, 0, 0);
-            }
+        for (int g = 0; g < 2 * AB; ++g) {  // (the weight is read once: non-temporal, so that x stays in the caches)
+            const int d = along(8 * g + (lane >> 3));
+            const uint32_t off = d < a.depth && w_row[g] != kOutOfRange ? w_row[g] + static_cast<uint32_t>(d) * 2u : kOutOfRange;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(w_rsrc, (lds_t*)(s_w + 8 * g * kFewStep), 16, static_cast<int>(off), 0, 0, 2);
         }
-        __builtin_amdgcn_sched_barrier(0);  // (the compiler would move each load to its product, to save registers that are there)
+#pragma unroll
+        for (int g = 0; g < 2 * MB; ++g) {
+            const int row = 8 * g + (lane >> 3), d = along(row);
+            const uint32_t off = d < a.depth ? static_cast<uint32_t>(row) * row_bytes + static_cast<uint32_t>(d) * 2u : kOutOfRange;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(x_rsrc, (lds_t*)(s_x + 8 * g * kFewStep), 16, static_cast<int>(off), 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_waitcnt(gemm_wait(0, 15));
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
-        for (int s = 0; s < kCount; ++s) {
+        for (int k = 0; k < 2; ++k) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+            for (int i = 0; i < AB; ++i) {
+                const u32x4_t w = operand(s_w, i, k);
 #pragma unroll
                 for (int j = 0; j < MB; ++j) {
-                    const u32x4_t x = *reinterpret_cast<const u32x4_t*>(s_x + (s * kRows + 16 * j + r) * kFewStep + 8 * ((4 * k + quarter) ^ ((r >> 1) & 7)));
-#pragma unroll
-                    for (int i = 0; i < AB; ++i) {
-                        acc[i][j] = gated_mfma16<Tag>(w[s][k][i], x, acc[i][j]);
-                    }
+                    acc[i][j] = gated_mfma16<Tag>(w, operand(s_x, j, k), acc[i][j]);
                 }
             }
         }
-        __builtin_amdgcn_s_waitcnt(gemm_wait(63, 0));  // (x is read before the next runs' is written)
+        __builtin_amdgcn_s_waitcnt(gemm_wait(63, 0));  // (a run is read before the next is written)
         __builtin_amdgcn_sched_barrier(0);
-    };
-    int run0 = wave;
-    for (; run0 + kFewWaves * (kUnroll - 1) < runs; run0 += kFewWaves * kUnroll) {
-        batch(std::integral_constant<int, kUnroll>{}, run0);
-    }
-    for (; run0 < runs; run0 += kFewWaves) {
-        batch(std::integral_constant<int, 1>{}, run0);
     }
     __syncthreads();  // (sums go where other wavefronts' x was)
     // a lane has weight rows 4 quarter .. + 3 of row r of x; the second half of the wavefronts hands its sums to the first

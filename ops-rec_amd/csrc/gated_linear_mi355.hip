@@ -16,7 +16,7 @@ using hstu::set_error;
 static_assert(OPS_REC_ACT_SILU == hstu::kActSilu && OPS_REC_ACT_GELU == hstu::kActGelu && OPS_REC_ACT_SIGMOID == hstu::kActSigmoid, "one numbering");
 
 constexpr int64_t kStep = 32;          // of a product's depth
-constexpr int64_t kFewRows = 64;       // of a workgroup of the kernel for few rows
+constexpr int64_t kFewRows = 96;       // of a workgroup of the kernel for few rows
 constexpr int64_t kMostCols = 1 << 21; // (256 rows of twice as many columns lie behind one descriptor of 2^31 bytes)
 constexpr int64_t kMostBytes = int64_t{1} << 31;  // behind one descriptor
 
@@ -105,14 +105,14 @@ const GatedTile& best_of(const GatedTile* tiles, int n, const gated_linear_param
 const GatedTile& forward_tile(const gated_linear_params* p) { return best_of(kernels_of(p->dtype).forward, hstu::kGatedForwardTiles, p); }
 const GatedTile& mixed_tile(const gated_linear_params* p) { return best_of(kernels_of(p->dtype).mixed_grad, hstu::kGatedMixedTiles, p); }
 
-// Up to 64 rows the kernel that streams the weight, unless the tiles are estimated faster: a compute unit reads 27 GB/s there (measured at 1 .. 64 rows of
-// 2048 x 5632 and 4096 x 11264; the latter's 33 .. 64 rows took 55 .. 74 us, 56 in tiles), and both take some 5 us besides.
+// Up to 96 rows the kernel that streams the weight, unless the tiles are estimated faster: a compute unit reads 45 GB/s there (48 and 64 rows of 2048 x 5632
+// and 4096 x 11264), and both take some 4 us besides.
 bool few_rows(const gated_linear_params* p)
 {
     if (p->rows > kFewRows) {
         return false;
     }
-    const double read = static_cast<double>(few_rows_read(p, few_rows_columns(p))) * static_cast<double>(p->cols) * 2.0 / 27e3;
+    const double read = static_cast<double>(few_rows_read(p, few_rows_columns(p))) * static_cast<double>(p->cols) * 2.0 / 45e3;
     return read <= 1.25 * cost_of(forward_tile(p), p->rows, p->inner, p->cols, 1);  // (whose steps were measured with weights in the caches)
 }
 

@@ -30,7 +30,9 @@ const GatedKernels& gated_table()
         {{gated_few_rows_kernel<Tag, 1, 1>, gated_few_rows_kernel<Tag, 1, 2>, gated_few_rows_kernel<Tag, 1, 3>, gated_few_rows_kernel<Tag, 1, 4>},
          {gated_few_rows_kernel<Tag, 2, 1>, gated_few_rows_kernel<Tag, 2, 2>, gated_few_rows_kernel<Tag, 2, 3>, gated_few_rows_kernel<Tag, 2, 4>},
          {gated_few_rows_kernel<Tag, 3, 1>, gated_few_rows_kernel<Tag, 3, 2>, gated_few_rows_kernel<Tag, 3, 3>, gated_few_rows_kernel<Tag, 3, 4>},
-         {gated_few_rows_kernel<Tag, 4, 1>, gated_few_rows_kernel<Tag, 4, 2>, gated_few_rows_kernel<Tag, 4, 3>, gated_few_rows_kernel<Tag, 4, 4>}},
+         {gated_few_rows_kernel<Tag, 4, 1>, gated_few_rows_kernel<Tag, 4, 2>, gated_few_rows_kernel<Tag, 4, 3>, gated_few_rows_kernel<Tag, 4, 4>},
+         {gated_few_rows_kernel<Tag, 5, 1>, gated_few_rows_kernel<Tag, 5, 2>, gated_few_rows_kernel<Tag, 5, 3>, gated_few_rows_kernel<Tag, 5, 4>},
+         {gated_few_rows_kernel<Tag, 6, 1>, gated_few_rows_kernel<Tag, 6, 2>, gated_few_rows_kernel<Tag, 6, 3>, gated_few_rows_kernel<Tag, 6, 4>}},
         gated_stage_kernel<Tag>,
         gated_sum_kernel<Tag>};
     return table;

@@ -21,7 +21,7 @@ struct GatedKernels {
     GatedTile mixed_grad[kGatedMixedTiles];
     GatedTile x_grad[kGatedXGradTiles];
     GatedTile weight_grad[kGatedWeightTiles];
-    void (*few_rows[4][4])(const GatedFewRowsArgs);  // up to 16, 32, 48, 64 rows; 8, 16, 24, 32 columns of hidden per workgroup
+    void (*few_rows[6][4])(const GatedFewRowsArgs);  // up to 16, 32, .. 96 rows; 8, 16, 24, 32 columns of hidden per workgroup
     void (*stage)(const GatedStageArgs);
     void (*sum)(const GatedSumArgs);
 };

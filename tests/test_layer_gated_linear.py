@@ -162,6 +162,15 @@ def test_the_widest():
     assert torch.count_nonzero(dw) == 0
 
 
+@pytest.mark.parametrize("inner", [1000, 4000, 6000, 8000])
+@pytest.mark.parametrize("rows", [16, 31, 33, 64, 80, 96])
+def test_few_rows(rows, inner):
+    """Every number of blocks of rows with 8, 16, 24 and 32 columns of hidden a workgroup, over depths that end inside a run and inside an operand."""
+    for cols in (72, 200):
+        assert name(rows, cols, inner) == "gated_few_rows"
+        check(rows, cols, inner, BF16 if inner % 3 else FP16, "silu", backward=False, seed=rows)
+
+
 def test_values_far_out():
     # gates whose exponentials overflow and underflow, and that are not finite
     x = torch.eye(8, dtype=BF16, device=DEV)
