@@ -8,11 +8,12 @@
 // Bound by the matrix units (and in the forward up to a depth of a few hundred by its stores).  A workgroup of four wavefronts has a tile of BM
 // rows by BN columns of the output, each wavefront a quarter of it in v_mfma_f32_32x32x16 blocks; the columns' side is the A operand, so that a lane
 // has outputs of one row, and its columns are placed in a permuted order that gives it runs of 8 consecutive ones: 16-byte pieces.
-// The depth goes by in steps of 32 through a ring of STAGES tiles in LDS, filled by direct-to-LDS loads and read while later ones are under way.
+// The depth goes by in steps of 32, or 64 where a tile has the LDS to itself, through a ring of STAGES tiles in LDS, filled by direct-to-LDS loads and read
+// while later ones are under way.  (Steps of 64 ask for whole 128-byte lines: 8191 x 2048 -> 5632 357 us in four stages of 32, 343 in two of 64.)
 // In the forward the BN columns are BN / 2 of the gate and the same BN / 2 of the other projection, dealt so that a wavefront has both
 // halves of a column in the same lane: activation and product never leave registers.
 //
-// A side whose rows run along the depth is kept in LDS by rows of 64 bytes (chunk index XOR-ed with (row / 4) % 4) and read as 16-byte operands;
+// A side whose rows run along the depth is kept in LDS by rows of 64 or 128 bytes (chunk index XOR-ed with (row / 4) % 4 or (row / 2) % 8) and read as 16-byte operands;
 // a side that is stored the other way -- the weight for d x, both sides of d W -- is kept as it lies, 32 rows of the tile's width, and read
 // back with the transposing LDS read (64-byte groups XOR-ed with row % 4): no operand is transposed through memory.
 //
@@ -26,7 +27,7 @@
 namespace hstu {
 
 constexpr int kGemmThreads = 256;
-constexpr int kGemmStep = 32;  // of the depth
+constexpr int kGemmStep = 32;  // of the depth, where not 64
 constexpr int kGemmForward = 0, kGemmXGrad = 1, kGemmWeightGrad = 2, kGemmMixedGrad = 3;
 constexpr int kGemmBand = 8;  // row tiles of a band
 
@@ -121,8 +122,8 @@ __device__ __forceinline__ u32x4_t gemm_rsrc(const void* base, uint32_t bytes)
 // s_waitcnt: at most `vm` memory requests and `lgkm` LDS accesses under way
 constexpr int gemm_wait(int vm, int lgkm) { return (vm & 15) | (7 << 4) | (lgkm << 8) | ((vm >> 4) << 14); }
 
-// WM x WN wavefronts, each with MB x NB blocks of 32 x 32; STAGES tiles of LDS
-template <typename Tag, int MODE, int WM, int WN, int MB, int NB, int STAGES, int PER_CU>
+// WM x WN wavefronts, each with MB x NB blocks of 32 x 32; STAGES tiles of LDS, STEP of the depth each
+template <typename Tag, int MODE, int WM, int WN, int MB, int NB, int STAGES, int PER_CU, int STEP>
 __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const GatedGemmArgs a)
 {
     static_assert(WM * WN == 4, "four wavefronts");
@@ -131,9 +132,10 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
     constexpr bool kBoth = MODE == kGemmForward || MODE == kGemmMixedGrad;  // the tile has both projections
     constexpr bool NT = !kBoth;                   // the columns' side is read transposed
     constexpr bool MT = MODE == kGemmWeightGrad;  // the rows' side is
-    constexpr int kReqsN = BN / 64, kReqsM = BM / 64, kReqs = kReqsN + kReqsM;  // direct-to-LDS instructions per wavefront and stage
+    static_assert(STEP == 32 || (STEP == 64 && kBoth), "sides stored across the depth go by steps of 32");
+    constexpr int kReqsN = BN * STEP / 2048, kReqsM = BM * STEP / 2048, kReqs = kReqsN + kReqsM;  // direct-to-LDS instructions per wavefront and stage
     static_assert(BM % 64 == 0 && BN % 64 == 0, "a stage's instructions are dealt evenly");
-    constexpr int kNElems = BN * kGemmStep, kStage = (BN + BM) * kGemmStep;
+    constexpr int kNElems = BN * STEP, kStage = (BN + BM) * STEP;
     constexpr int kEpiRow = kBoth ? kWaveN / 2 : 64 + 8;  // staged rows of up to 64 columns
     constexpr int kEpiPlanes = MODE == kGemmForward ? 4 : kBoth ? 2 : 1;
     // (a second piece where the stages' LDS has room for it)
@@ -204,8 +206,8 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
             req_off[i] = static_cast<uint32_t>(row) * (n_part ? n_row_bytes : m_row_bytes) + static_cast<uint32_t>(col) * 2u;
             req_depth[i] = row;
         } else {
-            const int lds_row = 16 * q + (lane >> 2);
-            const int chunk = (lane & 3) ^ ((lds_row >> 2) & 3);
+            const int lds_row = 512 / STEP * q + lane / (STEP / 8);
+            const int chunk = (lane % (STEP / 8)) ^ (STEP == 32 ? (lds_row >> 2) & 3 : (lds_row >> 1) & 7);
             int row = lds_row;
             if (n_part) {
                 // a wavefront's rows: half of the gate, half of the other projection
@@ -220,7 +222,7 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
     // lane (a scalar past a descriptor's end would not be).
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint16_t*)s_tiles));
     auto request = [&](int stage, int step) {
-        const int d0 = step * kGemmStep;
+        const int d0 = step * STEP;
         const auto each = [&](auto&& f) {
 #pragma unroll
             for (int i = 0; i < kReqs; ++i) {
@@ -228,11 +230,11 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
                 const int q = wave + 4 * (n_part ? i : i - kReqsN);
                 const uint32_t along = static_cast<uint32_t>(d0) * ((n_part ? NT : MT) ? (n_part ? n_row_bytes : m_row_bytes) : 2u);
                 // (forward: 16 LDS rows of one projection per instruction)
-                const bool upper = kBoth && n_part && (16 * q) % kWaveN >= kWaveN / 2;
+                const bool upper = kBoth && n_part && (512 / STEP * q) % kWaveN >= kWaveN / 2;
                 f(i, lds0 + static_cast<uint32_t>(2 * (stage * kStage + (n_part ? 0 : kNElems) + q * 512)), n_part ? (upper ? u_rsrc : n_rsrc) : m_rsrc, along);
             }
         };
-        if (d0 + kGemmStep <= depth) {
+        if (d0 + STEP <= depth) {
             each([&](int i, uint32_t to, u32x4_t rsrc, uint32_t along) { gemm_request(to, req_off[i], rsrc, along); });
         } else {
             each([&](int i, uint32_t to, u32x4_t rsrc, uint32_t along) {
@@ -244,9 +246,10 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
     // ---- operand reads: wavefront (wm, wn) has rows kWaveM wm .. and columns kWaveN wn .. of the tile.  Addresses within a stage: of a row-wise side,
     // block 0 for each half of the step (further blocks are constants away); of the other, each block (whose 64-byte groups are XOR-ed)
     const int r = lane & 31, half = lane >> 5;
-    const int swz = (r >> 2) & 3;
+    const int swz = STEP == 32 ? (r >> 2) & 3 : (r >> 1) & 7;
+    constexpr int kParts = STEP / 16;  // of a step, as deep as an instruction
     const int tr_row = 8 * half + ((lane & 15) >> 2);
-    int n_at[NT ? NB : 2], m_at[MT ? MB : 2];
+    int n_at[NT ? NB : kParts], m_at[MT ? MB : kParts];
     if constexpr (NT) {
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
@@ -255,8 +258,8 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
         }
     } else {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            n_at[kk] = (kWaveN * wn + r) * kGemmStep + ((2 * kk + half) ^ swz) * 8;
+        for (int kk = 0; kk < kParts; ++kk) {
+            n_at[kk] = (kWaveN * wn + r) * STEP + ((2 * kk + half) ^ swz) * 8;
         }
     }
     if constexpr (MT) {
@@ -267,8 +270,8 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
         }
     } else {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            m_at[kk] = kNElems + (kWaveM * wm + r) * kGemmStep + ((2 * kk + half) ^ swz) * 8;
+        for (int kk = 0; kk < kParts; ++kk) {
+            m_at[kk] = kNElems + (kWaveM * wm + r) * STEP + ((2 * kk + half) ^ swz) * 8;
         }
     }
     auto read_across = [&](const uint16_t* p, int width) -> u32x4_t {
@@ -337,11 +340,11 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
         }
     }
 
-    // A step is two halves of 16.  While the products of one half run, the operands of the next are read, so that the matrix pipe finds them
-    // there; the barrier that hands a stage over stands between the halves, when every wavefront has read all of the step before it:
+    // A step is two or four parts of 16.  While the products of one part run, the operands of the next are read, so that the matrix pipe finds them
+    // there; the barrier that hands a stage over stands ahead of the last part's products, when every wavefront has read all of the step:
     // its stage is free and is asked for again at once, STAGES steps ahead.  (Past the end the requests go on, out of range, so that their count
     // stays what the wait expects.)
-    const int n_steps = (depth + kGemmStep - 1) / kGemmStep;
+    const int n_steps = (depth + STEP - 1) / STEP;
     u32x4_t nv[2][NB], mv[2][MB];
     auto read = [&](int set, const uint16_t* st, int kk) {
         const uint16_t* const n_from = st + n_at[NT ? 0 : kk];
@@ -351,7 +354,7 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
             if constexpr (NT) {
                 nv[set][i] = read_across(st + n_at[i] + 16 * kk * BN, BN);
             } else {
-                nv[set][i] = *reinterpret_cast<const u32x4_t*>(n_from + 32 * i * kGemmStep);
+                nv[set][i] = *reinterpret_cast<const u32x4_t*>(n_from + 32 * i * STEP);
             }
         }
 #pragma unroll
@@ -359,7 +362,7 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
             if constexpr (MT) {
                 mv[set][j] = read_across(st + m_at[j] + 16 * kk * BM, BM);
             } else {
-                mv[set][j] = *reinterpret_cast<const u32x4_t*>(m_from + 32 * j * kGemmStep);
+                mv[set][j] = *reinterpret_cast<const u32x4_t*>(m_from + 32 * j * STEP);
             }
         }
     };
@@ -394,10 +397,13 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
     for (int t = 0; t < n_steps; ++t) {
         __builtin_amdgcn_sched_barrier(0);
         const uint16_t* const st = s_tiles + stage * kStage;
-        read(1, st, 1);
-        multiply(0);
-        order();
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int h = 0; h + 1 < kParts; ++h) {
+            read((h + 1) & 1, st, h + 1);
+            multiply(h & 1);
+            order();
+            __builtin_amdgcn_sched_barrier(0);
+        }
         __builtin_amdgcn_s_waitcnt(gemm_wait((STAGES - 2) * kReqs, 0));
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);

@@ -7,10 +7,10 @@
 
 namespace hstu {
 
-template <typename Tag, int MODE, int MB, int NB, int STAGES, int PER_CU>
+template <typename Tag, int MODE, int MB, int NB, int STAGES, int PER_CU, int STEP = kGemmStep>
 constexpr GatedTile gated_tile(const char* name, float alone, float step, float fixed)
 {
-    return {gated_gemm_kernel<Tag, MODE, 2, 2, MB, NB, STAGES, PER_CU>, name, 64 * NB / (MODE == kGemmForward || MODE == kGemmMixedGrad ? 2 : 1), 64 * MB, alone, step, fixed};
+    return {gated_gemm_kernel<Tag, MODE, 2, 2, MB, NB, STAGES, PER_CU, STEP>, name, 64 * NB / (MODE == kGemmForward || MODE == kGemmMixedGrad ? 2 : 1), 64 * MB, alone, step, fixed};
 }
 
 // (names: rows x columns of the products' tiles)
@@ -18,7 +18,7 @@ template <typename Tag>
 const GatedKernels& gated_table()
 {
     static const GatedKernels table = {
-        {gated_tile<Tag, kGemmForward, 4, 4, 4, 1>("gated_gemm_256x256", 0.66f, 0.75f, 10.0f), gated_tile<Tag, kGemmForward, 2, 4, 3, 2>("gated_gemm_128x256", 0.45f, 0.45f, 3.5f),
+        {gated_tile<Tag, kGemmForward, 4, 4, 2, 1, 64>("gated_gemm_256x256", 0.64f, 0.73f, 10.0f), gated_tile<Tag, kGemmForward, 2, 4, 3, 2>("gated_gemm_128x256", 0.45f, 0.45f, 3.5f),
          gated_tile<Tag, kGemmForward, 2, 2, 3, 3>("gated_gemm_128x128", 0.33f, 0.26f, 3.0f), gated_tile<Tag, kGemmForward, 1, 2, 3, 4>("gated_gemm_64x128", 0.25f, 0.17f, 2.0f)},
         {gated_tile<Tag, kGemmMixedGrad, 2, 4, 3, 2>("gated_gemm_128x256", 0.45f, 0.45f, 3.5f), gated_tile<Tag, kGemmMixedGrad, 2, 2, 3, 3>("gated_gemm_128x128", 0.33f, 0.26f, 3.0f),
          gated_tile<Tag, kGemmMixedGrad, 1, 2, 3, 4>("gated_gemm_64x128", 0.25f, 0.17f, 2.0f)},
