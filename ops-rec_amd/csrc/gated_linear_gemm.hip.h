@@ -33,6 +33,9 @@ constexpr int kGemmBand = 8;  // row tiles of a band
 
 __device__ __forceinline__ float gated_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f)); }
 
+// z, at most 30 from zero; NaN stays NaN (which the minimum of a maximum would make -30)
+__device__ __forceinline__ float gated_bounded(float z) { return z > 30.0f ? 30.0f : z < -30.0f ? -30.0f : z; }
+
 // act(z): silu, gelu by its tanh form -- z * sigmoid(2 sqrt(2 / pi) (z + 0.044715 z^3)) --, or the sigmoid.  (hardware exp2 and reciprocal, 1 ulp
 // each: the results are rounded to 8 or 11 bits.  Past |z| = 30 gelu's cube could make infinity times 0: its argument is bounded there, where the
 // sigmoid is 0 or 1 to all bits.)
@@ -42,7 +45,7 @@ __device__ __forceinline__ float gated_act(float z)
     if constexpr (ACT == kActSilu) {
         return z * gated_sigmoid(z);
     } else if constexpr (ACT == kActGelu) {
-        const float t = fminf(fmaxf(z, -30.0f), 30.0f);
+        const float t = gated_bounded(z);
         return z * gated_sigmoid(1.5957691216057308f * t * __builtin_fmaf(0.044715f * t, t, 1.0f));
     } else {
         return gated_sigmoid(z);
@@ -89,7 +92,7 @@ __device__ __forceinline__ void gated_act_slope(float z, float& act, float& slop
         act = z * s;
         slope = s * __builtin_fmaf(z, 1.0f - s, 1.0f);
     } else if constexpr (ACT == kActGelu) {
-        const float t = fminf(fmaxf(z, -30.0f), 30.0f);
+        const float t = gated_bounded(z);
         const float s = gated_sigmoid(1.5957691216057308f * t * __builtin_fmaf(0.044715f * t, t, 1.0f));
         act = z * s;
         slope = s * __builtin_fmaf(t * (1.0f - s), 1.5957691216057308f * __builtin_fmaf(0.134145f * t, t, 1.0f), 1.0f);
