@@ -85,6 +85,15 @@ auto operator_handle(const char* name, const char* overload)
 inline bool needs_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 inline bool needs_grad(const OptTensor& t) { return t.has_value() && needs_grad(*t); }
 
+// Forward-mode differentiation: operators without a formula for it refuse a tangent, which would be lost below autograd.
+inline bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+inline bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
+template <typename... T>
+void refuse_tangents(const char* op, const T&... inputs)
+{
+    TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(inputs) || ...), op, ": forward-mode differentiation is not implemented; do not pass inputs with a tangent");
+}
+
 inline Tensor unwrap(const OptTensor& t) { return t.value_or(Tensor()); }
 inline OptTensor wrap(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 

@@ -193,6 +193,7 @@ struct ResidualNormFunction : torch::autograd::Function<ResidualNormFunction> {
 Pair residual_norm_autograd(const Tensor& x, const Tensor& residual, const Tensor& gamma, const OptTensor& beta, const OptTensor& scale, double epsilon,
                             bool rms)
 {
+    refuse_tangents("residual_norm", x, residual, gamma, beta, scale);
     if (!at::GradMode::is_enabled() || !(needs_grad(x) || needs_grad(residual) || needs_grad(gamma) || needs_grad(beta) || needs_grad(scale))) {
         static const auto op = operator_handle<decltype(residual_norm)>("ops_rec::residual_norm", "");
         const at::AutoDispatchBelowADInplaceOrView below;
@@ -311,6 +312,7 @@ struct NormGateFunction : torch::autograd::Function<NormGateFunction> {
 Tensor norm_gate_autograd(const Tensor& x, const OptTensor& gate, const Tensor& gamma, const OptTensor& beta, const OptTensor& residual,
                           double residual_scale, int64_t groups, double epsilon, bool rms, bool silu)
 {
+    refuse_tangents("norm_gate", x, gate, gamma, beta, residual);
     if (!at::GradMode::is_enabled() || !(needs_grad(x) || needs_grad(gate) || needs_grad(gamma) || needs_grad(beta) || needs_grad(residual))) {
         static const auto op = operator_handle<decltype(norm_gate)>("ops_rec::norm_gate", "");
         const at::AutoDispatchBelowADInplaceOrView below;
@@ -404,6 +406,7 @@ struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
 Pair rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& frequencies, const OptTensor& seq_offset, const OptTensor& start,
                      const OptTensor& positions, bool interleaved, double magnitude, bool inverse)
 {
+    refuse_tangents("rotary", q, k, frequencies);
     if (!at::GradMode::is_enabled() || !(needs_grad(q) || needs_grad(k) || needs_grad(frequencies))) {
         static const auto op = operator_handle<decltype(rotary)>("ops_rec::rotary", "");
         const at::AutoDispatchBelowADInplaceOrView below;
@@ -525,6 +528,7 @@ struct GatedLinearFunction : torch::autograd::Function<GatedLinearFunction> {
 
 Pair gated_linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& bias, c10::string_view activation, bool keep)
 {
+    refuse_tangents("gated_linear", x, weight, bias);
     if (!at::GradMode::is_enabled() || !(needs_grad(x) || needs_grad(weight) || needs_grad(bias))) {
         static const auto op = operator_handle<decltype(gated_linear)>("ops_rec::gated_linear", "");
         const at::AutoDispatchBelowADInplaceOrView below;

@@ -18,6 +18,7 @@ import math
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _native
 from ._ops import _DTYPE_CODE, _PYTHON_KERNELS, _check, _lib_def, _lib_meta, _ptr
@@ -46,6 +47,12 @@ def _on_device(device, named) -> None:
     _check(device.type == "cuda", f"{named[0][0]} must be a GPU tensor, but it is on {device}")
     for name, t in named:
         _check(t is None or t.device == device, f"{name} must be on the device of {named[0][0]} ({device}), but it is on {getattr(t, 'device', None)}")
+
+
+def _no_tangents(op, *tensors) -> None:
+    """No formulas for forward-mode differentiation: a tangent would be lost."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{op}: forward-mode differentiation is not implemented; do not pass inputs with a tangent")
 
 
 def _rows(t: Optional[torch.Tensor]):
@@ -109,6 +116,7 @@ def residual_norm(x, residual, gamma, beta=None, scale=None, epsilon=1e-5, rms=F
     ``norm`` takes mean and variance over the columns, or with ``rms`` the root mean square alone.  x is fp32, bf16 or fp16, the residual stream of
     the same type or fp32, gamma, beta and scale (one value per column) all fp32 or all of the type of x.  Rows may be strided; arithmetic is fp32, and
     y is the norm of the sum as it is before it is rounded."""
+    _no_tangents("residual_norm", x, residual, gamma, beta, scale)
     _residual_norm_checks(x, residual, gamma, beta, scale, epsilon)
     _on_device(x.device, (("x", x), ("residual", residual), ("gamma", gamma), ("beta", beta), ("scale", scale)))
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
@@ -212,6 +220,7 @@ def norm_gate(x, gate, gamma, beta=None, residual=None, residual_scale=1.0, grou
 
     x is fp32, bf16 or fp16, the gate the same, the residual the same or fp32, gamma and beta (one value per column) both fp32 or both
     of the type of x.  Rows may be strided; arithmetic is fp32, rounded once."""
+    _no_tangents("norm_gate", x, gate, gamma, beta, residual)
     _norm_gate_checks(x, gate, gamma, beta, residual, groups, epsilon)
     _on_device(x.device, (("x", x), ("gate", gate), ("gamma", gamma), ("beta", beta), ("residual", residual)))
     stream_dtype = x.dtype if residual is None else residual.dtype
@@ -338,6 +347,7 @@ def rotary(q, k, frequencies, seq_offset=None, start=None, positions=None, inter
     cache holds already); or ``positions[row]``, for everything else (targets that stand at one place, gaps).  Rows of no sequence come
     out as zeros.  ``frequencies`` is fp64 (``rotary_frequencies``), and angles are formed in 64 bits.  q and k are fp32, bf16 or fp16, with any strides
     whose last is 1; the results are new and contiguous."""
+    _no_tangents("rotary", q, k, frequencies)
     _rotary_checks(q, k, frequencies, seq_offset, start, positions)
     _on_device(q.device, (("q", q), ("k", k), ("frequencies", frequencies), ("seq_offset", seq_offset), ("start", start), ("positions", positions)))
     q_out, k_out = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
@@ -413,6 +423,7 @@ def gated_linear(x, weight, bias=None, activation="silu", keep=False):
     prefer, the backward multiplies again, which takes 14 % more of a training step at 512 columns of x and 26 % at 2048.  Up to 192 columns that is faster,
     and mixed is empty either way.  ``activation`` is "silu", "gelu" (by its tanh form) or "sigmoid".  x, weight and bias are all bf16 or all fp16; cols
     and inner are multiples of 8.  Sums are fp32, and hidden is taken of them."""
+    _no_tangents("gated_linear", x, weight, bias)
     _gated_linear_checks(x, weight, bias, activation)
     _on_device(x.device, (("x", x), ("weight", weight), ("bias", bias)))
     inner = weight.size(0) // 2
