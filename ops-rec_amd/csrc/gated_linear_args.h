@@ -22,6 +22,7 @@ struct GatedGemmArgs {
     int chunks;
     int activation;
     int tiles_m, tiles_n;
+    uint32_t first, count;  // of the tiles of all chunks: what this launch has
 };
 
 // gated_few_rows_kernel (gated_linear_few_rows.hip.h)

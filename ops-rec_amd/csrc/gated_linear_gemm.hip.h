@@ -153,12 +153,11 @@ __global__ __launch_bounds__(kGemmThreads, PER_CU) void gated_gemm_kernel(const 
 
     // ---- the workgroup's tile
     const uint32_t tiles = static_cast<uint32_t>(a.tiles_m) * static_cast<uint32_t>(a.tiles_n);
-    const uint32_t all = tiles * static_cast<uint32_t>(a.chunks);
-    const uint32_t each = (all + 7u) >> 3;
-    const uint32_t place = (blockIdx.x & 7u) * each + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= each || place >= all) {
+    const uint32_t each = (a.count + 7u) >> 3, in_launch = (blockIdx.x & 7u) * each + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= each || in_launch >= a.count) {
         return;
     }
+    const uint32_t place = a.first + in_launch;
     const uint32_t part = place / tiles, tile = place - part * tiles;
     const uint32_t in_band = static_cast<uint32_t>(kGemmBand) * static_cast<uint32_t>(a.tiles_n);
     const uint32_t band = tile / in_band, at = tile - band * in_band;

@@ -19,6 +19,7 @@ constexpr int64_t kStep = 32;          // of a product's depth
 constexpr int64_t kFewRows = 96;       // of a workgroup of the kernel for few rows
 constexpr int64_t kMostCols = 1 << 21; // (256 rows of twice as many columns lie behind one descriptor of 2^31 bytes)
 constexpr int64_t kMostBytes = int64_t{1} << 31;  // behind one descriptor
+constexpr int64_t kMostWorkgroups = (1 << 24) - 8;  // of a launch, which has less than 2^32 threads; whole eights
 
 const hstu::GatedKernels& kernels_of(int dtype) { return dtype == HSTU_DT_BF16 ? hstu::gated_kernels_bf16() : hstu::gated_kernels_f16(); }
 
@@ -124,8 +125,16 @@ int launch_tiles(const GatedTile& t, GatedGemmArgs a, void* stream, const char* 
     if (all > 0x70000000) {
         return set_error(HSTU_ERR_INVALID, "%s would take %lld workgroups", what, static_cast<long long>(all));
     }
-    hipLaunchKernelGGL(t.kernel, dim3(static_cast<uint32_t>(ceil_div(all, 8) * 8)), dim3(256), 0, static_cast<hipStream_t>(stream), a);
-    return launched(what);
+    for (int64_t first = 0; first < all; first += kMostWorkgroups) {
+        const int64_t count = all - first < kMostWorkgroups ? all - first : kMostWorkgroups;
+        a.first = static_cast<uint32_t>(first);
+        a.count = static_cast<uint32_t>(count);
+        hipLaunchKernelGGL(t.kernel, dim3(static_cast<uint32_t>(ceil_div(count, 8) * 8)), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+        if (const int rc = launched(what); rc != HSTU_OK) {
+            return rc;
+        }
+    }
+    return HSTU_OK;
 }
 
 // A gradient's product: its tile, and the chunks its depth is cut into where the tiles are too few for the machine -- one or two workgroups to a compute
