@@ -177,7 +177,9 @@ HSTU_API int gated_linear_fwd(const gated_linear_params* params, void* stream);
 HSTU_API const char* gated_linear_fwd_kernel_name(const gated_linear_params* params);
 
 /* The gradients of gated_linear.  `fwd` describes the call as it was, with mixed as it was written (hidden is not read), or
- * NULL: g and u are then multiplied again. */
+ * NULL: g and u are then multiplied again.  The gradients of g and u are rounded to the type of x for the products behind them, half a step of it; in fp16 all
+ * of a call's are multiplied by a power of two first, chosen on the device by the largest, so that none is past 65504 and the steps of the smallest are 2^-22 of
+ * the largest at most. */
 typedef struct gated_linear_bwd_params {
     uint32_t struct_size; /* sizeof(gated_linear_bwd_params), checked */
     uint32_t reserved0;

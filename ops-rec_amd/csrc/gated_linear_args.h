@@ -4,6 +4,9 @@
 
 namespace hstu {
 
+// What d_mixed is multiplied by in fp16 where its values allow it: from 2^-11 to 255 for the largest (gated_range_kernel).
+constexpr float kGatedScale = 256.0f;
+
 constexpr int kActSilu = 0, kActGelu = 1, kActSigmoid = 2;
 
 // gated_gemm_kernel (gated_linear_gemm.hip.h): out[rows, cols] = a . b over `depth`
@@ -14,6 +17,8 @@ struct GatedGemmArgs {
     void* out;           // forward: hidden [rows, cols], or nullptr; d_mixed: [rows, 2 cols]; gradients: [rows, cols]
     void* mixed;         // forward: [rows, 3 cols] (kept_high), or nullptr
     const void* grad;    // d_mixed: the gradient of hidden [rows, cols]
+    float* range;        // d_mixed, fp16: the largest of each wavefront's values [tiles][4], or nullptr
+    const float* scale;  // fp16: [0] what d_mixed is multiplied by, [1] the inverse.  d_mixed: of a second pass, nullptr in the first; gradients: always
     float* partial;      // gradients in several chunks of the depth: [chunks][rows][cols]; d_mixed: column sums [2 row tiles][2 cols], or nullptr
     int64_t rows;
     int64_t depth;
@@ -44,6 +49,8 @@ struct GatedStageArgs {
     const void* mixed;  // [rows, 3 inner]
     void* d_mixed;      // [rows, 2 inner]
     float* partial;     // [slices][2 inner] column sums, or nullptr
+    float* range;       // as in GatedGemmArgs, [workgroups][4]
+    const float* scale;
     int64_t rows;
     int inner;
     int slices;
@@ -51,6 +58,7 @@ struct GatedStageArgs {
 };
 struct GatedSumArgs {
     const float* partial;  // [chunks][n]
+    const float* scale;    // fp16: as in GatedGemmArgs
     void* out;             // [n], 16-bit
     int64_t n;             // a multiple of 8
     int chunks;

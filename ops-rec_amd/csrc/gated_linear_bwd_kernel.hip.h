@@ -4,7 +4,7 @@
 //   d bias = column sums of d mixed, taken of the values before they are rounded
 //
 // Bound by HBM: 8 bytes read and 4 written per column of hidden.  (d mixed is rounded to the type of x, half a step of it: what the matrix instructions of
-// the products behind it multiply.)  A thread has 8 columns and walks over the rows of its slice; its
+// the products behind it multiply; in fp16 it is scaled ahead of that, kGatedScaled.)  A thread has 8 columns and walks over the rows of its slice; its
 // sums stay in registers, those of a workgroup's eight rows of threads meet in LDS, and a row of partial sums per workgroup goes to the workspace.
 #pragma once
 #include "gated_linear_gemm.hip.h"
@@ -24,6 +24,23 @@ __global__ __launch_bounds__(kStageThreads) void gated_stage_kernel(const GatedS
     const uint32_t slice = blockIdx.x / blocks;
     const int col = static_cast<int>(blockIdx.x - slice * blocks) * kStageCols + 8 * c;
     const bool have = col < a.inner;
+    float scale = kGatedScale, largest = 0.0f;
+    if constexpr (kGatedScaled<Tag>) {
+        if (a.scale != nullptr) {
+            scale = *a.scale;
+            if (scale == kGatedScale) {  // the first pass was enough
+                return;
+            }
+        }
+    }
+    const auto pack = [&](float x, float y) {
+        if constexpr (kGatedScaled<Tag>) {
+            largest = gated_larger(gated_larger(largest, x), y);
+            x *= scale;
+            y *= scale;
+        }
+        return pack2<Tag>(x, y);
+    };
     float dg[8], du[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -58,14 +75,19 @@ __global__ __launch_bounds__(kStageThreads) void gated_stage_kernel(const GatedS
                         dg[2 * e + h] += x[h];
                         du[2 * e + h] += y[h];
                     }
-                    og[e] = pack2<Tag>(x[0], x[1]);
-                    ou[e] = pack2<Tag>(y[0], y[1]);
+                    og[e] = pack(x[0], x[1]);
+                    ou[e] = pack(y[0], y[1]);
                 }
                 uint16_t* const to = static_cast<uint16_t*>(a.d_mixed) + row * 2 * a.inner + col;
                 *reinterpret_cast<u32x4_t*>(to) = og;
                 *reinterpret_cast<u32x4_t*>(to + a.inner) = ou;
             }
         });
+    }
+    if constexpr (kGatedScaled<Tag>) {
+        if (a.range != nullptr) {
+            gated_note_range(largest, a.range + static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64);
+        }
     }
     if (a.partial == nullptr) {
         return;
@@ -107,6 +129,13 @@ __global__ __launch_bounds__(256) void gated_sum_kernel(const GatedSumArgs a)
             const float4 lo = from[0], hi = from[1];
             t[0] += lo.x, t[1] += lo.y, t[2] += lo.z, t[3] += lo.w;
             t[4] += hi.x, t[5] += hi.y, t[6] += hi.z, t[7] += hi.w;
+        }
+        if constexpr (kGatedScaled<Tag>) {
+            const float back = a.scale[1];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                t[e] *= back;
+            }
         }
         const u32x4_t w = {pack2<Tag>(t[0], t[1]), pack2<Tag>(t[2], t[3]), pack2<Tag>(t[4], t[5]), pack2<Tag>(t[6], t[7])};
         reinterpret_cast<u32x4_t*>(a.out)[i] = w;

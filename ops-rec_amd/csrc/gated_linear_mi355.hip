@@ -7,6 +7,43 @@
 #include "hstu_error.h"
 #include "layer_args.h"
 
+namespace hstu {
+
+// The largest of n magnitudes of d_mixed -> the power of two it is multiplied by in fp16, and the inverse.  kGatedScale stays where the largest fits, and where a
+// step of fp16 from zero (2^-24) is 2^-22 of it at most; otherwise the largest comes to lie in [2^14, 2^15).
+constexpr int kRangeThreads = 1024;
+__global__ __launch_bounds__(kRangeThreads) void gated_range_kernel(const float* range, int64_t n, float* scale)
+{
+    __shared__ float s_largest[kRangeThreads / 64];
+    float largest = 0.0f;
+    for (int64_t i = threadIdx.x; i < n; i += kRangeThreads) {
+        largest = fmaxf(largest, range[i]);
+    }
+#pragma unroll
+    for (int i = 32; i > 0; i /= 2) {
+        largest = fmaxf(largest, __shfl_xor(largest, i));
+    }
+    if (threadIdx.x % 64 == 0) {
+        s_largest[threadIdx.x / 64] = largest;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < kRangeThreads / 64; ++i) {
+            largest = fmaxf(largest, s_largest[i]);
+        }
+        float by = kGatedScale;
+        if (largest > 0.0f && (largest * by > 65504.0f || largest * by < 0.125f)) {
+            int exponent = 0;
+            frexpf(largest, &exponent);  // largest < 2^exponent
+            by = ldexpf(1.0f, min(15 - exponent, 100));
+        }
+        scale[0] = by;
+        scale[1] = 1.0f / by;
+    }
+}
+
+}  // namespace hstu
+
 namespace {
 
 using hstu::GatedGemmArgs;
@@ -171,8 +208,9 @@ uint64_t rounded(uint64_t bytes) { return (bytes + 255u) & ~uint64_t{255}; }
 struct BackwardPlan {
     Product x, w;
     int slices;
-    uint64_t d_mixed, sums, x_partial, w_partial;  // bytes, in this order
-    uint64_t total() const { return d_mixed + sums + (x_partial > w_partial ? x_partial : w_partial); }
+    int64_t ranges;  // fp16: magnitudes that the pass of d_mixed notes, four a workgroup
+    uint64_t d_mixed, sums, range, x_partial, w_partial;  // bytes, in this order
+    uint64_t total() const { return d_mixed + sums + range + (x_partial > w_partial ? x_partial : w_partial); }
 };
 
 BackwardPlan plan_backward(const gated_linear_bwd_params* p)
@@ -187,6 +225,11 @@ BackwardPlan plan_backward(const gated_linear_bwd_params* p)
     b.slices = static_cast<int>(f.mixed == nullptr ? 2 * ceil_div(f.rows, mixed_tile(&f).rows) : useful < most ? useful : most);
     b.d_mixed = rounded(static_cast<uint64_t>(f.rows) * static_cast<uint64_t>(f.inner) * 4u);
     b.sums = p->bias_grad != nullptr ? rounded(static_cast<uint64_t>(b.slices) * static_cast<uint64_t>(f.inner) * 8u) : 0;
+    if (f.dtype == HSTU_DT_FP16) {  // (two floats of scale ahead of them)
+        const GatedTile& t = mixed_tile(&f);
+        b.ranges = 4 * (f.mixed == nullptr ? ceil_div(f.rows, t.rows) * ceil_div(f.inner, t.cols) : b.slices * blocks);
+        b.range = rounded(static_cast<uint64_t>(b.ranges + 2) * 4u);
+    }
     if (p->x_grad != nullptr) {
         b.x = plan(k.x_grad, hstu::kGatedXGradTiles, f.rows, f.cols, 2 * f.inner, f.cols * 2);
         b.x_partial = b.x.chunks > 1 ? static_cast<uint64_t>(b.x.chunks) * static_cast<uint64_t>(f.rows) * static_cast<uint64_t>(f.cols) * 4u : 0;
@@ -232,6 +275,7 @@ int launch_product(const hstu::GatedKernels& k, const Product& plan, GatedGemmAr
     }
     hstu::GatedSumArgs s{};
     s.partial = partial;
+    s.scale = a.scale;
     s.out = a.out;
     s.n = a.rows * a.cols;
     s.chunks = a.chunks;
@@ -322,9 +366,20 @@ HSTU_API int gated_linear_bwd(const gated_linear_bwd_params* p, void* workspace,
     const gated_linear_params& f = p->fwd;
     const hstu::GatedKernels& k = kernels_of(f.dtype);
     uint8_t* const ws = static_cast<uint8_t*>(workspace);
-    float* const partial = reinterpret_cast<float*>(ws + b.d_mixed + b.sums);
+    float* const scale = b.range != 0 ? reinterpret_cast<float*>(ws + b.d_mixed + b.sums) : nullptr;
+    float* const partial = reinterpret_cast<float*>(ws + b.d_mixed + b.sums + b.range);
 
     float* const sums = p->bias_grad != nullptr ? reinterpret_cast<float*>(ws + b.d_mixed) : nullptr;
+    // d_mixed: one pass, and in fp16 another that starts only where the first one's scale does not do (every launch is made: the host does not wait to see)
+    const auto in_range = [&](auto&& pass) {
+        int code = pass(scale == nullptr ? nullptr : scale + 2, nullptr);
+        if (code != HSTU_OK || scale == nullptr) {
+            return code;
+        }
+        hipLaunchKernelGGL(hstu::gated_range_kernel, dim3(1), dim3(hstu::kRangeThreads), 0, static_cast<hipStream_t>(stream), scale + 2, b.ranges, scale);
+        code = launched("gated_range_kernel");
+        return code != HSTU_OK ? code : pass(nullptr, scale);
+    };
     if (f.mixed == nullptr) {
         GatedGemmArgs a{};
         a.n_side = f.weight;
@@ -332,25 +387,33 @@ HSTU_API int gated_linear_bwd(const gated_linear_bwd_params* p, void* workspace,
         a.bias = f.bias;
         a.grad = p->grad;
         a.out = ws;
-        a.partial = sums;
         a.rows = f.rows;
         a.depth = a.chunk = f.cols;
         a.cols = static_cast<int>(f.inner);
         a.chunks = 1;
         a.activation = f.activation;
-        rc = launch_tiles(mixed_tile(&f), a, stream, "gated_gemm_kernel (d_mixed)");
+        rc = in_range([&](float* range, const float* by) {
+            a.range = range;
+            a.scale = by;
+            a.partial = by == nullptr ? sums : nullptr;
+            return launch_tiles(mixed_tile(&f), a, stream, "gated_gemm_kernel (d_mixed)");
+        });
     } else {
         hstu::GatedStageArgs s{};
         s.grad = p->grad;
         s.mixed = f.mixed;
         s.d_mixed = ws;
-        s.partial = sums;
         s.rows = f.rows;
         s.inner = static_cast<int>(f.inner);
         s.slices = b.slices;
         s.activation = f.activation;
-        hipLaunchKernelGGL(k.stage, dim3(static_cast<uint32_t>(b.slices * ceil_div(f.inner, 256))), dim3(256), 0, static_cast<hipStream_t>(stream), s);
-        rc = launched("gated_stage_kernel");
+        rc = in_range([&](float* range, const float* by) {
+            s.range = range;
+            s.scale = by;
+            s.partial = by == nullptr ? sums : nullptr;
+            hipLaunchKernelGGL(k.stage, dim3(static_cast<uint32_t>(b.slices * ceil_div(f.inner, 256))), dim3(256), 0, static_cast<hipStream_t>(stream), s);
+            return launched("gated_stage_kernel");
+        });
     }
     if (rc == HSTU_OK && p->bias_grad != nullptr) {
         hstu::NormSumsArgs n{};
@@ -366,6 +429,7 @@ HSTU_API int gated_linear_bwd(const gated_linear_bwd_params* p, void* workspace,
         GatedGemmArgs a{};
         a.n_side = f.weight;
         a.m_side = ws;
+        a.scale = scale;
         a.out = p->x_grad;
         a.rows = f.rows;
         a.depth = 2 * f.inner;
@@ -376,6 +440,7 @@ HSTU_API int gated_linear_bwd(const gated_linear_bwd_params* p, void* workspace,
         GatedGemmArgs a{};
         a.n_side = f.x;
         a.m_side = ws;
+        a.scale = scale;
         a.out = p->weight_grad;
         a.rows = 2 * f.inner;
         a.depth = f.rows;

@@ -1,10 +1,13 @@
 """gated_linear's backward where tests/test_layer_gated_linear.py does not go: values that are not finite, the ends of fp16, every tile of its products, what is kept above
 192 columns of x, and the largest sizes."""
 
+import math
+
 import pytest
 import torch
 
 import ops_rec
+import layer_reference as R
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -17,6 +20,55 @@ def _memory_goes_back():
     """Cached blocks go back to the device after each test: tests that count what the allocator takes find it as they expect it."""
     yield
     torch.cuda.empty_cache()
+
+
+def randn(gen, *shape, dtype, std=1.0):
+    return (torch.randn(*shape, generator=gen) * std).to(dtype)
+
+
+def act(name, z):
+    if name == "gelu":
+        return z * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z**3))
+    return torch.sigmoid(z) * (z if name == "silu" else 1)
+
+
+def growth(n):
+    """Of a sum of n products in fp32, relative to the sum of their magnitudes: n / 2^24 at most, and in trees and chains whose errors do not all go one way
+    2^-18 up to 2^12 products and sqrt(n) / 2^24 beyond."""
+    return max(2.0**-18, math.sqrt(n) * 2.0**-24)
+
+
+def definition(x, w, b, dh, activation):
+    """The gradients of x, weight and bias in 64 bits, on the device of the inputs, each with the room of a kernel that multiplies d_mixed in the inputs' type.
+
+    g and u are off by what their sums in fp32 are, and cut to 24 bits; the activations and their slopes have slopes of 1.13 at most, and the hardware's exponential
+    and reciprocal are off by 2^-22.  d_mixed is rounded by half a step, in fp16 at a scale at which a step from zero is 2^-22 of its largest value at most."""
+    half, inner = R.HALF_STEP[x.dtype], dh.size(1)
+    x64, w64, dh64 = x.double(), w.double(), dh.double()
+    b64 = torch.zeros(2 * inner, dtype=torch.float64, device=x.device) if b is None else b.double()
+    mixed, size = x64 @ w64.t() + b64, x64.abs() @ w64.abs().t() + b64.abs()
+    (g, u), (eg, eu) = mixed.chunk(2, dim=1), (growth(x.size(1)) * size).chunk(2, dim=1)
+    gl = g.detach().clone().requires_grad_(True)
+    a = act(activation, gl)
+    (slope,) = torch.autograd.grad(a.sum(), gl)
+    a = a.detach()
+    d = torch.cat([dh64 * u * slope, dh64 * a], dim=1)
+    rg, ru = (2.0**-15 * (t.abs() + e) + e for t, e in ((g, eg), (u, eu)))
+    room = torch.cat([dh64.abs() * (slope.abs() * ru + 1.13 * rg * (u.abs() + ru)), dh64.abs() * 1.13 * rg], dim=1) + 2.0**-20 * d.abs()
+    rounded = room + half * (d.abs() + room) + (2.0**-22 * d.abs().max() if x.dtype == FP16 else 0.0)
+    n = x.size(0)
+    return ((d @ w64, rounded @ w64.abs() + growth(2 * inner) * (d.abs() @ w64.abs())),
+            (d.t() @ x64, rounded.t() @ x64.abs() + growth(n) * (d.abs().t() @ x64.abs())),
+            (d.sum(0), room.sum(0) + growth(n) * d.abs().sum(0)))  # fmt: skip
+
+
+def compare(got, want, what):
+    ref, room = want
+    assert got.shape == ref.shape, what
+    room = R.HALF_STEP[got.dtype] * ref.abs() * (1 + 2.0**-7) + room + (2.0**-25 if got.dtype == FP16 else 0.0)
+    off = (got.detach().double() - ref).abs()
+    bad = ~(off <= room)
+    assert not bad.any(), (what, int(bad.sum()), off[bad].max().item(), room[bad].min().item())
 
 
 @pytest.mark.parametrize("activation", ["silu", "gelu", "sigmoid"])
@@ -67,3 +119,59 @@ def test_more_tiles_than_a_launch_has_workgroups():
     del hidden
     got = A.gated_linear_backward(repeated(dh, rows), many, w, None, torch.empty(0, dtype=torch.int16, device=DEV), "silu", [True, False, False])[0]
     assert is_repeated(got, dx)
+
+
+def ends_of_fp16(kind, cols, gen):
+    """x, weight, bias and the gradient of hidden in fp16, whose d_mixed is past 65504 ("past"), among the subnormals ("small"), or below all of them ("below"), while the
+    gradients of x and weight are well inside."""
+    rows, inner = 700, 72
+    grad, x, w, b = {"past": (2.0**13, 2.0**-11, 2.0**-7, 16.0), "small": (2.0**-12, 2.0**4, 2.0**-4, 2.0**-5), "below": (2.0**-24, 2.0**8, 2.0**-8, 2.0**-10)}[kind]
+    bias = randn(gen, 2 * inner, dtype=FP16, std=b)
+    weight = randn(gen, 2 * inner, cols, dtype=FP16, std=w)
+    if kind != "past":  # (u as small as its bias)
+        weight[inner:] = 0
+    if kind == "below":  # (and gates of about a half)
+        weight[:inner] *= 2.0**-4
+    return randn(gen, rows, cols, dtype=FP16, std=x), weight, bias, randn(gen, rows, inner, dtype=FP16, std=grad)
+
+
+@pytest.mark.parametrize("kind", ["past", "small", "below"])
+@pytest.mark.parametrize("cols,keep", [(64, False), (200, True), (200, False)])
+def test_the_ends_of_fp16(kind, cols, keep):
+    g = torch.Generator().manual_seed(cols)
+    x, w, b, dh = (t.to(DEV) for t in ends_of_fp16(kind, cols, g))
+    want = definition(x, w, b, dh, "silu")
+    assert all(t[0].abs().max() < 60000 for t in want[:2])
+    leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+    hidden, mixed = A.gated_linear(*leaves, b, "silu", keep)
+    assert (mixed.numel() != 0) == keep
+    for got, ref, name in zip(torch.autograd.grad(hidden, leaves, dh), want, ("x", "weight")):
+        compare(got, ref, name)
+
+
+@pytest.mark.parametrize("cols", [64, 200])
+def test_a_captured_step_follows_the_size_of_its_gradients(cols):
+    gen = torch.Generator().manual_seed(3)
+    x, w, b, dh = (t.to(DEV) for t in ends_of_fp16("past", cols, gen))
+    dh.mul_(2.0**-10)
+
+    def step():
+        mixed = A.gated_linear(x, w, b, "silu", True)[1]
+        return A.gated_linear_backward(dh, x, w, b, mixed, "silu", [True, True, False])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for by in (1.0, 2.0**10, 2.0**-25, 2.0**12, 2.0**3):
+        dh.mul_(by)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = definition(x, w, b, dh, "silu")
+        for got, ref, eager, name in zip(outs[:2], want, step(), ("x", "weight")):
+            assert torch.equal(got, eager)
+            compare(got, ref, name)
