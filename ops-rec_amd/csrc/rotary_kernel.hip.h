@@ -99,15 +99,21 @@ __device__ __forceinline__ int rotary_sequence(const void* offsets, int n, int i
 }
 
 // cos and sin of `turns` full turns, |turns| <= 1/2: the hardware's instructions take turns, and are exact enough for results of
-// 16 bits; fp32 results go through the library
+// 16 bits; fp32 results go through the library, and are turned on by what the 32 bits of its argument leave of the angle (up to 2^-26 of a turn, which would be
+// more than the rounding of the results)
 template <typename T>
-__device__ __forceinline__ void rotary_turn(float turns, float& c, float& s)
+__device__ __forceinline__ void rotary_turn(double turns, float& c, float& s)
 {
+    const float most = static_cast<float>(turns);
     if constexpr (ln_traits<T>::kPerChunk == 4) {
-        sincospif(2.0f * turns, &s, &c);
+        float c0, s0;
+        sincospif(2.0f * most, &s0, &c0);
+        const float rest = static_cast<float>(turns - most) * 6.2831853f;
+        c = __builtin_fmaf(-rest, s0, c0);
+        s = __builtin_fmaf(rest, c0, s0);
     } else {
-        c = __builtin_amdgcn_cosf(turns);
-        s = __builtin_amdgcn_sinf(turns);
+        c = __builtin_amdgcn_cosf(most);
+        s = __builtin_amdgcn_sinf(most);
     }
 }
 
@@ -177,7 +183,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
             const int at = INTERLEAVED ? (j < kValues / 2 ? c0 : c1) / 2 + j % (kValues / 2) : c0 + j;
             double turns = position * a.frequencies[min(at, a.pairs - 1)] * 0.15915494309189533577;  // 1 / (2 pi)
             turns -= rint(turns);
-            rotary_turn<T>(static_cast<float>(turns), cs[j], sn[j]);
+            rotary_turn<T>(turns, cs[j], sn[j]);
             cs[j] *= a.magnitude;
             sn[j] *= a.magnitude * a.sign;
         }
