@@ -10,7 +10,7 @@ namespace {
 
 using namespace ops_rec_binding;
 
-// set once by set_layer_fallbacks(); never released (calls may come during interpreter exit)
+// set once by set_layer_fallbacks(), with them kept_columns; never released (calls may come during interpreter exit)
 struct Fallbacks {
     PyObject* residual_norm = nullptr;
     PyObject* residual_norm_backward = nullptr;
@@ -20,6 +20,8 @@ struct Fallbacks {
     PyObject* gated_linear = nullptr;
     PyObject* gated_linear_backward = nullptr;
 } fallbacks;
+
+int64_t kept_columns = 0;  // _layer.KEPT_COLUMNS: up to so many columns of x nothing is kept for gated_linear's backward
 
 bool is_float(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
 
@@ -419,8 +421,6 @@ Pair rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& frequencies
 
 // -------------------------------------------------------------------------------------------------- gated projections ----
 
-constexpr int64_t kKeptColumns = 192;  // _layer.KEPT_COLUMNS
-
 // all of the description but hidden and mixed; false when the call is not in canonical form
 bool describe_gated_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, c10::string_view activation, gated_linear_params& p)
 {
@@ -452,7 +452,7 @@ Pair gated_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, 
     if (describe_gated_linear(x, weight, bias, activation, p)) {
         const c10::DeviceGuard guard(x.device());
         Tensor hidden = empty({p.rows, p.inner}, x.scalar_type(), x.device());
-        Tensor mixed = keep && p.cols > kKeptColumns ? empty({p.rows, 3 * p.inner}, at::kShort, x.device()) : empty({0}, at::kShort, x.device());
+        Tensor mixed = keep && p.cols > kept_columns ? empty({p.rows, 3 * p.inner}, at::kShort, x.device()) : empty({0}, at::kShort, x.device());
         p.hidden = hidden.data_ptr();
         p.mixed = ptr(mixed);
         const int rc = gated_linear_fwd(&p, stream_of(x));
@@ -543,7 +543,7 @@ Pair gated_linear_autograd(const Tensor& x, const Tensor& weight, const OptTenso
 void ops_rec_binding::define_layer(py::module_& m)
 {
     m.def("set_layer_fallbacks", [](py::object residual_norm_fn, py::object residual_norm_backward_fn, py::object norm_gate_fn, py::object norm_gate_backward_fn,
-                                    py::object rotary_fn, py::object gated_linear_fn, py::object gated_linear_backward_fn) {
+                                    py::object rotary_fn, py::object gated_linear_fn, py::object gated_linear_backward_fn, int64_t kept) {
         fallbacks.residual_norm = residual_norm_fn.release().ptr();
         fallbacks.residual_norm_backward = residual_norm_backward_fn.release().ptr();
         fallbacks.norm_gate = norm_gate_fn.release().ptr();
@@ -551,7 +551,9 @@ void ops_rec_binding::define_layer(py::module_& m)
         fallbacks.rotary = rotary_fn.release().ptr();
         fallbacks.gated_linear = gated_linear_fn.release().ptr();
         fallbacks.gated_linear_backward = gated_linear_backward_fn.release().ptr();
+        kept_columns = kept;
     });
+    m.def("kept_columns", [] { return kept_columns; });
 }
 
 TORCH_LIBRARY_IMPL(ops_rec, CUDA, m)

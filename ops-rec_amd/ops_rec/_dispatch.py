@@ -32,7 +32,7 @@ def _load():
                          _activation.distance_in_linear_silu, _activation.in_linear_silu_backward, _paged_fp8.hstu_paged_fp8,
                          _paged_fp8.hstu_paged_fp8_append, _paged_fp8.hstu_paged_fp8_evict)  # fmt: skip
     module.set_layer_fallbacks(_layer.residual_norm, _layer.residual_norm_backward, _layer.norm_gate, _layer.norm_gate_backward, _layer.rotary,
-                                _layer.gated_linear, _layer.gated_linear_backward)  # fmt: skip
+                                _layer.gated_linear, _layer.gated_linear_backward, _layer.KEPT_COLUMNS)  # fmt: skip
     return module
 
 

@@ -8,6 +8,7 @@ import torch
 
 import ops_rec
 import layer_reference as R
+from ops_rec import _dispatch, _layer
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -175,3 +176,20 @@ def test_a_captured_step_follows_the_size_of_its_gradients(cols):
         for got, ref, eager, name in zip(outs[:2], want, step(), ("x", "weight")):
             assert torch.equal(got, eager)
             compare(got, ref, name)
+
+
+def test_both_implementations_keep_from_the_same_width_on():
+    limit = _layer.KEPT_COLUMNS
+    assert _dispatch.binding is not None and _dispatch.binding.kept_columns() == limit
+    for cols in (limit - 8, limit, limit + 8):
+        g = torch.Generator().manual_seed(cols)
+        x, w, dh = (randn(g, *shape, dtype=BF16, std=0.3).to(DEV) for shape in ((130, cols), (80, cols), (130, 40)))
+        native, python = A.gated_linear(x, w, None, "silu", True), _layer.gated_linear(x, w, None, "silu", True)
+        assert all(torch.equal(a, b) for a, b in zip(native, python)) and (native[1].numel() != 0) == (cols > limit)
+        meta = torch.ops.ops_rec.gated_linear(x.to("meta"), w.to("meta"), None, "silu", True)
+        assert [t.shape for t in meta] == [t.shape for t in native]
+        want = definition(x, w, None, dh, "silu")
+        got = A.gated_linear_backward(dh, x, w, None, native[1], "silu", [True, True, False])
+        for a, b, ref, name in zip(got, _layer.gated_linear_backward(dh, x, w, None, python[1], "silu", [True, True, False]), want, ("x", "weight")):
+            assert torch.equal(a, b)
+            compare(a, ref, name)
