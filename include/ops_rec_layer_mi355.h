@@ -190,6 +190,15 @@ typedef struct gated_linear_bwd_params {
     void* bias_grad;   /* [2 * inner], or NULL */
 } gated_linear_bwd_params;
 
+/* the parts of a backward: the gradients of g and u, out of mixed or multiplied again, and the products behind them */
+#define OPS_REC_GATED_MIXED_GRAD 0
+#define OPS_REC_GATED_X_GRAD 1
+#define OPS_REC_GATED_WEIGHT_GRAD 2
+
+/* name of the kernel variant gated_linear_bwd would launch for a part, and the chunks its depth is cut into (chunks may be NULL); NULL for a part the call does
+ * not have, or after an error */
+HSTU_API const char* gated_linear_bwd_kernel_name(const gated_linear_bwd_params* params, int part, int64_t* chunks);
+
 HSTU_API int gated_linear_bwd_workspace_size(const gated_linear_bwd_params* params, uint64_t* workspace_bytes);
 HSTU_API int gated_linear_bwd(const gated_linear_bwd_params* params, void* workspace, uint64_t workspace_bytes, void* stream);
 

@@ -339,6 +339,23 @@ HSTU_API int gated_linear_fwd(const gated_linear_params* p, void* stream)
     return launch_tiles(forward_tile(p), a, stream, "gated_gemm_kernel (forward)");
 }
 
+HSTU_API const char* gated_linear_bwd_kernel_name(const gated_linear_bwd_params* p, int part, int64_t* chunks)
+{
+    if (validate(p) != HSTU_OK) {
+        return nullptr;
+    }
+    const BackwardPlan b = plan_backward(p);
+    const Product* product = part == OPS_REC_GATED_X_GRAD ? &b.x : part == OPS_REC_GATED_WEIGHT_GRAD ? &b.w : nullptr;
+    if (product != nullptr ? product->tile == nullptr : part != OPS_REC_GATED_MIXED_GRAD) {
+        set_error(HSTU_ERR_INVALID, "the call has no part %d", part);
+        return nullptr;
+    }
+    if (chunks != nullptr) {
+        *chunks = product != nullptr ? product->chunks : 1;
+    }
+    return product != nullptr ? product->tile->name : p->fwd.mixed != nullptr ? "gated_stage" : mixed_tile(&p->fwd).name;
+}
+
 HSTU_API int gated_linear_bwd_workspace_size(const gated_linear_bwd_params* p, uint64_t* workspace_bytes)
 {
     const int rc = validate(p);

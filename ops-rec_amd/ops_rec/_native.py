@@ -59,6 +59,7 @@ LAYER_SYMBOLS = (
     "rotary_fwd",
     "gated_linear_fwd",
     "gated_linear_fwd_kernel_name",
+    "gated_linear_bwd_kernel_name",
     "gated_linear_bwd_workspace_size",
     "gated_linear_bwd",
 )
@@ -422,6 +423,8 @@ def load() -> ctypes.CDLL:
     lib.hstu_paged_fp8_fwd_kernel_name.argtypes = [ctypes.POINTER(PagedFp8FwdParams)]
     lib.gated_linear_fwd_kernel_name.restype = ctypes.c_char_p
     lib.gated_linear_fwd_kernel_name.argtypes = [ctypes.POINTER(GatedLinearParams)]
+    lib.gated_linear_bwd_kernel_name.restype = ctypes.c_char_p
+    lib.gated_linear_bwd_kernel_name.argtypes = [ctypes.POINTER(GatedLinearBwdParams), ctypes.c_int, ctypes.POINTER(ctypes.c_int64)]
     lib.ln_mul_fwd.restype = ctypes.c_int
     lib.ln_mul_fwd.argtypes = [ctypes.POINTER(LnMulParams), ctypes.c_void_p]
     lib.ln_mul_fwd_kernel_name.restype = ctypes.c_char_p

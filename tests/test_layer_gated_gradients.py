@@ -1,6 +1,7 @@
 """gated_linear's backward where tests/test_layer_gated_linear.py does not go: values that are not finite, the ends of fp16, every tile of its products, what is kept above
 192 columns of x, and the largest sizes."""
 
+import ctypes
 import math
 
 import pytest
@@ -8,7 +9,7 @@ import torch
 
 import ops_rec
 import layer_reference as R
-from ops_rec import _dispatch, _layer
+from ops_rec import _dispatch, _layer, _native
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -193,3 +194,66 @@ def test_both_implementations_keep_from_the_same_width_on():
         for a, b, ref, name in zip(got, _layer.gated_linear_backward(dh, x, w, None, python[1], "silu", [True, True, False]), want, ("x", "weight")):
             assert torch.equal(a, b)
             compare(a, ref, name)
+
+
+def planned(rows, cols, inner, dtype=BF16, kept=False):
+    """(part, kernel, whether its depth is cut) of the three parts of a backward"""
+    p = _native.GatedLinearBwdParams()
+    p.struct_size = ctypes.sizeof(p)
+    none = torch.empty(0)
+    _layer._describe_gated_linear(p.fwd, torch.empty(rows, cols, dtype=dtype, device="meta"), torch.empty(2 * inner, cols, dtype=dtype, device="meta"), None, none, none, "silu")
+    p.fwd.x = p.fwd.weight = p.grad = p.x_grad = p.weight_grad = 0x1000  # never dereferenced
+    p.fwd.mixed = 0x1000 if kept else None
+    parts, chunks = [], ctypes.c_int64(0)
+    for part in range(3):
+        name = _native.load().gated_linear_bwd_kernel_name(ctypes.byref(p), part, ctypes.byref(chunks))
+        parts.append((part, name.decode().replace("gated_gemm_", ""), chunks.value > 1))
+    return parts
+
+
+# what is left over differs in every dimension of every tile: rows, columns of x, columns of hidden
+TILES = [(16, 8, 8), (16, 8, 416), (669, 8, 8), (4115, 8, 568), (16669, 8, 8), (18694, 8, 72), (17358, 136, 8), (4297, 136, 1568), (22779, 280, 8), (11595, 160, 1728),
+         (25679, 272, 8), (17548, 152, 1536), (18, 400, 4120), (5786, 2952, 8), (16, 4232, 1016), (11203, 520, 3744)]  # fmt: skip
+
+
+def test_every_tile_of_the_backward_is_among_them():
+    if torch.cuda.get_device_properties(0).multi_processor_count != 256:
+        pytest.skip("planned for 256 compute units")
+    tiles = {0: ["64x128", "128x128", "128x256"], 1: ["64x128", "128x128", "128x256", "192x256", "256x256"], 2: ["128x128", "128x256", "256x256"]}
+    expected = {(part, name, cut) for part, names in tiles.items() for name in names for cut in ((False, True) if part != 0 else (False,))}
+    assert {entry for size in TILES for entry in planned(*size)} == expected
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("rows,cols,inner", TILES)
+def test_every_tile_of_the_backward(rows, cols, inner, dtype):
+    g = torch.Generator().manual_seed(rows + cols)
+    x, w = randn(g, rows, cols, dtype=dtype).to(DEV), randn(g, 2 * inner, cols, dtype=dtype, std=1.5 / math.sqrt(cols)).to(DEV)
+    b, dh = randn(g, 2 * inner, dtype=dtype, std=0.5).to(DEV), randn(g, rows, inner, dtype=dtype).to(DEV)
+    mixed = A.gated_linear(x, w, b, "silu", True)[1]
+    want = definition(x, w, b, dh, "silu")
+    for kept in [torch.empty(0, dtype=torch.int16, device=DEV)] + ([mixed] if mixed.numel() else []):
+        for got, ref, name in zip(A.gated_linear_backward(dh, x, w, b, kept, "silu", [True] * 3), want, ("x", "weight", "bias")):
+            compare(got, ref, (name, kept.numel() != 0))
+
+
+@pytest.mark.parametrize("keep", [True, False])
+def test_rows_of_d_mixed_that_fill_a_descriptor(keep):
+    """256 rows of 2^22 columns are the 2^31 bytes that a tile of the x gradient may ask for; a gradient on a few columns alone, so that these are what the sums are made of."""
+    rows, cols, inner = 500, 200, 1 << 21
+    if torch.cuda.get_device_properties(0).multi_processor_count == 256:
+        assert planned(rows, cols, inner)[1:] == [(1, "256x256", True), (2, "256x256", True)]
+    g = torch.Generator().manual_seed(3)
+    some = torch.tensor([0, 1, 255, 70000, inner // 2 - 1, inner // 2, inner - 256, inner - 1], device=DEV)
+    both = torch.cat([some, some + inner])
+    x, few, dh = randn(g, rows, cols, dtype=BF16).to(DEV), randn(g, 16, cols, dtype=BF16, std=0.1).to(DEV), randn(g, rows, 8, dtype=BF16).to(DEV)
+    weight, grad = torch.zeros(2 * inner, cols, dtype=BF16, device=DEV), torch.zeros(rows, inner, dtype=BF16, device=DEV)
+    weight[both], grad[:, some] = few, dh
+    hidden, mixed = A.gated_linear(x, weight, None, "silu", keep)
+    assert (mixed.numel() != 0) == keep
+    dx, dw, _ = A.gated_linear_backward(grad, x, weight, None, mixed, "silu", [True, True, False])
+    want = definition(x, few, None, dh, "silu")
+    compare(dx, want[0], "x")
+    compare(dw[both], want[1], "weight")
+    dw[both] = 0
+    assert torch.count_nonzero(dw) == 0
