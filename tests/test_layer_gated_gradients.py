@@ -257,3 +257,57 @@ def test_rows_of_d_mixed_that_fill_a_descriptor(keep):
     compare(dw[both], want[1], "weight")
     dw[both] = 0
     assert torch.count_nonzero(dw) == 0
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu", "sigmoid"])
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("rows", [5, 40, 300])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_gradients_from_what_was_kept(activation, bias, rows, dtype):
+    """All that are wanted, and each choice of them: the same bits, and nothing in the place of the others."""
+    g = torch.Generator().manual_seed(rows)
+    cols, inner = 200, 264
+    x, w = randn(g, rows, cols, dtype=dtype).to(DEV), randn(g, 2 * inner, cols, dtype=dtype, std=1.5 / math.sqrt(cols)).to(DEV)
+    b, dh = randn(g, 2 * inner, dtype=dtype, std=0.5).to(DEV) if bias else None, randn(g, rows, inner, dtype=dtype).to(DEV)
+    mixed = A.gated_linear(x, w, b, activation, True)[1]
+    assert mixed.numel() != 0
+    grads = A.gated_linear_backward(dh, x, w, b, mixed, activation, [True, True, True])
+    for got, ref, name in list(zip(grads, definition(x, w, b, dh, activation), ("x", "weight", "bias")))[: 3 if bias else 2]:
+        compare(got, ref, name)
+    assert bias or grads[2].numel() == 0
+    for n in range(7):
+        wanted = [bool(n & 1), bool(n & 2), bool(n & 4)]
+        got = A.gated_linear_backward(dh, x, w, b, mixed, activation, wanted)
+        assert all(torch.equal(a, full) if want else a.numel() == 0 for a, full, want in zip(got, grads, wanted))
+    # through autograd, with inputs that need no gradient
+    leaves = [t if t is None else t.clone() for t in (x, w, b)]
+    for frozen in range(3 if bias else 2):
+        for i, t in enumerate(leaves):
+            if t is not None:
+                t.requires_grad_(i != frozen)
+        needed = [i for i, t in enumerate(leaves) if t is not None and i != frozen]
+        hidden = A.gated_linear(*leaves, activation, True)[0]
+        for i, got in zip(needed, torch.autograd.grad(hidden, [leaves[i] for i in needed], dh)):
+            assert torch.equal(got, grads[i])
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu", "sigmoid"])
+@pytest.mark.parametrize("cols", [64, 200])
+def test_gradients_of_gates_far_out(activation, cols):
+    """Gates whose exponentials overflow and underflow: their slopes are 0, 1 or those of the definition, and nothing is NaN."""
+    inner = 8
+    gates = torch.tensor([0.0, 200.0, -200.0, 1e30, -1e30, 3e38, -3e38, 60.0], dtype=BF16)
+    bias = torch.cat([gates, torch.ones(inner, dtype=BF16)]).to(DEV)
+    x, w = torch.zeros(6, cols, dtype=BF16, device=DEV), torch.zeros(2 * inner, cols, dtype=BF16, device=DEV)
+    x[:, 0] = 1.0
+    mixed = A.gated_linear(x, w, bias, activation, True)[1]
+    assert (mixed.numel() != 0) == (cols == 200)
+    dx, dw, db = A.gated_linear_backward(torch.ones(6, inner, dtype=BF16, device=DEV), x, w, bias, mixed, activation, [True, True, True])
+    z = torch.where(gates.double().abs() > 1000, 1000.0 * gates.double().sign(), gates.double()).requires_grad_(True)
+    (slope,) = torch.autograd.grad(act(activation, z).sum(), z)
+    value = torch.where(gates > 1000, gates.double() if activation != "sigmoid" else torch.ones(()).double(), act(activation, z.detach()))
+    want = 6 * torch.cat([slope, value])  # six rows, each with u = 1 and a gradient of 1
+    fits = want.abs() < 3.3e38
+    for got in (db.double().cpu(), dw[:, 0].double().cpu()):
+        assert torch.allclose(got[fits], want[fits], rtol=2.0**-7, atol=2.0**-126) and not torch.isnan(got).any()
+    assert torch.count_nonzero(dw[:, 1:]) == 0 and torch.count_nonzero(dx) == 0
