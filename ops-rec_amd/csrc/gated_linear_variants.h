@@ -9,8 +9,9 @@ struct GatedTile {
     const char* name;
     int cols;  // of the output, per workgroup (in the forward: of hidden)
     int rows;
-    // what a workgroup takes, in us (measured at 512 .. 4096 deep products; only their ratios matter): a step of the depth with a compute unit to itself, its
-    // share of a step where the units are full, and everything before the first and behind the last step
+    // what a workgroup takes, in us (measured at 512 .. 4096 deep products): a step of the depth with a compute unit to itself, its share of a step where
+    // the units are full, and everything before the first and behind the last step.  Among tiles their ratios decide; against the bytes of the kernel for few
+    // rows, and the traffic and the launch of partial outputs, their size
     float alone, step, fixed;
 };
 
