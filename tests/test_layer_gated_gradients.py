@@ -311,3 +311,27 @@ def test_gradients_of_gates_far_out(activation, cols):
     for got in (db.double().cpu(), dw[:, 0].double().cpu()):
         assert torch.allclose(got[fits], want[fits], rtol=2.0**-7, atol=2.0**-126) and not torch.isnan(got).any()
     assert torch.count_nonzero(dw[:, 1:]) == 0 and torch.count_nonzero(dx) == 0
+
+
+@pytest.mark.parametrize("filled", [0x7E, 0xFF])  # 8.5e37, NaN
+@pytest.mark.parametrize("rows,cols,inner", [(5, 200, 40), (300, 200, 264), (1000, 64, 1000), (2500, 72, 520)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_workspaces_that_hold_something(rows, cols, inner, dtype, filled):
+    """What a workspace held before reaches nothing: neither the gradients nor the power of two that fp16 is scaled by."""
+    g = torch.Generator().manual_seed(rows)
+    x, w = randn(g, rows, cols, dtype=dtype).to(DEV), randn(g, 2 * inner, cols, dtype=dtype, std=1.5 / math.sqrt(cols)).to(DEV)
+    b, dh = randn(g, 2 * inner, dtype=dtype, std=0.5).to(DEV), randn(g, rows, inner, dtype=dtype).to(DEV)
+    mixed = A.gated_linear(x, w, b, "silu", True)[1]
+    want = A.gated_linear_backward(dh, x, w, b, mixed, "silu", [True] * 3)
+    got = [torch.empty_like(t).fill_(-1.0) for t in want]
+    p = _native.GatedLinearBwdParams()
+    p.struct_size = ctypes.sizeof(p)
+    _layer._describe_gated_linear(p.fwd, x, w, b, None, mixed if mixed.numel() else None, "silu")
+    p.grad, p.x_grad, p.weight_grad, p.bias_grad = (t.data_ptr() for t in (dh, *got))
+    lib, size = _native.load(), ctypes.c_uint64(0)
+    assert lib.gated_linear_bwd_workspace_size(ctypes.byref(p), ctypes.byref(size)) == 0
+    space = torch.full((size.value + 512,), filled, dtype=torch.uint8, device=DEV)
+    assert lib.gated_linear_bwd(ctypes.byref(p), space.data_ptr(), size.value, torch.cuda.current_stream().cuda_stream) == 0, _native.last_error()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(bool(torch.isfinite(t).all()) for t in got)
+    assert bool((space[size.value :] == filled).all())
